@@ -1,0 +1,50 @@
+// What the translation units of the layer operators need of a context.  Not
+// part of the public ABI.
+#pragma once
+#include <cstddef>
+#include <cstdio>
+#include <cuda_runtime.h>
+
+#include "bm_sampler.h"
+
+enum { BM_WORK_SCAN = 0, BM_WORK_FP8 = 1, BM_WORK_KINDS = 2 };
+
+// The library's error channel: sets bm_last_error's text, returns code.
+int bm_detail_fail(int code, const char *msg);
+
+// The context's device (returned), SM count, device error word and stream.
+int bm_detail_ctx(bm_ctx_t *c, int *sms, int **d_err, cudaStream_t *stream);
+
+// The context's workspace of a kind, at least `bytes` long, zeroed when it was
+// allocated and never freed before the context.  Growing it allocates and
+// synchronises the device, so it fails under stream capture.
+int bm_detail_work(bm_ctx_t *c, int kind, size_t bytes, void **out);
+
+namespace bmc {
+
+inline int cuda_fail(cudaError_t e, const char *what) {
+    char buf[256];
+    snprintf(buf, sizeof(buf), "%s: %s", what, cudaGetErrorString(e));
+    return bm_detail_fail(e == cudaErrorMemoryAllocation ? BM_ERR_OOM : BM_ERR_CUDA, buf);
+}
+
+// Makes a context's device current, and the caller's again at the end.
+struct DeviceGuard {
+    int before = -1, now;
+    cudaError_t error;
+    explicit DeviceGuard(int device) : now(device) {
+        error = cudaGetDevice(&before);
+        if (error == cudaSuccess && before != now) error = cudaSetDevice(now);
+    }
+    ~DeviceGuard() {
+        if (before >= 0 && before != now) cudaSetDevice(before);
+    }
+};
+
+}  // namespace bmc
+
+#define BMC_CK(call)                                                     \
+    do {                                                                 \
+        cudaError_t e_ = (call);                                         \
+        if (e_ != cudaSuccess) return bmc::cuda_fail(e_, #call);         \
+    } while (0)

@@ -23,7 +23,9 @@
 
 #include <cuda_runtime.h>
 
+#include "bm_ctx.cuh"
 #include "bm_sampler.h"
+#include "bm_slots.cuh"
 
 namespace {
 
@@ -61,14 +63,61 @@ __global__ void decode_update_kernel(const int32_t *ids, int B, int32_t *ring, i
     if (out_id) out_id[r] = id;
 }
 
-}  // namespace
+// The map of a compaction, one CTA: row_of[r] = the row that moves to r
+// (active rows first, in order, stopped rows behind them, in order); live[r]
+// the same for active rows and -1 elsewhere; map a copy of row_of.
+__global__ void __launch_bounds__(1024)
+    compact_map_kernel(const int32_t *status, int B, int32_t *row_of, int32_t *live,
+                       int32_t *map) {
+    __shared__ int warp_sum[32], below;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int n_active = 0;
+    for (int r0 = 0; r0 < B; r0 += 1024) {
+        const int r = r0 + (int)threadIdx.x;
+        n_active += __syncthreads_count(r < B && status[r] == BM_DECODE_ACTIVE);
+    }
+    if (threadIdx.x == 0) below = 0;
+    for (int r0 = 0; r0 < B; r0 += 1024) {
+        const int r = r0 + (int)threadIdx.x;
+        const bool act = r < B && status[r] == BM_DECODE_ACTIVE;
+        const unsigned m = __ballot_sync(0xffffffffu, act);
+        if (lane == 0) warp_sum[warp] = __popc(m);
+        __syncthreads();
+        int before = below + __popc(m & ((1u << lane) - 1u)), all = 0;
+        for (int w = 0; w < 32; ++w) {
+            if (w < warp) before += warp_sum[w];
+            all += warp_sum[w];
+        }
+        if (r < B) {
+            // r - before stopped rows precede row r
+            const int to = act ? before : n_active + r - before;
+            row_of[to] = r;
+            live[to] = act ? r : -1;
+            if (map) map[to] = r;
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) below += all;
+        __syncthreads();
+    }
+}
 
-// the library's error channel (bm_sampler.cu): bm_last_error reads it
-int bm_detail_fail(int code, const char *msg);
+__global__ void __launch_bounds__(1024)
+    count_active_kernel(const int32_t *status, int B, int32_t *active) {
+    int n = 0;
+    for (int r0 = 0; r0 < B; r0 += 1024) {
+        const int r = r0 + (int)threadIdx.x;
+        n += __syncthreads_count(r < B && status[r] == BM_DECODE_ACTIVE);
+    }
+    if (threadIdx.x == 0) *active = n;
+}
+
+}  // namespace
 
 struct bm_decode {
     bm_ctx_t *ctx;
     int B, max_tokens, n_stop;
+    int rows;          // rows that a step takes
+    int32_t *d_move;   // [2 x B] the maps of a compaction
     int32_t *d_ring;   // [B x 256]
     int64_t *d_off;    // [B + 1], 256 r
     int32_t *d_pos;    // ids pushed so far (prompt included)
@@ -109,16 +158,33 @@ void release(bm_decode_t *d) {
     cudaFree(d->d_stop);
     cudaFree(d->d_active);
     cudaFree(d->d_id);
+    cudaFree(d->d_move);
     if (d->h_active) cudaFreeHost(d->h_active);
 }
 
 int launch_update(bm_decode_t *d, int32_t *d_out_id, cudaStream_t s) {
-    const int threads = 256, blocks = (d->B + threads - 1) / threads;
-    decode_update_kernel<<<blocks, threads, 0, s>>>(d->d_id, d->B, d->d_ring, d->d_pos, d->d_cur,
+    const int threads = 256, blocks = (d->rows + threads - 1) / threads;
+    decode_update_kernel<<<blocks, threads, 0, s>>>(d->d_id, d->rows, d->d_ring, d->d_pos, d->d_cur,
                                                     d->d_status, d->d_ngen, d->d_stop, d->n_stop,
                                                     d->max_tokens, d->d_active, d_out_id);
     DCK(cudaGetLastError());
     return BM_OK;
+}
+
+// The loop state's arrays as regions of B slots, then the caller's.
+int all_regions(const bm_decode_t *d, const bm_slot_region_t *more, int n_more,
+                bm_slot_region_t *out) {
+    int n = 0;
+    auto add = [&](void *base, int64_t row) {
+        out[n++] = bm_slot_region_t{base, row, row, row * d->B, 1, 0};
+    };
+    add(d->d_ring, HMAX * 4);
+    add(d->d_pos, 4);
+    add(d->d_cur, 4);
+    add(d->d_status, 4);
+    add(d->d_ngen, 4);
+    for (int i = 0; i < n_more; ++i) out[n++] = more[i];
+    return n;
 }
 
 }  // namespace
@@ -139,6 +205,7 @@ int bm_decode_create(bm_ctx_t *ctx, int B, int max_tokens, const int32_t *stop_i
     if (!d) return dfail(BM_ERR_OOM, "calloc");
     d->ctx = ctx;
     d->B = B;
+    d->rows = B;
     d->max_tokens = max_tokens;
     d->n_stop = n_stop;
     cudaError_t e = cudaSuccess;
@@ -154,6 +221,7 @@ int bm_decode_create(bm_ctx_t *ctx, int B, int max_tokens, const int32_t *stop_i
     al(reinterpret_cast<void **>(&d->d_stop), (size_t)n_stop * 4);
     al(reinterpret_cast<void **>(&d->d_active), 4);
     al(reinterpret_cast<void **>(&d->d_id), (size_t)B * 4);
+    al(reinterpret_cast<void **>(&d->d_move), (size_t)B * 8);
     if (e == cudaSuccess) e = cudaMallocHost(reinterpret_cast<void **>(&d->h_active), 4);
     if (e == cudaSuccess) {
         std::vector<int64_t> off((size_t)B + 1);
@@ -217,6 +285,7 @@ int bm_decode_reset(bm_decode_t *d, const int32_t *h_prompt, const int64_t *h_pr
     DCK(cudaMemset(d->d_status, 0, (size_t)B * 4));
     DCK(cudaMemset(d->d_ngen, 0, (size_t)B * 4));
     DCK(cudaMemcpy(d->d_active, &active, 4, cudaMemcpyHostToDevice));
+    d->rows = B;
     return BM_OK;
 }
 
@@ -224,7 +293,7 @@ int bm_decode_step(bm_decode_t *d, const float *d_logits, int V, int64_t ld,
                    const bm_knobs_t *d_knobs, int64_t knob_stride, const float *d_uniform,
                    int32_t *d_out_id, void *stream) {
     if (!d) return dfail(BM_ERR_INVALID_ARG, "decode is NULL");
-    int rc = bm_sample_batch(d->ctx, d_logits, d->B, V, ld, d->d_ring, d->d_off, d_knobs,
+    int rc = bm_sample_batch(d->ctx, d_logits, d->rows, V, ld, d->d_ring, d->d_off, d_knobs,
                              knob_stride, d_uniform, d->d_id, nullptr, nullptr, stream);
     if (rc != BM_OK) return rc;
     cudaStream_t s = stream ? static_cast<cudaStream_t>(stream)
@@ -237,13 +306,64 @@ int bm_decode_ternary_step(bm_decode_t *d, const float *d_hidden, int d_model,
                            float w_scale, int V, const bm_knobs_t *d_knobs, int64_t knob_stride,
                            const float *d_uniform, int32_t *d_out_id, void *stream) {
     if (!d) return dfail(BM_ERR_INVALID_ARG, "decode is NULL");
-    int rc = bm_ternary_sample_batch(d->ctx, d_hidden, d->B, d_model, d_norm_f, d_lmh_norm, d_w8,
+    int rc = bm_ternary_sample_batch(d->ctx, d_hidden, d->rows, d_model, d_norm_f, d_lmh_norm, d_w8,
                                      w_scale, V, d->d_ring, d->d_off, d_knobs, knob_stride,
                                      d_uniform, d->d_id, nullptr, nullptr, stream);
     if (rc != BM_OK) return rc;
     cudaStream_t s = stream ? static_cast<cudaStream_t>(stream)
                             : static_cast<cudaStream_t>(bm_ctx_stream(d->ctx));
     return launch_update(d, d_out_id, s);
+}
+
+int bm_decode_reorder(bm_decode_t *d, const int32_t *d_src, const bm_slot_region_t *regions,
+                      int n_regions, void *stream) {
+    if (!d) return dfail(BM_ERR_INVALID_ARG, "decode is NULL");
+    int rc = bms::check_regions(regions, n_regions);
+    if (rc != BM_OK) return rc;
+    if (!d_src || reinterpret_cast<uintptr_t>(d_src) % 4)
+        return dfail(BM_ERR_INVALID_ARG, "src NULL or not 4-byte aligned");
+    if (d->B > BM_SLOT_MAX) return dfail(BM_ERR_UNSUPPORTED, "B > BM_SLOT_MAX (8192)");
+    int sms, *err;
+    cudaStream_t s;
+    bmc::DeviceGuard guard(bm_detail_ctx(d->ctx, &sms, &err, &s));
+    DCK(guard.error);
+    if (stream) s = static_cast<cudaStream_t>(stream);
+    bm_slot_region_t r[2 * BM_SLOT_REGIONS];
+    const int n = all_regions(d, regions, n_regions, r);
+    DCK(bms::reorder(r, n, d_src, d->B, sms, s));
+    count_active_kernel<<<1, 1024, 0, s>>>(d->d_status, d->B, d->d_active);
+    DCK(cudaGetLastError());
+    return BM_OK;
+}
+
+int bm_decode_compact(bm_decode_t *d, const bm_slot_region_t *regions, int n_regions,
+                      int32_t *d_map, void *stream) {
+    if (!d) return dfail(BM_ERR_INVALID_ARG, "decode is NULL");
+    int rc = bms::check_regions(regions, n_regions);
+    if (rc != BM_OK) return rc;
+    if (reinterpret_cast<uintptr_t>(d_map) % 4)
+        return dfail(BM_ERR_INVALID_ARG, "map not 4-byte aligned");
+    if (d->B > BM_SLOT_MAX) return dfail(BM_ERR_UNSUPPORTED, "B > BM_SLOT_MAX (8192)");
+    int sms, *err;
+    cudaStream_t s;
+    bmc::DeviceGuard guard(bm_detail_ctx(d->ctx, &sms, &err, &s));
+    DCK(guard.error);
+    if (stream) s = static_cast<cudaStream_t>(stream);
+    int32_t *row_of = d->d_move, *live = d->d_move + d->B;
+    compact_map_kernel<<<1, 1024, 0, s>>>(d->d_status, d->B, row_of, live, d_map);
+    DCK(cudaGetLastError());
+    bm_slot_region_t r[2 * BM_SLOT_REGIONS];
+    const int n = all_regions(d, nullptr, 0, r);
+    DCK(bms::reorder(r, n, row_of, d->B, sms, s));
+    if (n_regions) DCK(bms::reorder(regions, n_regions, live, d->B, sms, s));
+    return BM_OK;
+}
+
+int bm_decode_set_rows(bm_decode_t *d, int rows) {
+    if (!d) return dfail(BM_ERR_INVALID_ARG, "decode is NULL");
+    if (rows < 1 || rows > d->B) return dfail(BM_ERR_INVALID_ARG, "rows outside [1, B]");
+    d->rows = rows;
+    return BM_OK;
 }
 
 int bm_decode_views(const bm_decode_t *d, bm_decode_views_t *v) {

@@ -28,6 +28,7 @@
 // 1239-1262); this bf16 variant has no counterpart there and is checked
 // against a CPU GEMM of the same bf16 operands.  Every wait is bounded.
 #include "bm_lmhead.cuh"
+#include "bm_tc.cuh"
 
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -56,7 +57,6 @@ constexpr size_t GEMM_SMEM = 1024 + (size_t)STAGES * STAGE_BYTES + 256;
 // column per thread)
 constexpr size_t EPI_STAGE = 32 * 256 * 4;
 constexpr size_t GEMM_SMEM_SUM = GEMM_SMEM + EPI_STAGE;
-constexpr unsigned long long WAIT_NS = 2000000000ull;  // bounded waits: 2 s
 
 // GPT-2 ids the reference never penalises (src/bitmamba.h:21-24).
 __device__ __forceinline__ bool protected_id(int id) {
@@ -71,41 +71,6 @@ __device__ __forceinline__ bool ahead(float a, int ia, float b, int ib) {
     return a > b || (a == b && ia < ib);
 }
 
-__device__ __forceinline__ uint32_t sa(const void *p) {
-    return (uint32_t)__cvta_generic_to_shared(p);
-}
-__device__ __forceinline__ unsigned long long gtimer() {
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-__device__ __forceinline__ void mbar_init(uint64_t *b, uint32_t n) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(sa(b)), "r"(n));
-}
-__device__ __forceinline__ void mbar_expect_tx(uint64_t *b, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(sa(b)),
-                 "r"(bytes)
-                 : "memory");
-}
-__device__ __forceinline__ bool mbar_try(uint64_t *b, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-        " selp.u32 %0, 1, 0, p;\n}"
-        : "=r"(ok)
-        : "r"(sa(b)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-__device__ __forceinline__ bool mbar_wait(uint64_t *b, uint32_t parity) {
-    if (mbar_try(b, parity)) return true;
-    const unsigned long long t0 = gtimer();
-    for (unsigned it = 0; it < (1u << 30); ++it) {
-        if (mbar_try(b, parity)) return true;
-        if (gtimer() - t0 > WAIT_NS) return false;
-    }
-    return false;
-}
 // 16-byte asynchronous global -> shared copy (every copy of a row in flight
 // at once), and the wait for this thread's copies
 __device__ __forceinline__ void cp_async16(void *dst, const void *src) {
@@ -113,21 +78,6 @@ __device__ __forceinline__ void cp_async16(void *dst, const void *src) {
 }
 __device__ __forceinline__ void cp_async_wait_own() {
     asm volatile("cp.async.commit_group;\n cp.async.wait_all;" ::: "memory");
-}
-// 2-D tiled TMA load into this CTA only: box at (x = k, y = row) into smem
-__device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, int x, int y,
-                                            uint64_t *bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, "
-        "{%2, %3}], [%4];" ::"r"(sa(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(sa(bar))
-        : "memory");
-}
-// Shared-memory matrix descriptor of a K-major tile with 128-byte swizzle:
-// rows of 128 bytes, 8-row groups 1024 bytes apart (SBO), version 1, layout 2.
-__device__ __forceinline__ uint64_t sdesc(uint32_t addr) {
-    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
-           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 __device__ __forceinline__ void umma_f16(uint32_t tmem, uint64_t da, uint64_t db, uint32_t idesc,
                                          uint32_t accumulate) {
@@ -143,27 +93,6 @@ __device__ __forceinline__ void umma_i8(uint32_t tmem, uint64_t da, uint64_t db,
         " tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}" ::"r"(tmem),
         "l"(da), "l"(db), "r"(idesc), "r"(accumulate));
 }
-__device__ __forceinline__ void umma_commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                     sa(bar))
-                 : "memory");
-}
-// 32 consecutive fp32 accumulator columns of this thread's lane
-__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
-        "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, "
-        "%28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
-          "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
-          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
-          "=r"(r[31])
-        : "r"(addr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-
 // Persistent: CTA c takes tiles c, c + grid, ... (M-tile index fastest, so
 // CTAs running together share W tiles).  Warp 0 lane 0 is the TMA producer,
 // warp 1 lane 0 issues the MMAs, warps 2-5 drain the accumulators.  Two
@@ -680,6 +609,11 @@ __global__ void gather_kernel(const uint4 *src, int64_t w16, const int *list, ui
 }
 
 }  // namespace
+
+cudaError_t byte_map(CUtensorMap *m, const void *base, int rows, int K, int box_rows) {
+    cudaError_t e = get_encode();
+    return e != cudaSuccess ? e : make_map(m, base, rows, K, box_rows, true);
+}
 
 cudaError_t prepare() {
     cudaError_t e = get_encode();

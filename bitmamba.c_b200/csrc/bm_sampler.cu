@@ -12,6 +12,7 @@
 #include <mutex>
 #include <vector>
 
+#include "bm_ctx.cuh"
 #include "bm_kernel.cuh"
 #include "bm_lmhead.cuh"
 #include "bm_sampler.h"
@@ -70,6 +71,13 @@ struct bm_ctx {
     unsigned char *h_stage;
     unsigned char *d_stage;
     size_t cap_stage;
+    // workspaces of the layer operators, by use.  A buffer that is outgrown is
+    // kept until the context goes: a captured graph may still name it
+    struct Work {
+        void *buf[24];
+        int n;
+        size_t cap;
+    } work[BM_WORK_KINDS];
 };
 
 namespace {
@@ -362,6 +370,8 @@ void bm_ctx_destroy(bm_ctx_t *c) {
     cudaFree(c->d_nl);
     cudaFree(c->d_a2);
     cudaFree(c->d_isc2);
+    for (auto &w : c->work)
+        for (int i = 0; i < w.n; ++i) cudaFree(w.buf[i]);
     if (c->h_stage) cudaFreeHost(c->h_stage);
     if (c->stream) cudaStreamDestroy(c->stream);
     free(c);
@@ -896,3 +906,35 @@ int bm_sample_row(float *logits, int V, const int *history, int history_len, flo
 
 // The library's error channel for the other translation units (bm_decode.cu).
 int bm_detail_fail(int code, const char *msg) { return fail(code, "%s", msg); }
+
+int bm_detail_ctx(bm_ctx_t *c, int *sms, int **d_err, cudaStream_t *stream) {
+    *sms = c->sms;
+    *d_err = c->d_err;
+    *stream = c->stream;
+    return c->device;
+}
+
+int bm_detail_work(bm_ctx_t *c, int kind, size_t bytes, void **out) {
+    auto &w = c->work[kind];
+    if (bytes > w.cap || w.n == 0) {
+        constexpr int most = (int)(sizeof(w.buf) / sizeof(w.buf[0]));
+        if (w.n == most) return fail(BM_ERR_OOM, "workspace grown %d times", most);
+        size_t n = 2 * w.cap;  // doubling: all buffers together stay under twice the largest
+        if (n < bytes) n = bytes;
+        n = (n + 255) & ~(size_t)255;
+        void *p = nullptr;
+        cudaError_t e = cudaMalloc(&p, n);
+        if (e != cudaSuccess) return cuda_fail(e, "cudaMalloc(workspace)");
+        e = cudaMemset(p, 0, n);
+        // the memset is not ordered against the context's stream
+        if (e == cudaSuccess) e = cudaDeviceSynchronize();
+        if (e != cudaSuccess) {
+            cudaFree(p);
+            return cuda_fail(e, "cudaMemset(workspace)");
+        }
+        w.buf[w.n++] = p;
+        w.cap = n;
+    }
+    *out = w.buf[w.n - 1];
+    return BM_OK;
+}

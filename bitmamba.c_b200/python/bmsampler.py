@@ -64,6 +64,24 @@ class ModelHeadInfo(ctypes.Structure):
                 ("d_w8", _P), ("d_packed", _P)]
 
 
+TYPES = {"f32": 0, "bf16": 1}  # BM_F32, BM_BF16
+
+
+class SsmLayerStruct(ctypes.Structure):
+    """bm_ssm_layer_t."""
+    _fields_ = [("n_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("n_slots", ctypes.c_int32), ("type", ctypes.c_int32), ("conv_w", _P),
+                ("conv_b", _P), ("dt_bias", _P), ("a_log", _P), ("d", _P), ("conv_state", _P),
+                ("h_state", _P)]
+
+
+class SlotRegion(ctypes.Structure):
+    """bm_slot_region_t."""
+    _fields_ = [("base", _P), ("row_bytes", ctypes.c_int64), ("row_pitch", ctypes.c_int64),
+                ("outer_pitch", ctypes.c_int64), ("n_outer", ctypes.c_int32),
+                ("reserved", ctypes.c_int32)]
+
+
 class DecodeViews(ctypes.Structure):
     """bm_decode_views_t: device pointers of a decode state."""
     _fields_ = [("ring", _P), ("ring_off", _P), ("current", _P), ("status", _P),
@@ -125,6 +143,20 @@ def lib():
         L.bm_model_head_info.argtypes = [_P, ctypes.POINTER(ModelHeadInfo)]
         L.bm_model_head_free.argtypes = [_P]
         L.bm_model_head_free.restype = None
+        L.bm_ssm_prefill.argtypes = [_P, _P, _P, _P, _P, _P, _P, ctypes.c_int64, ctypes.c_int,
+                                     _P, ctypes.c_int, _P, _P, _P, ctypes.c_int64, _P]
+        L.bm_ssm_step.argtypes = [_P, _P, _P, _P, _P, _P, _P, ctypes.c_int64, ctypes.c_int, _P,
+                                  _P, ctypes.c_int64, _P]
+        L.bm_slots_reorder.argtypes = [_P, _P, ctypes.c_int, _P, ctypes.c_int, _P]
+        L.bm_decode_reorder.argtypes = [_P, _P, _P, ctypes.c_int, _P]
+        L.bm_decode_compact.argtypes = [_P, _P, ctypes.c_int, _P, _P]
+        L.bm_decode_set_rows.argtypes = [_P, ctypes.c_int]
+        L.bm_fp8_quantize.argtypes = [_P, _P, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                      ctypes.c_int64, _P, _P, _P, ctypes.c_int64, _P]
+        L.bm_fp8_product.argtypes = [_P, _P, _P, ctypes.c_int64, ctypes.c_int, ctypes.c_int, _P,
+                                     _P, ctypes.c_int, _P, ctypes.c_int64, _P]
+        L.bm_fp8_logits.argtypes = [_P, _P, ctypes.c_int, ctypes.c_int, _P, _P, _P, ctypes.c_int,
+                                    _P, ctypes.c_int64, _P]
         L.bm_rng_seed.argtypes = [ctypes.c_uint64]
         L.bm_rng_seed.restype = None
         L.bm_rng_next.restype = ctypes.c_uint64
@@ -167,6 +199,28 @@ def knobs_array(temp, penalty, min_p, top_p, top_k) -> np.ndarray:
 
 def _ptr(a):
     return None if a is None else ctypes.c_void_p(a.ctypes.data)
+
+
+class SsmLayer:
+    """bm_ssm_layer_t: one layer's sizes, weights and slot states, as raw
+    device pointers (ints)."""
+
+    def __init__(self, n_heads, head_dim, n_slots, type, *, conv_w, conv_b, dt_bias, a_log, d,
+                 conv_state, h_state):
+        if type not in TYPES:
+            raise ValueError(f"type must be one of {sorted(TYPES)}")
+        self.struct = SsmLayerStruct(n_heads, head_dim, n_slots, TYPES[type], conv_w, conv_b,
+                                     dt_bias, a_log, d, conv_state, h_state)
+        self.ref = ctypes.byref(self.struct)
+
+
+def slot_regions(regions):
+    """An array of bm_slot_region_t from (base, row_bytes, row_pitch, n_outer,
+    outer_pitch) tuples."""
+    a = (SlotRegion * len(regions))()
+    for i, (base, row_bytes, row_pitch, n_outer, outer_pitch) in enumerate(regions):
+        a[i] = SlotRegion(base, row_bytes, row_pitch, outer_pitch, n_outer, 0)
+    return a
 
 
 class Context:
@@ -266,6 +320,40 @@ class Context:
             c(off_ptr) if off_ptr else None, c(knobs_ptr), knob_stride, c(u_ptr),
             c(out_id_ptr), c(out_prob_ptr) if out_prob_ptr else None,
             c(stats_ptr) if stats_ptr else None, c(stream) if stream else None))
+
+    def ssm_prefill(self, layer, x_ptr, z_ptr, b_ptr, c_ptr, dt_ptr, ld, rows, off_ptr, n_seq,
+                    slots_ptr, fresh_ptr, y_ptr, ldy, stream=None):
+        """bm_ssm_prefill on raw device pointers (ints; None where optional)."""
+        check(lib().bm_ssm_prefill(self._c, layer.ref, x_ptr, z_ptr, b_ptr, c_ptr, dt_ptr, ld,
+                                   rows, off_ptr, n_seq, slots_ptr, fresh_ptr, y_ptr, ldy, stream))
+
+    def ssm_step(self, layer, x_ptr, z_ptr, b_ptr, c_ptr, dt_ptr, ld, rows, slots_ptr, y_ptr, ldy,
+                 stream=None):
+        """bm_ssm_step on raw device pointers (ints; None where optional)."""
+        check(lib().bm_ssm_step(self._c, layer.ref, x_ptr, z_ptr, b_ptr, c_ptr, dt_ptr, ld, rows,
+                                slots_ptr, y_ptr, ldy, stream))
+
+    def slots_reorder(self, regions, src_ptr, n_slots, stream=None):
+        """bm_slots_reorder; regions from slot_regions()."""
+        check(lib().bm_slots_reorder(self._c, regions, len(regions), src_ptr, n_slots, stream))
+
+    def fp8_quantize(self, x_ptr, type, rows, d, ldx, norm_w_ptr, q_ptr, scale_ptr, ld_scale,
+                     stream=None):
+        """bm_fp8_quantize on raw device pointers (ints; norm_w None: no norm)."""
+        check(lib().bm_fp8_quantize(self._c, x_ptr, TYPES[type], rows, d, ldx, norm_w_ptr, q_ptr,
+                                    scale_ptr, ld_scale, stream))
+
+    def fp8_product(self, a_ptr, a_scale_ptr, ld_scale, rows, d, w_ptr, w_scale_ptr, n, out_ptr,
+                    ldo, stream=None):
+        """bm_fp8_product on raw device pointers (ints)."""
+        check(lib().bm_fp8_product(self._c, a_ptr, a_scale_ptr, ld_scale, rows, d, w_ptr,
+                                   w_scale_ptr, n, out_ptr, ldo, stream))
+
+    def fp8_logits(self, hidden_ptr, B, d_model, norm_w_ptr, w_ptr, w_scale_ptr, V, logits_ptr, ld,
+                   stream=None):
+        """bm_fp8_logits on raw device pointers (ints)."""
+        check(lib().bm_fp8_logits(self._c, hidden_ptr, B, d_model, norm_w_ptr, w_ptr, w_scale_ptr,
+                                  V, logits_ptr, ld, stream))
 
     def sample_host(self, logits, hist, hist_off, knobs, uniform, want_prob=True,
                     want_stats=True):
@@ -381,6 +469,19 @@ class Decode:
             self._d, c(hidden_ptr), d_model, c(norm_f_ptr) if norm_f_ptr else None,
             c(lmh_norm_ptr), c(w8_ptr), w_scale, V, c(knobs_ptr), knob_stride, c(u_ptr),
             c(out_id_ptr) if out_id_ptr else None, c(stream) if stream else None))
+
+    def reorder(self, src_ptr, regions=(), stream=None):
+        """bm_decode_reorder; regions from slot_regions()."""
+        check(lib().bm_decode_reorder(self._d, src_ptr, regions if len(regions) else None,
+                                      len(regions), stream))
+
+    def compact(self, regions=(), map_ptr=None, stream=None):
+        """bm_decode_compact; regions from slot_regions()."""
+        check(lib().bm_decode_compact(self._d, regions if len(regions) else None, len(regions),
+                                      map_ptr, stream))
+
+    def set_rows(self, rows):
+        check(lib().bm_decode_set_rows(self._d, rows))
 
     def views(self):
         v = DecodeViews()

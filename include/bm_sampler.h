@@ -278,6 +278,150 @@ int bm_ternary_sample_batch(bm_ctx_t *ctx, const float *d_hidden, int B, int d_m
                             float *d_out_prob, bm_row_stats_t *d_stats,
                             void *stream);
 
+/* ---- the state space mixer of a layer: prompts and single tokens ----------- */
+
+/*
+ * The part of a BitMamba layer between its two projections: the short causal
+ * convolution, the selective state space scan and the gate, in the form the
+ * packed model file holds (in_proj of 2 d_inner + 3 n_heads rows: one B, C
+ * and dt per head; conv1d of width BM_SSM_CONV over the d_inner channels; D
+ * per channel).  With C = n_heads * head_dim channels, h = c / head_dim the
+ * head of channel c, and per sequence t = 0, 1, ...
+ *
+ *   u_t[c] = silu(conv_b[c] + sum_{k < 4} conv_w[c][k] * x_{t-3+k}[c])
+ *   d      = softplus(dt_t[h] + dt_bias[h]),  a = exp(-exp(a_log[h]) * d)
+ *   s_t[c] = a * s_{t-1}[c] + d * B_t[h] * u_t[c]
+ *   y_t[c] = (C_t[h] * s_t[c] + D[c] * u_t[c]) * silu(z_t[c])
+ *
+ * evaluated in fp32; y is rounded once to its type.  Serves the layer loop
+ * that the reference runs as block_step and block_step_batch
+ * (src/block.c:272-448), between bm_ternary_logits or bm_fp8_logits as
+ * in_proj and out_proj.
+ */
+#define BM_SSM_CONV 4
+
+enum { BM_F32 = 0, BM_BF16 = 1 }; /* element types of activations */
+
+/* One layer: sizes, weights (fp32, device) and the states of n_slots
+ * sequences (device, caller's memory):
+ *   conv_state [n_slots x 3 x C] of `type`: the last three inputs x, oldest
+ *              first, exactly as they came;
+ *   h_state    [n_slots x C] fp32: s.
+ * head_dim >= 1; C <= 2^20.  16-byte aligned conv_w; the other weights and
+ * h_state 4-byte aligned, conv_state aligned to its type. */
+typedef struct {
+    int32_t n_heads, head_dim, n_slots, type;
+    const float *conv_w;  /* [C x 4], oldest input first */
+    const float *conv_b;  /* [C] */
+    const float *dt_bias; /* [n_heads] */
+    const float *a_log;   /* [n_heads] */
+    const float *d;       /* [C] */
+    void *conv_state;
+    float *h_state;
+} bm_ssm_layer_t;
+
+/*
+ * Prompts: `rows` token rows of n_seq sequences, sequence i owning the rows
+ * [d_seq_off[i], d_seq_off[i + 1]) (device int64, n_seq + 1 offsets that do
+ * not decrease).  d_x, d_z ([rows x C]) and d_b, d_c, d_dt ([rows x n_heads])
+ * are of the layer's type and share the row pitch ld (elements): columns of
+ * one projection row, or arrays of their own.  d_z NULL: no gate.
+ *   d_slots  [n_seq] slot of each sequence (NULL: slot i).  The slots of a
+ *            call must differ; a sequence whose slot is outside
+ *            [0, n_slots) is skipped (its y rows are left as they were).
+ *   d_fresh  [n_seq] non-zero: the sequence starts from a zero state, else it
+ *            continues from its slot's (NULL: all start from zero).
+ *   d_y      [rows x C] of the layer's type, row pitch ldy; must not overlap
+ *            the inputs.  Rows of no sequence are left as they were.
+ * Writes each sequence's state after its last token to its slot (an empty
+ * sequence: unchanged, or zeros when fresh); other slots are not touched.
+ * Stream-ordered (stream NULL: the context's stream).  The call uses a
+ * workspace of the context that grows with rows * C and is kept until the
+ * context is destroyed: the first call of a size must not be under stream
+ * capture, later ones may be.  Calls on one context must not overlap in time
+ * (two replayed graphs among them).  Errors of the kernel (a bounded wait)
+ * show in bm_ctx_check.
+ */
+int bm_ssm_prefill(bm_ctx_t *ctx, const bm_ssm_layer_t *layer, const void *d_x, const void *d_z,
+                   const void *d_b, const void *d_c, const void *d_dt, int64_t ld, int rows,
+                   const int64_t *d_seq_off, int n_seq, const int32_t *d_slots,
+                   const int32_t *d_fresh, void *d_y, int64_t ldy, void *stream);
+
+/* One token for each of `rows` sequences: row r continues the state in slot
+ * d_slots[r] (NULL: slot r; outside [0, n_slots): the row is skipped, its y
+ * left as it was) and updates it.  Arguments as above; no workspace. */
+int bm_ssm_step(bm_ctx_t *ctx, const bm_ssm_layer_t *layer, const void *d_x, const void *d_z,
+                const void *d_b, const void *d_c, const void *d_dt, int64_t ld, int rows,
+                const int32_t *d_slots, void *d_y, int64_t ldy, void *stream);
+
+/* ---- slots of a state cache -------------------------------------------------- */
+
+/* An array of n_slots rows in each of n_outer planes (layers), on the device:
+ * slot s of plane o is row_bytes bytes at base + o * outer_pitch +
+ * s * row_pitch.  Everything a multiple of 4; regions of which everything
+ * (base too) is a multiple of 16 move fastest.  Rows must not overlap. */
+typedef struct {
+    void *base;
+    int64_t row_bytes, row_pitch, outer_pitch;
+    int32_t n_outer, reserved;
+} bm_slot_region_t;
+
+#define BM_SLOT_REGIONS 8   /* regions per call */
+#define BM_SLOT_MAX 8192    /* slots per call */
+
+/*
+ * Slot s of every region takes what slot d_src[s] held before the call
+ * (device int32 [n_slots]), all slots as if at once: copies, one slot forked
+ * to many, permutations (beam search) and compaction, in place.  A slot whose
+ * d_src is itself, negative or >= n_slots is left as it is (a freed slot
+ * needs no move: bm_ssm_prefill's fresh sequences start from zero).  The
+ * region list is host memory.  Stream-ordered, no workspace.
+ */
+int bm_slots_reorder(bm_ctx_t *ctx, const bm_slot_region_t *regions, int n_regions,
+                     const int32_t *d_src, int n_slots, void *stream);
+
+/* ---- 8-bit floating point products with block scales ------------------------- */
+
+/*
+ * Activations to e4m3 with one scale per row and 128 columns: optionally
+ * x * (1 / sqrtf(mean(x^2) + 1e-6f)) * norm_w first (d_norm_w NULL: none),
+ * then scale = max|x| / 448 over the block (1 where max|x| <= 2^-100) and
+ * q = e4m3(x / scale), round to nearest even.  A NaN in a block makes its
+ * scale NaN and the block NaN.  d_x: [rows x d] of `type` (BM_F32, BM_BF16),
+ * row pitch ldx elements; d_q: [rows x d] e4m3 bytes; d_scale: scale of
+ * (row r, block b) at d_scale[b * ld_scale + r], ld_scale >= rows and a
+ * multiple of 4.  d % 16 == 0, d <= 16384; d_x and the row pitch aligned to 4
+ * elements, norm_w, q and d_scale 16-byte aligned.  Stream-ordered.
+ */
+int bm_fp8_quantize(bm_ctx_t *ctx, const void *d_x, int type, int rows, int d, int64_t ldx,
+                    const float *d_norm_w, uint8_t *d_q, float *d_scale, int64_t ld_scale,
+                    void *stream);
+
+/*
+ * out[m, n] = sum_b a_scale[b][m] * w_scale[n / 128][b]
+ *                   * sum_{k in block b} a[m, k] * w[n, k]
+ * for e4m3 a ([rows x d]) and w ([n x d]), row-major, blocks of 128 columns,
+ * on the fp8 tensor cores: the sum of a block by the tensor core, the scaled
+ * blocks added in fp32.  a_scale as bm_fp8_quantize writes it (ld_scale a
+ * multiple of 4), w_scale [ceil(n / 128) x ceil(d / 128)] row-major; out fp32,
+ * row pitch ldo >= n.  d % 16 == 0, d <= 16384; a, w and a_scale 16-byte
+ * aligned.  Stream-ordered; errors of the kernel show in bm_ctx_check.
+ */
+int bm_fp8_product(bm_ctx_t *ctx, const uint8_t *d_a, const float *d_a_scale, int64_t ld_scale,
+                   int rows, int d, const uint8_t *d_w, const float *d_w_scale, int n,
+                   float *d_out, int64_t ldo, void *stream);
+
+/*
+ * RMSNorm, quantisation and the product in one call: the counterpart of
+ * bm_lmhead_logits for an fp8 export (in_proj, out_proj or lm_head).  hidden
+ * fp32 [B x d_model], 16-byte aligned, norm weight as above.  The quantised
+ * rows live in a workspace of the context (as bm_ssm_prefill's: kept, grown
+ * by the first call of a size, one call at a time).
+ */
+int bm_fp8_logits(bm_ctx_t *ctx, const float *d_hidden, int B, int d_model, const float *d_norm_w,
+                  const uint8_t *d_w, const float *d_w_scale, int V, float *d_logits, int64_t ld,
+                  void *stream);
+
 /* ---- device-resident decode loop state ------------------------------------- */
 
 /*
@@ -347,6 +491,30 @@ int bm_decode_ternary_step(bm_decode_t *d, const float *d_hidden, int d_model,
                            const int8_t *d_w8, float w_scale, int V,
                            const bm_knobs_t *d_knobs, int64_t knob_stride,
                            const float *d_uniform, int32_t *d_out_id, void *stream);
+
+/*
+ * Rows moved within the state: row r takes what row d_src[r] held (device
+ * int32 [B], as bm_slots_reorder: fork a row to several samples, reorder
+ * beams), together with the slots of `regions` (n_slots = B; the rows' model
+ * states), and the active-row count follows.  B <= BM_SLOT_MAX.
+ * Stream-ordered.
+ */
+int bm_decode_reorder(bm_decode_t *d, const int32_t *d_src, const bm_slot_region_t *regions,
+                      int n_regions, void *stream);
+
+/*
+ * Active rows first, in order, stopped rows behind them: the loop state of
+ * every row moves, the slots of `regions` only for active rows (those of
+ * stopped rows are free: their contents are unspecified).  d_map (optional,
+ * [B]) receives the row each row came from.  Followed by bm_decode_set_rows,
+ * later steps cost only the rows that are left.
+ */
+int bm_decode_compact(bm_decode_t *d, const bm_slot_region_t *regions, int n_regions,
+                      int32_t *d_map, void *stream);
+
+/* Later steps take the first `rows` rows (1 <= rows <= B) and leave the others
+ * as they are; bm_decode_create and bm_decode_reset set rows = B. */
+int bm_decode_set_rows(bm_decode_t *d, int rows);
 
 /* Device pointers of the state (valid until bm_decode_destroy). */
 int bm_decode_views(const bm_decode_t *d, bm_decode_views_t *views);

@@ -1,0 +1,232 @@
+"""8-bit float quantisation and products with block scales (bm_fp8_quantize,
+bm_fp8_product, bm_fp8_logits) against their definitions in 64 bits."""
+import ctypes
+
+import numpy as np
+import pytest
+
+DEFAULT = 1
+U = 2.0 ** -24
+
+
+def pitch(rows):
+    return -(-rows // 4) * 4
+
+
+def quantize(gpu_ctx, x, w=None, ldx=None, lds=None):
+    import torch
+    rows, d = x.shape
+    lds = lds or pitch(rows)
+    q = torch.full((rows, d), 99, dtype=torch.uint8, device="cuda")
+    scale = torch.full((-(-d // 128), lds), -5.0, device="cuda")
+    torch.cuda.synchronize()
+    gpu_ctx.fp8_quantize(x.data_ptr(), "f32" if x.dtype == torch.float32 else "bf16", rows, d, ldx or x.stride(0),
+                         None if w is None else w.data_ptr(), q.data_ptr(), scale.data_ptr(), lds, DEFAULT)
+    torch.cuda.synchronize()
+    return q.view(torch.float8_e4m3fn), scale
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("rows,d", [(1, 16), (1, 128), (3, 144), (9, 512), (5, 528), (2, 2048), (33, 2064), (4, 4096),
+                                    (2, 4112), (3, 16384)])
+def test_quantize(gpu_ctx, type_, norm, rows, d):
+    """q is x / scale rounded to e4m3: half a step of the value (2^-4
+    relative, 2^-10 below the normal range), plus the roundings of the norm
+    (the mean's sum d u, then 6 u) and of the two divisions (2 u); scale is
+    max / 448 to the same roundings."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(d)
+    t = torch.float32 if type_ == "f32" else torch.bfloat16
+    x = (torch.randn(rows, d + 8, generator=g, device="cuda") * torch.exp(torch.randn(rows, d + 8, generator=g, device="cuda"))).to(t)
+    x[0, : min(d, 128)] = 0.0
+    w = (1 + 0.1 * torch.randn(d, generator=g, device="cuda")) if norm else None
+    q, scale = quantize(gpu_ctx, x[:, :d], w, ldx=d + 8, lds=pitch(rows) + 4)
+    v = x[:, :d].double().cpu().numpy()
+    eps = 2 * U
+    if norm:
+        v = v / np.sqrt((v * v).mean(1, keepdims=True) + 1e-6) * w.double().cpu().numpy()
+        eps += (d + 6) * U
+    KB = scale.shape[0]
+    for k in range(KB):
+        part = v[:, 128 * k:128 * (k + 1)]
+        top = np.abs(part).max(1)
+        want = np.where(top > 2.0 ** -100, top / 448.0, 1.0)
+        s = scale[k, :rows].double().cpu().numpy()
+        assert (np.abs(s - want) <= eps * want * 1.01).all()
+        got = q[:, 128 * k:128 * (k + 1)].double().cpu().numpy()
+        e = part / s[:, None]
+        step = np.maximum(2.0 ** -4 * np.abs(e), 2.0 ** -10)
+        assert (np.abs(got - e) <= step + 2 * eps * np.abs(e)).all()
+    assert (scale[:, rows:] == -5.0).all()  # behind the last row nothing is written
+
+
+@pytest.mark.gpu
+def test_quantize_rounds_to_even_exactly(gpu_ctx):
+    """With a block's largest value 448 the scale is 1: every half-way value
+    and every e4m3 value."""
+    import torch
+    v = torch.arange(0, 127, dtype=torch.uint8).view(torch.float8_e4m3fn).float()
+    half = (v[:-1] + v[1:]) / 2
+    x = torch.cat([v, half, -v, -half])
+    x = torch.nn.functional.pad(x, (0, -x.numel() % 127)).view(-1, 127)
+    x = torch.cat([x, torch.full((x.shape[0], 1), 448.0)], 1)
+    q, scale = quantize(gpu_ctx, x.cuda())
+    assert (scale[:, :x.shape[0]] == 1.0).all()
+    assert torch.equal(q.cpu().float(), x.to(torch.float8_e4m3fn).float())
+
+
+@pytest.mark.gpu
+def test_quantize_special_values(gpu_ctx):
+    import torch
+    x = torch.randn(6, 256, device="cuda")
+    x[0, 3] = float("nan")
+    x[1, 200] = float("inf")
+    x[2] = 0.0
+    x[3] = 1e-35
+    x[4, :128] = 3e38
+    q, s = quantize(gpu_ctx, x)
+    f = q.float()
+    assert s[0, 0].isnan() and f[0, :128].isnan().all() and not f[0, 128:].isnan().any()
+    assert s[1, 1].isinf() and f[1, 200].isnan() and (f[1, 128:200] == 0).all()
+    assert (s[:, 2:4] == 1.0).all() and (f[2:4] == 0).all()
+    assert (f[4, :128] == 448).all()
+
+
+def product_ref(a, asc, w, wsc):
+    M, K = a.shape
+    N = w.shape[0]
+    out, mag = np.zeros((M, N)), np.zeros((M, N))
+    for k in range(-(-K // 128)):
+        c = slice(128 * k, min(K, 128 * k + 128))
+        s = asc[k, :M, None] * np.repeat(wsc[:, k], 128)[None, :N]
+        out += (a[:, c] @ w[:, c].T) * s
+        mag += (np.abs(a[:, c]) @ np.abs(w[:, c]).T) * s
+    return out, mag
+
+
+def make(seed, M, K, N):
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    f8 = torch.float8_e4m3fn
+    a = (torch.randn(M, K, generator=g, device="cuda") * 60).clamp(-448, 448).to(f8)
+    w = (torch.randn(N, K, generator=g, device="cuda") * 60).clamp(-448, 448).to(f8)
+    KB, NB = -(-K // 128), -(-N // 128)
+    asc = torch.full((KB, pitch(M)), float("nan"), device="cuda")
+    asc[:, :M] = torch.rand(KB, M, generator=g, device="cuda") + 0.1
+    wsc = torch.rand(NB, KB, generator=g, device="cuda") + 0.1
+    return a, asc, w, wsc
+
+
+def product(gpu_ctx, a, asc, w, wsc, pad=0, stream=DEFAULT):
+    import torch
+    M, K = a.shape
+    N = w.shape[0]
+    out = torch.full((M, N + pad), -3.0, device="cuda")
+    torch.cuda.synchronize()
+    gpu_ctx.fp8_product(a.data_ptr(), asc.data_ptr(), asc.shape[1], M, K, w.data_ptr(), wsc.data_ptr(), N,
+                        out.data_ptr(), N + pad, stream)
+    torch.cuda.synchronize()
+    return out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 15, 17, 33, 64, 65, 100, 129, 256, 300])
+@pytest.mark.parametrize("K,N", [(16, 1), (128, 128), (144, 129), (1040, 1000), (2048, 515)])
+def test_product(gpu_ctx, M, K, N):
+    """The sum of a block of at most 128 products by the tensor core is off by
+    at most 128 roundings or truncations of its sum of magnitudes (2 u each),
+    the scale product and the scaled blocks' additions by one u each."""
+    a, asc, w, wsc = make(M * 7 + K, M, K, N)
+    out = product(gpu_ctx, a, asc, w, wsc, pad=M % 3)
+    f = lambda t: t.double().cpu().numpy()  # noqa: E731
+    want, mag = product_ref(f(a.float()), f(asc), f(w.float()), f(wsc))
+    got = f(out)
+    assert (np.abs(got[:, :N] - want) <= (256 + 2 + -(-K // 128)) * U * mag).all()
+    assert (got[:, N:] == -3.0).all()
+    gpu_ctx.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N", [(40, 16384, 300), (700, 512, 20000), (1, 4096, 40001), (513, 128, 385)])
+def test_product_many_tiles(gpu_ctx, M, K, N):
+    import torch
+    a, asc, w, wsc = make(M, M, K, N)
+    out = product(gpu_ctx, a, asc, w, wsc)
+    ad = a.double() * asc[:, :M].T.double().repeat_interleave(128, 1)[:, :K]
+    wd = w.double() * wsc.double().repeat_interleave(128, 0)[:N].repeat_interleave(128, 1)[:, :K]
+    want, mag = ad @ wd.T, ad.abs() @ wd.abs().T
+    assert ((out - want).abs() <= (256 + 2 + -(-K // 128)) * U * mag).all()
+    gpu_ctx.check()
+    assert torch.equal(out, product(gpu_ctx, a, asc, w, wsc))  # the same sums every time
+
+
+@pytest.mark.gpu
+def test_product_nan_stays_in_its_row_and_column(gpu_ctx):
+    a, asc, w, wsc = make(3, 20, 256, 300)
+    clean = product(gpu_ctx, a, asc, w, wsc)
+    a.view(dtype=__import__("torch").uint8)[4, 17] = 0x7F
+    w.view(dtype=__import__("torch").uint8)[200, 130] = 0x7F
+    got = product(gpu_ctx, a, asc, w, wsc)
+    nan = got.isnan()
+    assert nan[4].all() and nan[:, 200].all()
+    nan[4] = True
+    nan[:, 200] = True
+    assert ((got == clean) | nan).all() and int(nan.sum()) == 300 + 19
+
+
+@pytest.mark.gpu
+def test_logits_is_quantize_then_product(gpu_ctx):
+    import torch
+    B, d, V = 37, 2048, 1003
+    x = torch.randn(B, d, device="cuda")
+    nw = 1 + 0.02 * torch.randn(d, device="cuda")
+    _, _, w, wsc = make(5, 1, d, V)
+    out = torch.full((B, V + 1), -3.0, device="cuda")
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    gpu_ctx.fp8_logits(x.data_ptr(), B, d, nw.data_ptr(), w.data_ptr(), wsc.data_ptr(), V, out.data_ptr(), V + 1,
+                       s.cuda_stream)
+    torch.cuda.synchronize()
+    q, sc = quantize(gpu_ctx, x, nw)
+    assert torch.equal(out[:, :V], product(gpu_ctx, q, sc, w, wsc))
+    assert (out[:, V] == -3.0).all()
+    # captured, replayed on another input
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        gpu_ctx.fp8_logits(x.data_ptr(), B, d, nw.data_ptr(), w.data_ptr(), wsc.data_ptr(), V, out.data_ptr(), V + 1,
+                           torch.cuda.current_stream().cuda_stream)
+    x.normal_()
+    torch.cuda.synchronize()
+    g.replay()
+    torch.cuda.synchronize()
+    q, sc = quantize(gpu_ctx, x, nw)
+    assert torch.equal(out[:, :V], product(gpu_ctx, q, sc, w, wsc))
+
+
+def test_refusals(sampler_lib):
+    L = sampler_lib.lib()
+    ctx = ctypes.create_string_buffer(1 << 16)
+    q = 1 << 20
+    quant = dict(ctx=ctx, x=q, type=0, rows=5, d=256, ldx=256, w=q, q=q, s=q, lds=8, stream=None)
+    prod = dict(ctx=ctx, a=q, asc=q, lds=8, rows=5, d=256, w=q, wsc=q, n=100, out=q, ldo=100, stream=None)
+    logits = dict(ctx=ctx, x=q, B=5, d=256, nw=q, w=q, wsc=q, V=100, out=q, ld=100, stream=None)
+
+    def refuses(f, base, **ch):
+        a = dict(base)
+        a.update(ch)
+        return f(*a.values()) in (-1, -4)
+
+    for ch in (dict(ctx=None), dict(x=None), dict(x=q + 8), dict(type=2), dict(rows=-1), dict(d=0), dict(d=8), dict(d=24),
+               dict(d=16400), dict(ldx=252), dict(ldx=258), dict(w=q + 4), dict(q=None), dict(q=q + 4), dict(s=None),
+               dict(s=q + 4), dict(lds=4), dict(lds=6)):
+        assert refuses(L.bm_fp8_quantize, quant, **ch), ch
+    for ch in (dict(ctx=None), dict(a=None), dict(a=q + 8), dict(asc=None), dict(asc=q + 4), dict(lds=4), dict(lds=6),
+               dict(rows=-1), dict(d=24), dict(d=16400), dict(w=None), dict(w=q + 8), dict(wsc=None), dict(wsc=q + 2),
+               dict(n=0), dict(out=None), dict(out=q + 2), dict(ldo=99)):
+        assert refuses(L.bm_fp8_product, prod, **ch), ch
+    for ch in (dict(ctx=None), dict(x=None), dict(x=q + 4), dict(B=-1), dict(d=24), dict(nw=q + 4), dict(V=0), dict(ld=99)):
+        assert refuses(L.bm_fp8_logits, logits, **ch), ch
+    for f, base, k in ((L.bm_fp8_quantize, quant, "rows"), (L.bm_fp8_product, prod, "rows"), (L.bm_fp8_logits, logits, "B")):
+        assert f(*{**base, k: 0}.values()) == 0
