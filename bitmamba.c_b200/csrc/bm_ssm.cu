@@ -71,40 +71,428 @@ __device__ __forceinline__ Head head_of(const Args &p, int64_t row, int h) {
     return r;
 }
 
-// One thread per channel of a sequence, token after token.
+// ---------------------------------------------------------------- prompts --
+//
+// The token axis of all sequences together is cut into tiles of LC rows; a
+// CTA takes one tile of NT * VEC channels, a thread VEC channels of it from
+// the tile's first row to its last, with the convolution's window, the state
+// and the outputs in registers.  The recurrence is linear, so a tile first
+// runs from a zero state:
+//   s_t = local_t + (a_first ... a_t) * s_in,    s_out = S + A * s_in
+// and the C s_t of its outputs is completed when s_in arrives: outputs wait
+// in registers, x and z are read once and y is written once.
+//
+// s_in comes from the tiles before (CTAs take tiles in order, by a ticket, so
+// whoever is waited for is running or done).  Each thread publishes its
+// channels' {epoch, A, S} as one 16-byte word, then looks back for the nearest
+// tile whose word is final ({epoch, FINAL, s_out}: it holds a sequence start,
+// or has completed its own look-back) and applies the A, S of the tiles in
+// between in order.  That is the chain s = A s + S that each of them applies
+// too, so the result does not depend on how far back the final word was.
+// Words carry the launch's epoch (a counter in the workspace that the last
+// CTA advances), so nothing is cleared between launches or graph replays.
+
+constexpr float FINAL = -1.0f;  // in the place of A (a product of decays, >= 0)
+constexpr unsigned long long WAIT_NS = 2000000000ull;  // bounded waits: 2 s
+
+struct Control {
+    unsigned ticket, done, epoch;
+};
+constexpr size_t CONTROL_BYTES = 256;
+
+__device__ __forceinline__ uint4 load_word(const uint4 *p) {
+    unsigned long long lo, hi;
+    asm volatile("{\n .reg .b128 w;\n ld.relaxed.gpu.global.b128 w, [%2];\n mov.b128 {%0, %1}, w;\n}"
+                 : "=l"(lo), "=l"(hi)
+                 : "l"(p)
+                 : "memory");
+    return make_uint4((unsigned)lo, (unsigned)(lo >> 32), (unsigned)hi, (unsigned)(hi >> 32));
+}
+__device__ __forceinline__ void store_word(uint4 *p, uint4 v) {
+    const unsigned long long lo = v.x | ((unsigned long long)v.y << 32),
+                             hi = v.z | ((unsigned long long)v.w << 32);
+    asm volatile("{\n .reg .b128 w;\n mov.b128 w, {%0, %1};\n st.relaxed.gpu.global.b128 [%2], w;\n}" ::"l"(lo),
+                 "l"(hi), "l"(p)
+                 : "memory");
+}
+__device__ __forceinline__ unsigned long long gtimer() {
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+
+// VEC consecutive elements as they lie in memory, and as fp32.
+template <typename T, int VEC>
+struct Raw;
 template <typename T>
-__global__ void __launch_bounds__(128) prefill_kernel(const Args p) {
-    const int ch = blockIdx.x * 128 + threadIdx.x, s = blockIdx.y;
-    if (ch >= p.l.C) return;
-    const int slot = p.slots ? p.slots[s] : s;
-    if (slot < 0 || slot >= p.l.n_slots) return;
-    const int64_t r0 = max((int64_t)0, p.off[s]), r1 = min((int64_t)p.rows, p.off[s + 1]);
-    const bool fresh = !p.fresh || p.fresh[s] != 0;
-    T *cs = static_cast<T *>(p.l.conv) + ((int64_t)slot * 3) * p.l.C + ch;
-    float *hs = p.l.h + (int64_t)slot * p.l.C + ch;
-    const T zero = from_f<T>(0.0f);
-    T x3 = fresh ? zero : cs[0], x2 = fresh ? zero : cs[p.l.C], x1 = fresh ? zero : cs[2 * p.l.C];
-    float h = fresh ? 0.0f : *hs;
-    const float4 w = reinterpret_cast<const float4 *>(p.l.conv_w)[ch];
-    const float bias = p.l.conv_b[ch], d = p.l.d[ch];
-    const int hd = ch / p.l.P;
-    for (int64_t r = r0; r < r1; ++r) {
-        const Head k = head_of<T>(p, r, hd);
-        const T x0 = static_cast<const T *>(p.x)[r * p.ld + ch];
-        const float u = silu(fmaf(
-            w.w, to_f(x0), fmaf(w.z, to_f(x1), fmaf(w.y, to_f(x2), fmaf(w.x, to_f(x3), bias)))));
-        h = fmaf(k.a, h, k.g * u);
-        float y = fmaf(k.c, h, d * u);
-        if (p.z) y *= silu(to_f(static_cast<const T *>(p.z)[r * p.ld + ch]));
-        static_cast<T *>(p.y)[r * p.ldy + ch] = from_f<T>(y);
-        x3 = x2;
-        x2 = x1;
-        x1 = x0;
+struct Raw<T, 1> {
+    T v;
+    __device__ __forceinline__ void load(const T *p) { v = *p; }
+    __device__ __forceinline__ void zero() { v = from_f<T>(0.0f); }
+    __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = to_f(v); }
+};
+template <>
+struct Raw<__nv_bfloat16, 2> {
+    uint32_t v;
+    __device__ __forceinline__ void load(const __nv_bfloat16 *p) {
+        v = *reinterpret_cast<const uint32_t *>(p);
     }
-    cs[0] = x3;
-    cs[p.l.C] = x2;
-    cs[2 * p.l.C] = x1;
-    *hs = h;
+    __device__ __forceinline__ void zero() { v = 0; }
+    __device__ __forceinline__ void get(float (&f)[2]) const {
+        f[0] = __uint_as_float(v << 16);
+        f[1] = __uint_as_float(v & 0xffff0000u);
+    }
+};
+__device__ __forceinline__ void put(float *p, const float (&f)[1]) { *p = f[0]; }
+__device__ __forceinline__ void put(float *p, const float (&f)[2]) {
+    *reinterpret_cast<float2 *>(p) = make_float2(f[0], f[1]);
+}
+__device__ __forceinline__ void put(__nv_bfloat16 *p, const float (&f)[1]) {
+    *p = __float2bfloat16_rn(f[0]);
+}
+__device__ __forceinline__ void put(__nv_bfloat16 *p, const float (&f)[2]) {
+    *reinterpret_cast<__nv_bfloat162 *>(p) = __floats2bfloat162_rn(f[0], f[1]);
+}
+
+// What the tile's rows are, found by one warp (lane = row, LC <= 32).
+struct Rows {
+    unsigned valid, start, end;  // row of a sequence with a slot; its first, its last
+    int place0;                  // the first row's place in its sequence
+    int slot[32];
+    int fresh[32];
+};
+
+template <int LC>
+__device__ __forceinline__ void find_rows(const Args &p, int64_t r0, int lane, Rows *out) {
+    const unsigned all = 0xffffffffu;
+    // how many offsets are <= r0: 32 probes a step
+    int lo = 0, n = p.n_seq + 1;
+    while (n > 32) {
+        const int stride = (n + 31) / 32, at = lane * stride;
+        const unsigned m = __ballot_sync(all, at < n && p.off[lo + at] <= r0);
+        if (m == 0) {
+            n = 0;
+            break;
+        }
+        const int k = __popc(m) - 1;
+        lo += k * stride;
+        n = min(stride, n - k * stride);
+    }
+    int base = lo + __popc(__ballot_sync(all, lane < n && p.off[lo + lane] <= r0));
+    // and <= this lane's row: the offsets from there on, 32 at a time
+    const int64_t r = r0 + lane, last = r0 + LC - 1;
+    int count = base;
+    for (;;) {
+        const int64_t v = base + lane <= p.n_seq ? p.off[base + lane] : INT64_MAX;
+        const unsigned m = __ballot_sync(all, v <= last);
+        for (int j = 0; j < __popc(m); ++j)
+            count += __shfl_sync(all, v, j) <= r;
+        if (m != all) break;
+        base += 32;
+    }
+    const int sid = count - 1;
+    bool valid = lane < LC && r < p.rows && sid >= 0 && sid < p.n_seq;
+    int slot = -1, fresh = 1;
+    int64_t o0 = 0, o1 = 0;
+    if (valid) {
+        slot = p.slots ? p.slots[sid] : sid;
+        fresh = p.fresh ? p.fresh[sid] != 0 : 1;
+        o0 = max((int64_t)0, p.off[sid]);
+        o1 = min(p.off[sid + 1], (int64_t)p.rows);
+        valid = slot >= 0 && slot < p.l.n_slots;
+    }
+    const unsigned mv = __ballot_sync(all, valid), ms = __ballot_sync(all, valid && r == o0),
+                   me = __ballot_sync(all, valid && r == o1 - 1);
+    out->slot[lane] = slot;
+    out->fresh[lane] = fresh;
+    if (lane == 0) {
+        out->valid = mv;
+        out->start = ms;
+        out->end = me;
+        out->place0 = (int)min((int64_t)3, r0 - o0);
+    }
+}
+
+template <typename T, int VEC, int LC, int NT>
+__global__ void __launch_bounds__(NT)
+    prefill_kernel(const Args p, Control *ctl, uint4 *words, int n_cb, int *err) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ unsigned s_ticket, s_epoch;
+    __shared__ Rows rows;
+    float4 *tab = reinterpret_cast<float4 *>(smem);  // [LC][heads of the CTA]: a, g, c
+    const int C = p.l.C, tid = threadIdx.x, lane = tid & 31;
+    if (tid == 0) {
+        s_epoch = *reinterpret_cast<volatile unsigned *>(&ctl->epoch) + 1;
+        s_ticket = atomicAdd(&ctl->ticket, 1u);
+    }
+    __syncthreads();
+    const unsigned epoch = s_epoch;
+    const int tile = (int)(s_ticket / (unsigned)n_cb), cb = (int)(s_ticket % (unsigned)n_cb);
+    const int64_t r0 = (int64_t)tile * LC;
+    const int c0 = cb * NT * VEC, ch = c0 + tid * VEC;
+    const bool on = ch < C;
+    const T *px = static_cast<const T *>(p.x) + ch, *pz = static_cast<const T *>(p.z) + ch;
+
+    // the tile's inputs, and the three rows above it, all in flight at once
+    Raw<T, VEC> x[LC], above[3];
+#pragma unroll
+    for (int t = 0; t < LC; ++t) {
+        x[t].zero();
+        if (on && r0 + t < p.rows) x[t].load(px + (r0 + t) * p.ld);
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        above[k].zero();
+        if (on && r0 > k && r0 - 1 - k < p.rows) above[k].load(px + (r0 - 1 - k) * p.ld);
+    }
+    if (tid < 32) find_rows<LC>(p, r0, lane, &rows);
+    // the scalars of the tile's rows and the CTA's heads
+    const int h0 = c0 / p.l.P, nh = (min(c0 + NT * VEC, C) - 1) / p.l.P - h0 + 1;
+    for (int i = tid; i < LC * nh; i += NT) {
+        const int t = i / nh, h = i - t * nh;
+        Head k{0.0f, 0.0f, 0.0f};
+        if (r0 + t < p.rows) k = head_of<T>(p, r0 + t, h0 + h);
+        tab[i] = make_float4(k.a, k.g, k.c, 0.0f);
+    }
+    float4 w[VEC];
+    float bias[VEC], dd[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+        w[v] = on ? reinterpret_cast<const float4 *>(p.l.conv_w)[ch + v] : make_float4(0, 0, 0, 0);
+        bias[v] = on ? p.l.conv_b[ch + v] : 0.0f;
+        dd[v] = on ? p.l.d[ch + v] : 0.0f;
+    }
+    __syncthreads();
+    const unsigned valid = rows.valid, start = rows.start, end = rows.end;
+    const float4 *tb = tab + ((on ? ch : c0) / p.l.P - h0);
+
+    // x1, x2, x3: the inputs 1, 2, 3 tokens back; from the slot before the
+    // sequence's first
+    float x1[VEC], x2[VEC], x3[VEC], h[VEC];
+    auto conv_at = [&](int slot, int j) {
+        return static_cast<T *>(p.l.conv) + ((int64_t)slot * 3 + j) * C + ch;
+    };
+    auto back = [&](int k, int place, int t, float (&f)[VEC]) {
+        // the input k tokens before a token at `place` < k of its sequence
+        Raw<T, VEC> r;
+        r.zero();
+        if (on && !rows.fresh[t]) r.load(conv_at(rows.slot[t], 3 + place - k));
+        r.get(f);
+    };
+    auto keep = [&](int slot, const float (&a)[VEC], const float (&b)[VEC], const float (&c)[VEC],
+                    const float (&s)[VEC]) {
+        if (!on) return;
+        put(conv_at(slot, 0), a);
+        put(conv_at(slot, 1), b);
+        put(conv_at(slot, 2), c);
+        put(p.l.h + (int64_t)slot * C + ch, s);
+    };
+    above[0].get(x1);
+    above[1].get(x2);
+    above[2].get(x3);
+    if ((valid & 1u) && !(start & 1u)) {
+        if (rows.place0 < 3) back(3, rows.place0, 0, x3);
+        if (rows.place0 < 2) back(2, rows.place0, 0, x2);
+    }
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) h[v] = 0.0f;
+
+    float y[LC][VEC], A = 1.0f;
+    // the end of the sequence that came in from the tile before
+    float Ae = 0.0f, he[VEC], e1[VEC], e2[VEC], e3[VEC];
+    int end_slot = -1;
+#pragma unroll
+    for (int t = 0; t < LC; ++t) {
+        if (start >> t & 1u) {
+            back(1, 0, t, x1);
+            back(2, 0, t, x2);
+            back(3, 0, t, x3);
+            A = 0.0f;
+#pragma unroll
+            for (int v = 0; v < VEC; ++v)
+                h[v] = on && !rows.fresh[t] ? p.l.h[(int64_t)rows.slot[t] * C + ch + v] : 0.0f;
+        }
+        const float4 k = tb[t * nh];
+        float xt[VEC];
+        x[t].get(xt);
+        A *= k.x;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            const float u = silu(fmaf(w[v].w, xt[v], fmaf(w[v].z, x1[v], fmaf(w[v].y, x2[v], fmaf(w[v].x, x3[v], bias[v])))));
+            h[v] = fmaf(k.x, h[v], k.y * u);
+            y[t][v] = fmaf(k.z, h[v], dd[v] * u);
+            x3[v] = x2[v];
+            x2[v] = x1[v];
+            x1[v] = xt[v];
+        }
+        if (end >> t & 1u) {
+            if (start & ((2u << t) - 1u)) {
+                keep(rows.slot[t], x3, x2, x1, h);
+            } else {
+                // completed and written below, behind the look-back: the
+                // tiles before have read the slot by then
+                end_slot = rows.slot[t];
+                Ae = A;
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) {
+                    he[v] = h[v];
+                    e1[v] = x1[v];
+                    e2[v] = x2[v];
+                    e3[v] = x3[v];
+                }
+            }
+        }
+    }
+
+    // the gates, in flight during the look-back
+    Raw<T, VEC> z[LC];
+#pragma unroll
+    for (int t = 0; t < LC; ++t) {
+        z[t].zero();
+        if (p.z && on && (valid >> t & 1u)) z[t].load(pz + (r0 + t) * p.ld);
+    }
+
+    // Every tile but the last publishes, whatever its rows are, so that offsets
+    // that contradict each other make no tile wait for a word that never comes.
+    const bool need_in = tile > 0 && (valid & 1u) && !(start & 1u);
+    const bool need_out = (tile + 1) * (int64_t)LC < p.rows;
+    const int cw = (C + VEC - 1) / VEC;
+    uint4 *own = words + (int64_t)tile * cw + ch / VEC;
+    auto publish = [&](float a, const float (&s)[VEC]) {
+        if (on) store_word(own, make_uint4(epoch, __float_as_uint(a), __float_as_uint(s[0]), __float_as_uint(s[VEC - 1])));
+    };
+    // with a start in the tile its last state does not depend on what comes in
+    if (need_out) publish(start || !need_in ? FINAL : A, h);
+    if (need_in) {
+        float hin[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) hin[v] = 0.0f;
+        if (on) {
+            int j = 1;  // tiles back
+            uint4 wd;
+            bool gave_up = false;
+            unsigned long long t0 = 0;
+            for (;;) {
+                wd = load_word(own - (int64_t)j * cw);
+                if (wd.x != epoch) {
+                    if (t0 == 0) t0 = gtimer();
+                    if (gtimer() - t0 > WAIT_NS) {
+                        gave_up = true;
+                        break;
+                    }
+                    continue;
+                }
+                if (__uint_as_float(wd.y) == FINAL || j == tile) break;  // (tile 0's is final)
+                ++j;
+            }
+            if (gave_up) {
+                atomicOr(err, 8);
+            } else {
+                hin[0] = __uint_as_float(wd.z);
+                if (VEC > 1) hin[VEC - 1] = __uint_as_float(wd.w);
+                for (--j; j > 0; --j) {
+                    wd = load_word(own - (int64_t)j * cw);
+                    // a final word that came meanwhile is the same chain's value
+                    const float a = __uint_as_float(wd.y);
+                    const bool fin = a == FINAL;
+                    hin[0] = fin ? __uint_as_float(wd.z) : fmaf(a, hin[0], __uint_as_float(wd.z));
+                    if (VEC > 1)
+                        hin[VEC - 1] = fin ? __uint_as_float(wd.w) : fmaf(a, hin[VEC - 1], __uint_as_float(wd.w));
+                }
+            }
+        }
+        if (need_out && !start) {
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) h[v] = fmaf(A, hin[v], h[v]);
+            publish(FINAL, h);
+        }
+        if (end_slot >= 0) {
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) he[v] = fmaf(Ae, hin[v], he[v]);
+            keep(end_slot, e3, e2, e1, he);
+        }
+        const int first = start ? __ffs(start) - 1 : LC;
+#pragma unroll
+        for (int t = 0; t < LC; ++t) {
+            if (t < first) {
+                const float4 k = tb[t * nh];
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) {
+                    hin[v] *= k.x;
+                    y[t][v] = fmaf(k.z, hin[v], y[t][v]);
+                }
+            }
+        }
+    }
+    if (on) {
+        T *py = static_cast<T *>(p.y) + ch;
+#pragma unroll
+        for (int t = 0; t < LC; ++t) {
+            if (!(valid >> t & 1u)) continue;
+            float o[VEC], zt[VEC];
+            z[t].get(zt);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) o[v] = p.z ? y[t][v] * silu(zt[v]) : y[t][v];
+            put(py + (r0 + t) * p.ldy, o);
+        }
+    }
+    // sequences without tokens that start afresh: a zero state
+    if (tile == 0) {
+        __shared__ int empty[NT], n_empty;
+        for (int s0 = 0; s0 < p.n_seq; s0 += NT) {
+            const int s = s0 + tid;
+            int slot = -1;
+            if (s < p.n_seq && !(p.fresh && p.fresh[s] == 0) &&
+                max((int64_t)0, p.off[s]) >= min((int64_t)p.rows, p.off[s + 1])) {
+                slot = p.slots ? p.slots[s] : s;
+                if (slot >= p.l.n_slots) slot = -1;
+            }
+            if (!__syncthreads_or(slot >= 0)) continue;
+            if (tid == 0) n_empty = 0;
+            __syncthreads();
+            if (slot >= 0) empty[atomicAdd(&n_empty, 1)] = slot;
+            __syncthreads();
+            const float none[VEC] = {};
+            for (int i = 0; i < n_empty; ++i) keep(empty[i], none, none, none, none);
+            __syncthreads();
+        }
+    }
+    __syncthreads();
+    if (tid == 0) {
+        __threadfence();
+        if (atomicAdd(&ctl->done, 1u) == gridDim.x - 1) {
+            ctl->ticket = 0;
+            ctl->done = 0;
+            __threadfence();
+            ctl->epoch = epoch;
+        }
+    }
+}
+
+struct Launch {
+    Args a;
+    Control *ctl;
+    uint4 *words;
+    int *err;
+    cudaStream_t s;
+};
+
+template <typename T, int VEC, int LC, int NT>
+cudaError_t launch_prefill(const Launch &l) {
+    const int C = l.a.l.C, P = l.a.l.P;
+    const int n_cb = (C + NT * VEC - 1) / (NT * VEC);
+    const int64_t tiles = l.a.rows > 0 ? ((int64_t)l.a.rows + LC - 1) / LC : 1;
+    if (tiles * n_cb > INT32_MAX) return cudaErrorInvalidValue;
+    const int heads = min((NT * VEC + P - 2) / P + 1, l.a.l.H);
+    const size_t smem = (size_t)LC * heads * sizeof(float4);
+    auto *k = prefill_kernel<T, VEC, LC, NT>;
+    constexpr int most = LC * NT * VEC * (int)sizeof(float4);  // a head per channel
+    if (smem > 40000) {
+        const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+        if (e != cudaSuccess) return e;
+    }
+    k<<<(int)(tiles * n_cb), NT, smem, l.s>>>(l.a, l.ctl, l.words, n_cb, l.err);
+    return cudaGetLastError();
 }
 
 template <typename T>
@@ -201,21 +589,42 @@ int bm_ssm_prefill(bm_ctx_t *ctx, const bm_ssm_layer_t *layer, const void *d_x, 
     if (n_seq == 0) return BM_OK;
     if (!d_seq_off || misaligned(d_seq_off, 8))
         return bm_detail_fail(BM_ERR_INVALID_ARG, "seq_off NULL or not 8-byte aligned");
-    if (n_seq > 65535) return bm_detail_fail(BM_ERR_UNSUPPORTED, "n_seq > 65535");
     a.off = d_seq_off;
     a.n_seq = n_seq;
     a.fresh = d_fresh;
-    int sms, *err;
-    cudaStream_t s;
-    bmc::DeviceGuard guard(bm_detail_ctx(ctx, &sms, &err, &s));
+    const size_t e = layer->type == BM_F32 ? 4 : 2;
+    // two channels a thread: the words of a pair must be one head's, and every
+    // pair aligned
+    const bool pairs = layer->type == BM_BF16 && a.l.P % 2 == 0 && ld % 2 == 0 && ldy % 2 == 0 &&
+                       !misaligned(d_x, 2 * e) && !misaligned(d_z, 2 * e) &&
+                       !misaligned(d_y, 2 * e) && !misaligned(layer->conv_state, 2 * e) &&
+                       !misaligned(layer->h_state, 8);
+    int sms;
+    Launch l{};
+    bmc::DeviceGuard guard(bm_detail_ctx(ctx, &sms, &l.err, &l.s));
     BMC_CK(guard.error);
-    if (stream) s = static_cast<cudaStream_t>(stream);
-    const dim3 grid((unsigned)((a.l.C + 127) / 128), (unsigned)n_seq);
+    if (stream) l.s = static_cast<cudaStream_t>(stream);
+    l.a = a;
+    constexpr int LONG = 32, SHORT = 8, NT = 128;
+    const int vec = pairs ? 2 : 1;
+    const int64_t ctas = ((int64_t)rows + LONG - 1) / LONG * ((a.l.C + NT * vec - 1) / (NT * vec));
+    const bool few = ctas < 2 * sms;
+    const int64_t tiles = ((int64_t)rows + (few ? SHORT : LONG) - 1) / (few ? SHORT : LONG);
+    void *work;
+    const int r = bm_detail_work(ctx, BM_WORK_SCAN,
+                                 CONTROL_BYTES + (size_t)tiles * ((a.l.C + vec - 1) / vec) * sizeof(uint4), &work);
+    if (r != BM_OK) return r;
+    l.ctl = static_cast<Control *>(work);
+    l.words = reinterpret_cast<uint4 *>(static_cast<unsigned char *>(work) + CONTROL_BYTES);
+    using bf16 = __nv_bfloat16;
+    cudaError_t ce;
     if (layer->type == BM_F32)
-        prefill_kernel<float><<<grid, 128, 0, s>>>(a);
+        ce = few ? launch_prefill<float, 1, SHORT, NT>(l) : launch_prefill<float, 1, LONG, NT>(l);
+    else if (pairs)
+        ce = few ? launch_prefill<bf16, 2, SHORT, NT>(l) : launch_prefill<bf16, 2, LONG, NT>(l);
     else
-        prefill_kernel<__nv_bfloat16><<<grid, 128, 0, s>>>(a);
-    BMC_CK(cudaGetLastError());
+        ce = few ? launch_prefill<bf16, 1, SHORT, NT>(l) : launch_prefill<bf16, 1, LONG, NT>(l);
+    BMC_CK(ce);
     return BM_OK;
 }
 
