@@ -50,7 +50,13 @@ __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) {
     return __float2bfloat16_rn(v);
 }
 
-__device__ __forceinline__ float silu(float v) { return __fdividef(v, 1.0f + __expf(-v)); }
+// v / (1 + e^-v): where e^-v overflows the quotient's limit, -0
+__device__ __forceinline__ float silu(float v) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * -1.44269504f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return v * r;
+}
 __device__ __forceinline__ float softplus(float v) {
     return fmaxf(v, 0.0f) + log1pf(expf(-fabsf(v)));
 }
@@ -84,15 +90,19 @@ __device__ __forceinline__ Head head_of(const Args &p, int64_t row, int h) {
 //
 // s_in comes from the tiles before (CTAs take tiles in order, by a ticket, so
 // whoever is waited for is running or done).  Each thread publishes its
-// channels' {epoch, A, S} as one 16-byte word, then looks back for the nearest
-// tile whose word is final ({epoch, FINAL, s_out}: it holds a sequence start,
-// or has completed its own look-back) and applies the A, S of the tiles in
-// between in order.  That is the chain s = A s + S that each of them applies
-// too, so the result does not depend on how far back the final word was.
-// Words carry the launch's epoch (a counter in the workspace that the last
-// CTA advances), so nothing is cleared between launches or graph replays.
+// channels' S and each head its A, then looks back for the nearest tile whose
+// s_out is final (it holds a sequence start, or has completed its own
+// look-back) and applies the A and S of the tiles in between in order.  That
+// is the chain s = A s + S that each of them applies too, so the result does
+// not depend on how far back the final word was.
+//
+// A value is published as 8 bytes {tag, value} written at once, tag = 2 *
+// epoch + (final or not): whoever reads the launch's tag has the value.  (16
+// bytes in one relaxed b128 access were seen torn here: halves of two
+// successive stores.)  The epoch is a counter in the workspace that the
+// launch's last CTA advances, so nothing is cleared between launches or graph
+// replays; a tag comes again after 2^31 launches.
 
-constexpr float FINAL = -1.0f;  // in the place of A (a product of decays, >= 0)
 constexpr unsigned long long WAIT_NS = 2000000000ull;  // bounded waits: 2 s
 
 struct Control {
@@ -100,19 +110,41 @@ struct Control {
 };
 constexpr size_t CONTROL_BYTES = 256;
 
-__device__ __forceinline__ uint4 load_word(const uint4 *p) {
-    unsigned long long lo, hi;
-    asm volatile("{\n .reg .b128 w;\n ld.relaxed.gpu.global.b128 w, [%2];\n mov.b128 {%0, %1}, w;\n}"
-                 : "=l"(lo), "=l"(hi)
-                 : "l"(p)
-                 : "memory");
-    return make_uint4((unsigned)lo, (unsigned)(lo >> 32), (unsigned)hi, (unsigned)(hi >> 32));
+// The words of VEC channels: {tag, S} each.
+template <int VEC>
+struct Words {
+    unsigned tag[VEC];
+    float s[VEC];
+};
+__device__ __forceinline__ void split(unsigned long long w, unsigned *tag, float *s) {
+    *tag = (unsigned)w;
+    *s = __uint_as_float((unsigned)(w >> 32));
 }
-__device__ __forceinline__ void store_word(uint4 *p, uint4 v) {
-    const unsigned long long lo = v.x | ((unsigned long long)v.y << 32),
-                             hi = v.z | ((unsigned long long)v.w << 32);
-    asm volatile("{\n .reg .b128 w;\n mov.b128 w, {%0, %1};\n st.relaxed.gpu.global.b128 [%2], w;\n}" ::"l"(lo),
-                 "l"(hi), "l"(p)
+__device__ __forceinline__ unsigned long long join(unsigned tag, float s) {
+    return tag | ((unsigned long long)__float_as_uint(s) << 32);
+}
+using Word64 = unsigned long long;
+__device__ __forceinline__ Words<1> load_words(const Word64 *p, Words<1>) {
+    Words<1> r;
+    Word64 w;
+    asm volatile("ld.relaxed.gpu.global.b64 %0, [%1];" : "=l"(w) : "l"(p) : "memory");
+    split(w, &r.tag[0], &r.s[0]);
+    return r;
+}
+__device__ __forceinline__ Words<2> load_words(const Word64 *p, Words<2>) {
+    Words<2> r;
+    Word64 w0, w1;
+    asm volatile("ld.relaxed.gpu.global.v2.b64 {%0, %1}, [%2];" : "=l"(w0), "=l"(w1) : "l"(p) : "memory");
+    split(w0, &r.tag[0], &r.s[0]);
+    split(w1, &r.tag[1], &r.s[1]);
+    return r;
+}
+__device__ __forceinline__ void store_words(Word64 *p, unsigned tag, const float (&s)[1]) {
+    asm volatile("st.relaxed.gpu.global.b64 [%0], %1;" ::"l"(p), "l"(join(tag, s[0])) : "memory");
+}
+__device__ __forceinline__ void store_words(Word64 *p, unsigned tag, const float (&s)[2]) {
+    asm volatile("st.relaxed.gpu.global.v2.b64 [%0], {%1, %2};" ::"l"(p), "l"(join(tag, s[0])),
+                 "l"(join(tag, s[1]))
                  : "memory");
 }
 __device__ __forceinline__ unsigned long long gtimer() {
@@ -121,11 +153,32 @@ __device__ __forceinline__ unsigned long long gtimer() {
     return t;
 }
 
+// Copies to shared memory, each thread for itself: 4 bytes asynchronously, a
+// 2-byte element through a register.
+__device__ __forceinline__ void stage(void *dst, const void *src, bool on, float) {
+    const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(d), "l"(src), "r"(on ? 4 : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void stage(void *dst, const void *src, bool on, uint32_t) {
+    stage(dst, src, on, 0.0f);
+}
+__device__ __forceinline__ void stage(void *dst, const void *src, bool on, __nv_bfloat16) {
+    *static_cast<__nv_bfloat16 *>(dst) =
+        on ? *static_cast<const __nv_bfloat16 *>(src) : __float2bfloat16_rn(0.0f);
+}
+template <int N>
+__device__ __forceinline__ void stage_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void stage_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
 // VEC consecutive elements as they lie in memory, and as fp32.
 template <typename T, int VEC>
 struct Raw;
 template <typename T>
 struct Raw<T, 1> {
+    using Word = T;
     T v;
     __device__ __forceinline__ void load(const T *p) { v = *p; }
     __device__ __forceinline__ void zero() { v = from_f<T>(0.0f); }
@@ -133,6 +186,7 @@ struct Raw<T, 1> {
 };
 template <>
 struct Raw<__nv_bfloat16, 2> {
+    using Word = uint32_t;
     uint32_t v;
     __device__ __forceinline__ void load(const __nv_bfloat16 *p) {
         v = *reinterpret_cast<const uint32_t *>(p);
@@ -152,6 +206,64 @@ __device__ __forceinline__ void put(__nv_bfloat16 *p, const float (&f)[1]) {
 }
 __device__ __forceinline__ void put(__nv_bfloat16 *p, const float (&f)[2]) {
     *reinterpret_cast<__nv_bfloat162 *>(p) = __floats2bfloat162_rn(f[0], f[1]);
+}
+
+// The state that comes into a tile, from the words of the tiles before: `own`
+// is this thread's word of this tile, `dec` its head's, with cw and H words a
+// tile.  BACK tiles are read at a time; false when a word did not come in
+// time.
+template <int VEC>
+__device__ __forceinline__ bool look_back(const Word64 *own, int cw, const Word64 *dec, int H,
+                                          int tile, unsigned tag, float (&hin)[VEC]) {
+    constexpr int BACK = 4;
+    Words<VEC> w[BACK];
+    Words<1> a[BACK];
+    auto load = [&](int i, int j) {
+        w[i] = load_words(own - (int64_t)j * cw, Words<VEC>());
+        a[i] = load_words(dec - (int64_t)j * H, Words<1>());
+    };
+    auto final_at = [&](int i) { return w[i].tag[0] == tag + 1 && w[i].tag[VEC - 1] == tag + 1; };
+    // (a word that became final meanwhile holds what the chain gives)
+    auto apply = [&](int i) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v)
+            hin[v] = w[i].tag[v] == tag + 1 ? w[i].s[v] : fmaf(a[i].s[0], hin[v], w[i].s[v]);
+    };
+    unsigned long long t0 = 0;
+    for (int j = 1;;) {
+#pragma unroll
+        for (int i = 0; i < BACK; ++i) load(i, min(j + i, tile));
+        // the nearest final tile before any that is not ready, and how many
+        // are ready
+        int at = -1, ready = BACK;
+#pragma unroll
+        for (int i = BACK - 1; i >= 0; --i) {
+            if (final_at(i)) {
+                at = i;
+            } else if ((w[i].tag[0] | 1u) != tag + 1 || (w[i].tag[VEC - 1] | 1u) != tag + 1 || a[i].tag[0] != tag) {
+                at = -1;
+                ready = i;
+            }
+        }
+        if (at >= 0) {
+#pragma unroll
+            for (int i = BACK - 1; i >= 0; --i)
+                if (i <= at) apply(i);
+            for (--j; j > 0; j -= BACK) {
+#pragma unroll
+                for (int i = 0; i < BACK; ++i) load(i, max(j - i, 1));
+#pragma unroll
+                for (int i = 0; i < BACK; ++i)
+                    if (j - i > 0) apply(i);
+            }
+            return true;
+        }
+        j += ready;  // (never beyond tile: tile 0 is final)
+        if (ready == 0) {
+            if (t0 == 0) t0 = gtimer();
+            if (gtimer() - t0 > WAIT_NS) return false;
+        }
+    }
 }
 
 // What the tile's rows are, found by one warp (lane = row, LC <= 32).
@@ -213,13 +325,20 @@ __device__ __forceinline__ void find_rows(const Args &p, int64_t r0, int lane, R
     }
 }
 
+// Shared memory of a CTA: x and z of the tile (each thread its own), then the
+// head scalars [LC][heads] (a, g, c).
 template <typename T, int VEC, int LC, int NT>
-__global__ void __launch_bounds__(NT)
-    prefill_kernel(const Args p, Control *ctl, uint4 *words, int n_cb, int *err) {
+constexpr size_t STAGED = (size_t)LC * NT * VEC * sizeof(T);  // x, or z
+
+template <typename T, int VEC, int LC, int NT, int PER_SM>
+__global__ void __launch_bounds__(NT, PER_SM)
+    prefill_kernel(const Args p, Control *ctl, Word64 *words, Word64 *decays, int n_cb, int *err) {
+    using Word = typename Raw<T, VEC>::Word;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ unsigned s_ticket, s_epoch;
     __shared__ Rows rows;
-    float4 *tab = reinterpret_cast<float4 *>(smem);  // [LC][heads of the CTA]: a, g, c
+    Word *sx = reinterpret_cast<Word *>(smem) + threadIdx.x, *sz = sx + LC * NT;
+    float4 *tab = reinterpret_cast<float4 *>(smem + 2 * STAGED<T, VEC, LC, NT>);
     const int C = p.l.C, tid = threadIdx.x, lane = tid & 31;
     if (tid == 0) {
         s_epoch = *reinterpret_cast<volatile unsigned *>(&ctl->epoch) + 1;
@@ -229,21 +348,31 @@ __global__ void __launch_bounds__(NT)
     const unsigned epoch = s_epoch;
     const int tile = (int)(s_ticket / (unsigned)n_cb), cb = (int)(s_ticket % (unsigned)n_cb);
     const int64_t r0 = (int64_t)tile * LC;
+    const int live_rows = (int)min((int64_t)LC, p.rows - r0);
     const int c0 = cb * NT * VEC, ch = c0 + tid * VEC;
     const bool on = ch < C;
-    const T *px = static_cast<const T *>(p.x) + ch, *pz = static_cast<const T *>(p.z) + ch;
 
-    // the tile's inputs, and the three rows above it, all in flight at once
-    Raw<T, VEC> x[LC], above[3];
+    // the tile's inputs and gates and the three rows above, all in flight at
+    // once; the gates are waited for last
+    const T *px = static_cast<const T *>(p.x) + (on ? ch + r0 * p.ld : 0);
+    {
+        const T *q = px;
 #pragma unroll
-    for (int t = 0; t < LC; ++t) {
-        x[t].zero();
-        if (on && r0 + t < p.rows) x[t].load(px + (r0 + t) * p.ld);
+        for (int t = 0; t < LC; ++t, q += p.ld) stage(sx + t * NT, t < live_rows ? q : px, on && t < live_rows, Word());
+        stage_commit();
+        if (p.z) {
+            const T *pz = static_cast<const T *>(p.z) + (on ? ch + r0 * p.ld : 0);
+            q = pz;
+#pragma unroll
+            for (int t = 0; t < LC; ++t, q += p.ld) stage(sz + t * NT, t < live_rows ? q : pz, on && t < live_rows, Word());
+        }
+        stage_commit();
     }
+    Raw<T, VEC> above[3];
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
         above[k].zero();
-        if (on && r0 > k && r0 - 1 - k < p.rows) above[k].load(px + (r0 - 1 - k) * p.ld);
+        if (on && r0 > k && r0 - 1 - k < p.rows) above[k].load(px - (k + 1) * p.ld);
     }
     if (tid < 32) find_rows<LC>(p, r0, lane, &rows);
     // the scalars of the tile's rows and the CTA's heads
@@ -251,7 +380,7 @@ __global__ void __launch_bounds__(NT)
     for (int i = tid; i < LC * nh; i += NT) {
         const int t = i / nh, h = i - t * nh;
         Head k{0.0f, 0.0f, 0.0f};
-        if (r0 + t < p.rows) k = head_of<T>(p, r0 + t, h0 + h);
+        if (t < live_rows) k = head_of<T>(p, r0 + t, h0 + h);
         tab[i] = make_float4(k.a, k.g, k.c, 0.0f);
     }
     float4 w[VEC];
@@ -297,6 +426,7 @@ __global__ void __launch_bounds__(NT)
 #pragma unroll
     for (int v = 0; v < VEC; ++v) h[v] = 0.0f;
 
+    stage_wait<1>();
     float y[LC][VEC], A = 1.0f;
     // the end of the sequence that came in from the tile before
     float Ae = 0.0f, he[VEC], e1[VEC], e2[VEC], e3[VEC];
@@ -314,7 +444,9 @@ __global__ void __launch_bounds__(NT)
         }
         const float4 k = tb[t * nh];
         float xt[VEC];
-        x[t].get(xt);
+        Raw<T, VEC> xr;
+        xr.v = sx[t * NT];
+        xr.get(xt);
         A *= k.x;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
@@ -344,67 +476,33 @@ __global__ void __launch_bounds__(NT)
         }
     }
 
-    // the gates, in flight during the look-back
-    Raw<T, VEC> z[LC];
-#pragma unroll
-    for (int t = 0; t < LC; ++t) {
-        z[t].zero();
-        if (p.z && on && (valid >> t & 1u)) z[t].load(pz + (r0 + t) * p.ld);
-    }
-
     // Every tile but the last publishes, whatever its rows are, so that offsets
     // that contradict each other make no tile wait for a word that never comes.
     const bool need_in = tile > 0 && (valid & 1u) && !(start & 1u);
     const bool need_out = (tile + 1) * (int64_t)LC < p.rows;
-    const int cw = (C + VEC - 1) / VEC;
-    uint4 *own = words + (int64_t)tile * cw + ch / VEC;
-    auto publish = [&](float a, const float (&s)[VEC]) {
-        if (on) store_word(own, make_uint4(epoch, __float_as_uint(a), __float_as_uint(s[0]), __float_as_uint(s[VEC - 1])));
-    };
+    Word64 *own = words + (int64_t)tile * C + ch;
+    const int head = (on ? ch : c0) / p.l.P;
+    Word64 *dec = decays + (int64_t)tile * p.l.H + head;
+    const unsigned tag = 2 * epoch;
     // with a start in the tile its last state does not depend on what comes in
-    if (need_out) publish(start || !need_in ? FINAL : A, h);
+    const bool is_final = start || !need_in;
+    if (need_out && on) {
+        store_words(own, is_final ? tag + 1 : tag, h);
+        // one thread a head (or more, with the same value)
+        if (!is_final && (tid == 0 || ch % p.l.P < VEC)) {
+            const float a[1] = {A};
+            store_words(dec, tag, a);
+        }
+    }
     if (need_in) {
         float hin[VEC];
 #pragma unroll
         for (int v = 0; v < VEC; ++v) hin[v] = 0.0f;
-        if (on) {
-            int j = 1;  // tiles back
-            uint4 wd;
-            bool gave_up = false;
-            unsigned long long t0 = 0;
-            for (;;) {
-                wd = load_word(own - (int64_t)j * cw);
-                if (wd.x != epoch) {
-                    if (t0 == 0) t0 = gtimer();
-                    if (gtimer() - t0 > WAIT_NS) {
-                        gave_up = true;
-                        break;
-                    }
-                    continue;
-                }
-                if (__uint_as_float(wd.y) == FINAL || j == tile) break;  // (tile 0's is final)
-                ++j;
-            }
-            if (gave_up) {
-                atomicOr(err, 8);
-            } else {
-                hin[0] = __uint_as_float(wd.z);
-                if (VEC > 1) hin[VEC - 1] = __uint_as_float(wd.w);
-                for (--j; j > 0; --j) {
-                    wd = load_word(own - (int64_t)j * cw);
-                    // a final word that came meanwhile is the same chain's value
-                    const float a = __uint_as_float(wd.y);
-                    const bool fin = a == FINAL;
-                    hin[0] = fin ? __uint_as_float(wd.z) : fmaf(a, hin[0], __uint_as_float(wd.z));
-                    if (VEC > 1)
-                        hin[VEC - 1] = fin ? __uint_as_float(wd.w) : fmaf(a, hin[VEC - 1], __uint_as_float(wd.w));
-                }
-            }
-        }
+        if (on && !look_back<VEC>(own, C, dec, p.l.H, tile, tag, hin)) atomicOr(err, 8);
         if (need_out && !start) {
 #pragma unroll
             for (int v = 0; v < VEC; ++v) h[v] = fmaf(A, hin[v], h[v]);
-            publish(FINAL, h);
+            if (on) store_words(own, tag + 1, h);
         }
         if (end_slot >= 0) {
 #pragma unroll
@@ -424,16 +522,19 @@ __global__ void __launch_bounds__(NT)
             }
         }
     }
+    stage_wait<0>();
     if (on) {
-        T *py = static_cast<T *>(p.y) + ch;
+        T *py = static_cast<T *>(p.y) + ch + r0 * p.ldy;
 #pragma unroll
-        for (int t = 0; t < LC; ++t) {
+        for (int t = 0; t < LC; ++t, py += p.ldy) {
             if (!(valid >> t & 1u)) continue;
             float o[VEC], zt[VEC];
-            z[t].get(zt);
+            Raw<T, VEC> zr;
+            zr.v = sz[t * NT];
+            zr.get(zt);
 #pragma unroll
             for (int v = 0; v < VEC; ++v) o[v] = p.z ? y[t][v] * silu(zt[v]) : y[t][v];
-            put(py + (r0 + t) * p.ldy, o);
+            put(py, o);
         }
     }
     // sequences without tokens that start afresh: a zero state
@@ -472,26 +573,26 @@ __global__ void __launch_bounds__(NT)
 struct Launch {
     Args a;
     Control *ctl;
-    uint4 *words;
+    Word64 *words, *decays;
     int *err;
     cudaStream_t s;
 };
 
-template <typename T, int VEC, int LC, int NT>
+template <typename T, int VEC, int LC, int NT, int PER_SM>
 cudaError_t launch_prefill(const Launch &l) {
     const int C = l.a.l.C, P = l.a.l.P;
     const int n_cb = (C + NT * VEC - 1) / (NT * VEC);
     const int64_t tiles = l.a.rows > 0 ? ((int64_t)l.a.rows + LC - 1) / LC : 1;
     if (tiles * n_cb > INT32_MAX) return cudaErrorInvalidValue;
     const int heads = min((NT * VEC + P - 2) / P + 1, l.a.l.H);
-    const size_t smem = (size_t)LC * heads * sizeof(float4);
-    auto *k = prefill_kernel<T, VEC, LC, NT>;
-    constexpr int most = LC * NT * VEC * (int)sizeof(float4);  // a head per channel
-    if (smem > 40000) {
-        const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-        if (e != cudaSuccess) return e;
-    }
-    k<<<(int)(tiles * n_cb), NT, smem, l.s>>>(l.a, l.ctl, l.words, n_cb, l.err);
+    constexpr size_t staged = 2 * STAGED<T, VEC, LC, NT>;
+    auto *k = prefill_kernel<T, VEC, LC, NT, PER_SM>;
+    // the most any call takes: a head per channel
+    constexpr int most = (int)(staged + LC * NT * VEC * sizeof(float4));
+    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    if (e != cudaSuccess) return e;
+    k<<<(int)(tiles * n_cb), NT, staged + (size_t)LC * heads * sizeof(float4), l.s>>>(
+        l.a, l.ctl, l.words, l.decays, n_cb, l.err);
     return cudaGetLastError();
 }
 
@@ -611,19 +712,22 @@ int bm_ssm_prefill(bm_ctx_t *ctx, const bm_ssm_layer_t *layer, const void *d_x, 
     const bool few = ctas < 2 * sms;
     const int64_t tiles = ((int64_t)rows + (few ? SHORT : LONG) - 1) / (few ? SHORT : LONG);
     void *work;
+    // a word per tile and channel, then one per tile and head
+    const size_t n_words = ((size_t)tiles * a.l.C + 1) / 2 * 2;
     const int r = bm_detail_work(ctx, BM_WORK_SCAN,
-                                 CONTROL_BYTES + (size_t)tiles * ((a.l.C + vec - 1) / vec) * sizeof(uint4), &work);
+                                 CONTROL_BYTES + (n_words + (size_t)tiles * a.l.H) * sizeof(Word64), &work);
     if (r != BM_OK) return r;
     l.ctl = static_cast<Control *>(work);
-    l.words = reinterpret_cast<uint4 *>(static_cast<unsigned char *>(work) + CONTROL_BYTES);
+    l.words = reinterpret_cast<Word64 *>(static_cast<unsigned char *>(work) + CONTROL_BYTES);
+    l.decays = l.words + n_words;
     using bf16 = __nv_bfloat16;
     cudaError_t ce;
     if (layer->type == BM_F32)
-        ce = few ? launch_prefill<float, 1, SHORT, NT>(l) : launch_prefill<float, 1, LONG, NT>(l);
+        ce = few ? launch_prefill<float, 1, SHORT, NT, 4>(l) : launch_prefill<float, 1, LONG, NT, 6>(l);
     else if (pairs)
-        ce = few ? launch_prefill<bf16, 2, SHORT, NT>(l) : launch_prefill<bf16, 2, LONG, NT>(l);
+        ce = few ? launch_prefill<bf16, 2, SHORT, NT, 4>(l) : launch_prefill<bf16, 2, LONG, NT, 4>(l);
     else
-        ce = few ? launch_prefill<bf16, 1, SHORT, NT>(l) : launch_prefill<bf16, 1, LONG, NT>(l);
+        ce = few ? launch_prefill<bf16, 1, SHORT, NT, 4>(l) : launch_prefill<bf16, 1, LONG, NT, 6>(l);
     BMC_CK(ce);
     return BM_OK;
 }
