@@ -79,18 +79,24 @@ __device__ __forceinline__ Head head_of(const Args &p, int64_t row, int h) {
 
 // ---------------------------------------------------------------- prompts --
 //
-// The token axis of all sequences together is cut into tiles of LC rows; a
-// CTA takes one tile of NT * VEC channels, a thread VEC channels of it from
-// the tile's first row to its last, with the convolution's window, the state
-// and the outputs in registers.  The recurrence is linear, so a tile first
-// runs from a zero state:
+// The token axis of all sequences together is cut into tiles of ST * LC rows; a
+// CTA takes one tile of CG * VEC channels, a thread VEC channels of one of the
+// tile's ST parts from its first row to its last, with the convolution's
+// window, the state and the outputs in registers.  The recurrence is linear,
+// so a part first runs from a zero state:
 //   s_t = local_t + (a_first ... a_t) * s_in,    s_out = S + A * s_in
 // and the C s_t of its outputs is completed when s_in arrives: outputs wait
-// in registers, x and z are read once and y is written once.
+// in registers, x and z are read once and y is written once.  The parts of a
+// tile are joined in shared memory, the tiles through published words.
+//
+// Narrow and long tiles (64 or 128 bytes of a row) keep few tiles of the same
+// channels in flight and the chain over them short: with 128 threads side by
+// side and tiles of 32 rows, 37 tiles of each channel were in flight and the
+// look-back cost more than the scan (65536 x 4096 bf16: 1.98 ms).
 //
 // s_in comes from the tiles before (CTAs take tiles in order, by a ticket, so
-// whoever is waited for is running or done).  Each thread publishes its
-// channels' S and each head its A, then looks back for the nearest tile whose
+// whoever is waited for is running or done).  Each tile publishes its
+// channels' S and its heads' A, then looks back for the nearest tile whose
 // s_out is final (it holds a sequence start, or has completed its own
 // look-back) and applies the A and S of the tiles in between in order.  That
 // is the chain s = A s + S that each of them applies too, so the result does
@@ -155,17 +161,13 @@ __device__ __forceinline__ unsigned long long gtimer() {
 
 // Copies to shared memory, each thread for itself: 4 bytes asynchronously, a
 // 2-byte element through a register.
-__device__ __forceinline__ void stage(void *dst, const void *src, bool on, float) {
+__device__ __forceinline__ void stage(void *dst, const void *src, float) {
     const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(d), "l"(src), "r"(on ? 4 : 0)
-                 : "memory");
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(d), "l"(src) : "memory");
 }
-__device__ __forceinline__ void stage(void *dst, const void *src, bool on, uint32_t) {
-    stage(dst, src, on, 0.0f);
-}
-__device__ __forceinline__ void stage(void *dst, const void *src, bool on, __nv_bfloat16) {
-    *static_cast<__nv_bfloat16 *>(dst) =
-        on ? *static_cast<const __nv_bfloat16 *>(src) : __float2bfloat16_rn(0.0f);
+__device__ __forceinline__ void stage(void *dst, const void *src, uint32_t) { stage(dst, src, 0.0f); }
+__device__ __forceinline__ void stage(void *dst, const void *src, __nv_bfloat16) {
+    *static_cast<__nv_bfloat16 *>(dst) = *static_cast<const __nv_bfloat16 *>(src);
 }
 template <int N>
 __device__ __forceinline__ void stage_wait() {
@@ -266,80 +268,56 @@ __device__ __forceinline__ bool look_back(const Word64 *own, int cw, const Word6
     }
 }
 
-// What the tile's rows are, found by one warp (lane = row, LC <= 32).
-struct Rows {
-    unsigned valid, start, end;  // row of a sequence with a slot; its first, its last
-    int place0;                  // the first row's place in its sequence
-    int slot[32];
-    int fresh[32];
-};
-
-template <int LC>
-__device__ __forceinline__ void find_rows(const Args &p, int64_t r0, int lane, Rows *out) {
+// How many offsets are <= r (a warp's lanes together, 32 probes a step).
+__device__ __forceinline__ int count_offsets(const int64_t *off, int n_off, int64_t r, int lane) {
     const unsigned all = 0xffffffffu;
-    // how many offsets are <= r0: 32 probes a step
-    int lo = 0, n = p.n_seq + 1;
+    int lo = 0, n = n_off;
     while (n > 32) {
         const int stride = (n + 31) / 32, at = lane * stride;
-        const unsigned m = __ballot_sync(all, at < n && p.off[lo + at] <= r0);
-        if (m == 0) {
-            n = 0;
-            break;
-        }
+        const unsigned m = __ballot_sync(all, at < n && off[lo + at] <= r);
+        if (m == 0) return lo;
         const int k = __popc(m) - 1;
         lo += k * stride;
         n = min(stride, n - k * stride);
     }
-    int base = lo + __popc(__ballot_sync(all, lane < n && p.off[lo + lane] <= r0));
-    // and <= this lane's row: the offsets from there on, 32 at a time
-    const int64_t r = r0 + lane, last = r0 + LC - 1;
-    int count = base;
-    for (;;) {
-        const int64_t v = base + lane <= p.n_seq ? p.off[base + lane] : INT64_MAX;
-        const unsigned m = __ballot_sync(all, v <= last);
-        for (int j = 0; j < __popc(m); ++j)
-            count += __shfl_sync(all, v, j) <= r;
-        if (m != all) break;
-        base += 32;
-    }
-    const int sid = count - 1;
-    bool valid = lane < LC && r < p.rows && sid >= 0 && sid < p.n_seq;
-    int slot = -1, fresh = 1;
-    int64_t o0 = 0, o1 = 0;
-    if (valid) {
-        slot = p.slots ? p.slots[sid] : sid;
-        fresh = p.fresh ? p.fresh[sid] != 0 : 1;
-        o0 = max((int64_t)0, p.off[sid]);
-        o1 = min(p.off[sid + 1], (int64_t)p.rows);
-        valid = slot >= 0 && slot < p.l.n_slots;
-    }
-    const unsigned mv = __ballot_sync(all, valid), ms = __ballot_sync(all, valid && r == o0),
-                   me = __ballot_sync(all, valid && r == o1 - 1);
-    out->slot[lane] = slot;
-    out->fresh[lane] = fresh;
-    if (lane == 0) {
-        out->valid = mv;
-        out->start = ms;
-        out->end = me;
-        out->place0 = (int)min((int64_t)3, r0 - o0);
-    }
+    return lo + __popc(__ballot_sync(all, lane < n && off[lo + lane] <= r));
 }
 
-// Shared memory of a CTA: x and z of the tile (each thread its own), then the
-// head scalars [LC][heads] (a, g, c).
-template <typename T, int VEC, int LC, int NT>
-constexpr size_t STAGED = (size_t)LC * NT * VEC * sizeof(T);  // x, or z
+// A tile's rows.  info: slot << 3 | fresh << 2 | place in the sequence (3 and
+// above: 3), or -1 for a row of no sequence; the masks have a bit per row.
+template <int ROWS>
+struct Rows {
+    int first, last;  // offsets <= the tile's first and last row
+    int info[ROWS];
+    unsigned valid[ROWS / 32], start[ROWS / 32], end[ROWS / 32];
+};
 
-template <typename T, int VEC, int LC, int NT, int PER_SM>
-__global__ void __launch_bounds__(NT, PER_SM)
-    prefill_kernel(const Args p, Control *ctl, Word64 *words, Word64 *decays, int n_cb, int *err) {
+// Shared memory of a CTA: x and z of the tile, then the head scalars
+// [rows][heads] (a, g, c).  With 16 words a row the odd parts are shifted by
+// 16 banks, so that the two parts of a warp do not meet.
+template <typename T, int VEC, int CG, int ST, int LC>
+struct Tile {
+    static constexpr int NT = CG * ST, ROWS = ST * LC;
+    static constexpr int PAD = CG == 16 ? 16 : 0;  // words per part
+    static constexpr int WORDS = ROWS * CG + ST * PAD;
+    static constexpr size_t STAGED = 2 * (size_t)WORDS * VEC * sizeof(T);
+};
+
+template <typename T, int VEC, int CG, int ST, int LC, int PER_SM>
+__global__ void __launch_bounds__(CG *ST, PER_SM)
+    prefill_kernel(const Args p, Control *ctl, Word64 *words, Word64 *decays, int n_cb, int wide,
+                   int *err) {
+    using L = Tile<T, VEC, CG, ST, LC>;
     using Word = typename Raw<T, VEC>::Word;
+    constexpr int NT = L::NT, ROWS = L::ROWS;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ unsigned s_ticket, s_epoch;
-    __shared__ Rows rows;
-    Word *sx = reinterpret_cast<Word *>(smem) + threadIdx.x, *sz = sx + LC * NT;
-    float4 *tab = reinterpret_cast<float4 *>(smem + 2 * STAGED<T, VEC, LC, NT>);
+    __shared__ Rows<ROWS> rows;
+    __shared__ float part_s[ST][CG * VEC], part_a[ST][CG], came[CG * VEC];
+    Word *const sx = reinterpret_cast<Word *>(smem), *const sz = sx + L::WORDS;
+    float4 *const tab = reinterpret_cast<float4 *>(smem + L::STAGED);
     const int C = p.l.C, tid = threadIdx.x, lane = tid & 31;
+    const int cg = tid % CG, part = tid / CG;
     if (tid == 0) {
         s_epoch = *reinterpret_cast<volatile unsigned *>(&ctl->epoch) + 1;
         s_ticket = atomicAdd(&ctl->ticket, 1u);
@@ -347,37 +325,46 @@ __global__ void __launch_bounds__(NT, PER_SM)
     __syncthreads();
     const unsigned epoch = s_epoch;
     const int tile = (int)(s_ticket / (unsigned)n_cb), cb = (int)(s_ticket % (unsigned)n_cb);
-    const int64_t r0 = (int64_t)tile * LC;
-    const int live_rows = (int)min((int64_t)LC, p.rows - r0);
-    const int c0 = cb * NT * VEC, ch = c0 + tid * VEC;
+    const int64_t r0 = (int64_t)tile * ROWS;
+    const int live_rows = (int)min((int64_t)ROWS, p.rows - r0);
+    const int c0 = cb * CG * VEC, ch = c0 + cg * VEC;
     const bool on = ch < C;
 
-    // the tile's inputs and gates and the three rows above, all in flight at
-    // once; the gates are waited for last
-    const T *px = static_cast<const T *>(p.x) + (on ? ch + r0 * p.ld : 0);
-    {
-        const T *q = px;
-#pragma unroll
-        for (int t = 0; t < LC; ++t, q += p.ld) stage(sx + t * NT, t < live_rows ? q : px, on && t < live_rows, Word());
-        stage_commit();
-        if (p.z) {
-            const T *pz = static_cast<const T *>(p.z) + (on ? ch + r0 * p.ld : 0);
-            q = pz;
-#pragma unroll
-            for (int t = 0; t < LC; ++t, q += p.ld) stage(sz + t * NT, t < live_rows ? q : pz, on && t < live_rows, Word());
+    // the tile's inputs and gates, all in flight at once; the gates are waited
+    // for last
+    for (int k = 0; k < (p.z ? 2 : 1); ++k) {
+        const T *src = static_cast<const T *>(k ? p.z : p.x) + r0 * p.ld;
+        Word *dst = k ? sz : sx;
+        if (wide) {  // 16 bytes at a time
+            constexpr int E = 16 / (int)sizeof(T), CH = CG * VEC / E;  // elements, chunks of a row
+            const int i = tid % CH;
+            const T *q = src + c0 + i * E;
+            for (int r = tid / CH; r < live_rows; r += NT / CH) {
+                const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst + r * CG + r / LC * L::PAD + i * (E / VEC));
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(q + r * p.ld) : "memory");
+            }
+        } else if (on) {
+            for (int r = part; r < live_rows; r += ST)
+                stage(dst + r * CG + r / LC * L::PAD + cg, src + ch + r * p.ld, Word());
         }
         stage_commit();
     }
+    if (!p.z) stage_commit();
     Raw<T, VEC> above[3];
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
         above[k].zero();
-        if (on && r0 > k && r0 - 1 - k < p.rows) above[k].load(px - (k + 1) * p.ld);
+        if (on && part == 0 && r0 > k && r0 - 1 - k < p.rows)
+            above[k].load(static_cast<const T *>(p.x) + ch + (r0 - 1 - k) * p.ld);
     }
-    if (tid < 32) find_rows<LC>(p, r0, lane, &rows);
-    // the scalars of the tile's rows and the CTA's heads
-    const int h0 = c0 / p.l.P, nh = (min(c0 + NT * VEC, C) - 1) / p.l.P - h0 + 1;
-    for (int i = tid; i < LC * nh; i += NT) {
+    // the rows' sequences
+    if (tid < 64) {
+        const int n = count_offsets(p.off, p.n_seq + 1, tid < 32 ? r0 : r0 + live_rows - 1, lane);
+        if (lane == 0) (tid < 32 ? rows.first : rows.last) = n;
+    }
+    // the scalars of the rows and the CTA's heads
+    const int h0 = c0 / p.l.P, nh = (min(c0 + CG * VEC, C) - 1) / p.l.P - h0 + 1;
+    for (int i = tid; i < ROWS * nh; i += NT) {
         const int t = i / nh, h = i - t * nh;
         Head k{0.0f, 0.0f, 0.0f};
         if (t < live_rows) k = head_of<T>(p, r0 + t, h0 + h);
@@ -392,8 +379,49 @@ __global__ void __launch_bounds__(NT, PER_SM)
         dd[v] = on ? p.l.d[ch + v] : 0.0f;
     }
     __syncthreads();
-    const unsigned valid = rows.valid, start = rows.start, end = rows.end;
-    const float4 *tb = tab + ((on ? ch : c0) / p.l.P - h0);
+    for (int i = tid; i < (ROWS + NT - 1) / NT * NT; i += NT) {
+        const int64_t r = r0 + i;
+        // the offsets <= r, of which the tile has only a few
+        int lo = rows.first, hi = max(rows.first, rows.last);
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (p.off[mid] <= r) lo = mid + 1;
+            else hi = mid;
+        }
+        const int sid = lo - 1;
+        int info = -1;
+        bool first = false, last = false;
+        if (i < live_rows && sid >= 0 && sid < p.n_seq) {
+            const int slot = p.slots ? p.slots[sid] : sid;
+            if (slot >= 0 && slot < p.l.n_slots) {
+                const int64_t o0 = max((int64_t)0, p.off[sid]), o1 = min(p.off[sid + 1], (int64_t)p.rows);
+                const int fresh = p.fresh ? p.fresh[sid] != 0 : 1;
+                info = slot << 3 | fresh << 2 | (int)max((int64_t)0, min((int64_t)3, r - o0));
+                first = r == o0;
+                last = r == o1 - 1;
+            }
+        }
+        const unsigned mv = __ballot_sync(0xffffffffu, info >= 0), ms = __ballot_sync(0xffffffffu, first),
+                       me = __ballot_sync(0xffffffffu, last);
+        if (i < ROWS) {
+            rows.info[i] = info;
+            if (lane == 0) {
+                rows.valid[i / 32] = mv;
+                rows.start[i / 32] = ms;
+                rows.end[i / 32] = me;
+            }
+        }
+    }
+    stage_wait<1>();
+    __syncthreads();
+    constexpr unsigned mask = LC == 32 ? 0xffffffffu : (1u << LC % 32) - 1u;
+    const int b0 = part * LC;
+    const unsigned valid = rows.valid[b0 / 32] >> b0 % 32 & mask, start = rows.start[b0 / 32] >> b0 % 32 & mask,
+                   end = rows.end[b0 / 32] >> b0 % 32 & mask;
+    const int *info = rows.info + b0;
+    const int head = (on ? ch : c0) / p.l.P;
+    const float4 *tb = tab + b0 * nh + head - h0;
+    const Word *xw = sx + b0 * CG + part * L::PAD + cg, *zw = sz + b0 * CG + part * L::PAD + cg;
 
     // x1, x2, x3: the inputs 1, 2, 3 tokens back; from the slot before the
     // sequence's first
@@ -405,7 +433,7 @@ __global__ void __launch_bounds__(NT, PER_SM)
         // the input k tokens before a token at `place` < k of its sequence
         Raw<T, VEC> r;
         r.zero();
-        if (on && !rows.fresh[t]) r.load(conv_at(rows.slot[t], 3 + place - k));
+        if (on && !(info[t] & 4)) r.load(conv_at(info[t] >> 3, 3 + place - k));
         r.get(f);
     };
     auto keep = [&](int slot, const float (&a)[VEC], const float (&b)[VEC], const float (&c)[VEC],
@@ -416,19 +444,23 @@ __global__ void __launch_bounds__(NT, PER_SM)
         put(conv_at(slot, 2), c);
         put(p.l.h + (int64_t)slot * C + ch, s);
     };
+    if (part > 0) {
+#pragma unroll
+        for (int k = 0; k < 3; ++k) above[k].v = xw[-(k + 1) * CG - L::PAD];
+    }
     above[0].get(x1);
     above[1].get(x2);
     above[2].get(x3);
     if ((valid & 1u) && !(start & 1u)) {
-        if (rows.place0 < 3) back(3, rows.place0, 0, x3);
-        if (rows.place0 < 2) back(2, rows.place0, 0, x2);
+        const int place = info[0] & 3;
+        if (place < 3) back(3, place, 0, x3);
+        if (place < 2) back(2, place, 0, x2);
     }
 #pragma unroll
     for (int v = 0; v < VEC; ++v) h[v] = 0.0f;
 
-    stage_wait<1>();
     float y[LC][VEC], A = 1.0f;
-    // the end of the sequence that came in from the tile before
+    // the end of the sequence that came in from the part before
     float Ae = 0.0f, he[VEC], e1[VEC], e2[VEC], e3[VEC];
     int end_slot = -1;
 #pragma unroll
@@ -437,15 +469,14 @@ __global__ void __launch_bounds__(NT, PER_SM)
             back(1, 0, t, x1);
             back(2, 0, t, x2);
             back(3, 0, t, x3);
-            A = 0.0f;
 #pragma unroll
             for (int v = 0; v < VEC; ++v)
-                h[v] = on && !rows.fresh[t] ? p.l.h[(int64_t)rows.slot[t] * C + ch + v] : 0.0f;
+                h[v] = on && !(info[t] & 4) ? p.l.h[(int64_t)(info[t] >> 3) * C + ch + v] : 0.0f;
         }
         const float4 k = tb[t * nh];
         float xt[VEC];
         Raw<T, VEC> xr;
-        xr.v = sx[t * NT];
+        xr.v = xw[t * CG];
         xr.get(xt);
         A *= k.x;
 #pragma unroll
@@ -459,11 +490,11 @@ __global__ void __launch_bounds__(NT, PER_SM)
         }
         if (end >> t & 1u) {
             if (start & ((2u << t) - 1u)) {
-                keep(rows.slot[t], x3, x2, x1, h);
+                keep(info[t] >> 3, x3, x2, x1, h);
             } else {
-                // completed and written below, behind the look-back: the
-                // tiles before have read the slot by then
-                end_slot = rows.slot[t];
+                // completed and written below, when the state that came in is
+                // known: whoever starts from the slot has read it by then
+                end_slot = info[t] >> 3;
                 Ae = A;
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) {
@@ -476,64 +507,94 @@ __global__ void __launch_bounds__(NT, PER_SM)
         }
     }
 
-    // Every tile but the last publishes, whatever its rows are, so that offsets
-    // that contradict each other make no tile wait for a word that never comes.
-    const bool need_in = tile > 0 && (valid & 1u) && !(start & 1u);
-    const bool need_out = (tile + 1) * (int64_t)LC < p.rows;
-    Word64 *own = words + (int64_t)tile * C + ch;
-    const int head = (on ? ch : c0) / p.l.P;
-    Word64 *dec = decays + (int64_t)tile * p.l.H + head;
-    const unsigned tag = 2 * epoch;
-    // with a start in the tile its last state does not depend on what comes in
-    const bool is_final = start || !need_in;
-    if (need_out && on) {
-        store_words(own, is_final ? tag + 1 : tag, h);
-        // one thread a head (or more, with the same value)
-        if (!is_final && (tid == 0 || ch % p.l.P < VEC)) {
-            const float a[1] = {A};
-            store_words(dec, tag, a);
+    // the parts' S and A; with a start in a part its S is the state itself
+    const float SET = -1.0f;  // in the place of A (a product of decays, >= 0)
+    if (start) A = SET;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) part_s[part][cg * VEC + v] = h[v];
+    part_a[part][cg] = A;
+    auto pass = [&](int i, float (&s)[VEC]) {  // the state through part i
+        const float a = part_a[i][cg];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            const float local = part_s[i][cg * VEC + v];
+            s[v] = a == SET ? local : fmaf(a, s[v], local);
         }
+    };
+    __syncthreads();
+    float hin[VEC];
+    if (part == 0) {
+        // Every tile but the last publishes, whatever its rows are, so that
+        // offsets that contradict each other make no tile wait for a word that
+        // never comes.
+        const bool need_in = tile > 0 && (valid & 1u) && !(start & 1u);
+        const bool need_out = (tile + 1) * (int64_t)ROWS < p.rows;
+        Word64 *own = words + (int64_t)tile * C + ch, *dec = decays + (int64_t)tile * p.l.H + head;
+        const unsigned tag = 2 * epoch;
+        float S[VEC], all = 1.0f;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) S[v] = hin[v] = 0.0f;
+        bool is_final = !need_in;
+        if (need_out) {
+#pragma unroll 4
+            for (int i = 0; i < ST; ++i) {
+                pass(i, S);
+                is_final |= part_a[i][cg] == SET;
+                all *= part_a[i][cg];
+            }
+            if (on) {
+                store_words(own, is_final ? tag + 1 : tag, S);
+                // one thread a head (or more, with the same value)
+                if (!is_final && (tid == 0 || ch % p.l.P < VEC)) {
+                    const float a[1] = {all};
+                    store_words(dec, tag, a);
+                }
+            }
+        }
+        if (need_in && on && !look_back<VEC>(own, C, dec, p.l.H, tile, tag, hin)) atomicOr(err, 8);
+        if (need_out && !is_final && on) {
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) S[v] = fmaf(all, hin[v], S[v]);
+            store_words(own, tag + 1, S);
+        }
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) came[cg * VEC + v] = hin[v];
     }
-    if (need_in) {
-        float hin[VEC];
+    stage_wait<0>();
+    __syncthreads();
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) hin[v] = 0.0f;
-        if (on && !look_back<VEC>(own, C, dec, p.l.H, tile, tag, hin)) atomicOr(err, 8);
-        if (need_out && !start) {
+    for (int v = 0; v < VEC; ++v) hin[v] = came[cg * VEC + v];
+    for (int i = 0; i < part; ++i) pass(i, hin);
+    if (end_slot >= 0) {
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) h[v] = fmaf(A, hin[v], h[v]);
-            if (on) store_words(own, tag + 1, h);
-        }
-        if (end_slot >= 0) {
+        for (int v = 0; v < VEC; ++v) he[v] = fmaf(Ae, hin[v], he[v]);
+        keep(end_slot, e3, e2, e1, he);
+    }
+    const int first = start ? __ffs(start) - 1 : LC;
+    if (on) {
+        T *py = static_cast<T *>(p.y) + ch + (r0 + b0) * p.ldy;
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) he[v] = fmaf(Ae, hin[v], he[v]);
-            keep(end_slot, e3, e2, e1, he);
-        }
-        const int first = start ? __ffs(start) - 1 : LC;
+        for (int t = 0; t < LC; ++t, py += p.ldy) {
+            float o[VEC];
 #pragma unroll
-        for (int t = 0; t < LC; ++t) {
+            for (int v = 0; v < VEC; ++v) o[v] = y[t][v];
             if (t < first) {
                 const float4 k = tb[t * nh];
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) {
                     hin[v] *= k.x;
-                    y[t][v] = fmaf(k.z, hin[v], y[t][v]);
+                    o[v] = fmaf(k.z, hin[v], o[v]);
                 }
             }
-        }
-    }
-    stage_wait<0>();
-    if (on) {
-        T *py = static_cast<T *>(p.y) + ch + r0 * p.ldy;
-#pragma unroll
-        for (int t = 0; t < LC; ++t, py += p.ldy) {
             if (!(valid >> t & 1u)) continue;
-            float o[VEC], zt[VEC];
-            Raw<T, VEC> zr;
-            zr.v = sz[t * NT];
-            zr.get(zt);
+            if (p.z) {
+                Raw<T, VEC> zr;
+                float zt[VEC];
+                zr.v = zw[t * CG];
+                zr.get(zt);
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) o[v] = p.z ? y[t][v] * silu(zt[v]) : y[t][v];
+                for (int v = 0; v < VEC; ++v) o[v] *= silu(zt[v]);
+            }
             put(py, o);
         }
     }
@@ -554,7 +615,7 @@ __global__ void __launch_bounds__(NT, PER_SM)
             if (slot >= 0) empty[atomicAdd(&n_empty, 1)] = slot;
             __syncthreads();
             const float none[VEC] = {};
-            for (int i = 0; i < n_empty; ++i) keep(empty[i], none, none, none, none);
+            for (int i = part; i < n_empty; i += ST) keep(empty[i], none, none, none, none);
             __syncthreads();
         }
     }
@@ -572,28 +633,40 @@ __global__ void __launch_bounds__(NT, PER_SM)
 
 struct Launch {
     Args a;
-    Control *ctl;
-    Word64 *words, *decays;
+    bm_ctx_t *ctx;
+    int sms;
     int *err;
     cudaStream_t s;
 };
 
-template <typename T, int VEC, int LC, int NT, int PER_SM>
-cudaError_t launch_prefill(const Launch &l) {
-    const int C = l.a.l.C, P = l.a.l.P;
-    const int n_cb = (C + NT * VEC - 1) / (NT * VEC);
-    const int64_t tiles = l.a.rows > 0 ? ((int64_t)l.a.rows + LC - 1) / LC : 1;
-    if (tiles * n_cb > INT32_MAX) return cudaErrorInvalidValue;
-    const int heads = min((NT * VEC + P - 2) / P + 1, l.a.l.H);
-    constexpr size_t staged = 2 * STAGED<T, VEC, LC, NT>;
-    auto *k = prefill_kernel<T, VEC, LC, NT, PER_SM>;
-    // the most any call takes: a head per channel
-    constexpr int most = (int)(staged + LC * NT * VEC * sizeof(float4));
-    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-    if (e != cudaSuccess) return e;
-    k<<<(int)(tiles * n_cb), NT, staged + (size_t)LC * heads * sizeof(float4), l.s>>>(
-        l.a, l.ctl, l.words, l.decays, n_cb, l.err);
-    return cudaGetLastError();
+template <typename T, int VEC, int CG, int ST, int LC, int PER_SM>
+int launch_prefill(const Launch &l) {
+    using L = Tile<T, VEC, CG, ST, LC>;
+    const Args &a = l.a;
+    const int C = a.l.C, P = a.l.P;
+    const int n_cb = (C + CG * VEC - 1) / (CG * VEC);
+    const int64_t tiles = a.rows > 0 ? ((int64_t)a.rows + L::ROWS - 1) / L::ROWS : 1;
+    if (tiles * n_cb > INT32_MAX)
+        return bm_detail_fail(BM_ERR_UNSUPPORTED, "rows * channels too large for one call");
+    // a word per tile and channel, then one per tile and head
+    const size_t n_words = ((size_t)tiles * C + 1) / 2 * 2;
+    void *work;
+    const int rc = bm_detail_work(l.ctx, BM_WORK_SCAN,
+                                  CONTROL_BYTES + (n_words + (size_t)tiles * a.l.H) * sizeof(Word64), &work);
+    if (rc != BM_OK) return rc;
+    Word64 *words = reinterpret_cast<Word64 *>(static_cast<unsigned char *>(work) + CONTROL_BYTES);
+    const int heads = min((CG * VEC + P - 2) / P + 1, a.l.H);
+    auto *k = prefill_kernel<T, VEC, CG, ST, LC, PER_SM>;
+    // the most any call takes: heads of VEC channels
+    constexpr int most = (int)(L::STAGED + (size_t)L::ROWS * (CG + VEC - 1) * sizeof(float4));
+    static_assert(most <= 220 * 1024, "shared memory");
+    BMC_CK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+    auto even = [&](const void *q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; };
+    const int wide = C % (CG * VEC) == 0 && even(a.x) && even(a.z) && a.ld * (int64_t)sizeof(T) % 16 == 0;
+    k<<<(int)(tiles * n_cb), L::NT, L::STAGED + (size_t)L::ROWS * heads * sizeof(float4), l.s>>>(
+        a, static_cast<Control *>(work), words, words + n_words, n_cb, wide, l.err);
+    BMC_CK(cudaGetLastError());
+    return BM_OK;
 }
 
 template <typename T>
@@ -700,36 +773,20 @@ int bm_ssm_prefill(bm_ctx_t *ctx, const bm_ssm_layer_t *layer, const void *d_x, 
                        !misaligned(d_x, 2 * e) && !misaligned(d_z, 2 * e) &&
                        !misaligned(d_y, 2 * e) && !misaligned(layer->conv_state, 2 * e) &&
                        !misaligned(layer->h_state, 8);
-    int sms;
     Launch l{};
-    bmc::DeviceGuard guard(bm_detail_ctx(ctx, &sms, &l.err, &l.s));
+    l.ctx = ctx;
+    bmc::DeviceGuard guard(bm_detail_ctx(ctx, &l.sms, &l.err, &l.s));
     BMC_CK(guard.error);
     if (stream) l.s = static_cast<cudaStream_t>(stream);
     l.a = a;
-    constexpr int LONG = 32, SHORT = 8, NT = 128;
-    const int vec = pairs ? 2 : 1;
-    const int64_t ctas = ((int64_t)rows + LONG - 1) / LONG * ((a.l.C + NT * vec - 1) / (NT * vec));
-    const bool few = ctas < 2 * sms;
-    const int64_t tiles = ((int64_t)rows + (few ? SHORT : LONG) - 1) / (few ? SHORT : LONG);
-    void *work;
-    // a word per tile and channel, then one per tile and head
-    const size_t n_words = ((size_t)tiles * a.l.C + 1) / 2 * 2;
-    const int r = bm_detail_work(ctx, BM_WORK_SCAN,
-                                 CONTROL_BYTES + (n_words + (size_t)tiles * a.l.H) * sizeof(Word64), &work);
-    if (r != BM_OK) return r;
-    l.ctl = static_cast<Control *>(work);
-    l.words = reinterpret_cast<Word64 *>(static_cast<unsigned char *>(work) + CONTROL_BYTES);
-    l.decays = l.words + n_words;
+    // long parts unless that leaves SMs without a CTA
     using bf16 = __nv_bfloat16;
-    cudaError_t ce;
+    const bool few = ((int64_t)rows + 255) / 256 * ((a.l.C + 31) / 32) < 2 * l.sms;
     if (layer->type == BM_F32)
-        ce = few ? launch_prefill<float, 1, SHORT, NT, 4>(l) : launch_prefill<float, 1, LONG, NT, 6>(l);
-    else if (pairs)
-        ce = few ? launch_prefill<bf16, 2, SHORT, NT, 4>(l) : launch_prefill<bf16, 2, LONG, NT, 4>(l);
-    else
-        ce = few ? launch_prefill<bf16, 1, SHORT, NT, 4>(l) : launch_prefill<bf16, 1, LONG, NT, 6>(l);
-    BMC_CK(ce);
-    return BM_OK;
+        return few ? launch_prefill<float, 1, 32, 4, 8, 4>(l) : launch_prefill<float, 1, 32, 8, 32, 3>(l);
+    if (pairs)
+        return few ? launch_prefill<bf16, 2, 16, 8, 8, 4>(l) : launch_prefill<bf16, 2, 16, 16, 32, 2>(l);
+    return few ? launch_prefill<bf16, 1, 32, 4, 8, 4>(l) : launch_prefill<bf16, 1, 32, 8, 32, 3>(l);
 }
 
 int bm_ssm_step(bm_ctx_t *ctx, const bm_ssm_layer_t *layer, const void *d_x, const void *d_z,
