@@ -50,12 +50,49 @@ __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) {
     return __float2bfloat16_rn(v);
 }
 
+// One channel or two: two take the packed fp32 instructions, which do the
+// arithmetic of a pair in one issue slot.
+template <int VEC>
+struct Vec;
+template <>
+struct Vec<1> {
+    using type = float;
+};
+template <>
+struct Vec<2> {
+    using type = float2;
+};
+__device__ __forceinline__ float vfma(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ float2 vfma(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float vmul(float a, float b) { return a * b; }
+__device__ __forceinline__ float2 vmul(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float vadd(float a, float b) { return a + b; }
+__device__ __forceinline__ float2 vadd(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ void vset(float &v, float a, float) { v = a; }
+__device__ __forceinline__ void vset(float2 &v, float a, float b) { v = make_float2(a, b); }
+__device__ __forceinline__ float lane0(float v) { return v; }
+__device__ __forceinline__ float lane0(float2 v) { return v.x; }
+__device__ __forceinline__ float lane1(float v) { return v; }
+__device__ __forceinline__ float lane1(float2 v) { return v.y; }
+__device__ __forceinline__ float ex2(float v) {
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(v));
+    return v;
+}
+__device__ __forceinline__ float rcp(float v) {
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(v));
+    return v;
+}
 // v / (1 + e^-v): where e^-v overflows the quotient's limit, -0
-__device__ __forceinline__ float silu(float v) {
-    float e, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * -1.44269504f));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-    return v * r;
+template <typename V>
+__device__ __forceinline__ V silu(V v) {
+    V k, one, e;
+    vset(k, -1.44269504f, -1.44269504f);
+    vset(one, 1.0f, 1.0f);
+    const V t = vmul(v, k);
+    vset(e, ex2(lane0(t)), ex2(lane1(t)));
+    e = vadd(e, one);
+    vset(e, rcp(lane0(e)), rcp(lane1(e)));
+    return vmul(v, e);
 }
 __device__ __forceinline__ float softplus(float v) {
     return fmaxf(v, 0.0f) + log1pf(expf(-fabsf(v)));
@@ -116,41 +153,42 @@ struct Control {
 };
 constexpr size_t CONTROL_BYTES = 256;
 
-// The words of VEC channels: {tag, S} each.
-template <int VEC>
-struct Words {
-    unsigned tag[VEC];
-    float s[VEC];
-};
-__device__ __forceinline__ void split(unsigned long long w, unsigned *tag, float *s) {
-    *tag = (unsigned)w;
-    *s = __uint_as_float((unsigned)(w >> 32));
-}
-__device__ __forceinline__ unsigned long long join(unsigned tag, float s) {
-    return tag | ((unsigned long long)__float_as_uint(s) << 32);
-}
+// The words of one or two channels: {tag, S} each.
 using Word64 = unsigned long long;
-__device__ __forceinline__ Words<1> load_words(const Word64 *p, Words<1>) {
-    Words<1> r;
+template <typename V>
+struct Words;
+template <>
+struct Words<float> {
+    unsigned tag, tag1;
+    float s;
+};
+template <>
+struct Words<float2> {
+    unsigned tag, tag1;
+    float2 s;
+};
+__device__ __forceinline__ Word64 join(unsigned tag, float s) {
+    return tag | ((Word64)__float_as_uint(s) << 32);
+}
+__device__ __forceinline__ void load_words(const Word64 *p, Words<float> &r) {
     Word64 w;
     asm volatile("ld.relaxed.gpu.global.b64 %0, [%1];" : "=l"(w) : "l"(p) : "memory");
-    split(w, &r.tag[0], &r.s[0]);
-    return r;
+    r.tag = r.tag1 = (unsigned)w;
+    r.s = __uint_as_float((unsigned)(w >> 32));
 }
-__device__ __forceinline__ Words<2> load_words(const Word64 *p, Words<2>) {
-    Words<2> r;
+__device__ __forceinline__ void load_words(const Word64 *p, Words<float2> &r) {
     Word64 w0, w1;
     asm volatile("ld.relaxed.gpu.global.v2.b64 {%0, %1}, [%2];" : "=l"(w0), "=l"(w1) : "l"(p) : "memory");
-    split(w0, &r.tag[0], &r.s[0]);
-    split(w1, &r.tag[1], &r.s[1]);
-    return r;
+    r.tag = (unsigned)w0;
+    r.tag1 = (unsigned)w1;
+    r.s = make_float2(__uint_as_float((unsigned)(w0 >> 32)), __uint_as_float((unsigned)(w1 >> 32)));
 }
-__device__ __forceinline__ void store_words(Word64 *p, unsigned tag, const float (&s)[1]) {
-    asm volatile("st.relaxed.gpu.global.b64 [%0], %1;" ::"l"(p), "l"(join(tag, s[0])) : "memory");
+__device__ __forceinline__ void store_words(Word64 *p, unsigned tag, float s) {
+    asm volatile("st.relaxed.gpu.global.b64 [%0], %1;" ::"l"(p), "l"(join(tag, s)) : "memory");
 }
-__device__ __forceinline__ void store_words(Word64 *p, unsigned tag, const float (&s)[2]) {
-    asm volatile("st.relaxed.gpu.global.v2.b64 [%0], {%1, %2};" ::"l"(p), "l"(join(tag, s[0])),
-                 "l"(join(tag, s[1]))
+__device__ __forceinline__ void store_words(Word64 *p, unsigned tag, float2 s) {
+    asm volatile("st.relaxed.gpu.global.v2.b64 [%0], {%1, %2};" ::"l"(p), "l"(join(tag, s.x)),
+                 "l"(join(tag, s.y))
                  : "memory");
 }
 __device__ __forceinline__ unsigned long long gtimer() {
@@ -164,6 +202,10 @@ __device__ __forceinline__ unsigned long long gtimer() {
 __device__ __forceinline__ void stage(void *dst, const void *src, float) {
     const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(d), "l"(src) : "memory");
+}
+__device__ __forceinline__ void stage(void *dst, const void *src, float2) {
+    const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(d), "l"(src) : "memory");
 }
 __device__ __forceinline__ void stage(void *dst, const void *src, uint32_t) { stage(dst, src, 0.0f); }
 __device__ __forceinline__ void stage(void *dst, const void *src, __nv_bfloat16) {
@@ -182,54 +224,52 @@ template <typename T>
 struct Raw<T, 1> {
     using Word = T;
     T v;
-    __device__ __forceinline__ void load(const T *p) { v = *p; }
     __device__ __forceinline__ void zero() { v = from_f<T>(0.0f); }
-    __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = to_f(v); }
+    __device__ __forceinline__ float get() const { return to_f(v); }
+};
+template <>
+struct Raw<float, 2> {
+    using Word = float2;
+    float2 v;
+    __device__ __forceinline__ void zero() { v = make_float2(0.0f, 0.0f); }
+    __device__ __forceinline__ float2 get() const { return v; }
 };
 template <>
 struct Raw<__nv_bfloat16, 2> {
     using Word = uint32_t;
     uint32_t v;
-    __device__ __forceinline__ void load(const __nv_bfloat16 *p) {
-        v = *reinterpret_cast<const uint32_t *>(p);
-    }
     __device__ __forceinline__ void zero() { v = 0; }
-    __device__ __forceinline__ void get(float (&f)[2]) const {
-        f[0] = __uint_as_float(v << 16);
-        f[1] = __uint_as_float(v & 0xffff0000u);
+    __device__ __forceinline__ float2 get() const {
+        return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
     }
 };
-__device__ __forceinline__ void put(float *p, const float (&f)[1]) { *p = f[0]; }
-__device__ __forceinline__ void put(float *p, const float (&f)[2]) {
-    *reinterpret_cast<float2 *>(p) = make_float2(f[0], f[1]);
-}
-__device__ __forceinline__ void put(__nv_bfloat16 *p, const float (&f)[1]) {
-    *p = __float2bfloat16_rn(f[0]);
-}
-__device__ __forceinline__ void put(__nv_bfloat16 *p, const float (&f)[2]) {
-    *reinterpret_cast<__nv_bfloat162 *>(p) = __floats2bfloat162_rn(f[0], f[1]);
+__device__ __forceinline__ void put(float *p, float f) { *p = f; }
+__device__ __forceinline__ void put(float *p, float2 f) { *reinterpret_cast<float2 *>(p) = f; }
+__device__ __forceinline__ void put(__nv_bfloat16 *p, float f) { *p = __float2bfloat16_rn(f); }
+__device__ __forceinline__ void put(__nv_bfloat16 *p, float2 f) {
+    *reinterpret_cast<__nv_bfloat162 *>(p) = __floats2bfloat162_rn(f.x, f.y);
 }
 
 // The state that comes into a tile, from the words of the tiles before: `own`
 // is this thread's word of this tile, `dec` its head's, with cw and H words a
 // tile.  BACK tiles are read at a time; false when a word did not come in
 // time.
-template <int VEC>
+template <typename V>
 __device__ __forceinline__ bool look_back(const Word64 *own, int cw, const Word64 *dec, int H,
-                                          int tile, unsigned tag, float (&hin)[VEC]) {
+                                          int tile, unsigned tag, V &hin) {
     constexpr int BACK = 4;
-    Words<VEC> w[BACK];
-    Words<1> a[BACK];
+    Words<V> w[BACK];
+    Words<float> a[BACK];
     auto load = [&](int i, int j) {
-        w[i] = load_words(own - (int64_t)j * cw, Words<VEC>());
-        a[i] = load_words(dec - (int64_t)j * H, Words<1>());
+        load_words(own - (int64_t)j * cw, w[i]);
+        load_words(dec - (int64_t)j * H, a[i]);
     };
-    auto final_at = [&](int i) { return w[i].tag[0] == tag + 1 && w[i].tag[VEC - 1] == tag + 1; };
     // (a word that became final meanwhile holds what the chain gives)
     auto apply = [&](int i) {
-#pragma unroll
-        for (int v = 0; v < VEC; ++v)
-            hin[v] = w[i].tag[v] == tag + 1 ? w[i].s[v] : fmaf(a[i].s[0], hin[v], w[i].s[v]);
+        V aa;
+        vset(aa, a[i].s, a[i].s);
+        const V r = vfma(aa, hin, w[i].s);
+        vset(hin, w[i].tag == tag + 1 ? lane0(w[i].s) : lane0(r), w[i].tag1 == tag + 1 ? lane1(w[i].s) : lane1(r));
     };
     unsigned long long t0 = 0;
     for (int j = 1;;) {
@@ -240,9 +280,9 @@ __device__ __forceinline__ bool look_back(const Word64 *own, int cw, const Word6
         int at = -1, ready = BACK;
 #pragma unroll
         for (int i = BACK - 1; i >= 0; --i) {
-            if (final_at(i)) {
+            if (w[i].tag == tag + 1 && w[i].tag1 == tag + 1) {
                 at = i;
-            } else if ((w[i].tag[0] | 1u) != tag + 1 || (w[i].tag[VEC - 1] | 1u) != tag + 1 || a[i].tag[0] != tag) {
+            } else if ((w[i].tag | 1u) != tag + 1 || (w[i].tag1 | 1u) != tag + 1 || a[i].tag != tag) {
                 at = -1;
                 ready = i;
             }
@@ -292,334 +332,398 @@ struct Rows {
     unsigned valid[ROWS / 32], start[ROWS / 32], end[ROWS / 32];
 };
 
-// Shared memory of a CTA: x and z of the tile, then the head scalars
-// [rows][heads] (a, g, c).  With 16 words a row the odd parts are shifted by
-// 16 banks, so that the two parts of a warp do not meet.
+// Shared memory of a CTA: x and z of the tile, then two buffers of the head
+// scalars [heads][rows] (a, a, g, g | c, c, q, q: each twice for the packed
+// instructions; q = C * the product of the part's decays up to the row) and of
+// the parts' decays [heads][ST].  Odd parts are shifted by half a warp's words,
+// so that the two parts of a warp do not meet in the banks.
 template <typename T, int VEC, int CG, int ST, int LC>
 struct Tile {
     static constexpr int NT = CG * ST, ROWS = ST * LC;
     static constexpr int PAD = CG == 16 ? 16 : 0;  // words per part
     static constexpr int WORDS = ROWS * CG + ST * PAD;
     static constexpr size_t STAGED = 2 * (size_t)WORDS * VEC * sizeof(T);
+    static constexpr size_t PER_HEAD = 2 * (size_t)(ROWS * 32 + ST * 4);
 };
 
+// Persistent: while a CTA looks back and finishes a tile, the next one's
+// inputs, weights, head scalars and row descriptions are on their way.
 template <typename T, int VEC, int CG, int ST, int LC, int PER_SM>
 __global__ void __launch_bounds__(CG *ST, PER_SM)
-    prefill_kernel(const Args p, Control *ctl, Word64 *words, Word64 *decays, int n_cb, int wide,
-                   int *err) {
+    prefill_kernel(const Args p, Control *ctl, Word64 *words, Word64 *decays, int n_cb, int n_items,
+                   int max_heads, int wide, int *err) {
     using L = Tile<T, VEC, CG, ST, LC>;
     using Word = typename Raw<T, VEC>::Word;
+    using V = typename Vec<VEC>::type;
     constexpr int NT = L::NT, ROWS = L::ROWS;
+    static_assert(LC <= 32 && 32 % LC == 0 && ROWS % 32 == 0 && NT >= 96, "tile");
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ unsigned s_ticket, s_epoch;
-    __shared__ Rows<ROWS> rows;
-    __shared__ float part_s[ST][CG * VEC], part_a[ST][CG], came[CG * VEC];
+    __shared__ int s_next;
+    __shared__ unsigned s_epoch;
+    __shared__ Rows<ROWS> rows_[2];
+    __shared__ V part_s[ST][CG], came[CG];
+    __shared__ float part_a[ST][CG];
     Word *const sx = reinterpret_cast<Word *>(smem), *const sz = sx + L::WORDS;
-    float4 *const tab = reinterpret_cast<float4 *>(smem + L::STAGED);
-    const int C = p.l.C, tid = threadIdx.x, lane = tid & 31;
-    const int cg = tid % CG, part = tid / CG;
-    if (tid == 0) {
-        s_epoch = *reinterpret_cast<volatile unsigned *>(&ctl->epoch) + 1;
-        s_ticket = atomicAdd(&ctl->ticket, 1u);
-    }
-    __syncthreads();
-    const unsigned epoch = s_epoch;
-    const int tile = (int)(s_ticket / (unsigned)n_cb), cb = (int)(s_ticket % (unsigned)n_cb);
-    const int64_t r0 = (int64_t)tile * ROWS;
-    const int live_rows = (int)min((int64_t)ROWS, p.rows - r0);
-    const int c0 = cb * CG * VEC, ch = c0 + cg * VEC;
-    const bool on = ch < C;
+    float4 *const tabs = reinterpret_cast<float4 *>(smem + L::STAGED);
+    float *const decs = reinterpret_cast<float *>(tabs + 2 * max_heads * ROWS * 2);
+    const int C = p.l.C, P = p.l.P, tid = threadIdx.x, lane = tid & 31;
+    const int cg = tid % CG, part = tid / CG, b0 = part * LC;
+    constexpr unsigned mask = LC == 32 ? 0xffffffffu : (1u << LC % 32) - 1u;
+    const float SET = -1.0f;  // in the place of A (a product of decays, >= 0)
 
-    // the tile's inputs and gates, all in flight at once; the gates are waited
-    // for last
-    for (int k = 0; k < (p.z ? 2 : 1); ++k) {
-        const T *src = static_cast<const T *>(k ? p.z : p.x) + r0 * p.ld;
-        Word *dst = k ? sz : sx;
+    // ---- the steps that get an item ready
+    auto stage_in = [&](int item, const void *from, Word *dst) {
+        const int tile = item / n_cb, c0 = item % n_cb * (CG * VEC);
+        const int64_t r0 = (int64_t)tile * ROWS;
+        const int live = (int)min((int64_t)ROWS, p.rows - r0);
+        const T *src = static_cast<const T *>(from) + r0 * p.ld + c0;
         if (wide) {  // 16 bytes at a time
             constexpr int E = 16 / (int)sizeof(T), CH = CG * VEC / E;  // elements, chunks of a row
             const int i = tid % CH;
-            const T *q = src + c0 + i * E;
-            for (int r = tid / CH; r < live_rows; r += NT / CH) {
+            const T *q = src + i * E + tid / CH * p.ld;
+            for (int r = tid / CH; r < live; r += NT / CH, q += NT / CH * p.ld) {
                 const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst + r * CG + r / LC * L::PAD + i * (E / VEC));
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(q + r * p.ld) : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(q) : "memory");
             }
-        } else if (on) {
-            for (int r = part; r < live_rows; r += ST)
-                stage(dst + r * CG + r / LC * L::PAD + cg, src + ch + r * p.ld, Word());
+        } else if (c0 + cg * VEC < C) {
+            for (int r = part; r < live; r += ST)
+                stage(dst + r * CG + r / LC * L::PAD + cg, src + cg * VEC + r * p.ld, Word());
+        }
+    };
+    V w0, w1, w2, w3, bias, dd;
+    Raw<T, VEC> above[3];
+    auto load_weights = [&](int item) {
+        const int tile = item / n_cb, ch = item % n_cb * (CG * VEC) + cg * VEC;
+        const int64_t r0 = (int64_t)tile * ROWS;
+        const bool on = ch < C;
+        float4 a = make_float4(0, 0, 0, 0), b = a;
+        if (on) {
+            a = reinterpret_cast<const float4 *>(p.l.conv_w)[ch];
+            b = reinterpret_cast<const float4 *>(p.l.conv_w)[ch + VEC - 1];
+        }
+        vset(w0, a.x, b.x);
+        vset(w1, a.y, b.y);
+        vset(w2, a.z, b.z);
+        vset(w3, a.w, b.w);
+        vset(bias, on ? p.l.conv_b[ch] : 0.0f, on ? p.l.conv_b[ch + VEC - 1] : 0.0f);
+        vset(dd, on ? p.l.d[ch] : 0.0f, on ? p.l.d[ch + VEC - 1] : 0.0f);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {  // the three rows above the tile
+            above[k].zero();
+            if (on && part == 0 && r0 > k && r0 - 1 - k < p.rows)
+                above[k].v = *reinterpret_cast<const Word *>(static_cast<const T *>(p.x) + ch + (r0 - 1 - k) * p.ld);
+        }
+    };
+    auto count = [&](int item, int buf, int warp) {  // warps 1 and 2
+        const int64_t r0 = (int64_t)(item / n_cb) * ROWS;
+        const int64_t r = warp == 1 ? r0 : min((int64_t)p.rows, r0 + ROWS) - 1;
+        const int n = count_offsets(p.off, p.n_seq + 1, r, lane);
+        if (lane == 0) (warp == 1 ? rows_[buf].first : rows_[buf].last) = n;
+    };
+    // entries i, i + step, ...: consecutive lanes are consecutive rows
+    auto head_table = [&](int item, int buf, int i0, int step) {
+        const int tile = item / n_cb, c0 = item % n_cb * (CG * VEC);
+        const int64_t r0 = (int64_t)tile * ROWS;
+        const int h0 = c0 / P, nh = (min(c0 + CG * VEC, C) - 1) / P - h0 + 1;
+        float4 *tab = tabs + buf * max_heads * ROWS * 2;
+        float *dec = decs + buf * max_heads * ST;
+        for (int i = i0; i < nh * ROWS; i += step) {
+            const int h = i / ROWS, t = i % ROWS;
+            Head k{0.0f, 0.0f, 0.0f};
+            if (r0 + t < p.rows) k = head_of<T>(p, r0 + t, h0 + h);
+            float prod = k.a;
+#pragma unroll
+            for (int o = 1; o < LC; o <<= 1) {
+                const float before = __shfl_up_sync(0xffffffffu, prod, o, LC);
+                if (t % LC >= o) prod *= before;
+            }
+            tab[i * 2] = make_float4(k.a, k.a, k.g, k.g);
+            tab[i * 2 + 1] = make_float4(k.c, k.c, k.c * prod, k.c * prod);
+            if (t % LC == LC - 1) dec[h * ST + t / LC] = prod;
+        }
+    };
+    auto describe_rows = [&](int item, int buf) {
+        const int64_t r0 = (int64_t)(item / n_cb) * ROWS;
+        Rows<ROWS> &rows = rows_[buf];
+        for (int i = tid; i < (ROWS + NT - 1) / NT * NT; i += NT) {
+            const int64_t r = r0 + i;
+            // the offsets <= r, of which the tile has only a few
+            int lo = rows.first, hi = max(rows.first, rows.last);
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (p.off[mid] <= r) lo = mid + 1;
+                else hi = mid;
+            }
+            const int sid = lo - 1;
+            int info = -1;
+            bool first = false, last = false;
+            if (i < ROWS && r < p.rows && sid >= 0 && sid < p.n_seq) {
+                const int slot = p.slots ? p.slots[sid] : sid;
+                if (slot >= 0 && slot < p.l.n_slots) {
+                    const int64_t o0 = max((int64_t)0, p.off[sid]), o1 = min(p.off[sid + 1], (int64_t)p.rows);
+                    const int fresh = p.fresh ? p.fresh[sid] != 0 : 1;
+                    info = slot << 3 | fresh << 2 | (int)max((int64_t)0, min((int64_t)3, r - o0));
+                    first = r == o0;
+                    last = r == o1 - 1;
+                }
+            }
+            const unsigned mv = __ballot_sync(0xffffffffu, info >= 0), ms = __ballot_sync(0xffffffffu, first),
+                           me = __ballot_sync(0xffffffffu, last);
+            if (i < ROWS) {
+                rows.info[i] = info;
+                if (lane == 0) {
+                    rows.valid[i / 32] = mv;
+                    rows.start[i / 32] = ms;
+                    rows.end[i / 32] = me;
+                }
+            }
+        }
+    };
+
+    if (tid == 0) {
+        s_epoch = *reinterpret_cast<volatile unsigned *>(&ctl->epoch) + 1;
+        s_next = (int)atomicAdd(&ctl->ticket, 1u);
+    }
+    __syncthreads();
+    const unsigned epoch = s_epoch, tag = 2 * epoch;
+    int item = s_next, buf = 0;
+    if (item < n_items) {
+        stage_in(item, p.x, sx);
+        stage_commit();
+        if (p.z) stage_in(item, p.z, sz);
+        stage_commit();
+        load_weights(item);
+        if (tid >= 32 && tid < 96) count(item, 0, tid / 32);
+        head_table(item, 0, tid, NT);
+        __syncthreads();
+        describe_rows(item, 0);
+    }
+    while (item < n_items) {
+        stage_wait<1>();  // x; the gates may still be on their way
+        __syncthreads();
+        if (tid == 0) s_next = (int)atomicAdd(&ctl->ticket, 1u);
+        const int tile = item / n_cb, cb = item % n_cb;
+        const int64_t r0 = (int64_t)tile * ROWS;
+        const int c0 = cb * CG * VEC, ch = c0 + cg * VEC;
+        const bool on = ch < C;
+        const Rows<ROWS> &rows = rows_[buf];
+        const unsigned valid = rows.valid[b0 / 32] >> b0 % 32 & mask, start = rows.start[b0 / 32] >> b0 % 32 & mask,
+                       end = rows.end[b0 / 32] >> b0 % 32 & mask;
+        const int *info = rows.info + b0;
+        const int head = (on ? ch : c0) / P, hh = head - c0 / P;
+        const float4 *tb = tabs + ((buf * max_heads + hh) * ROWS + b0) * 2;
+        const Word *xw = sx + b0 * CG + part * L::PAD + cg, *zw = sz + b0 * CG + part * L::PAD + cg;
+
+        // x1, x2, x3: the inputs 1, 2, 3 tokens back; from the slot before the
+        // sequence's first
+        auto conv_at = [&](int slot, int j) {
+            return static_cast<T *>(p.l.conv) + ((int64_t)slot * 3 + j) * C + ch;
+        };
+        auto back = [&](int k, int place, int t) {
+            // the input k tokens before a token at `place` < k of its sequence
+            Raw<T, VEC> r;
+            r.zero();
+            if (on && !(info[t] & 4)) r.v = *reinterpret_cast<const Word *>(conv_at(info[t] >> 3, 3 + place - k));
+            return r.get();
+        };
+        auto keep = [&](int slot, V a, V b, V c, V s) {
+            if (!on) return;
+            put(conv_at(slot, 0), a);
+            put(conv_at(slot, 1), b);
+            put(conv_at(slot, 2), c);
+            put(p.l.h + (int64_t)slot * C + ch, s);
+        };
+        if (part > 0) {
+#pragma unroll
+            for (int k = 0; k < 3; ++k) above[k].v = xw[-(k + 1) * CG - L::PAD];
+        }
+        V x1 = above[0].get(), x2 = above[1].get(), x3 = above[2].get();
+        if ((valid & 1u) && !(start & 1u)) {
+            const int place = info[0] & 3;
+            if (place < 3) x3 = back(3, place, 0);
+            if (place < 2) x2 = back(2, place, 0);
+        }
+        V h, y[LC];
+        vset(h, 0.0f, 0.0f);
+        // the end of the sequence that came in from the part before
+        float Ae = 0.0f;
+        V he = h, e1 = h, e2 = h, e3 = h;
+        int end_slot = -1;
+        auto token = [&](int t) {
+            const float4 k0 = tb[t * 2], k1 = tb[t * 2 + 1];
+            V a, g, c;
+            vset(a, k0.x, k0.y);
+            vset(g, k0.z, k0.w);
+            vset(c, k1.x, k1.y);
+            Raw<T, VEC> xr;
+            xr.v = xw[t * CG];
+            const V xt = xr.get();
+            const V u = silu(vfma(w3, xt, vfma(w2, x1, vfma(w1, x2, vfma(w0, x3, bias)))));
+            h = vfma(a, h, vmul(g, u));
+            y[t] = vfma(c, h, vmul(dd, u));
+            x3 = x2;
+            x2 = x1;
+            x1 = xt;
+            return k0.x;
+        };
+        if (valid == mask && !start && !end) {
+#pragma unroll
+            for (int t = 0; t < LC; ++t) token(t);
+        } else {
+            float A = 1.0f;
+#pragma unroll
+            for (int t = 0; t < LC; ++t) {
+                if (start >> t & 1u) {
+                    x1 = back(1, 0, t);
+                    x2 = back(2, 0, t);
+                    x3 = back(3, 0, t);
+                    const float *hs = p.l.h + (int64_t)(info[t] >> 3) * C + ch;
+                    const bool from = on && !(info[t] & 4);
+                    vset(h, from ? hs[0] : 0.0f, from ? hs[VEC - 1] : 0.0f);
+                }
+                A *= token(t);
+                if (end >> t & 1u) {
+                    if (start & ((2u << t) - 1u)) {
+                        keep(info[t] >> 3, x3, x2, x1, h);
+                    } else {
+                        // completed and written below, when the state that came
+                        // in is known: whoever starts from the slot has read it
+                        // by then
+                        end_slot = info[t] >> 3;
+                        Ae = A;
+                        he = h;
+                        e1 = x1;
+                        e2 = x2;
+                        e3 = x3;
+                    }
+                }
+            }
+        }
+        // the parts' S and A; with a start in a part its S is the state itself
+        part_s[part][cg] = h;
+        part_a[part][cg] = start ? SET : decs[(buf * max_heads + hh) * ST + part];
+        auto pass = [&](int i, V s) {  // the state through part i
+            const float a = part_a[i][cg];
+            const V local = part_s[i][cg];
+            V aa;
+            vset(aa, a, a);
+            const V r = vfma(aa, s, local);
+            return a == SET ? local : r;
+        };
+        __syncthreads();
+
+        // the next item on its way; part 0 joins the parts and looks back
+        const int next = s_next;
+        const bool more = next < n_items;
+        if (more) {
+            stage_in(next, p.x, sx);
+            load_weights(next);
         }
         stage_commit();
-    }
-    if (!p.z) stage_commit();
-    Raw<T, VEC> above[3];
-#pragma unroll
-    for (int k = 0; k < 3; ++k) {
-        above[k].zero();
-        if (on && part == 0 && r0 > k && r0 - 1 - k < p.rows)
-            above[k].load(static_cast<const T *>(p.x) + ch + (r0 - 1 - k) * p.ld);
-    }
-    // the rows' sequences
-    if (tid < 64) {
-        const int n = count_offsets(p.off, p.n_seq + 1, tid < 32 ? r0 : r0 + live_rows - 1, lane);
-        if (lane == 0) (tid < 32 ? rows.first : rows.last) = n;
-    }
-    // the scalars of the rows and the CTA's heads
-    const int h0 = c0 / p.l.P, nh = (min(c0 + CG * VEC, C) - 1) / p.l.P - h0 + 1;
-    for (int i = tid; i < ROWS * nh; i += NT) {
-        const int t = i / nh, h = i - t * nh;
-        Head k{0.0f, 0.0f, 0.0f};
-        if (t < live_rows) k = head_of<T>(p, r0 + t, h0 + h);
-        tab[i] = make_float4(k.a, k.g, k.c, 0.0f);
-    }
-    float4 w[VEC];
-    float bias[VEC], dd[VEC];
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-        w[v] = on ? reinterpret_cast<const float4 *>(p.l.conv_w)[ch + v] : make_float4(0, 0, 0, 0);
-        bias[v] = on ? p.l.conv_b[ch + v] : 0.0f;
-        dd[v] = on ? p.l.d[ch + v] : 0.0f;
-    }
-    __syncthreads();
-    for (int i = tid; i < (ROWS + NT - 1) / NT * NT; i += NT) {
-        const int64_t r = r0 + i;
-        // the offsets <= r, of which the tile has only a few
-        int lo = rows.first, hi = max(rows.first, rows.last);
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (p.off[mid] <= r) lo = mid + 1;
-            else hi = mid;
-        }
-        const int sid = lo - 1;
-        int info = -1;
-        bool first = false, last = false;
-        if (i < live_rows && sid >= 0 && sid < p.n_seq) {
-            const int slot = p.slots ? p.slots[sid] : sid;
-            if (slot >= 0 && slot < p.l.n_slots) {
-                const int64_t o0 = max((int64_t)0, p.off[sid]), o1 = min(p.off[sid + 1], (int64_t)p.rows);
-                const int fresh = p.fresh ? p.fresh[sid] != 0 : 1;
-                info = slot << 3 | fresh << 2 | (int)max((int64_t)0, min((int64_t)3, r - o0));
-                first = r == o0;
-                last = r == o1 - 1;
-            }
-        }
-        const unsigned mv = __ballot_sync(0xffffffffu, info >= 0), ms = __ballot_sync(0xffffffffu, first),
-                       me = __ballot_sync(0xffffffffu, last);
-        if (i < ROWS) {
-            rows.info[i] = info;
-            if (lane == 0) {
-                rows.valid[i / 32] = mv;
-                rows.start[i / 32] = ms;
-                rows.end[i / 32] = me;
-            }
-        }
-    }
-    stage_wait<1>();
-    __syncthreads();
-    constexpr unsigned mask = LC == 32 ? 0xffffffffu : (1u << LC % 32) - 1u;
-    const int b0 = part * LC;
-    const unsigned valid = rows.valid[b0 / 32] >> b0 % 32 & mask, start = rows.start[b0 / 32] >> b0 % 32 & mask,
-                   end = rows.end[b0 / 32] >> b0 % 32 & mask;
-    const int *info = rows.info + b0;
-    const int head = (on ? ch : c0) / p.l.P;
-    const float4 *tb = tab + b0 * nh + head - h0;
-    const Word *xw = sx + b0 * CG + part * L::PAD + cg, *zw = sz + b0 * CG + part * L::PAD + cg;
-
-    // x1, x2, x3: the inputs 1, 2, 3 tokens back; from the slot before the
-    // sequence's first
-    float x1[VEC], x2[VEC], x3[VEC], h[VEC];
-    auto conv_at = [&](int slot, int j) {
-        return static_cast<T *>(p.l.conv) + ((int64_t)slot * 3 + j) * C + ch;
-    };
-    auto back = [&](int k, int place, int t, float (&f)[VEC]) {
-        // the input k tokens before a token at `place` < k of its sequence
-        Raw<T, VEC> r;
-        r.zero();
-        if (on && !(info[t] & 4)) r.load(conv_at(info[t] >> 3, 3 + place - k));
-        r.get(f);
-    };
-    auto keep = [&](int slot, const float (&a)[VEC], const float (&b)[VEC], const float (&c)[VEC],
-                    const float (&s)[VEC]) {
-        if (!on) return;
-        put(conv_at(slot, 0), a);
-        put(conv_at(slot, 1), b);
-        put(conv_at(slot, 2), c);
-        put(p.l.h + (int64_t)slot * C + ch, s);
-    };
-    if (part > 0) {
-#pragma unroll
-        for (int k = 0; k < 3; ++k) above[k].v = xw[-(k + 1) * CG - L::PAD];
-    }
-    above[0].get(x1);
-    above[1].get(x2);
-    above[2].get(x3);
-    if ((valid & 1u) && !(start & 1u)) {
-        const int place = info[0] & 3;
-        if (place < 3) back(3, place, 0, x3);
-        if (place < 2) back(2, place, 0, x2);
-    }
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) h[v] = 0.0f;
-
-    float y[LC][VEC], A = 1.0f;
-    // the end of the sequence that came in from the part before
-    float Ae = 0.0f, he[VEC], e1[VEC], e2[VEC], e3[VEC];
-    int end_slot = -1;
-#pragma unroll
-    for (int t = 0; t < LC; ++t) {
-        if (start >> t & 1u) {
-            back(1, 0, t, x1);
-            back(2, 0, t, x2);
-            back(3, 0, t, x3);
-#pragma unroll
-            for (int v = 0; v < VEC; ++v)
-                h[v] = on && !(info[t] & 4) ? p.l.h[(int64_t)(info[t] >> 3) * C + ch + v] : 0.0f;
-        }
-        const float4 k = tb[t * nh];
-        float xt[VEC];
-        Raw<T, VEC> xr;
-        xr.v = xw[t * CG];
-        xr.get(xt);
-        A *= k.x;
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            const float u = silu(fmaf(w[v].w, xt[v], fmaf(w[v].z, x1[v], fmaf(w[v].y, x2[v], fmaf(w[v].x, x3[v], bias[v])))));
-            h[v] = fmaf(k.x, h[v], k.y * u);
-            y[t][v] = fmaf(k.z, h[v], dd[v] * u);
-            x3[v] = x2[v];
-            x2[v] = x1[v];
-            x1[v] = xt[v];
-        }
-        if (end >> t & 1u) {
-            if (start & ((2u << t) - 1u)) {
-                keep(info[t] >> 3, x3, x2, x1, h);
-            } else {
-                // completed and written below, when the state that came in is
-                // known: whoever starts from the slot has read it by then
-                end_slot = info[t] >> 3;
-                Ae = A;
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) {
-                    he[v] = h[v];
-                    e1[v] = x1[v];
-                    e2[v] = x2[v];
-                    e3[v] = x3[v];
-                }
-            }
-        }
-    }
-
-    // the parts' S and A; with a start in a part its S is the state itself
-    const float SET = -1.0f;  // in the place of A (a product of decays, >= 0)
-    if (start) A = SET;
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) part_s[part][cg * VEC + v] = h[v];
-    part_a[part][cg] = A;
-    auto pass = [&](int i, float (&s)[VEC]) {  // the state through part i
-        const float a = part_a[i][cg];
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            const float local = part_s[i][cg * VEC + v];
-            s[v] = a == SET ? local : fmaf(a, s[v], local);
-        }
-    };
-    __syncthreads();
-    float hin[VEC];
-    if (part == 0) {
-        // Every tile but the last publishes, whatever its rows are, so that
-        // offsets that contradict each other make no tile wait for a word that
-        // never comes.
-        const bool need_in = tile > 0 && (valid & 1u) && !(start & 1u);
-        const bool need_out = (tile + 1) * (int64_t)ROWS < p.rows;
-        Word64 *own = words + (int64_t)tile * C + ch, *dec = decays + (int64_t)tile * p.l.H + head;
-        const unsigned tag = 2 * epoch;
-        float S[VEC], all = 1.0f;
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) S[v] = hin[v] = 0.0f;
-        bool is_final = !need_in;
-        if (need_out) {
+        if (tid < 32) {
+            if (part == 0) {
+                // Every tile but the last publishes, whatever its rows are, so
+                // that offsets that contradict each other make no tile wait
+                // for a word that never comes.
+                const bool need_in = tile > 0 && (valid & 1u) && !(start & 1u);
+                const bool need_out = r0 + ROWS < p.rows;
+                Word64 *own = words + (int64_t)tile * C + ch, *dec = decays + (int64_t)tile * p.l.H + head;
+                float all = 1.0f;
+                V S, hin;
+                vset(S, 0.0f, 0.0f);
+                vset(hin, 0.0f, 0.0f);
+                bool is_final = !need_in;
+                if (need_out) {
 #pragma unroll 4
-            for (int i = 0; i < ST; ++i) {
-                pass(i, S);
-                is_final |= part_a[i][cg] == SET;
-                all *= part_a[i][cg];
-            }
-            if (on) {
-                store_words(own, is_final ? tag + 1 : tag, S);
-                // one thread a head (or more, with the same value)
-                if (!is_final && (tid == 0 || ch % p.l.P < VEC)) {
-                    const float a[1] = {all};
-                    store_words(dec, tag, a);
+                    for (int i = 0; i < ST; ++i) {
+                        S = pass(i, S);
+                        is_final |= part_a[i][cg] == SET;
+                        all *= part_a[i][cg];
+                    }
+                    if (on) {
+                        store_words(own, is_final ? tag + 1 : tag, S);
+                        // one thread a head (or more, with the same value)
+                        if (!is_final && (tid == 0 || ch % P < VEC)) store_words(dec, tag, all);
+                    }
                 }
-            }
-        }
-        if (need_in && on && !look_back<VEC>(own, C, dec, p.l.H, tile, tag, hin)) atomicOr(err, 8);
-        if (need_out && !is_final && on) {
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) S[v] = fmaf(all, hin[v], S[v]);
-            store_words(own, tag + 1, S);
-        }
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) came[cg * VEC + v] = hin[v];
-    }
-    stage_wait<0>();
-    __syncthreads();
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) hin[v] = came[cg * VEC + v];
-    for (int i = 0; i < part; ++i) pass(i, hin);
-    if (end_slot >= 0) {
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) he[v] = fmaf(Ae, hin[v], he[v]);
-        keep(end_slot, e3, e2, e1, he);
-    }
-    const int first = start ? __ffs(start) - 1 : LC;
-    if (on) {
-        T *py = static_cast<T *>(p.y) + ch + (r0 + b0) * p.ldy;
-#pragma unroll
-        for (int t = 0; t < LC; ++t, py += p.ldy) {
-            float o[VEC];
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) o[v] = y[t][v];
-            if (t < first) {
-                const float4 k = tb[t * nh];
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) {
-                    hin[v] *= k.x;
-                    o[v] = fmaf(k.z, hin[v], o[v]);
+                if (need_in && on && !look_back(own, C, dec, p.l.H, tile, tag, hin)) atomicOr(err, 8);
+                if (need_out && !is_final && on) {
+                    V aa;
+                    vset(aa, all, all);
+                    store_words(own, tag + 1, vfma(aa, hin, S));
                 }
+                came[cg] = hin;
             }
-            if (!(valid >> t & 1u)) continue;
-            if (p.z) {
-                Raw<T, VEC> zr;
-                float zt[VEC];
-                zr.v = zw[t * CG];
-                zr.get(zt);
+            __syncwarp();
+        } else if (more) {
+            if (tid < 96) count(next, buf ^ 1, tid / 32);
+            head_table(next, buf ^ 1, tid - 32, NT - 32);
+        }
+        stage_wait<1>();  // z
+        __syncthreads();
+        V hin = came[cg];
+        for (int i = 0; i < part; ++i) hin = pass(i, hin);
+        if (end_slot >= 0) {
+            V aa;
+            vset(aa, Ae, Ae);
+            keep(end_slot, e3, e2, e1, vfma(aa, hin, he));
+        }
+        if (on) {
+            const int first = start ? __ffs(start) - 1 : LC;
+            T *py = static_cast<T *>(p.y) + ch + (r0 + b0) * p.ldy;
+            auto finish = [&](int t, bool fix) {
+                V o = y[t];
+                if (fix) {
+                    const float2 q2 = *reinterpret_cast<const float2 *>(&tb[t * 2 + 1].z);
+                    V q;
+                    vset(q, q2.x, q2.y);
+                    o = vfma(q, hin, o);
+                }
+                if (p.z) {
+                    Raw<T, VEC> zr;
+                    zr.v = zw[t * CG];
+                    o = vmul(o, silu(zr.get()));
+                }
+                put(py, o);
+            };
+            if (valid == mask && !start) {
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) o[v] *= silu(zt[v]);
+                for (int t = 0; t < LC; ++t, py += p.ldy) finish(t, true);
+            } else {
+#pragma unroll
+                for (int t = 0; t < LC; ++t, py += p.ldy)
+                    if (valid >> t & 1u) finish(t, t < first);
             }
-            put(py, o);
         }
-    }
-    // sequences without tokens that start afresh: a zero state
-    if (tile == 0) {
-        __shared__ int empty[NT], n_empty;
-        for (int s0 = 0; s0 < p.n_seq; s0 += NT) {
-            const int s = s0 + tid;
-            int slot = -1;
-            if (s < p.n_seq && !(p.fresh && p.fresh[s] == 0) &&
-                max((int64_t)0, p.off[s]) >= min((int64_t)p.rows, p.off[s + 1])) {
-                slot = p.slots ? p.slots[s] : s;
-                if (slot >= p.l.n_slots) slot = -1;
+        // sequences without tokens that start afresh: a zero state
+        if (tile == 0) {
+            __shared__ int empty[NT], n_empty;
+            for (int s0 = 0; s0 < p.n_seq; s0 += NT) {
+                const int s = s0 + tid;
+                int slot = -1;
+                if (s < p.n_seq && !(p.fresh && p.fresh[s] == 0) &&
+                    max((int64_t)0, p.off[s]) >= min((int64_t)p.rows, p.off[s + 1])) {
+                    slot = p.slots ? p.slots[s] : s;
+                    if (slot >= p.l.n_slots) slot = -1;
+                }
+                if (!__syncthreads_or(slot >= 0)) continue;
+                if (tid == 0) n_empty = 0;
+                __syncthreads();
+                if (slot >= 0) empty[atomicAdd(&n_empty, 1)] = slot;
+                __syncthreads();
+                V none;
+                vset(none, 0.0f, 0.0f);
+                for (int i = part; i < n_empty; i += ST) keep(empty[i], none, none, none, none);
+                __syncthreads();
             }
-            if (!__syncthreads_or(slot >= 0)) continue;
-            if (tid == 0) n_empty = 0;
-            __syncthreads();
-            if (slot >= 0) empty[atomicAdd(&n_empty, 1)] = slot;
-            __syncthreads();
-            const float none[VEC] = {};
-            for (int i = part; i < n_empty; i += ST) keep(empty[i], none, none, none, none);
-            __syncthreads();
         }
+        if (more) describe_rows(next, buf ^ 1);
+        __syncthreads();  // z and the parts are free
+        if (more && p.z) stage_in(next, p.z, sz);
+        stage_commit();
+        item = next;
+        buf ^= 1;
     }
-    __syncthreads();
     if (tid == 0) {
         __threadfence();
         if (atomicAdd(&ctl->done, 1u) == gridDim.x - 1) {
@@ -646,7 +750,8 @@ int launch_prefill(const Launch &l) {
     const int C = a.l.C, P = a.l.P;
     const int n_cb = (C + CG * VEC - 1) / (CG * VEC);
     const int64_t tiles = a.rows > 0 ? ((int64_t)a.rows + L::ROWS - 1) / L::ROWS : 1;
-    if (tiles * n_cb > INT32_MAX)
+    const int64_t items = tiles * n_cb;
+    if (items > INT32_MAX / 2)
         return bm_detail_fail(BM_ERR_UNSUPPORTED, "rows * channels too large for one call");
     // a word per tile and channel, then one per tile and head
     const size_t n_words = ((size_t)tiles * C + 1) / 2 * 2;
@@ -657,14 +762,15 @@ int launch_prefill(const Launch &l) {
     Word64 *words = reinterpret_cast<Word64 *>(static_cast<unsigned char *>(work) + CONTROL_BYTES);
     const int heads = min((CG * VEC + P - 2) / P + 1, a.l.H);
     auto *k = prefill_kernel<T, VEC, CG, ST, LC, PER_SM>;
-    // the most any call takes: heads of VEC channels
-    constexpr int most = (int)(L::STAGED + (size_t)L::ROWS * (CG + VEC - 1) * sizeof(float4));
-    static_assert(most <= 220 * 1024, "shared memory");
+    constexpr int most = 200 * 1024;
+    const size_t bytes = L::STAGED + (size_t)heads * L::PER_HEAD;
+    if (bytes > most) return bm_detail_fail(BM_ERR_UNSUPPORTED, "too many heads in a tile");
     BMC_CK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
     auto even = [&](const void *q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; };
     const int wide = C % (CG * VEC) == 0 && even(a.x) && even(a.z) && a.ld * (int64_t)sizeof(T) % 16 == 0;
-    k<<<(int)(tiles * n_cb), L::NT, L::STAGED + (size_t)L::ROWS * heads * sizeof(float4), l.s>>>(
-        a, static_cast<Control *>(work), words, words + n_words, n_cb, wide, l.err);
+    const int64_t grid = items < (int64_t)PER_SM * l.sms ? items : (int64_t)PER_SM * l.sms;
+    k<<<(int)grid, L::NT, bytes, l.s>>>(a, static_cast<Control *>(work), words, words + n_words, n_cb,
+                                        (int)items, heads, wide, l.err);
     BMC_CK(cudaGetLastError());
     return BM_OK;
 }
@@ -767,9 +873,8 @@ int bm_ssm_prefill(bm_ctx_t *ctx, const bm_ssm_layer_t *layer, const void *d_x, 
     a.n_seq = n_seq;
     a.fresh = d_fresh;
     const size_t e = layer->type == BM_F32 ? 4 : 2;
-    // two channels a thread: the words of a pair must be one head's, and every
-    // pair aligned
-    const bool pairs = layer->type == BM_BF16 && a.l.P % 2 == 0 && ld % 2 == 0 && ldy % 2 == 0 &&
+    // two channels a thread: a pair is one head's, and every pair is aligned
+    const bool pairs = a.l.P % 2 == 0 && a.l.P >= 16 && ld % 2 == 0 && ldy % 2 == 0 &&
                        !misaligned(d_x, 2 * e) && !misaligned(d_z, 2 * e) &&
                        !misaligned(d_y, 2 * e) && !misaligned(layer->conv_state, 2 * e) &&
                        !misaligned(layer->h_state, 8);
@@ -779,14 +884,17 @@ int bm_ssm_prefill(bm_ctx_t *ctx, const bm_ssm_layer_t *layer, const void *d_x, 
     BMC_CK(guard.error);
     if (stream) l.s = static_cast<cudaStream_t>(stream);
     l.a = a;
-    // long parts unless that leaves SMs without a CTA
+    // Tall tiles unless that leaves SMs without work.  One channel a thread,
+    // in small tiles, for what cannot be paired and for heads so small that
+    // their scalars would fill the shared memory.
     using bf16 = __nv_bfloat16;
     const bool few = ((int64_t)rows + 255) / 256 * ((a.l.C + 31) / 32) < 2 * l.sms;
-    if (layer->type == BM_F32)
-        return few ? launch_prefill<float, 1, 32, 4, 8, 4>(l) : launch_prefill<float, 1, 32, 8, 32, 3>(l);
-    if (pairs)
-        return few ? launch_prefill<bf16, 2, 16, 8, 8, 4>(l) : launch_prefill<bf16, 2, 16, 16, 32, 2>(l);
-    return few ? launch_prefill<bf16, 1, 32, 4, 8, 4>(l) : launch_prefill<bf16, 1, 32, 8, 32, 3>(l);
+    if (layer->type == BM_F32) {
+        if (!pairs) return launch_prefill<float, 1, 32, 4, 8, 4>(l);
+        return few ? launch_prefill<float, 2, 16, 8, 8, 4>(l) : launch_prefill<float, 2, 16, 8, 16, 4>(l);
+    }
+    if (!pairs) return launch_prefill<bf16, 1, 32, 4, 8, 4>(l);
+    return few ? launch_prefill<bf16, 2, 16, 8, 8, 4>(l) : launch_prefill<bf16, 2, 16, 16, 16, 2>(l);
 }
 
 int bm_ssm_step(bm_ctx_t *ctx, const bm_ssm_layer_t *layer, const void *d_x, const void *d_z,
