@@ -116,106 +116,44 @@ __device__ __forceinline__ Head head_of(const Args &p, int64_t row, int h) {
 
 // ---------------------------------------------------------------- prompts --
 //
-// The token axis of all sequences together is cut into tiles of ST * LC rows; a
-// CTA takes one tile of CG * VEC channels, a thread VEC channels of one of the
-// tile's ST parts from its first row to its last, with the convolution's
-// window, the state and the outputs in registers.  The recurrence is linear,
-// so a part first runs from a zero state:
+// The token axis of all sequences together is cut into tiles of ST * LC rows.
+// A CTA takes CG * VEC channels and goes down the tiles; a thread has VEC
+// channels of one of a tile's ST parts, with the convolution's window, the
+// state and the outputs in registers.  The recurrence is linear, so a part
+// first runs from a zero state:
 //   s_t = local_t + (a_first ... a_t) * s_in,    s_out = S + A * s_in
-// and the C s_t of its outputs is completed when s_in arrives: outputs wait
-// in registers, x and z are read once and y is written once.  The parts of a
-// tile are joined in shared memory, the tiles through published words.
+// the parts' (A, S) are joined by a scan over the lanes of a warp, and the
+// outputs, which waited in registers, get their C a_first ... a_t s_in: x and
+// z are read once, y is written once.  The next tile's x and z are copied to
+// shared memory meanwhile.
 //
-// Narrow and long tiles (64 or 128 bytes of a row) keep few tiles of the same
-// channels in flight and the chain over them short: with 128 threads side by
-// side and tiles of 32 rows, 37 tiles of each channel were in flight and the
-// look-back cost more than the scan (65536 x 4096 bf16: 1.98 ms).
+// A CTA's channels are 64 to 128 bytes of a row, so a few dozen to hundreds of
+// CTAs share a prompt with nothing between them.  Where that leaves SMs idle
+// (few channels, many rows), the rows are cut into segments too: a first
+// launch takes each segment's (A, S) from a zero state, the second starts
+// every segment from those before it, and a third writes the states of
+// sequences that ended in another segment than they began in (before that,
+// their first segment may still have to read the slot).
 //
-// s_in comes from the tiles before (CTAs take tiles in order, by a ticket, so
-// whoever is waited for is running or done).  Each tile publishes its
-// channels' S and its heads' A, then looks back for the nearest tile whose
-// s_out is final (it holds a sequence start, or has completed its own
-// look-back) and applies the A and S of the tiles in between in order.  That
-// is the chain s = A s + S that each of them applies too, so the result does
-// not depend on how far back the final word was.
-//
-// A value is published as 8 bytes {tag, value} written at once, tag = 2 *
-// epoch + (final or not): whoever reads the launch's tag has the value.  (16
-// bytes in one relaxed b128 access were seen torn here: halves of two
-// successive stores.)  The epoch is a counter in the workspace that the
-// launch's last CTA advances, so nothing is cleared between launches or graph
-// replays; a tag comes again after 2^31 launches.
+// Measured against it: tiles joined by published words and a look-back (one
+// launch, any number of CTAs on an axis) took 0.91 ms for 65536 x 4096 bf16
+// and 123 us for 4099 x 4096 fp32; the chain over the tiles was what it spent
+// its time on.
 
-constexpr unsigned long long WAIT_NS = 2000000000ull;  // bounded waits: 2 s
-
-struct Control {
-    unsigned ticket, done, epoch;
-};
-constexpr size_t CONTROL_BYTES = 256;
-
-// The words of one or two channels: {tag, S} each.
-using Word64 = unsigned long long;
-template <typename V>
-struct Words;
-template <>
-struct Words<float> {
-    unsigned tag, tag1;
-    float s;
-};
-template <>
-struct Words<float2> {
-    unsigned tag, tag1;
-    float2 s;
-};
-__device__ __forceinline__ Word64 join(unsigned tag, float s) {
-    return tag | ((Word64)__float_as_uint(s) << 32);
-}
-__device__ __forceinline__ void load_words(const Word64 *p, Words<float> &r) {
-    Word64 w;
-    asm volatile("ld.relaxed.gpu.global.b64 %0, [%1];" : "=l"(w) : "l"(p) : "memory");
-    r.tag = r.tag1 = (unsigned)w;
-    r.s = __uint_as_float((unsigned)(w >> 32));
-}
-__device__ __forceinline__ void load_words(const Word64 *p, Words<float2> &r) {
-    Word64 w0, w1;
-    asm volatile("ld.relaxed.gpu.global.v2.b64 {%0, %1}, [%2];" : "=l"(w0), "=l"(w1) : "l"(p) : "memory");
-    r.tag = (unsigned)w0;
-    r.tag1 = (unsigned)w1;
-    r.s = make_float2(__uint_as_float((unsigned)(w0 >> 32)), __uint_as_float((unsigned)(w1 >> 32)));
-}
-__device__ __forceinline__ void store_words(Word64 *p, unsigned tag, float s) {
-    asm volatile("st.relaxed.gpu.global.b64 [%0], %1;" ::"l"(p), "l"(join(tag, s)) : "memory");
-}
-__device__ __forceinline__ void store_words(Word64 *p, unsigned tag, float2 s) {
-    asm volatile("st.relaxed.gpu.global.v2.b64 [%0], {%1, %2};" ::"l"(p), "l"(join(tag, s.x)),
-                 "l"(join(tag, s.y))
-                 : "memory");
-}
-__device__ __forceinline__ unsigned long long gtimer() {
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-
-// Copies to shared memory, each thread for itself: 4 bytes asynchronously, a
-// 2-byte element through a register.
+// Copies to shared memory: 4 or 8 bytes asynchronously, a 2-byte element
+// through a register.
 __device__ __forceinline__ void stage(void *dst, const void *src, float) {
     const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(d), "l"(src) : "memory");
-}
-__device__ __forceinline__ void stage(void *dst, const void *src, float2) {
-    const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(d), "l"(src) : "memory");
 }
 __device__ __forceinline__ void stage(void *dst, const void *src, uint32_t) { stage(dst, src, 0.0f); }
 __device__ __forceinline__ void stage(void *dst, const void *src, __nv_bfloat16) {
     *static_cast<__nv_bfloat16 *>(dst) = *static_cast<const __nv_bfloat16 *>(src);
 }
-template <int N>
-__device__ __forceinline__ void stage_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+__device__ __forceinline__ void stage(void *dst, const void *src, float2) {
+    const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(d), "l"(src) : "memory");
 }
-__device__ __forceinline__ void stage_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 
 // VEC consecutive elements as they lie in memory, and as fp32.
 template <typename T, int VEC>
@@ -250,152 +188,178 @@ __device__ __forceinline__ void put(__nv_bfloat16 *p, float2 f) {
     *reinterpret_cast<__nv_bfloat162 *>(p) = __floats2bfloat162_rn(f.x, f.y);
 }
 
-// The state that comes into a tile, from the words of the tiles before: `own`
-// is this thread's word of this tile, `dec` its head's, with cw and H words a
-// tile.  BACK tiles are read at a time; false when a word did not come in
-// time.
-template <typename V>
-__device__ __forceinline__ bool look_back(const Word64 *own, int cw, const Word64 *dec, int H,
-                                          int tile, unsigned tag, V &hin) {
-    constexpr int BACK = 4;
-    Words<V> w[BACK];
-    Words<float> a[BACK];
-    auto load = [&](int i, int j) {
-        load_words(own - (int64_t)j * cw, w[i]);
-        load_words(dec - (int64_t)j * H, a[i]);
-    };
-    // (a word that became final meanwhile holds what the chain gives)
-    auto apply = [&](int i) {
-        V aa;
-        vset(aa, a[i].s, a[i].s);
-        const V r = vfma(aa, hin, w[i].s);
-        vset(hin, w[i].tag == tag + 1 ? lane0(w[i].s) : lane0(r), w[i].tag1 == tag + 1 ? lane1(w[i].s) : lane1(r));
-    };
-    unsigned long long t0 = 0;
-    for (int j = 1;;) {
-#pragma unroll
-        for (int i = 0; i < BACK; ++i) load(i, min(j + i, tile));
-        // the nearest final tile before any that is not ready, and how many
-        // are ready
-        int at = -1, ready = BACK;
-#pragma unroll
-        for (int i = BACK - 1; i >= 0; --i) {
-            if (w[i].tag == tag + 1 && w[i].tag1 == tag + 1) {
-                at = i;
-            } else if ((w[i].tag | 1u) != tag + 1 || (w[i].tag1 | 1u) != tag + 1 || a[i].tag != tag) {
-                at = -1;
-                ready = i;
-            }
-        }
-        if (at >= 0) {
-#pragma unroll
-            for (int i = BACK - 1; i >= 0; --i)
-                if (i <= at) apply(i);
-            for (--j; j > 0; j -= BACK) {
-#pragma unroll
-                for (int i = 0; i < BACK; ++i) load(i, max(j - i, 1));
-#pragma unroll
-                for (int i = 0; i < BACK; ++i)
-                    if (j - i > 0) apply(i);
-            }
-            return true;
-        }
-        j += ready;  // (never beyond tile: tile 0 is final)
-        if (ready == 0) {
-            if (t0 == 0) t0 = gtimer();
-            if (gtimer() - t0 > WAIT_NS) return false;
-        }
-    }
+// In the place of A (a product of decays, >= 0): a sequence starts in there,
+// S is the state itself.  Not A = 0, which a state that is not finite would
+// survive.
+constexpr float SET = -1.0f;
+__device__ __forceinline__ float through(float a, float s, float S) { return a == SET ? S : fmaf(a, s, S); }
+__device__ __forceinline__ float2 through(float a, float2 s, float2 S) {
+    return a == SET ? S : __ffma2_rn(make_float2(a, a), s, S);
+}
+__device__ __forceinline__ float through(float a1, float a2) { return a2 == SET || a1 == SET ? SET : a1 * a2; }
+__device__ __forceinline__ float shfl_up(float v, int o, int w) { return __shfl_up_sync(0xffffffffu, v, o, w); }
+__device__ __forceinline__ float2 shfl_up(float2 v, int o, int w) {
+    return make_float2(shfl_up(v.x, o, w), shfl_up(v.y, o, w));
+}
+__device__ __forceinline__ float shfl_at(float v, int l, int w) { return __shfl_sync(0xffffffffu, v, l, w); }
+__device__ __forceinline__ float2 shfl_at(float2 v, int l, int w) {
+    return make_float2(shfl_at(v.x, l, w), shfl_at(v.y, l, w));
 }
 
-// How many offsets are <= r (a warp's lanes together, 32 probes a step).
-__device__ __forceinline__ int count_offsets(const int64_t *off, int n_off, int64_t r, int lane) {
-    const unsigned all = 0xffffffffu;
-    int lo = 0, n = n_off;
-    while (n > 32) {
-        const int stride = (n + 31) / 32, at = lane * stride;
-        const unsigned m = __ballot_sync(all, at < n && off[lo + at] <= r);
-        if (m == 0) return lo;
-        const int k = __popc(m) - 1;
-        lo += k * stride;
-        n = min(stride, n - k * stride);
-    }
-    return lo + __popc(__ballot_sync(all, lane < n && off[lo + lane] <= r));
-}
-
-// A tile's rows.  info: slot << 3 | fresh << 2 | place in the sequence (3 and
-// above: 3), or -1 for a row of no sequence; the masks have a bit per row.
-template <int ROWS>
-struct Rows {
-    int first, last;  // offsets <= the tile's first and last row
-    int info[ROWS];
-    unsigned valid[ROWS / 32], start[ROWS / 32], end[ROWS / 32];
+// Segments of the token axis, and what their launches hand on (in the
+// context's workspace): S [seg][C], A [seg][H], the states to write [seg][C]
+// with the inputs [seg][3][C], and their slots [seg][CTA] (-1: none).
+struct Segments {
+    int n, rows;  // rows of a segment, a multiple of the tile
+    float *S, *A, *h;
+    void *conv;
+    int *slot;
 };
 
-// Shared memory of a CTA: x and z of the tile, then two buffers of the head
-// scalars [heads][rows] (a, a, g, g | c, c, q, q: each twice for the packed
-// instructions; q = C * the product of the part's decays up to the row) and of
-// the parts' decays [heads][ST].  Odd parts are shifted by half a warp's words,
-// so that the two parts of a warp do not meet in the banks.
+constexpr int SEQ_CACHE = 1024;  // sequences whose offsets a CTA keeps in shared memory
+
 template <typename T, int VEC, int CG, int ST, int LC>
 struct Tile {
     static constexpr int NT = CG * ST, ROWS = ST * LC;
-    static constexpr int PAD = CG == 16 ? 16 : 0;  // words per part
+    // words: odd parts are shifted by 16 banks, so that the two parts of a
+    // warp do not meet
+    static constexpr int PAD = CG == 16 && VEC * sizeof(T) == 4 ? 16 : 0;
     static constexpr int WORDS = ROWS * CG + ST * PAD;
-    static constexpr size_t STAGED = 2 * (size_t)WORDS * VEC * sizeof(T);
-    static constexpr size_t PER_HEAD = 2 * (size_t)(ROWS * 32 + ST * 4);
+    // x and z, twice
+    static constexpr size_t STAGED = 4 * (size_t)WORDS * VEC * sizeof(T);
+    // a head's scalars (a, g, c, C times the part's decays so far) and its
+    // parts' decays, twice
+    static constexpr size_t PER_HEAD = 2 * (size_t)(ROWS * 16 + ST * 4);
 };
 
-// Persistent: while a CTA looks back and finishes a tile, the next one's
-// inputs, weights, head scalars and row descriptions are on their way.
-template <typename T, int VEC, int CG, int ST, int LC, int PER_SM>
+// SUMS: only the segment's (A, S).
+template <typename T, int VEC, int CG, int ST, int LC, int PER_SM, bool SUMS>
 __global__ void __launch_bounds__(CG *ST, PER_SM)
-    prefill_kernel(const Args p, Control *ctl, Word64 *words, Word64 *decays, int n_cb, int n_items,
-                   int max_heads, int wide, int *err) {
+    prefill_kernel(const Args p, const Segments g, int heads, int wide) {
     using L = Tile<T, VEC, CG, ST, LC>;
-    using Word = typename Raw<T, VEC>::Word;
+    using R = Raw<T, VEC>;
+    using Word = typename R::Word;
     using V = typename Vec<VEC>::type;
     constexpr int NT = L::NT, ROWS = L::ROWS;
-    static_assert(LC <= 32 && 32 % LC == 0 && ROWS % 32 == 0 && NT >= 96, "tile");
+    static_assert(LC <= 32 && 32 % LC == 0 && ST <= 32 && ROWS % 32 == 0 && ROWS <= NT && LC >= 3, "tile");
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ int s_next;
-    __shared__ unsigned s_epoch;
-    __shared__ Rows<ROWS> rows_[2];
-    __shared__ V part_s[ST][CG], came[CG];
-    __shared__ float part_a[ST][CG];
-    Word *const sx = reinterpret_cast<Word *>(smem), *const sz = sx + L::WORDS;
+    __shared__ int s_off[SEQ_CACHE + 1], s_info[SEQ_CACHE];
+    __shared__ int row_info[ROWS];
+    __shared__ unsigned row_valid[ROWS / 32], row_start[ROWS / 32], row_end[ROWS / 32];
+    __shared__ int last_begin, last_end, last_info, n_list, list[NT];
+    __shared__ V part_s[ST][CG + 1], came[ST][CG + 1], halo[3][CG];
+    __shared__ float part_a[ST][CG + 1];
+    Word *const staged = reinterpret_cast<Word *>(smem);  // x0, z0, x1, z1
     float4 *const tabs = reinterpret_cast<float4 *>(smem + L::STAGED);
-    float *const decs = reinterpret_cast<float *>(tabs + 2 * max_heads * ROWS * 2);
+    float *const decs = reinterpret_cast<float *>(tabs + 2 * heads * ROWS);
     const int C = p.l.C, P = p.l.P, tid = threadIdx.x, lane = tid & 31;
     const int cg = tid % CG, part = tid / CG, b0 = part * LC;
+    const int seg = blockIdx.y, c0 = blockIdx.x * (CG * VEC), ch = c0 + cg * VEC;
+    const int seg0 = seg * g.rows, seg1 = min(p.rows, seg0 + g.rows);
+    const bool on = ch < C;
+    const int h0 = c0 / P, nh = (min(c0 + CG * VEC, C) - 1) / P - h0 + 1, hh = (on ? ch : c0) / P - h0;
     constexpr unsigned mask = LC == 32 ? 0xffffffffu : (1u << LC % 32) - 1u;
-    const float SET = -1.0f;  // in the place of A (a product of decays, >= 0)
+    const bool gate = p.z && !SUMS;
 
-    // ---- the steps that get an item ready
-    auto stage_in = [&](int item, const void *from, Word *dst) {
-        const int tile = item / n_cb, c0 = item % n_cb * (CG * VEC);
-        const int64_t r0 = (int64_t)tile * ROWS;
-        const int live = (int)min((int64_t)ROWS, p.rows - r0);
-        const T *src = static_cast<const T *>(from) + r0 * p.ld + c0;
-        if (wide) {  // 16 bytes at a time
-            constexpr int E = 16 / (int)sizeof(T), CH = CG * VEC / E;  // elements, chunks of a row
-            const int i = tid % CH;
-            const T *q = src + i * E + tid / CH * p.ld;
-            for (int r = tid / CH; r < live; r += NT / CH, q += NT / CH * p.ld) {
-                const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst + r * CG + r / LC * L::PAD + i * (E / VEC));
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(q) : "memory");
+    auto stage_in = [&](int r0, int buf) {
+        const int live = min(ROWS, seg1 - r0);
+        for (int k = 0; k < (gate ? 2 : 1); ++k) {
+            const T *src = static_cast<const T *>(k ? p.z : p.x) + r0 * p.ld + c0;
+            Word *dst = staged + (2 * buf + k) * L::WORDS;
+            if (wide) {  // 16 bytes at a time
+                constexpr int E = 16 / (int)sizeof(T), CH = CG * VEC / E;  // elements, chunks of a row
+                constexpr int STEP = NT / CH;                             // rows a pass
+                const int i = tid % CH, r = tid / CH;
+                const T *q = src + i * E + r * p.ld;
+                Word *d = dst + r * CG + i * (E / VEC);
+#pragma unroll
+                for (int n = 0; n < ROWS / STEP; ++n, q += STEP * p.ld) {
+                    const int at = r + n * STEP;
+                    if (at < live) {
+                        const uint32_t a =
+                            (uint32_t)__cvta_generic_to_shared(d + n * STEP * CG + at / LC * L::PAD);
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(a), "l"(q) : "memory");
+                    }
+                }
+            } else if (on) {
+                for (int r = part; r < live; r += ST)
+                    stage(dst + r * CG + r / LC * L::PAD + cg, src + cg * VEC + r * p.ld, Word());
             }
-        } else if (c0 + cg * VEC < C) {
-            for (int r = part; r < live; r += ST)
-                stage(dst + r * CG + r / LC * L::PAD + cg, src + cg * VEC + r * p.ld, Word());
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    // consecutive lanes are consecutive rows
+    auto head_table = [&](int r0, int buf) {
+        for (int i = tid; i < nh * ROWS; i += NT) {
+            const int h = i / ROWS, t = i % ROWS;
+            Head k{0.0f, 0.0f, 0.0f};
+            if (r0 + t < seg1) k = head_of<T>(p, r0 + t, h0 + h);
+            float prod = k.a;
+#pragma unroll
+            for (int o = 1; o < LC; o <<= 1) {
+                const float before = shfl_up(prod, o, LC);
+                if (t % LC >= o) prod *= before;
+            }
+            tabs[buf * heads * ROWS + i] = make_float4(k.a, k.g, k.c, k.c * prod);
+            if (t % LC == LC - 1) decs[(buf * heads + h) * ST + t / LC] = prod;
         }
     };
+    const bool cached = p.n_seq <= SEQ_CACHE;
+    auto off_at = [&](int i) {
+        return cached ? s_off[i] : (int)max((int64_t)0, min((int64_t)p.rows, p.off[i]));
+    };
+    // slot << 4 | fresh << 2, or -1
+    auto load_info = [&](int s) {
+        const int slot = p.slots ? p.slots[s] : s;
+        const int fresh = p.fresh ? p.fresh[s] != 0 : 1;
+        return slot >= 0 && slot < p.l.n_slots ? slot << 4 | fresh << 2 : -1;
+    };
+    // What the rows of a tile are, a thread a row.  row_info: slot << 4 | began
+    // before the segment << 3 | fresh << 2 | place in the sequence (3 and
+    // above: 3), or -1 for a row of no sequence; the masks have a bit per row.
+    auto describe_rows = [&](int r0) {
+        if (tid >= ROWS) return;
+        const int r = r0 + tid;
+        int lo = 0, hi = p.n_seq + 1;  // the offsets <= r
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (off_at(mid) <= r) lo = mid + 1;
+            else hi = mid;
+        }
+        const int sid = lo - 1;
+        int info = -1, o0 = 0, o1 = 0;
+        if (r < seg1 && sid >= 0 && sid < p.n_seq) {
+            info = cached ? s_info[sid] : load_info(sid);
+            o0 = off_at(sid);
+            o1 = off_at(sid + 1);
+            if (info >= 0) info |= (o0 < seg0 ? 8 : 0) | max(0, min(3, r - o0));
+        }
+        const unsigned all = 0xffffffffu;
+        const unsigned mv = __ballot_sync(all, info >= 0), ms = __ballot_sync(all, info >= 0 && r == o0),
+                       me = __ballot_sync(all, info >= 0 && r == o1 - 1);
+        row_info[tid] = info;
+        if (lane == 0) {
+            row_valid[tid / 32] = mv;
+            row_start[tid / 32] = ms;
+            row_end[tid / 32] = me;
+        }
+        if (tid == ROWS - 1) {
+            last_begin = o0;
+            last_end = o1;
+            last_info = info;
+        }
+    };
+
+    // ---- before the first tile
+    if (cached) {
+        for (int i = tid; i <= p.n_seq; i += NT) {
+            s_off[i] = (int)max((int64_t)0, min((int64_t)p.rows, p.off[i]));
+            if (i < p.n_seq) s_info[i] = load_info(i);
+        }
+    }
+    if (seg0 < seg1) stage_in(seg0, 0);
     V w0, w1, w2, w3, bias, dd;
-    Raw<T, VEC> above[3];
-    auto load_weights = [&](int item) {
-        const int tile = item / n_cb, ch = item % n_cb * (CG * VEC) + cg * VEC;
-        const int64_t r0 = (int64_t)tile * ROWS;
-        const bool on = ch < C;
+    {
         float4 a = make_float4(0, 0, 0, 0), b = a;
         if (on) {
             a = reinterpret_cast<const float4 *>(p.l.conv_w)[ch];
@@ -407,189 +371,137 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
         vset(w3, a.w, b.w);
         vset(bias, on ? p.l.conv_b[ch] : 0.0f, on ? p.l.conv_b[ch + VEC - 1] : 0.0f);
         vset(dd, on ? p.l.d[ch] : 0.0f, on ? p.l.d[ch + VEC - 1] : 0.0f);
+    }
+    if (part == 0) {  // the three rows above
 #pragma unroll
-        for (int k = 0; k < 3; ++k) {  // the three rows above the tile
-            above[k].zero();
-            if (on && part == 0 && r0 > k && r0 - 1 - k < p.rows)
-                above[k].v = *reinterpret_cast<const Word *>(static_cast<const T *>(p.x) + ch + (r0 - 1 - k) * p.ld);
+        for (int k = 0; k < 3; ++k) {
+            R r;
+            r.zero();
+            if (on && seg0 > k && seg0 < seg1)
+                r.v = *reinterpret_cast<const Word *>(static_cast<const T *>(p.x) + ch + (seg0 - 1 - k) * p.ld);
+            halo[k][cg] = r.get();
         }
-    };
-    auto count = [&](int item, int buf, int warp) {  // warps 1 and 2
-        const int64_t r0 = (int64_t)(item / n_cb) * ROWS;
-        const int64_t r = warp == 1 ? r0 : min((int64_t)p.rows, r0 + ROWS) - 1;
-        const int n = count_offsets(p.off, p.n_seq + 1, r, lane);
-        if (lane == 0) (warp == 1 ? rows_[buf].first : rows_[buf].last) = n;
-    };
-    // entries i, i + step, ...: consecutive lanes are consecutive rows
-    auto head_table = [&](int item, int buf, int i0, int step) {
-        const int tile = item / n_cb, c0 = item % n_cb * (CG * VEC);
-        const int64_t r0 = (int64_t)tile * ROWS;
-        const int h0 = c0 / P, nh = (min(c0 + CG * VEC, C) - 1) / P - h0 + 1;
-        float4 *tab = tabs + buf * max_heads * ROWS * 2;
-        float *dec = decs + buf * max_heads * ST;
-        for (int i = i0; i < nh * ROWS; i += step) {
-            const int h = i / ROWS, t = i % ROWS;
-            Head k{0.0f, 0.0f, 0.0f};
-            if (r0 + t < p.rows) k = head_of<T>(p, r0 + t, h0 + h);
-            float prod = k.a;
-#pragma unroll
-            for (int o = 1; o < LC; o <<= 1) {
-                const float before = __shfl_up_sync(0xffffffffu, prod, o, LC);
-                if (t % LC >= o) prod *= before;
-            }
-            tab[i * 2] = make_float4(k.a, k.a, k.g, k.g);
-            tab[i * 2 + 1] = make_float4(k.c, k.c, k.c * prod, k.c * prod);
-            if (t % LC == LC - 1) dec[h * ST + t / LC] = prod;
+    }
+    // the scan's view of the threads: a lane a part
+    const int sp = tid % ST, sc = tid / ST, sch = c0 + sc * VEC;
+    V carry;  // the state that comes into the tile, for channels sch
+    vset(carry, 0.0f, 0.0f);
+    float all = 1.0f;  // (SUMS) the decays of the segment so far
+    if (!SUMS && sch < C) {
+        for (int j = 0; j < seg; ++j) {
+            const float *S = g.S + (int64_t)j * C + sch;
+            V v;
+            vset(v, S[0], S[VEC - 1]);
+            carry = through(g.A[(int64_t)j * p.l.H + sch / P], carry, v);
         }
+    }
+    head_table(seg0, 0);
+    __syncthreads();
+    describe_rows(seg0);
+
+    auto conv_at = [&](int slot, int j) {
+        return static_cast<T *>(p.l.conv) + ((int64_t)slot * 3 + j) * C + ch;
     };
-    auto describe_rows = [&](int item, int buf) {
-        const int64_t r0 = (int64_t)(item / n_cb) * ROWS;
-        Rows<ROWS> &rows = rows_[buf];
-        for (int i = tid; i < (ROWS + NT - 1) / NT * NT; i += NT) {
-            const int64_t r = r0 + i;
-            // the offsets <= r, of which the tile has only a few
-            int lo = rows.first, hi = max(rows.first, rows.last);
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (p.off[mid] <= r) lo = mid + 1;
-                else hi = mid;
-            }
-            const int sid = lo - 1;
-            int info = -1;
-            bool first = false, last = false;
-            if (i < ROWS && r < p.rows && sid >= 0 && sid < p.n_seq) {
-                const int slot = p.slots ? p.slots[sid] : sid;
-                if (slot >= 0 && slot < p.l.n_slots) {
-                    const int64_t o0 = max((int64_t)0, p.off[sid]), o1 = min(p.off[sid + 1], (int64_t)p.rows);
-                    const int fresh = p.fresh ? p.fresh[sid] != 0 : 1;
-                    info = slot << 3 | fresh << 2 | (int)max((int64_t)0, min((int64_t)3, r - o0));
-                    first = r == o0;
-                    last = r == o1 - 1;
-                }
-            }
-            const unsigned mv = __ballot_sync(0xffffffffu, info >= 0), ms = __ballot_sync(0xffffffffu, first),
-                           me = __ballot_sync(0xffffffffu, last);
-            if (i < ROWS) {
-                rows.info[i] = info;
-                if (lane == 0) {
-                    rows.valid[i / 32] = mv;
-                    rows.start[i / 32] = ms;
-                    rows.end[i / 32] = me;
-                }
-            }
-        }
+    auto back = [&](int k, int place, int info) {
+        // the input k tokens before a token at `place` < k of its sequence
+        R r;
+        r.zero();
+        if (on && !(info & 4)) r.v = *reinterpret_cast<const Word *>(conv_at(info >> 4, 3 + place - k));
+        return r.get();
+    };
+    auto keep = [&](int slot, V a, V b, V c, V s) {
+        if (!on || SUMS) return;
+        put(conv_at(slot, 0), a);
+        put(conv_at(slot, 1), b);
+        put(conv_at(slot, 2), c);
+        put(p.l.h + (int64_t)slot * C + ch, s);
     };
 
-    if (tid == 0) {
-        s_epoch = *reinterpret_cast<volatile unsigned *>(&ctl->epoch) + 1;
-        s_next = (int)atomicAdd(&ctl->ticket, 1u);
-    }
-    __syncthreads();
-    const unsigned epoch = s_epoch, tag = 2 * epoch;
-    int item = s_next, buf = 0;
-    if (item < n_items) {
-        stage_in(item, p.x, sx);
-        stage_commit();
-        if (p.z) stage_in(item, p.z, sz);
-        stage_commit();
-        load_weights(item);
-        if (tid >= 32 && tid < 96) count(item, 0, tid / 32);
-        head_table(item, 0, tid, NT);
+    bool plain = false;
+    int left_slot = -1;  // the slot of a state left to the third launch
+    int buf = 0;
+    for (int r0 = seg0; r0 < seg1; r0 += ROWS, buf ^= 1) {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
         __syncthreads();
-        describe_rows(item, 0);
-    }
-    while (item < n_items) {
-        stage_wait<1>();  // x; the gates may still be on their way
-        __syncthreads();
-        if (tid == 0) s_next = (int)atomicAdd(&ctl->ticket, 1u);
-        const int tile = item / n_cb, cb = item % n_cb;
-        const int64_t r0 = (int64_t)tile * ROWS;
-        const int c0 = cb * CG * VEC, ch = c0 + cg * VEC;
-        const bool on = ch < C;
-        const Rows<ROWS> &rows = rows_[buf];
-        const unsigned valid = rows.valid[b0 / 32] >> b0 % 32 & mask, start = rows.start[b0 / 32] >> b0 % 32 & mask,
-                       end = rows.end[b0 / 32] >> b0 % 32 & mask;
-        const int *info = rows.info + b0;
-        const int head = (on ? ch : c0) / P, hh = head - c0 / P;
-        const float4 *tb = tabs + ((buf * max_heads + hh) * ROWS + b0) * 2;
-        const Word *xw = sx + b0 * CG + part * L::PAD + cg, *zw = sz + b0 * CG + part * L::PAD + cg;
+        const int r1 = r0 + ROWS;
+        if (r1 < seg1) stage_in(r1, buf ^ 1);
+        unsigned valid = mask, start = 0, end = 0;
+        if (!plain) {
+            valid = row_valid[b0 / 32] >> b0 % 32 & mask;
+            start = row_start[b0 / 32] >> b0 % 32 & mask;
+            end = row_end[b0 / 32] >> b0 % 32 & mask;
+        }
+        const int *info = row_info + b0;
+        const float4 *tb = tabs + (buf * heads + hh) * ROWS + b0;
+        const Word *xw = staged + 2 * buf * L::WORDS + b0 * CG + part * L::PAD + cg, *zw = xw + L::WORDS;
 
         // x1, x2, x3: the inputs 1, 2, 3 tokens back; from the slot before the
         // sequence's first
-        auto conv_at = [&](int slot, int j) {
-            return static_cast<T *>(p.l.conv) + ((int64_t)slot * 3 + j) * C + ch;
-        };
-        auto back = [&](int k, int place, int t) {
-            // the input k tokens before a token at `place` < k of its sequence
-            Raw<T, VEC> r;
-            r.zero();
-            if (on && !(info[t] & 4)) r.v = *reinterpret_cast<const Word *>(conv_at(info[t] >> 3, 3 + place - k));
-            return r.get();
-        };
-        auto keep = [&](int slot, V a, V b, V c, V s) {
-            if (!on) return;
-            put(conv_at(slot, 0), a);
-            put(conv_at(slot, 1), b);
-            put(conv_at(slot, 2), c);
-            put(p.l.h + (int64_t)slot * C + ch, s);
-        };
-        if (part > 0) {
-#pragma unroll
-            for (int k = 0; k < 3; ++k) above[k].v = xw[-(k + 1) * CG - L::PAD];
-        }
-        V x1 = above[0].get(), x2 = above[1].get(), x3 = above[2].get();
-        if ((valid & 1u) && !(start & 1u)) {
-            const int place = info[0] & 3;
-            if (place < 3) x3 = back(3, place, 0);
-            if (place < 2) x2 = back(2, place, 0);
+        V x1, x2, x3;
+        if (part == 0) {
+            x1 = halo[0][cg];
+            x2 = halo[1][cg];
+            x3 = halo[2][cg];
+        } else {
+            R r;
+            r.v = xw[-CG - L::PAD];
+            x1 = r.get();
+            r.v = xw[-2 * CG - L::PAD];
+            x2 = r.get();
+            r.v = xw[-3 * CG - L::PAD];
+            x3 = r.get();
         }
         V h, y[LC];
         vset(h, 0.0f, 0.0f);
         // the end of the sequence that came in from the part before
         float Ae = 0.0f;
         V he = h, e1 = h, e2 = h, e3 = h;
-        int end_slot = -1;
+        int end_info = -1;
         auto token = [&](int t) {
-            const float4 k0 = tb[t * 2], k1 = tb[t * 2 + 1];
-            V a, g, c;
-            vset(a, k0.x, k0.y);
-            vset(g, k0.z, k0.w);
-            vset(c, k1.x, k1.y);
-            Raw<T, VEC> xr;
+            const float4 k = tb[t];
+            V a, gg, c;
+            vset(a, k.x, k.x);
+            vset(gg, k.y, k.y);
+            vset(c, k.z, k.z);
+            R xr;
             xr.v = xw[t * CG];
             const V xt = xr.get();
             const V u = silu(vfma(w3, xt, vfma(w2, x1, vfma(w1, x2, vfma(w0, x3, bias)))));
-            h = vfma(a, h, vmul(g, u));
-            y[t] = vfma(c, h, vmul(dd, u));
+            h = vfma(a, h, vmul(gg, u));
+            if (!SUMS) y[t] = vfma(c, h, vmul(dd, u));
             x3 = x2;
             x2 = x1;
             x1 = xt;
-            return k0.x;
+            return k.x;
         };
-        if (valid == mask && !start && !end) {
+        if (valid == mask && !start && !end && (plain || (info[0] & 3) == 3)) {
 #pragma unroll
             for (int t = 0; t < LC; ++t) token(t);
         } else {
+            if ((valid & 1u) && !(start & 1u)) {
+                const int place = info[0] & 3;
+                if (place < 3) x3 = back(3, place, info[0]);
+                if (place < 2) x2 = back(2, place, info[0]);
+            }
             float A = 1.0f;
 #pragma unroll
             for (int t = 0; t < LC; ++t) {
                 if (start >> t & 1u) {
-                    x1 = back(1, 0, t);
-                    x2 = back(2, 0, t);
-                    x3 = back(3, 0, t);
-                    const float *hs = p.l.h + (int64_t)(info[t] >> 3) * C + ch;
+                    x1 = back(1, 0, info[t]);
+                    x2 = back(2, 0, info[t]);
+                    x3 = back(3, 0, info[t]);
+                    const float *hs = p.l.h + (int64_t)(info[t] >> 4) * C + ch;
                     const bool from = on && !(info[t] & 4);
                     vset(h, from ? hs[0] : 0.0f, from ? hs[VEC - 1] : 0.0f);
                 }
                 A *= token(t);
                 if (end >> t & 1u) {
                     if (start & ((2u << t) - 1u)) {
-                        keep(info[t] >> 3, x3, x2, x1, h);
+                        keep(info[t] >> 4, x3, x2, x1, h);
                     } else {
-                        // completed and written below, when the state that came
-                        // in is known: whoever starts from the slot has read it
-                        // by then
-                        end_slot = info[t] >> 3;
+                        // completed and written below, when the state that
+                        // came in is known
+                        end_info = info[t];
                         Ae = A;
                         he = h;
                         e1 = x1;
@@ -599,88 +511,76 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
                 }
             }
         }
-        // the parts' S and A; with a start in a part its S is the state itself
         part_s[part][cg] = h;
-        part_a[part][cg] = start ? SET : decs[(buf * max_heads + hh) * ST + part];
-        auto pass = [&](int i, V s) {  // the state through part i
-            const float a = part_a[i][cg];
-            const V local = part_s[i][cg];
-            V aa;
-            vset(aa, a, a);
-            const V r = vfma(aa, s, local);
-            return a == SET ? local : r;
-        };
+        part_a[part][cg] = start ? SET : decs[(buf * heads + hh) * ST + part];
+        if (r1 < seg1) head_table(r1, buf ^ 1);
         __syncthreads();
-
-        // the next item on its way; part 0 joins the parts and looks back
-        const int next = s_next;
-        const bool more = next < n_items;
-        if (more) {
-            stage_in(next, p.x, sx);
-            load_weights(next);
+        if (part == ST - 1) {
+            halo[0][cg] = x1;
+            halo[1][cg] = x2;
+            halo[2][cg] = x3;
         }
-        stage_commit();
-        if (tid < 32) {
-            if (part == 0) {
-                // Every tile but the last publishes, whatever its rows are, so
-                // that offsets that contradict each other make no tile wait
-                // for a word that never comes.
-                const bool need_in = tile > 0 && (valid & 1u) && !(start & 1u);
-                const bool need_out = r0 + ROWS < p.rows;
-                Word64 *own = words + (int64_t)tile * C + ch, *dec = decays + (int64_t)tile * p.l.H + head;
-                float all = 1.0f;
-                V S, hin;
-                vset(S, 0.0f, 0.0f);
-                vset(hin, 0.0f, 0.0f);
-                bool is_final = !need_in;
-                if (need_out) {
-#pragma unroll 4
-                    for (int i = 0; i < ST; ++i) {
-                        S = pass(i, S);
-                        is_final |= part_a[i][cg] == SET;
-                        all *= part_a[i][cg];
-                    }
-                    if (on) {
-                        store_words(own, is_final ? tag + 1 : tag, S);
-                        // one thread a head (or more, with the same value)
-                        if (!is_final && (tid == 0 || ch % P < VEC)) store_words(dec, tag, all);
-                    }
+        {
+            float a = part_a[sp][sc];
+            V S = part_s[sp][sc];
+#pragma unroll
+            for (int o = 1; o < ST; o <<= 1) {
+                const float a1 = shfl_up(a, o, ST);
+                const V S1 = shfl_up(S, o, ST);
+                if (sp >= o) {
+                    S = through(a, S1, S);
+                    a = through(a1, a);
                 }
-                if (need_in && on && !look_back(own, C, dec, p.l.H, tile, tag, hin)) atomicOr(err, 8);
-                if (need_out && !is_final && on) {
-                    V aa;
-                    vset(aa, all, all);
-                    store_words(own, tag + 1, vfma(aa, hin, S));
-                }
-                came[cg] = hin;
             }
-            __syncwarp();
-        } else if (more) {
-            if (tid < 96) count(next, buf ^ 1, tid / 32);
-            head_table(next, buf ^ 1, tid - 32, NT - 32);
+            const float a1 = shfl_up(a, 1, ST), an = shfl_at(a, ST - 1, ST);
+            const V S1 = shfl_up(S, 1, ST), Sn = shfl_at(S, ST - 1, ST);
+            came[sp][sc] = sp == 0 ? carry : through(a1, carry, S1);
+            carry = through(an, carry, Sn);
+            all = through(all, an);
         }
-        stage_wait<1>();  // z
+        // the next tile's rows: inside the sequence of this tile's last row,
+        // nothing has to be looked up
+        if (r1 < seg1) {
+            const bool same = (plain || (row_info[ROWS - 1] >= 0 && last_info >= 0)) && r1 >= last_begin + 3 &&
+                              r1 + ROWS < last_end && r1 + ROWS <= seg1;
+            if (!same) {
+                __syncthreads();  // every thread is done with this tile's rows
+                describe_rows(r1);
+            }
+            plain = same;
+        }
         __syncthreads();
-        V hin = came[cg];
-        for (int i = 0; i < part; ++i) hin = pass(i, hin);
-        if (end_slot >= 0) {
+        const V hin = came[part][cg];
+        if (!SUMS && end_info >= 0) {
             V aa;
             vset(aa, Ae, Ae);
-            keep(end_slot, e3, e2, e1, vfma(aa, hin, he));
+            const V s = vfma(aa, hin, he);
+            if (end_info & 8) {
+                left_slot = end_info >> 4;
+                if (on) {
+                    T *cv = static_cast<T *>(g.conv) + (int64_t)seg * 3 * C + ch;
+                    put(cv, e3);
+                    put(cv + C, e2);
+                    put(cv + 2 * C, e1);
+                    put(g.h + (int64_t)seg * C + ch, s);
+                }
+            } else {
+                keep(end_info >> 4, e3, e2, e1, s);
+            }
         }
-        if (on) {
+        if (!SUMS && on) {
             const int first = start ? __ffs(start) - 1 : LC;
             T *py = static_cast<T *>(p.y) + ch + (r0 + b0) * p.ldy;
             auto finish = [&](int t, bool fix) {
                 V o = y[t];
                 if (fix) {
-                    const float2 q2 = *reinterpret_cast<const float2 *>(&tb[t * 2 + 1].z);
-                    V q;
-                    vset(q, q2.x, q2.y);
-                    o = vfma(q, hin, o);
+                    const float q = tb[t].w;
+                    V qq;
+                    vset(qq, q, q);
+                    o = vfma(qq, hin, o);
                 }
-                if (p.z) {
-                    Raw<T, VEC> zr;
+                if (gate) {
+                    R zr;
                     zr.v = zw[t * CG];
                     o = vmul(o, silu(zr.get()));
                 }
@@ -695,51 +595,64 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
                     if (valid >> t & 1u) finish(t, t < first);
             }
         }
-        // sequences without tokens that start afresh: a zero state
-        if (tile == 0) {
-            __shared__ int empty[NT], n_empty;
-            for (int s0 = 0; s0 < p.n_seq; s0 += NT) {
-                const int s = s0 + tid;
-                int slot = -1;
-                if (s < p.n_seq && !(p.fresh && p.fresh[s] == 0) &&
-                    max((int64_t)0, p.off[s]) >= min((int64_t)p.rows, p.off[s + 1])) {
-                    slot = p.slots ? p.slots[s] : s;
-                    if (slot >= p.l.n_slots) slot = -1;
-                }
-                if (!__syncthreads_or(slot >= 0)) continue;
-                if (tid == 0) n_empty = 0;
-                __syncthreads();
-                if (slot >= 0) empty[atomicAdd(&n_empty, 1)] = slot;
-                __syncthreads();
-                V none;
-                vset(none, 0.0f, 0.0f);
-                for (int i = part; i < n_empty; i += ST) keep(empty[i], none, none, none, none);
-                __syncthreads();
+    }
+    if (SUMS) {
+        if (sp == 0 && sch < C) {
+            float *S = g.S + (int64_t)seg * C + sch;
+            S[0] = lane0(carry);
+            S[VEC - 1] = lane1(carry);
+            // (threads of the same head, and CTAs, write the same value)
+            g.A[(int64_t)seg * p.l.H + sch / P] = all;
+        }
+        return;
+    }
+    if (g.n > 1) {
+        const int left = __syncthreads_or(left_slot + 1) ? 1 : 0;
+        if (tid == 0) list[0] = -1;
+        __syncthreads();
+        if (left && left_slot >= 0) list[0] = left_slot;  // (one sequence: one slot)
+        __syncthreads();
+        if (tid == 0) g.slot[seg * gridDim.x + blockIdx.x] = list[0];
+    }
+    // sequences without tokens that start afresh: a zero state
+    if (seg == 0) {
+        for (int s0 = 0; s0 < p.n_seq; s0 += NT) {
+            const int s = s0 + tid;
+            int slot = -1;
+            if (s < p.n_seq && off_at(s) >= off_at(s + 1)) {
+                const int i = cached ? s_info[s] : load_info(s);
+                if (i >= 0 && (i & 4)) slot = i >> 4;
             }
-        }
-        if (more) describe_rows(next, buf ^ 1);
-        __syncthreads();  // z and the parts are free
-        if (more && p.z) stage_in(next, p.z, sz);
-        stage_commit();
-        item = next;
-        buf ^= 1;
-    }
-    if (tid == 0) {
-        __threadfence();
-        if (atomicAdd(&ctl->done, 1u) == gridDim.x - 1) {
-            ctl->ticket = 0;
-            ctl->done = 0;
-            __threadfence();
-            ctl->epoch = epoch;
+            if (!__syncthreads_or(slot >= 0)) continue;
+            if (tid == 0) n_list = 0;
+            __syncthreads();
+            if (slot >= 0) list[atomicAdd(&n_list, 1)] = slot;
+            __syncthreads();
+            V none;
+            vset(none, 0.0f, 0.0f);
+            for (int i = part; i < n_list; i += ST) keep(list[i], none, none, none, none);
+            __syncthreads();
         }
     }
+}
+
+// The third launch: states that segments left, to their slots.
+template <typename T>
+__global__ void __launch_bounds__(128) left_kernel(const Layer l, const Segments g, int channels, int n_cb) {
+    const int ch = blockIdx.x * 128 + threadIdx.x, seg = blockIdx.y;
+    if (ch >= l.C) return;
+    const int slot = g.slot[seg * n_cb + ch / channels];
+    if (slot < 0) return;
+    const T *from = static_cast<const T *>(g.conv) + (int64_t)seg * 3 * l.C + ch;
+    T *to = static_cast<T *>(l.conv) + (int64_t)slot * 3 * l.C + ch;
+    for (int k = 0; k < 3; ++k) to[k * l.C] = from[k * l.C];
+    l.h[(int64_t)slot * l.C + ch] = g.h[(int64_t)seg * l.C + ch];
 }
 
 struct Launch {
     Args a;
     bm_ctx_t *ctx;
     int sms;
-    int *err;
     cudaStream_t s;
 };
 
@@ -747,30 +660,45 @@ template <typename T, int VEC, int CG, int ST, int LC, int PER_SM>
 int launch_prefill(const Launch &l) {
     using L = Tile<T, VEC, CG, ST, LC>;
     const Args &a = l.a;
-    const int C = a.l.C, P = a.l.P;
+    const int C = a.l.C, P = a.l.P, H = a.l.H;
     const int n_cb = (C + CG * VEC - 1) / (CG * VEC);
-    const int64_t tiles = a.rows > 0 ? ((int64_t)a.rows + L::ROWS - 1) / L::ROWS : 1;
-    const int64_t items = tiles * n_cb;
-    if (items > INT32_MAX / 2)
-        return bm_detail_fail(BM_ERR_UNSUPPORTED, "rows * channels too large for one call");
-    // a word per tile and channel, then one per tile and head
-    const size_t n_words = ((size_t)tiles * C + 1) / 2 * 2;
-    void *work;
-    const int rc = bm_detail_work(l.ctx, BM_WORK_SCAN,
-                                  CONTROL_BYTES + (n_words + (size_t)tiles * a.l.H) * sizeof(Word64), &work);
-    if (rc != BM_OK) return rc;
-    Word64 *words = reinterpret_cast<Word64 *>(static_cast<unsigned char *>(work) + CONTROL_BYTES);
-    const int heads = min((CG * VEC + P - 2) / P + 1, a.l.H);
-    auto *k = prefill_kernel<T, VEC, CG, ST, LC, PER_SM>;
-    constexpr int most = 200 * 1024;
+    const int tiles = a.rows > 0 ? (int)(((int64_t)a.rows + L::ROWS - 1) / L::ROWS) : 1;
+    // segments for SMs that would be idle, of at least two tiles each
+    int segs = l.sms * PER_SM / n_cb;
+    if (segs > tiles / 2) segs = tiles / 2;
+    if (segs > 64) segs = 64;
+    if (segs < 1) segs = 1;
+    Segments g{};
+    g.rows = (tiles + segs - 1) / segs * L::ROWS;
+    g.n = segs = (int)(((int64_t)tiles * L::ROWS + g.rows - 1) / g.rows);
+    if (segs > 1) {
+        void *work;
+        const size_t words = (size_t)segs * ((size_t)2 * C + H + 3 * C + n_cb);
+        const int rc = bm_detail_work(l.ctx, BM_WORK_SCAN, words * 4 + 64, &work);
+        if (rc != BM_OK) return rc;
+        g.S = static_cast<float *>(work);
+        g.h = g.S + (size_t)segs * C;
+        g.conv = g.h + (size_t)segs * C;
+        g.A = g.h + (size_t)segs * 4 * C;
+        g.slot = reinterpret_cast<int *>(g.A + (size_t)segs * H);
+    }
+    int heads = (CG * VEC + P - 2) / P + 1;
+    if (heads > H) heads = H;
     const size_t bytes = L::STAGED + (size_t)heads * L::PER_HEAD;
+    constexpr int most = 202 * 1024;
     if (bytes > most) return bm_detail_fail(BM_ERR_UNSUPPORTED, "too many heads in a tile");
-    BMC_CK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
     auto even = [&](const void *q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; };
     const int wide = C % (CG * VEC) == 0 && even(a.x) && even(a.z) && a.ld * (int64_t)sizeof(T) % 16 == 0;
-    const int64_t grid = items < (int64_t)PER_SM * l.sms ? items : (int64_t)PER_SM * l.sms;
-    k<<<(int)grid, L::NT, bytes, l.s>>>(a, static_cast<Control *>(work), words, words + n_words, n_cb,
-                                        (int)items, heads, wide, l.err);
+    auto *main = prefill_kernel<T, VEC, CG, ST, LC, PER_SM, false>;
+    BMC_CK(cudaFuncSetAttribute(main, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+    if (segs > 1) {
+        auto *sums = prefill_kernel<T, VEC, CG, ST, LC, PER_SM, true>;
+        BMC_CK(cudaFuncSetAttribute(sums, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+        sums<<<dim3((unsigned)n_cb, (unsigned)segs - 1), L::NT, bytes, l.s>>>(a, g, heads, wide);
+    }
+    main<<<dim3((unsigned)n_cb, (unsigned)segs), L::NT, bytes, l.s>>>(a, g, heads, wide);
+    if (segs > 1)
+        left_kernel<T><<<dim3((unsigned)(C + 127) / 128, (unsigned)segs), 128, 0, l.s>>>(a.l, g, CG * VEC, n_cb);
     BMC_CK(cudaGetLastError());
     return BM_OK;
 }
@@ -878,23 +806,23 @@ int bm_ssm_prefill(bm_ctx_t *ctx, const bm_ssm_layer_t *layer, const void *d_x, 
                        !misaligned(d_x, 2 * e) && !misaligned(d_z, 2 * e) &&
                        !misaligned(d_y, 2 * e) && !misaligned(layer->conv_state, 2 * e) &&
                        !misaligned(layer->h_state, 8);
+    if (layer->n_slots > (1 << 27)) return bm_detail_fail(BM_ERR_UNSUPPORTED, "n_slots > 2^27");
+    if (rows > INT32_MAX - 65536) return bm_detail_fail(BM_ERR_UNSUPPORTED, "rows > 2^31 - 65537");
     Launch l{};
     l.ctx = ctx;
-    bmc::DeviceGuard guard(bm_detail_ctx(ctx, &l.sms, &l.err, &l.s));
+    int *err;
+    bmc::DeviceGuard guard(bm_detail_ctx(ctx, &l.sms, &err, &l.s));
     BMC_CK(guard.error);
     if (stream) l.s = static_cast<cudaStream_t>(stream);
     l.a = a;
-    // Tall tiles unless that leaves SMs without work.  One channel a thread,
-    // in small tiles, for what cannot be paired and for heads so small that
-    // their scalars would fill the shared memory.
+    // Small tiles for few rows.  One channel a thread for what cannot be paired
+    // and for heads so small that the scalars of a tall tile's rows would not
+    // fit the shared memory.
     using bf16 = __nv_bfloat16;
-    const bool few = ((int64_t)rows + 255) / 256 * ((a.l.C + 31) / 32) < 2 * l.sms;
-    if (layer->type == BM_F32) {
-        if (!pairs) return launch_prefill<float, 1, 32, 4, 8, 4>(l);
-        return few ? launch_prefill<float, 2, 16, 8, 8, 4>(l) : launch_prefill<float, 2, 16, 8, 16, 4>(l);
-    }
-    if (!pairs) return launch_prefill<bf16, 1, 32, 4, 8, 4>(l);
-    return few ? launch_prefill<bf16, 2, 16, 8, 8, 4>(l) : launch_prefill<bf16, 2, 16, 16, 16, 2>(l);
+    const bool f32 = layer->type == BM_F32;
+    if (!pairs) return f32 ? launch_prefill<float, 1, 32, 16, 8, 1>(l) : launch_prefill<bf16, 1, 32, 16, 8, 1>(l);
+    if (rows <= 64) return f32 ? launch_prefill<float, 2, 16, 8, 8, 4>(l) : launch_prefill<bf16, 2, 16, 8, 8, 4>(l);
+    return f32 ? launch_prefill<float, 2, 16, 32, 8, 1>(l) : launch_prefill<bf16, 2, 16, 32, 16, 1>(l);
 }
 
 int bm_ssm_step(bm_ctx_t *ctx, const bm_ssm_layer_t *layer, const void *d_x, const void *d_z,
