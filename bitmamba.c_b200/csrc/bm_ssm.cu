@@ -9,6 +9,7 @@
 // and 1 ulp) are not multiplied up.
 #include <climits>
 #include <cstdint>
+#include <cstdlib>
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -37,6 +38,7 @@ struct Args {
     const int64_t *off;
     int n_seq;
     const int32_t *fresh;
+    const float4 *tab;  // the head scalars of all rows (heads_kernel)
 };
 
 __device__ __forceinline__ float to_f(float v) { return v; }
@@ -66,6 +68,13 @@ __device__ __forceinline__ float vfma(float a, float b, float c) { return fmaf(a
 __device__ __forceinline__ float2 vfma(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
 __device__ __forceinline__ float vmul(float a, float b) { return a * b; }
 __device__ __forceinline__ float2 vmul(float2 a, float2 b) { return __fmul2_rn(a, b); }
+// a scalar with a pair: plain instructions, the packed ones would want it twice
+__device__ __forceinline__ float sfma(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ float2 sfma(float a, float2 b, float2 c) {
+    return make_float2(fmaf(a, b.x, c.x), fmaf(a, b.y, c.y));
+}
+__device__ __forceinline__ float smul(float a, float b) { return a * b; }
+__device__ __forceinline__ float2 smul(float a, float2 b) { return make_float2(a * b.x, a * b.y); }
 __device__ __forceinline__ float vadd(float a, float b) { return a + b; }
 __device__ __forceinline__ float2 vadd(float2 a, float2 b) { return __fadd2_rn(a, b); }
 __device__ __forceinline__ void vset(float &v, float a, float) { v = a; }
@@ -103,15 +112,19 @@ __device__ __forceinline__ float softplus(float v) {
 struct Head {
     float a, g, c;
 };
+__device__ __forceinline__ Head head_of(float dt, float rate, float b, float c) {
+    const float d = softplus(dt);
+    Head r;
+    r.a = expf(-rate * d);
+    r.g = d * b;
+    r.c = c;
+    return r;
+}
 template <typename T>
 __device__ __forceinline__ Head head_of(const Args &p, int64_t row, int h) {
     const int64_t at = row * p.ld + h;
-    const float d = softplus(to_f(static_cast<const T *>(p.dt)[at]) + p.l.dt_bias[h]);
-    Head r;
-    r.a = expf(-expf(p.l.a_log[h]) * d);
-    r.g = d * to_f(static_cast<const T *>(p.b)[at]);
-    r.c = to_f(static_cast<const T *>(p.c)[at]);
-    return r;
+    return head_of(to_f(static_cast<const T *>(p.dt)[at]) + p.l.dt_bias[h], expf(p.l.a_log[h]),
+                   to_f(static_cast<const T *>(p.b)[at]), to_f(static_cast<const T *>(p.c)[at]));
 }
 
 // ---------------------------------------------------------------- prompts --
@@ -227,13 +240,40 @@ struct Tile {
     static constexpr int WORDS = ROWS * CG + ST * PAD;
     // x and z, twice
     static constexpr size_t STAGED = 4 * (size_t)WORDS * VEC * sizeof(T);
-    // a head's scalars (a, g, c, C times the part's decays so far) and its
-    // parts' decays, twice
-    static constexpr size_t PER_HEAD = 2 * (size_t)(ROWS * 16 + ST * 4);
+    // a head's scalars (a, g, c, the part's decays up to the row), twice
+    static constexpr size_t PER_HEAD = 2 * (size_t)ROWS * 16;
 };
 
-// SUMS: only the segment's (A, S).
-template <typename T, int VEC, int CG, int ST, int LC, int PER_SM, bool SUMS>
+// The head scalars of all rows, [part of LC rows][head][LC]: a thread a head
+// and part.  Each head's are needed by every CTA that has channels of it;
+// worked out by each of them they took a third of a long prompt's instructions.
+template <typename T, int LC>
+__global__ void __launch_bounds__(128) heads_kernel(const Args p, float4 *tab) {
+    const int64_t i = (int64_t)blockIdx.x * 128 + threadIdx.x;
+    const int64_t part = i / p.l.H;
+    const int h = (int)(i - part * p.l.H);
+    if (part * LC >= p.rows) return;
+    float4 *out = tab + i * LC;
+    const float bias = p.l.dt_bias[h], rate = expf(p.l.a_log[h]);
+    T dt[LC], b[LC], c[LC];
+#pragma unroll
+    for (int t = 0; t < LC; ++t) {
+        const int64_t at = min(part * LC + t, (int64_t)p.rows - 1) * p.ld + h;
+        dt[t] = static_cast<const T *>(p.dt)[at];
+        b[t] = static_cast<const T *>(p.b)[at];
+        c[t] = static_cast<const T *>(p.c)[at];
+    }
+    float prod = 1.0f;
+#pragma unroll
+    for (int t = 0; t < LC; ++t) {
+        const Head k = head_of(to_f(dt[t]) + bias, rate, to_f(b[t]), to_f(c[t]));
+        prod *= k.a;
+        out[t] = make_float4(k.a, k.g, k.c, prod);
+    }
+}
+
+// SUMS: only the segment's (A, S).  PRE: the head scalars come from p.tab.
+template <typename T, int VEC, int CG, int ST, int LC, int PER_SM, bool PRE, bool SUMS>
 __global__ void __launch_bounds__(CG *ST, PER_SM)
     prefill_kernel(const Args p, const Segments g, int heads, int wide) {
     using L = Tile<T, VEC, CG, ST, LC>;
@@ -241,7 +281,7 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
     using Word = typename R::Word;
     using V = typename Vec<VEC>::type;
     constexpr int NT = L::NT, ROWS = L::ROWS;
-    static_assert(LC <= 32 && 32 % LC == 0 && ST <= 32 && ROWS % 32 == 0 && ROWS <= NT && LC >= 3, "tile");
+    static_assert(LC <= 32 && 32 % LC == 0 && ST <= 32 && ROWS % 32 == 0 && NT % 32 == 0 && LC >= 3, "tile");
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ int s_off[SEQ_CACHE + 1], s_info[SEQ_CACHE];
     __shared__ int row_info[ROWS];
@@ -251,7 +291,6 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
     __shared__ float part_a[ST][CG + 1];
     Word *const staged = reinterpret_cast<Word *>(smem);  // x0, z0, x1, z1
     float4 *const tabs = reinterpret_cast<float4 *>(smem + L::STAGED);
-    float *const decs = reinterpret_cast<float *>(tabs + 2 * heads * ROWS);
     const int C = p.l.C, P = p.l.P, tid = threadIdx.x, lane = tid & 31;
     const int cg = tid % CG, part = tid / CG, b0 = part * LC;
     const int seg = blockIdx.y, c0 = blockIdx.x * (CG * VEC), ch = c0 + cg * VEC;
@@ -286,6 +325,17 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
                     stage(dst + r * CG + r / LC * L::PAD + cg, src + cg * VEC + r * p.ld, Word());
             }
         }
+        if (PRE) {
+            const int parts = (live + LC - 1) / LC * LC;
+            for (int i = tid; i < nh * ROWS; i += NT) {
+                const int h = i / ROWS, t = i % ROWS;
+                if (t >= parts) continue;
+                const uint32_t a = (uint32_t)__cvta_generic_to_shared(tabs + buf * heads * ROWS + i);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(a),
+                             "l"(p.tab + ((int64_t)(r0 + t) / LC * p.l.H + h0 + h) * LC + t % LC)
+                             : "memory");
+            }
+        }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     // consecutive lanes are consecutive rows
@@ -300,8 +350,7 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
                 const float before = shfl_up(prod, o, LC);
                 if (t % LC >= o) prod *= before;
             }
-            tabs[buf * heads * ROWS + i] = make_float4(k.a, k.g, k.c, k.c * prod);
-            if (t % LC == LC - 1) decs[(buf * heads + h) * ST + t / LC] = prod;
+            tabs[buf * heads * ROWS + i] = make_float4(k.a, k.g, k.c, prod);
         }
     };
     const bool cached = p.n_seq <= SEQ_CACHE;
@@ -318,35 +367,36 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
     // before the segment << 3 | fresh << 2 | place in the sequence (3 and
     // above: 3), or -1 for a row of no sequence; the masks have a bit per row.
     auto describe_rows = [&](int r0) {
-        if (tid >= ROWS) return;
-        const int r = r0 + tid;
-        int lo = 0, hi = p.n_seq + 1;  // the offsets <= r
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (off_at(mid) <= r) lo = mid + 1;
-            else hi = mid;
-        }
-        const int sid = lo - 1;
-        int info = -1, o0 = 0, o1 = 0;
-        if (r < seg1 && sid >= 0 && sid < p.n_seq) {
-            info = cached ? s_info[sid] : load_info(sid);
-            o0 = off_at(sid);
-            o1 = off_at(sid + 1);
-            if (info >= 0) info |= (o0 < seg0 ? 8 : 0) | max(0, min(3, r - o0));
-        }
-        const unsigned all = 0xffffffffu;
-        const unsigned mv = __ballot_sync(all, info >= 0), ms = __ballot_sync(all, info >= 0 && r == o0),
-                       me = __ballot_sync(all, info >= 0 && r == o1 - 1);
-        row_info[tid] = info;
-        if (lane == 0) {
-            row_valid[tid / 32] = mv;
-            row_start[tid / 32] = ms;
-            row_end[tid / 32] = me;
-        }
-        if (tid == ROWS - 1) {
-            last_begin = o0;
-            last_end = o1;
-            last_info = info;
+        for (int i = tid; i < ROWS; i += NT) {  // (whole warps)
+            const int r = r0 + i;
+            int lo = 0, hi = p.n_seq + 1;  // the offsets <= r
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (off_at(mid) <= r) lo = mid + 1;
+                else hi = mid;
+            }
+            const int sid = lo - 1;
+            int info = -1, o0 = 0, o1 = 0;
+            if (r < seg1 && sid >= 0 && sid < p.n_seq) {
+                info = cached ? s_info[sid] : load_info(sid);
+                o0 = off_at(sid);
+                o1 = off_at(sid + 1);
+                if (info >= 0) info |= (o0 < seg0 ? 8 : 0) | max(0, min(3, r - o0));
+            }
+            const unsigned all = 0xffffffffu;
+            const unsigned mv = __ballot_sync(all, info >= 0), ms = __ballot_sync(all, info >= 0 && r == o0),
+                           me = __ballot_sync(all, info >= 0 && r == o1 - 1);
+            row_info[i] = info;
+            if (lane == 0) {
+                row_valid[i / 32] = mv;
+                row_start[i / 32] = ms;
+                row_end[i / 32] = me;
+            }
+            if (i == ROWS - 1) {
+                last_begin = o0;
+                last_end = o1;
+                last_info = info;
+            }
         }
     };
 
@@ -395,7 +445,7 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
             carry = through(g.A[(int64_t)j * p.l.H + sch / P], carry, v);
         }
     }
-    head_table(seg0, 0);
+    if (!PRE) head_table(seg0, 0);
     __syncthreads();
     describe_rows(seg0);
 
@@ -459,16 +509,12 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
         int end_info = -1;
         auto token = [&](int t) {
             const float4 k = tb[t];
-            V a, gg, c;
-            vset(a, k.x, k.x);
-            vset(gg, k.y, k.y);
-            vset(c, k.z, k.z);
             R xr;
             xr.v = xw[t * CG];
             const V xt = xr.get();
             const V u = silu(vfma(w3, xt, vfma(w2, x1, vfma(w1, x2, vfma(w0, x3, bias)))));
-            h = vfma(a, h, vmul(gg, u));
-            if (!SUMS) y[t] = vfma(c, h, vmul(dd, u));
+            h = sfma(k.x, h, smul(k.y, u));
+            if (!SUMS) y[t] = sfma(k.z, h, vmul(dd, u));
             x3 = x2;
             x2 = x1;
             x1 = xt;
@@ -512,8 +558,8 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
             }
         }
         part_s[part][cg] = h;
-        part_a[part][cg] = start ? SET : decs[(buf * heads + hh) * ST + part];
-        if (r1 < seg1) head_table(r1, buf ^ 1);
+        part_a[part][cg] = start ? SET : tb[LC - 1].w;
+        if (!PRE && r1 < seg1) head_table(r1, buf ^ 1);
         __syncthreads();
         if (part == ST - 1) {
             halo[0][cg] = x1;
@@ -574,10 +620,9 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
             auto finish = [&](int t, bool fix) {
                 V o = y[t];
                 if (fix) {
-                    const float q = tb[t].w;
-                    V qq;
-                    vset(qq, q, q);
-                    o = vfma(qq, hin, o);
+                    const float2 cq = *reinterpret_cast<const float2 *>(&tb[t].z);
+                    const float q = cq.x * cq.y;
+                    o = sfma(q, hin, o);
                 }
                 if (gate) {
                     R zr;
@@ -656,10 +701,10 @@ struct Launch {
     cudaStream_t s;
 };
 
-template <typename T, int VEC, int CG, int ST, int LC, int PER_SM>
-int launch_prefill(const Launch &l) {
+template <typename T, int VEC, int CG, int ST, int LC, int PER_SM, bool PRE>
+int launch_prefill(Launch &l) {
     using L = Tile<T, VEC, CG, ST, LC>;
-    const Args &a = l.a;
+    Args &a = l.a;
     const int C = a.l.C, P = a.l.P, H = a.l.H;
     const int n_cb = (C + CG * VEC - 1) / (CG * VEC);
     const int tiles = a.rows > 0 ? (int)(((int64_t)a.rows + L::ROWS - 1) / L::ROWS) : 1;
@@ -671,16 +716,24 @@ int launch_prefill(const Launch &l) {
     Segments g{};
     g.rows = (tiles + segs - 1) / segs * L::ROWS;
     g.n = segs = (int)(((int64_t)tiles * L::ROWS + g.rows - 1) / g.rows);
-    if (segs > 1) {
+    const int64_t parts = ((int64_t)a.rows + LC - 1) / LC;
+    const size_t tab_bytes = PRE ? (size_t)parts * H * LC * sizeof(float4) : 0;
+    if (segs > 1 || PRE) {
         void *work;
-        const size_t words = (size_t)segs * ((size_t)2 * C + H + 3 * C + n_cb);
-        const int rc = bm_detail_work(l.ctx, BM_WORK_SCAN, words * 4 + 64, &work);
+        const size_t words = segs > 1 ? (size_t)segs * ((size_t)2 * C + H + 3 * C + n_cb) : 0;
+        const int rc = bm_detail_work(l.ctx, BM_WORK_SCAN, tab_bytes + words * 4, &work);
         if (rc != BM_OK) return rc;
-        g.S = static_cast<float *>(work);
+        a.tab = static_cast<const float4 *>(work);
+        g.S = reinterpret_cast<float *>(static_cast<unsigned char *>(work) + tab_bytes);
         g.h = g.S + (size_t)segs * C;
         g.conv = g.h + (size_t)segs * C;
         g.A = g.h + (size_t)segs * 4 * C;
         g.slot = reinterpret_cast<int *>(g.A + (size_t)segs * H);
+    }
+    if (PRE) {
+        const int64_t blocks = (parts * H + 127) / 128;
+        if (blocks > INT32_MAX) return bm_detail_fail(BM_ERR_UNSUPPORTED, "rows * heads too large for one call");
+        heads_kernel<T, LC><<<(unsigned)blocks, 128, 0, l.s>>>(a, const_cast<float4 *>(a.tab));
     }
     int heads = (CG * VEC + P - 2) / P + 1;
     if (heads > H) heads = H;
@@ -689,10 +742,10 @@ int launch_prefill(const Launch &l) {
     if (bytes > most) return bm_detail_fail(BM_ERR_UNSUPPORTED, "too many heads in a tile");
     auto even = [&](const void *q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; };
     const int wide = C % (CG * VEC) == 0 && even(a.x) && even(a.z) && a.ld * (int64_t)sizeof(T) % 16 == 0;
-    auto *main = prefill_kernel<T, VEC, CG, ST, LC, PER_SM, false>;
+    auto *main = prefill_kernel<T, VEC, CG, ST, LC, PER_SM, PRE, false>;
     BMC_CK(cudaFuncSetAttribute(main, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
     if (segs > 1) {
-        auto *sums = prefill_kernel<T, VEC, CG, ST, LC, PER_SM, true>;
+        auto *sums = prefill_kernel<T, VEC, CG, ST, LC, PER_SM, PRE, true>;
         BMC_CK(cudaFuncSetAttribute(sums, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
         sums<<<dim3((unsigned)n_cb, (unsigned)segs - 1), L::NT, bytes, l.s>>>(a, g, heads, wide);
     }
@@ -820,9 +873,15 @@ int bm_ssm_prefill(bm_ctx_t *ctx, const bm_ssm_layer_t *layer, const void *d_x, 
     // fit the shared memory.
     using bf16 = __nv_bfloat16;
     const bool f32 = layer->type == BM_F32;
-    if (!pairs) return f32 ? launch_prefill<float, 1, 32, 16, 8, 1>(l) : launch_prefill<bf16, 1, 32, 16, 8, 1>(l);
-    if (rows <= 64) return f32 ? launch_prefill<float, 2, 16, 8, 8, 4>(l) : launch_prefill<bf16, 2, 16, 8, 8, 4>(l);
-    return f32 ? launch_prefill<float, 2, 16, 32, 8, 1>(l) : launch_prefill<bf16, 2, 16, 32, 16, 1>(l);
+    if (!pairs)
+        return f32 ? launch_prefill<float, 1, 32, 16, 8, 1, false>(l) : launch_prefill<bf16, 1, 32, 16, 8, 1, false>(l);
+    if (rows <= 64)
+        return f32 ? launch_prefill<float, 2, 16, 8, 8, 4, false>(l) : launch_prefill<bf16, 2, 16, 8, 8, 4, false>(l);
+    static const int which = getenv("BM_T") ? atoi(getenv("BM_T")) : 0;
+    if (which == 0) return f32 ? launch_prefill<float, 2, 16, 32, 8, 1, true>(l) : launch_prefill<bf16, 2, 16, 32, 16, 1, true>(l);
+    if (which == 1) return f32 ? launch_prefill<float, 2, 8, 32, 8, 2, true>(l) : launch_prefill<bf16, 2, 8, 32, 16, 2, true>(l);
+    if (which == 2) return f32 ? launch_prefill<float, 2, 8, 32, 8, 3, true>(l) : launch_prefill<bf16, 2, 8, 32, 8, 3, true>(l);
+    return f32 ? launch_prefill<float, 2, 16, 16, 8, 2, true>(l) : launch_prefill<bf16, 2, 16, 32, 8, 1, true>(l);
 }
 
 int bm_ssm_step(bm_ctx_t *ctx, const bm_ssm_layer_t *layer, const void *d_x, const void *d_z,
