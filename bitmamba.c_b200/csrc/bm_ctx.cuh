@@ -1,7 +1,9 @@
 // What the translation units of the layer operators need of a context.  Not
 // part of the public ABI.
 #pragma once
+#include <atomic>
 #include <cstddef>
+#include <cstdint>
 #include <cstdio>
 #include <cuda_runtime.h>
 
@@ -38,6 +40,21 @@ struct DeviceGuard {
     }
     ~DeviceGuard() {
         if (before >= 0 && before != now) cudaSetDevice(before);
+    }
+};
+
+// Lets a kernel take `bytes` of dynamic shared memory on a device: always the
+// same number for a kernel, so that calls of several threads agree, and set
+// once a device (the call costs as much as a launch).
+struct SharedMemory {
+    std::atomic<uint64_t> done{0};  // a bit per device, the first 64
+    cudaError_t allow(const void *kernel, int bytes, int device) {
+        const uint64_t bit = device < 64 ? 1ull << device : 0;
+        if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+        const cudaError_t e =
+            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+        return e;
     }
 };
 

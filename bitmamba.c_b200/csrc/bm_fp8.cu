@@ -342,9 +342,11 @@ cudaError_t launch_product(const uint8_t *a, const uint8_t *w, const ProductArgs
     CUtensorMap mw, ma;
     cudaError_t e = byte_map(&mw, w, p.N, p.K, BV);
     if (e == cudaSuccess) e = byte_map(&ma, a, p.M, p.K, NB);
+    int device = 0;
+    static bmc::SharedMemory shm;
+    if (e == cudaSuccess) e = cudaGetDevice(&device);
     if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(product_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 (int)S::SMEM);
+        e = shm.allow(reinterpret_cast<const void *>(product_kernel<NB>), (int)S::SMEM, device);
     if (e != cudaSuccess) return e;
     const int64_t tiles = (int64_t)((p.M + NB - 1) / NB) * ((p.N + BV - 1) / BV);
     if (tiles > INT32_MAX / 2) return cudaErrorInvalidValue;

@@ -134,10 +134,12 @@ cudaError_t reorder(const bm_slot_region_t *regions, int n_regions, const int32_
     // 64 KB of pieces (three CTAs per SM), more where that is under 16 bytes a slot
     const int room = n_slots * 16 > 65536 ? n_slots * 16 : 65536;
     const size_t bytes = ((size_t)n_slots * 4 + 15) / 16 * 16 + (size_t)room;
-    // the most that any call takes, so that calls of several threads agree
+    // the most that any call takes
     constexpr int most = BM_SLOT_MAX * 4 + BM_SLOT_MAX * 16;
-    cudaError_t e =
-        cudaFuncSetAttribute(reorder_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    int device;
+    cudaError_t e = cudaGetDevice(&device);
+    static bmc::SharedMemory shm;
+    if (e == cudaSuccess) e = shm.allow(reinterpret_cast<const void *>(reorder_kernel), most, device);
     if (e != cudaSuccess) return e;
     reorder_kernel<<<sms * 3, NT, bytes, s>>>(g, d_src, n_slots, room);
     return cudaGetLastError();

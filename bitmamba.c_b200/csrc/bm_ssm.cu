@@ -9,7 +9,6 @@
 // and 1 ulp) are not multiplied up.
 #include <climits>
 #include <cstdint>
-#include <cstdlib>
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -38,7 +37,9 @@ struct Args {
     const int64_t *off;
     int n_seq;
     const int32_t *fresh;
-    const float4 *tab;  // the head scalars of all rows (heads_kernel)
+    // the head scalars of all rows, and the parts' decays (heads_kernel)
+    const float4 *tab;
+    const float *dec;
 };
 
 __device__ __forceinline__ float to_f(float v) { return v; }
@@ -234,21 +235,22 @@ constexpr int SEQ_CACHE = 1024;  // sequences whose offsets a CTA keeps in share
 template <typename T, int VEC, int CG, int ST, int LC>
 struct Tile {
     static constexpr int NT = CG * ST, ROWS = ST * LC;
-    // words: odd parts are shifted by 16 banks, so that the two parts of a
-    // warp do not meet
-    static constexpr int PAD = CG == 16 && VEC * sizeof(T) == 4 ? 16 : 0;
+    // words: a part is shifted by CG words against the one before, so that the
+    // parts of a warp (of half a warp, for 8-byte words) meet in no bank
+    static constexpr int PAD = CG * VEC * sizeof(T) >= 128 ? 0 : CG;
     static constexpr int WORDS = ROWS * CG + ST * PAD;
     // x and z, twice
     static constexpr size_t STAGED = 4 * (size_t)WORDS * VEC * sizeof(T);
-    // a head's scalars (a, g, c, the part's decays up to the row), twice
-    static constexpr size_t PER_HEAD = 2 * (size_t)ROWS * 16;
+    // a head's scalars (a, g, c, C times the part's decays up to the row) and
+    // its parts' decays, twice
+    static constexpr size_t PER_HEAD = 2 * (size_t)(ROWS * 16 + ST * 4);
 };
 
-// The head scalars of all rows, [part of LC rows][head][LC]: a thread a head
-// and part.  Each head's are needed by every CTA that has channels of it;
+// The head scalars of all rows, [part of LC rows][head][LC], and the parts'
+// decays, [part][head]: a thread a head and part.  Each head's are needed by every CTA that has channels of it;
 // worked out by each of them they took a third of a long prompt's instructions.
 template <typename T, int LC>
-__global__ void __launch_bounds__(128) heads_kernel(const Args p, float4 *tab) {
+__global__ void __launch_bounds__(128) heads_kernel(const Args p, float4 *tab, float *dec) {
     const int64_t i = (int64_t)blockIdx.x * 128 + threadIdx.x;
     const int64_t part = i / p.l.H;
     const int h = (int)(i - part * p.l.H);
@@ -268,8 +270,9 @@ __global__ void __launch_bounds__(128) heads_kernel(const Args p, float4 *tab) {
     for (int t = 0; t < LC; ++t) {
         const Head k = head_of(to_f(dt[t]) + bias, rate, to_f(b[t]), to_f(c[t]));
         prod *= k.a;
-        out[t] = make_float4(k.a, k.g, k.c, prod);
+        out[t] = make_float4(k.a, k.g, k.c, k.c * prod);
     }
+    dec[i] = prod;
 }
 
 // SUMS: only the segment's (A, S).  PRE: the head scalars come from p.tab.
@@ -287,10 +290,15 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
     __shared__ int row_info[ROWS];
     __shared__ unsigned row_valid[ROWS / 32], row_start[ROWS / 32], row_end[ROWS / 32];
     __shared__ int last_begin, last_end, last_info, n_list, list[NT];
+    // the state and inputs that the first sequence starting in a part of the
+    // next tile takes from its slot
+    __shared__ V init_h[ST][CG];
+    __shared__ Word init_x[ST][3][CG];
     __shared__ V part_s[ST][CG + 1], came[ST][CG + 1], halo[3][CG];
     __shared__ float part_a[ST][CG + 1];
     Word *const staged = reinterpret_cast<Word *>(smem);  // x0, z0, x1, z1
     float4 *const tabs = reinterpret_cast<float4 *>(smem + L::STAGED);
+    float *const decs = reinterpret_cast<float *>(tabs + 2 * heads * ROWS);
     const int C = p.l.C, P = p.l.P, tid = threadIdx.x, lane = tid & 31;
     const int cg = tid % CG, part = tid / CG, b0 = part * LC;
     const int seg = blockIdx.y, c0 = blockIdx.x * (CG * VEC), ch = c0 + cg * VEC;
@@ -311,14 +319,19 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
                 const int i = tid % CH, r = tid / CH;
                 const T *q = src + i * E + r * p.ld;
                 Word *d = dst + r * CG + i * (E / VEC);
+                static_assert(STEP % LC == 0, "a pass is whole parts");
+                const uint32_t a0 = (uint32_t)__cvta_generic_to_shared(d + r / LC * L::PAD);
+                auto copy = [&](int n) {
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                                     a0 + n * (STEP * CG + STEP / LC * L::PAD) * (int)sizeof(Word)),
+                                 "l"(q)
+                                 : "memory");
+                };
+                if (live == ROWS) {
 #pragma unroll
-                for (int n = 0; n < ROWS / STEP; ++n, q += STEP * p.ld) {
-                    const int at = r + n * STEP;
-                    if (at < live) {
-                        const uint32_t a =
-                            (uint32_t)__cvta_generic_to_shared(d + n * STEP * CG + at / LC * L::PAD);
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(a), "l"(q) : "memory");
-                    }
+                    for (int n = 0; n < ROWS / STEP; ++n, q += STEP * p.ld) copy(n);
+                } else {
+                    for (int n = 0; r + n * STEP < live; ++n, q += STEP * p.ld) copy(n);
                 }
             } else if (on) {
                 for (int r = part; r < live; r += ST)
@@ -334,6 +347,8 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(a),
                              "l"(p.tab + ((int64_t)(r0 + t) / LC * p.l.H + h0 + h) * LC + t % LC)
                              : "memory");
+                if (t % LC == 0)
+                    stage(decs + (buf * heads + h) * ST + t / LC, p.dec + (int64_t)(r0 + t) / LC * p.l.H + h0 + h, 0.0f);
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -350,7 +365,8 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
                 const float before = shfl_up(prod, o, LC);
                 if (t % LC >= o) prod *= before;
             }
-            tabs[buf * heads * ROWS + i] = make_float4(k.a, k.g, k.c, prod);
+            tabs[buf * heads * ROWS + i] = make_float4(k.a, k.g, k.c, k.c * prod);
+            if (t % LC == LC - 1) decs[(buf * heads + h) * ST + t / LC] = prod;
         }
     };
     const bool cached = p.n_seq <= SEQ_CACHE;
@@ -401,12 +417,6 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
     };
 
     // ---- before the first tile
-    if (cached) {
-        for (int i = tid; i <= p.n_seq; i += NT) {
-            s_off[i] = (int)max((int64_t)0, min((int64_t)p.rows, p.off[i]));
-            if (i < p.n_seq) s_info[i] = load_info(i);
-        }
-    }
     if (seg0 < seg1) stage_in(seg0, 0);
     V w0, w1, w2, w3, bias, dd;
     {
@@ -421,6 +431,12 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
         vset(w3, a.w, b.w);
         vset(bias, on ? p.l.conv_b[ch] : 0.0f, on ? p.l.conv_b[ch + VEC - 1] : 0.0f);
         vset(dd, on ? p.l.d[ch] : 0.0f, on ? p.l.d[ch + VEC - 1] : 0.0f);
+    }
+    if (cached) {
+        for (int i = tid; i <= p.n_seq; i += NT) {
+            s_off[i] = (int)max((int64_t)0, min((int64_t)p.rows, p.off[i]));
+            if (i < p.n_seq) s_info[i] = load_info(i);
+        }
     }
     if (part == 0) {  // the three rows above
 #pragma unroll
@@ -466,6 +482,19 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
         put(conv_at(slot, 2), c);
         put(p.l.h + (int64_t)slot * C + ch, s);
     };
+
+    auto fetch_init = [&]() {
+        const unsigned start = row_start[b0 / 32] >> b0 % 32 & mask;
+        if (!start) return;
+        const int info = row_info[b0 + __ffs(start) - 1];
+        if (!on || (info & 4)) return;
+        stage(&init_h[part][cg], p.l.h + (int64_t)(info >> 4) * C + ch, V());
+#pragma unroll
+        for (int k = 0; k < 3; ++k) stage(&init_x[part][k][cg], conv_at(info >> 4, k), Word());
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    __syncthreads();
+    fetch_init();
 
     bool plain = false;
     int left_slot = -1;  // the slot of a state left to the third launch
@@ -533,12 +562,23 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
 #pragma unroll
             for (int t = 0; t < LC; ++t) {
                 if (start >> t & 1u) {
-                    x1 = back(1, 0, info[t]);
-                    x2 = back(2, 0, info[t]);
-                    x3 = back(3, 0, info[t]);
-                    const float *hs = p.l.h + (int64_t)(info[t] >> 4) * C + ch;
                     const bool from = on && !(info[t] & 4);
-                    vset(h, from ? hs[0] : 0.0f, from ? hs[VEC - 1] : 0.0f);
+                    if (from && (start & ((1u << t) - 1u)) == 0) {  // fetched
+                        R r;
+                        r.v = init_x[part][2][cg];
+                        x1 = r.get();
+                        r.v = init_x[part][1][cg];
+                        x2 = r.get();
+                        r.v = init_x[part][0][cg];
+                        x3 = r.get();
+                        h = init_h[part][cg];
+                    } else {
+                        x1 = back(1, 0, info[t]);
+                        x2 = back(2, 0, info[t]);
+                        x3 = back(3, 0, info[t]);
+                        const float *hs = p.l.h + (int64_t)(info[t] >> 4) * C + ch;
+                        vset(h, from ? hs[0] : 0.0f, from ? hs[VEC - 1] : 0.0f);
+                    }
                 }
                 A *= token(t);
                 if (end >> t & 1u) {
@@ -558,7 +598,7 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
             }
         }
         part_s[part][cg] = h;
-        part_a[part][cg] = start ? SET : tb[LC - 1].w;
+        part_a[part][cg] = start ? SET : decs[(buf * heads + hh) * ST + part];
         if (!PRE && r1 < seg1) head_table(r1, buf ^ 1);
         __syncthreads();
         if (part == ST - 1) {
@@ -596,6 +636,7 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
             plain = same;
         }
         __syncthreads();
+        if (r1 < seg1 && !plain) fetch_init();
         const V hin = came[part][cg];
         if (!SUMS && end_info >= 0) {
             V aa;
@@ -620,9 +661,7 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
             auto finish = [&](int t, bool fix) {
                 V o = y[t];
                 if (fix) {
-                    const float2 cq = *reinterpret_cast<const float2 *>(&tb[t].z);
-                    const float q = cq.x * cq.y;
-                    o = sfma(q, hin, o);
+                    o = sfma(tb[t].w, hin, o);
                 }
                 if (gate) {
                     R zr;
@@ -697,7 +736,7 @@ __global__ void __launch_bounds__(128) left_kernel(const Layer l, const Segments
 struct Launch {
     Args a;
     bm_ctx_t *ctx;
-    int sms;
+    int device, sms;
     cudaStream_t s;
 };
 
@@ -717,13 +756,14 @@ int launch_prefill(Launch &l) {
     g.rows = (tiles + segs - 1) / segs * L::ROWS;
     g.n = segs = (int)(((int64_t)tiles * L::ROWS + g.rows - 1) / g.rows);
     const int64_t parts = ((int64_t)a.rows + LC - 1) / LC;
-    const size_t tab_bytes = PRE ? (size_t)parts * H * LC * sizeof(float4) : 0;
+    const size_t tab_bytes = PRE ? (size_t)parts * H * (LC * sizeof(float4) + sizeof(float)) : 0;
     if (segs > 1 || PRE) {
         void *work;
         const size_t words = segs > 1 ? (size_t)segs * ((size_t)2 * C + H + 3 * C + n_cb) : 0;
         const int rc = bm_detail_work(l.ctx, BM_WORK_SCAN, tab_bytes + words * 4, &work);
         if (rc != BM_OK) return rc;
         a.tab = static_cast<const float4 *>(work);
+        a.dec = reinterpret_cast<const float *>(a.tab + (PRE ? parts * H * LC : 0));
         g.S = reinterpret_cast<float *>(static_cast<unsigned char *>(work) + tab_bytes);
         g.h = g.S + (size_t)segs * C;
         g.conv = g.h + (size_t)segs * C;
@@ -733,20 +773,22 @@ int launch_prefill(Launch &l) {
     if (PRE) {
         const int64_t blocks = (parts * H + 127) / 128;
         if (blocks > INT32_MAX) return bm_detail_fail(BM_ERR_UNSUPPORTED, "rows * heads too large for one call");
-        heads_kernel<T, LC><<<(unsigned)blocks, 128, 0, l.s>>>(a, const_cast<float4 *>(a.tab));
+        heads_kernel<T, LC><<<(unsigned)blocks, 128, 0, l.s>>>(a, const_cast<float4 *>(a.tab), const_cast<float *>(a.dec));
     }
     int heads = (CG * VEC + P - 2) / P + 1;
     if (heads > H) heads = H;
     const size_t bytes = L::STAGED + (size_t)heads * L::PER_HEAD;
-    constexpr int most = 202 * 1024;
+    // a pair's head has 16 channels or more (bm_ssm_prefill)
+    constexpr int most = (int)(L::STAGED + (VEC == 2 ? (CG * VEC + 14) / 16 + 1 : CG) * L::PER_HEAD);
     if (bytes > most) return bm_detail_fail(BM_ERR_UNSUPPORTED, "too many heads in a tile");
     auto even = [&](const void *q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; };
     const int wide = C % (CG * VEC) == 0 && even(a.x) && even(a.z) && a.ld * (int64_t)sizeof(T) % 16 == 0;
     auto *main = prefill_kernel<T, VEC, CG, ST, LC, PER_SM, PRE, false>;
-    BMC_CK(cudaFuncSetAttribute(main, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+    static bmc::SharedMemory shm[2];
+    BMC_CK(shm[0].allow(reinterpret_cast<const void *>(main), most, l.device));
     if (segs > 1) {
         auto *sums = prefill_kernel<T, VEC, CG, ST, LC, PER_SM, PRE, true>;
-        BMC_CK(cudaFuncSetAttribute(sums, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+        BMC_CK(shm[1].allow(reinterpret_cast<const void *>(sums), most, l.device));
         sums<<<dim3((unsigned)n_cb, (unsigned)segs - 1), L::NT, bytes, l.s>>>(a, g, heads, wide);
     }
     main<<<dim3((unsigned)n_cb, (unsigned)segs), L::NT, bytes, l.s>>>(a, g, heads, wide);
@@ -864,7 +906,8 @@ int bm_ssm_prefill(bm_ctx_t *ctx, const bm_ssm_layer_t *layer, const void *d_x, 
     Launch l{};
     l.ctx = ctx;
     int *err;
-    bmc::DeviceGuard guard(bm_detail_ctx(ctx, &l.sms, &err, &l.s));
+    l.device = bm_detail_ctx(ctx, &l.sms, &err, &l.s);
+    bmc::DeviceGuard guard(l.device);
     BMC_CK(guard.error);
     if (stream) l.s = static_cast<cudaStream_t>(stream);
     l.a = a;
@@ -877,11 +920,10 @@ int bm_ssm_prefill(bm_ctx_t *ctx, const bm_ssm_layer_t *layer, const void *d_x, 
         return f32 ? launch_prefill<float, 1, 32, 16, 8, 1, false>(l) : launch_prefill<bf16, 1, 32, 16, 8, 1, false>(l);
     if (rows <= 64)
         return f32 ? launch_prefill<float, 2, 16, 8, 8, 4, false>(l) : launch_prefill<bf16, 2, 16, 8, 8, 4, false>(l);
-    static const int which = getenv("BM_T") ? atoi(getenv("BM_T")) : 0;
-    if (which == 0) return f32 ? launch_prefill<float, 2, 16, 32, 8, 1, true>(l) : launch_prefill<bf16, 2, 16, 32, 16, 1, true>(l);
-    if (which == 1) return f32 ? launch_prefill<float, 2, 8, 32, 8, 2, true>(l) : launch_prefill<bf16, 2, 8, 32, 16, 2, true>(l);
-    if (which == 2) return f32 ? launch_prefill<float, 2, 8, 32, 8, 3, true>(l) : launch_prefill<bf16, 2, 8, 32, 8, 3, true>(l);
-    return f32 ? launch_prefill<float, 2, 16, 16, 8, 2, true>(l) : launch_prefill<bf16, 2, 16, 32, 8, 1, true>(l);
+    // the head scalars of few tiles cost less in the CTAs than a launch
+    if (rows <= 2048)
+        return f32 ? launch_prefill<float, 2, 16, 32, 8, 1, false>(l) : launch_prefill<bf16, 2, 16, 32, 8, 1, false>(l);
+    return f32 ? launch_prefill<float, 2, 16, 32, 8, 1, true>(l) : launch_prefill<bf16, 2, 16, 32, 16, 1, true>(l);
 }
 
 int bm_ssm_step(bm_ctx_t *ctx, const bm_ssm_layer_t *layer, const void *d_x, const void *d_z,
