@@ -9,10 +9,14 @@
 // back, scale it and add it to fp32 sums in registers while the tensor core
 // works on the next buffer.
 //
-// The tile is 128 rows of w (the accumulator's lanes) by NB rows of a (its
-// columns).  With w on the lanes a warp's store covers 32 consecutive outputs
-// of one row whatever the row pitch, the w scale is one value per tile and
-// block, and few rows of a cost a narrow tile instead of a padded one.
+// Two shapes of tile:
+//   few rows    128 rows of w (the accumulator's lanes) by NB = 16 .. 128 rows
+//               of a (its columns), so that a few rows cost a narrow tile
+//               instead of a padded one.  Bound by the bytes of w.
+//   many rows   128 rows of a (lanes) by 256 rows of w: a thread's scale is
+//               one value for its 128 columns.  (With w on the lanes every
+//               column has its own scale, and fetching 128 of them a block
+//               took twice as long as the tensor core's work.)
 #include <cstdint>
 
 #include <cuda_bf16.h>
@@ -126,20 +130,7 @@ cudaError_t quantize(const T *x, int rows, int d, int64_t ldx, const float *norm
 
 // -------------------------------------------------------------- product --
 
-constexpr int BV = 128, BKB = 128;  // rows of w per tile, bytes (columns) of K per block
-constexpr int RING = 4;             // blocks of scales in shared memory
-
-template <int NB>
-struct Shape {
-    static constexpr int PW = NB >= 64 ? 8 : 4;      // promotion warps
-    static constexpr int CW = NB / (PW / 4);         // columns per promotion warp
-    static constexpr int TB = NB == 256 ? 2 : 4;     // tensor memory buffers
-    static constexpr int COLS = TB * NB;             // a power of two >= 32
-    static constexpr int STAGE = BV * BKB + NB * BKB;
-    static constexpr int STAGES = (192 * 1024) / STAGE;
-    static constexpr int THREADS = 32 * (3 + PW);
-    static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + RING * NB * 4 + 512;
-};
+constexpr int BKB = 128;  // bytes (columns) of K per block
 
 __device__ __forceinline__ void umma_f8(uint32_t tmem, uint64_t da, uint64_t db, uint32_t idesc,
                                         uint32_t accumulate) {
@@ -148,7 +139,22 @@ __device__ __forceinline__ void umma_f8(uint32_t tmem, uint64_t da, uint64_t db,
         " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}" ::"r"(tmem),
         "l"(da), "l"(db), "r"(idesc), "r"(accumulate));
 }
-__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&r)[16]) {
+// consecutive fp32 accumulator columns of this thread's lane; the registers
+// hold them after tmem_wait
+__device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+        "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, "
+        "%28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+          "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+          "=r"(r[31])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
         "%11, %12, %13, %14, %15}, [%16];"
@@ -156,11 +162,37 @@ __device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&r)[16]) {
           "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
           "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(addr));
+}
+// (the registers pass through, so that no use moves before the wait)
+template <int N>
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[N]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
 }
 __device__ __forceinline__ void arrive(uint64_t *b) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(sa(b)) : "memory");
 }
+__device__ __forceinline__ void tmem_alloc(uint32_t *slot, uint32_t cols) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sa(slot)),
+                 "r"(cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t cols) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
+}
+__device__ __forceinline__ void before_sync() {
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void after_sync() {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+// both operands e4m3 (formats 0) and K-major, D fp32, 128 lanes, n columns
+__host__ __device__ constexpr uint32_t f8_desc(int n) {
+    return (1u << 4) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+}
+__device__ __forceinline__ float as_f(uint32_t v) { return __uint_as_float(v); }
 
 struct ProductArgs {
     const float *sa, *sw;
@@ -170,33 +202,53 @@ struct ProductArgs {
     int *err;
 };
 
-// Persistent: CTA c takes tiles c, c + grid, ... (rows of a fastest, so CTAs
-// running together share w tiles).  Warp 0 lane 0 is the TMA producer, warp 1
-// lane 0 issues the MMAs, warp 2 multiplies and stages the scales, the
-// promotion warps add.
+// ---- few rows
+//
+// Persistent CTAs with one tile after the other, or (split > 1) a cluster of
+// `split` CTAs per tile, each with a part of K: the others hand their sums to
+// the first through its shared memory, which adds them in order.  The scales
+// of a stay in shared memory, those of w in the lanes of a warp.
 template <int NB>
-__global__ void __launch_bounds__(Shape<NB>::THREADS, 1)
-    product_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmA,
-                   const ProductArgs p) {
-    using S = Shape<NB>;
+struct Few {
+    static constexpr int BV = 128;
+    static constexpr int PW = NB >= 64 ? 8 : 4;  // promotion warps
+    static constexpr int CW = NB / (PW / 4);     // columns per promotion warp
+    static constexpr int TB = 4;                 // tensor memory buffers
+    static constexpr int COLS = TB * NB;         // a power of two >= 32
+    static constexpr int STAGE = BV * BKB + NB * BKB;
+    static constexpr int THREADS = 32 * (2 + PW);
+    static constexpr int MAX_STAGES = 12;
+    static constexpr size_t BARS = (2 * MAX_STAGES + 2 * TB) * 8 + 16;
+    static constexpr int SMEM = 220 * 1024;
+    // as many stages as fit beside the scales of kb blocks
+    static int stages(int kb) {
+        const int n = (int)((SMEM - 1024 - BARS - (size_t)kb * NB * 4) / STAGE);
+        return n < MAX_STAGES ? n : MAX_STAGES;
+    }
+};
+
+template <int NB>
+__global__ void __launch_bounds__(Few<NB>::THREADS, 1)
+    few_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmA,
+                    const ProductArgs p, int stages, int split) {
+    using S = Few<NB>;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
-    unsigned char *smem = reinterpret_cast<unsigned char *>(
-        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    float *ring = reinterpret_cast<float *>(smem + S::STAGES * S::STAGE);
-    uint64_t *full = reinterpret_cast<uint64_t *>(ring + RING * NB);
-    uint64_t *empty = full + S::STAGES;
-    uint64_t *accf = empty + S::STAGES;  // [TB] a block's sums are complete
-    uint64_t *acce = accf + S::TB;       // [TB] they are read
-    uint64_t *sf = acce + S::TB;         // [RING] scales staged
-    uint64_t *se = sf + RING;            // [RING] scales read
-    uint32_t *tslot = reinterpret_cast<uint32_t *>(se + RING);
+    // (an offset, so that the compiler still knows it for shared memory)
+    unsigned char *const smem = smem_raw + ((1024u - (sa(smem_raw) & 1023u)) & 1023u);
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + stages * S::STAGE);
+    uint64_t *empty = full + S::MAX_STAGES;
+    uint64_t *accf = empty + S::MAX_STAGES;  // [TB] a block's sums are complete
+    uint64_t *acce = accf + S::TB;           // [TB] they are read
+    uint32_t *tslot = reinterpret_cast<uint32_t *>(acce + S::TB);
     int *abort_ = reinterpret_cast<int *>(tslot + 1);
+    float *scales = reinterpret_cast<float *>(tslot + 4);  // [blocks][NB]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int MT = (p.M + NB - 1) / NB, NT = (p.N + BV - 1) / BV, KB = (p.K + BKB - 1) / BKB;
-    const int tiles = MT * NT;
+    const int tiles = (p.N + S::BV - 1) / S::BV, KB = (p.K + BKB - 1) / BKB;
+    const int rank = blockIdx.x % split, first = blockIdx.x / split, step = gridDim.x / split;
+    const int kb0 = (int)((int64_t)KB * rank / split), nkb = (int)((int64_t)KB * (rank + 1) / split) - kb0;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < S::STAGES; ++i) {
+        for (int i = 0; i < stages; ++i) {
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], 1);
         }
@@ -204,163 +256,413 @@ __global__ void __launch_bounds__(Shape<NB>::THREADS, 1)
             mbar_init(&accf[i], 1);
             mbar_init(&acce[i], S::PW);
         }
-        for (int i = 0; i < RING; ++i) {
-            mbar_init(&sf[i], 1);
-            mbar_init(&se[i], S::PW);
-        }
         *abort_ = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                         sa(tslot)),
-                     "r"((uint32_t)S::COLS)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    if (warp == 0) tmem_alloc(tslot, S::COLS);
+    before_sync();
     __syncthreads();
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    after_sync();
     const uint32_t tmem = *tslot;
     auto fail = [&]() { atomicOr(abort_, 1); };
     auto aborted = [&]() { return *reinterpret_cast<volatile int *>(abort_) != 0; };
 
     if (threadIdx.x == 0) {
-        int g = 0;
-        for (int t = blockIdx.x; t < tiles && !aborted(); t += gridDim.x) {
-            const int m0 = (t % MT) * NB, n0 = (t / MT) * BV;
-            for (int kb = 0; kb < KB; ++kb, ++g) {
-                const int s = g % S::STAGES;
-                if (g >= S::STAGES && !mbar_wait(&empty[s], ((g / S::STAGES) - 1) & 1)) {
+        int s = 0, ph = 1;
+        for (int t = first; t < tiles && !aborted(); t += step) {
+            for (int kb = 0; kb < nkb; ++kb) {
+                if (!mbar_wait(&empty[s], ph)) {  // (a fresh barrier is past phase 1)
                     fail();
                     break;
                 }
                 unsigned char *st = smem + (size_t)s * S::STAGE;
                 mbar_expect_tx(&full[s], S::STAGE);
-                tma_load_2d(st, &tmW, kb * BKB, n0, &full[s]);
-                tma_load_2d(st + BV * BKB, &tmA, kb * BKB, m0, &full[s]);
+                tma_load_2d(st, &tmW, (kb0 + kb) * BKB, t * S::BV, &full[s]);
+                tma_load_2d(st + S::BV * BKB, &tmA, (kb0 + kb) * BKB, 0, &full[s]);
+                if (++s == stages) {
+                    s = 0;
+                    ph ^= 1;
+                }
             }
         }
     } else if (threadIdx.x == 32) {
-        // e4m3 x e4m3 -> fp32 (formats 0, D format 1), both K-major
-        const uint32_t idesc = (1u << 4) | ((uint32_t)(NB >> 3) << 17) | ((uint32_t)(BV >> 4) << 24);
-        int g = 0;
-        for (int t = blockIdx.x; t < tiles && !aborted(); t += gridDim.x) {
-            for (int kb = 0; kb < KB; ++kb, ++g) {
-                const int s = g % S::STAGES, b = g % S::TB;
-                if ((g >= S::TB && !mbar_wait(&acce[b], ((g / S::TB) - 1) & 1)) ||
-                    !mbar_wait(&full[s], (g / S::STAGES) & 1)) {
+        int s = 0, ph = 0, g = 0;
+        for (int t = first; t < tiles && !aborted(); t += step) {
+            for (int kb = 0; kb < nkb; ++kb, ++g) {
+                const int b = g % S::TB;
+                if (!mbar_wait(&acce[b], (g / S::TB + 1) & 1) || !mbar_wait(&full[s], ph)) {
                     fail();
                     break;
                 }
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t w0 = sa(smem + (size_t)s * S::STAGE), a0 = w0 + BV * BKB;
-                const uint32_t acc = tmem + (uint32_t)(b * NB);
+                after_sync();
+                const uint32_t w0 = sa(smem + (size_t)s * S::STAGE), a0 = w0 + S::BV * BKB;
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    umma_f8(acc, sdesc(w0 + k * 32), sdesc(a0 + k * 32), idesc, k > 0 ? 1u : 0u);
+                    umma_f8(tmem + (uint32_t)(b * NB), sdesc(w0 + k * 32), sdesc(a0 + k * 32), f8_desc(NB),
+                            k > 0 ? 1u : 0u);
                 umma_commit(&empty[s]);
                 umma_commit(&accf[b]);
-            }
-        }
-    } else if (warp == 2) {
-        int g = 0;
-        for (int t = blockIdx.x; t < tiles && !aborted(); t += gridDim.x) {
-            const int m0 = (t % MT) * NB, nt = t / MT;
-            for (int kb = 0; kb < KB; ++kb, ++g) {
-                const int r = g % RING;
-                const bool ok = g < RING || mbar_wait(&se[r], ((g / RING) - 1) & 1);
-                if (__any_sync(0xffffffffu, !ok)) {
-                    fail();
-                    break;
+                if (++s == stages) {
+                    s = 0;
+                    ph ^= 1;
                 }
-                const float sw = p.sw[(int64_t)nt * KB + kb];
-                for (int c = lane; c < NB; c += 32)
-                    ring[r * NB + c] = m0 + c < p.M ? p.sa[kb * p.ld_scale + m0 + c] * sw : 0.0f;
-                __syncwarp();
-                if (lane == 0) arrive(&sf[r]);
             }
         }
-    } else if (warp >= 3) {
-        const int q = warp & 3, c0 = ((warp - 3) >> 2) * S::CW;
+    } else if (warp >= 2) {
+        for (int i = threadIdx.x - 64; i < nkb * NB; i += 32 * S::PW) {
+            const int m = i % NB;
+            scales[i] = m < p.M ? p.sa[(kb0 + i / NB) * p.ld_scale + m] : 0.0f;
+        }
+        asm volatile("bar.sync 1, %0;" ::"r"(32 * S::PW) : "memory");
+        const int q = warp & 3, c0 = ((warp - 2) >> 2) * S::CW;
+        constexpr int LD = S::CW < 32 ? 16 : 32;
         int g = 0;
-        for (int t = blockIdx.x; t < tiles && !aborted(); t += gridDim.x) {
-            const int m0 = (t % MT) * NB, n0 = (t / MT) * BV;
-            float acc[S::CW];
+        // 32 blocks' scales of w in the lanes, the next ones on their way
+        auto load_sw = [&](int t, int kb) {
+            return t < tiles && kb + lane < nkb ? p.sw[(int64_t)t * KB + kb0 + kb + lane] : 0.0f;
+        };
+        float sw_next = load_sw(first, 0);
+        // (a cluster's barriers are reached whatever failed)
+        for (int t = first; t < tiles && (split > 1 || !aborted()); t += step) {
+            float2 acc[S::CW / 2];
 #pragma unroll
-            for (int j = 0; j < S::CW; ++j) acc[j] = 0.0f;
+            for (int j = 0; j < S::CW / 2; ++j) acc[j] = make_float2(0.0f, 0.0f);
             bool good = true;
-            for (int kb = 0; kb < KB; ++kb, ++g) {
-                const int b = g % S::TB, r = g % RING;
-                const bool ok = mbar_wait(&sf[r], (g / RING) & 1) && mbar_wait(&accf[b], (g / S::TB) & 1);
+            float sw = 0.0f;
+            for (int kb = 0; kb < nkb; ++kb, ++g) {
+                if (kb % 32 == 0) {
+                    sw = sw_next;
+                    sw_next = kb + 32 < nkb ? load_sw(t, kb + 32) : load_sw(t + step, 0);
+                }
+                const int b = g % S::TB;
+                const bool ok = mbar_wait(&accf[b], (g / S::TB) & 1);
                 if (__any_sync(0xffffffffu, !ok)) {
                     fail();
                     good = false;
                     break;
                 }
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                after_sync();
                 const uint32_t tb = tmem + (uint32_t)(b * NB + c0) + ((uint32_t)(q * 32) << 16);
-                const float *sc = ring + r * NB + c0;
+                const float k = __shfl_sync(0xffffffffu, sw, kb % 32);
+                const float2 k2 = make_float2(k, k);
+                const float4 *sc = reinterpret_cast<const float4 *>(scales + kb * NB + c0);
 #pragma unroll
-                for (int c = 0; c < S::CW; c += 16) {
-                    uint32_t v[16];
-                    tmem_ld16(tb + c, v);
+                for (int c = 0; c < S::CW; c += LD) {
+                    uint32_t v[LD];
+                    tmem_load(tb + c, v);
+                    float4 f[LD / 4];
 #pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        acc[c + j] = fmaf(__uint_as_float(v[j]), sc[c + j], acc[c + j]);
-                }
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) {
-                    arrive(&acce[b]);
-                    arrive(&se[r]);
+                    for (int j = 0; j < LD / 4; ++j) f[j] = sc[c / 4 + j];
+                    tmem_wait(v);
+                    if (c + LD == S::CW) {  // the sums are read: the buffer is free
+                        before_sync();
+                        __syncwarp();
+                        if (lane == 0) arrive(&acce[b]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < LD; j += 4) {
+                        const int at = (c + j) / 2;
+                        acc[at] = __ffma2_rn(make_float2(as_f(v[j]), as_f(v[j + 1])),
+                                             __fmul2_rn(make_float2(f[j / 4].x, f[j / 4].y), k2), acc[at]);
+                        acc[at + 1] = __ffma2_rn(make_float2(as_f(v[j + 2]), as_f(v[j + 3])),
+                                                 __fmul2_rn(make_float2(f[j / 4].z, f[j / 4].w), k2), acc[at + 1]);
+                    }
                 }
             }
-            const int n = n0 + q * 32 + lane;
+            // sums of this CTA's part of K to the first of the cluster: [rank
+            // - 1][column][lane of w], over its stages, which are idle by then
+            // (its tensor core has read them, else it had not got this far)
+            const int at = (c0 * 128 + q * 32 + lane) * 4;
+            if (split > 1) {
+                asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+                if (rank > 0) {
+                    const uint32_t mine = sa(smem) + (uint32_t)((rank - 1) * NB * 128 * 4 + at);
+                    uint32_t theirs;
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(theirs) : "r"(mine));
+#pragma unroll
+                    for (int j = 0; j < S::CW; ++j)
+                        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(theirs + j * 512),
+                                     "f"(j % 2 ? acc[j / 2].y : acc[j / 2].x)
+                                     : "memory");
+                }
+                asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+                if (rank > 0) break;
+                for (int r = 0; r < split - 1; ++r) {
+                    const float *from = reinterpret_cast<const float *>(smem + (size_t)r * NB * 128 * 4 + at);
+#pragma unroll
+                    for (int j = 0; j < S::CW; ++j) {
+                        if (j % 2) acc[j / 2].y += from[j * 128];
+                        else acc[j / 2].x += from[j * 128];
+                    }
+                }
+            }
+            const int n = t * S::BV + q * 32 + lane;
             if (good && n < p.N) {
-                float *o = p.out + (int64_t)(m0 + c0) * p.ldo + n;
+                float *o = p.out + (int64_t)c0 * p.ldo + n;
 #pragma unroll
                 for (int j = 0; j < S::CW; ++j, o += p.ldo)
-                    if (m0 + c0 + j < p.M) *o = acc[j];
+                    if (c0 + j < p.M) *o = j % 2 ? acc[j / 2].y : acc[j / 2].x;
             }
         }
     }
+    if (split > 1 && warp < 2) {
+        // the cluster's two barriers, for the warps without sums
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
     __syncwarp();
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    before_sync();
     __syncthreads();
-    if (warp == 0)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
-                     "r"((uint32_t)S::COLS)
-                     : "memory");
+    if (warp == 0) tmem_free(tmem, S::COLS);
     if (threadIdx.x == 0 && *abort_) atomicOr(p.err, 4);
 }
 
 template <int NB>
-cudaError_t launch_product(const uint8_t *a, const uint8_t *w, const ProductArgs &p, int sms,
-                           cudaStream_t s) {
-    using S = Shape<NB>;
+cudaError_t few_rows(const uint8_t *a, const uint8_t *w, const ProductArgs &p, int sms, cudaStream_t s) {
+    using S = Few<NB>;
     CUtensorMap mw, ma;
-    cudaError_t e = byte_map(&mw, w, p.N, p.K, BV);
+    cudaError_t e = byte_map(&mw, w, p.N, p.K, S::BV);
     if (e == cudaSuccess) e = byte_map(&ma, a, p.M, p.K, NB);
     int device = 0;
     static bmc::SharedMemory shm;
     if (e == cudaSuccess) e = cudaGetDevice(&device);
-    if (e == cudaSuccess)
-        e = shm.allow(reinterpret_cast<const void *>(product_kernel<NB>), (int)S::SMEM, device);
+    auto *k = few_rows_kernel<NB>;
+    if (e == cudaSuccess) e = shm.allow(reinterpret_cast<const void *>(k), S::SMEM, device);
     if (e != cudaSuccess) return e;
-    const int64_t tiles = (int64_t)((p.M + NB - 1) / NB) * ((p.N + BV - 1) / BV);
+    const int tiles = (p.N + S::BV - 1) / S::BV, KB = (p.K + BKB - 1) / BKB;
+    // part of K each where tiles alone leave SMs idle: at least four blocks,
+    // and the others' sums fit over two thirds of the stages
+    int split = 1;
+    while (split < 4 && tiles * split * 2 <= sms && KB >= split * 2 * 4 && (split * 2 - 1) * NB <= 256) split *= 2;
+    const int blocks = (KB + split - 1) / split, stages = S::stages(blocks);
+    cudaLaunchConfig_t c{};
+    cudaLaunchAttribute at[1];
+    c.gridDim = dim3((unsigned)(split > 1 ? tiles * split : tiles < sms ? tiles : sms));
+    c.blockDim = dim3(S::THREADS);
+    c.dynamicSmemBytes = S::SMEM;
+    c.stream = s;
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)split;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    c.attrs = at;
+    c.numAttrs = split > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&c, k, mw, ma, p, stages, split);
+}
+
+// ---- many rows
+//
+// Persistent: CTA c takes tiles c, c + grid, ... (rows of a fastest, so CTAs
+// running together share w tiles).  Warp 0 lane 0 is the TMA producer, warp 1
+// lane 0 issues the MMAs, warps 4 to 11 promote: each has 32 rows by 128
+// columns, a scale of a per thread and of w per warp.  128 sums and 64 values
+// on their way from tensor memory take more registers than an equal share, so
+// the first four warps give theirs up: 128 * 72 + 256 * 216 = 384 * 168, what
+// the block was launched with.
+constexpr int BM = 128, BN = 256, STAGES = 4, PROMOTE = 8, TBUF = 2;
+constexpr int STAGE_BYTES = (BM + BN) * BKB;
+constexpr int MANY_THREADS = 32 * (4 + PROMOTE);
+constexpr int TURN = 17 * 32 * 4;  // a warp's 32 x 16 values on their way out
+constexpr int KRING = 8;           // blocks whose scales a thread has at hand
+constexpr size_t MANY_SMEM =
+    1024 + (size_t)STAGES * STAGE_BYTES + PROMOTE * TURN + KRING * PROMOTE * 32 * 4 + 256;
+
+__global__ void __launch_bounds__(MANY_THREADS, 1)
+    many_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
+                     const ProductArgs p) {
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    // (an offset, so that the compiler still knows it for shared memory)
+    unsigned char *const smem = smem_raw + ((1024u - (sa(smem_raw) & 1023u)) & 1023u);
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + STAGES * STAGE_BYTES + PROMOTE * TURN +
+                                                  KRING * PROMOTE * 32 * 4);
+    uint64_t *empty = full + STAGES;
+    uint64_t *accf = empty + STAGES;
+    uint64_t *acce = accf + TBUF;
+    uint32_t *tslot = reinterpret_cast<uint32_t *>(acce + TBUF);
+    int *abort_ = reinterpret_cast<int *>(tslot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int MT = (p.M + BM - 1) / BM, NTL = (p.N + BN - 1) / BN, KB = (p.K + BKB - 1) / BKB;
+    const int tiles = MT * NTL;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < STAGES; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < TBUF; ++i) {
+            mbar_init(&accf[i], 1);
+            mbar_init(&acce[i], PROMOTE);
+        }
+        *abort_ = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) tmem_alloc(tslot, TBUF * BN);
+    before_sync();
+    __syncthreads();
+    after_sync();
+    const uint32_t tmem = *tslot;
+    auto fail = [&]() { atomicOr(abort_, 1); };
+    auto aborted = [&]() { return *reinterpret_cast<volatile int *>(abort_) != 0; };
+
+    if (warp < 4)
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    else
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    if (threadIdx.x == 0) {
+        int g = 0;
+        for (int t = blockIdx.x; t < tiles && !aborted(); t += gridDim.x) {
+            const int m0 = t % MT * BM, n0 = t / MT * BN;
+            for (int kb = 0; kb < KB; ++kb, ++g) {
+                const int s = g % STAGES;
+                if (!mbar_wait(&empty[s], (g / STAGES + 1) & 1)) {
+                    fail();
+                    break;
+                }
+                unsigned char *st = smem + (size_t)s * STAGE_BYTES;
+                mbar_expect_tx(&full[s], STAGE_BYTES);
+                tma_load_2d(st, &tmA, kb * BKB, m0, &full[s]);
+                tma_load_2d(st + BM * BKB, &tmW, kb * BKB, n0, &full[s]);
+            }
+        }
+    } else if (threadIdx.x == 32) {
+        int g = 0;
+        for (int t = blockIdx.x; t < tiles && !aborted(); t += gridDim.x) {
+            for (int kb = 0; kb < KB; ++kb, ++g) {
+                const int s = g % STAGES, b = g % TBUF;
+                if (!mbar_wait(&acce[b], (g / TBUF + 1) & 1) || !mbar_wait(&full[s], (g / STAGES) & 1)) {
+                    fail();
+                    break;
+                }
+                after_sync();
+                const uint32_t a0 = sa(smem + (size_t)s * STAGE_BYTES), w0 = a0 + BM * BKB;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    umma_f8(tmem + (uint32_t)(b * BN), sdesc(a0 + k * 32), sdesc(w0 + k * 32), f8_desc(BN),
+                            k > 0 ? 1u : 0u);
+                umma_commit(&empty[s]);
+                umma_commit(&accf[b]);
+            }
+        }
+    } else if (warp >= 4) {
+        const int q = warp & 3, half = (warp - 4) >> 2, c0 = half * 128;
+        float *turn = reinterpret_cast<float *>(smem + STAGES * STAGE_BYTES + (warp - 4) * TURN);
+        const int NSW = (p.N + 127) / 128;
+        int g = 0;
+        // This thread's scale for each block, in a ring of its own: four blocks
+        // are loaded while the four before are used, and multiplied only then
+        // (a product right behind the loads would wait for them).
+        float *kr = reinterpret_cast<float *>(smem + STAGES * STAGE_BYTES + PROMOTE * TURN) + threadIdx.x - 128;
+        const float *pa = nullptr, *pw = nullptr;
+        int ahead_t = blockIdx.x, ahead_kb = 0;
+        float va[4], vw[4];
+        auto load4 = [&]() {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (ahead_kb == 0) {
+                    const int m = ahead_t % MT * BM + q * 32 + lane, nb = ahead_t / MT * 2 + half;
+                    pa = ahead_t < tiles && m < p.M && nb < NSW ? p.sa + m : nullptr;
+                    pw = p.sw + (int64_t)nb * KB;
+                }
+                va[i] = pa ? *pa : 0.0f;
+                vw[i] = pa ? *pw : 0.0f;
+                if (pa) pa += p.ld_scale;
+                ++pw;
+                if (++ahead_kb == KB) {
+                    ahead_kb = 0;
+                    ahead_t += gridDim.x;
+                }
+            }
+        };
+        load4();
+        for (int t = blockIdx.x; t < tiles && !aborted(); t += gridDim.x) {
+            const int m0 = t % MT * BM + q * 32, n0 = t / MT * BN + c0;
+            float acc[128];
+#pragma unroll
+            for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
+            bool good = true;
+            for (int kb = 0; kb < KB; ++kb, ++g) {
+                if (g % 4 == 0) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) kr[(g + i) % KRING * (PROMOTE * 32)] = va[i] * vw[i];
+                    load4();
+                }
+                const float k = kr[g % KRING * (PROMOTE * 32)];
+                const int b = g % TBUF;
+                const bool ok = mbar_wait(&accf[b], (g / TBUF) & 1);
+                if (__any_sync(0xffffffffu, !ok)) {
+                    fail();
+                    good = false;
+                    break;
+                }
+                after_sync();
+                const uint32_t tb = tmem + (uint32_t)(b * BN + c0) + ((uint32_t)(q * 32) << 16);
+#pragma unroll
+                for (int c = 0; c < 128; c += 64) {
+                    uint32_t v[2][32];
+                    tmem_load(tb + c, v[0]);
+                    tmem_load(tb + c + 32, v[1]);
+                    tmem_wait(v[0]);
+                    tmem_wait(v[1]);
+                    if (c == 64) {  // the sums are read: the buffer is free
+                        before_sync();
+                        __syncwarp();
+                        if (lane == 0) arrive(&acce[b]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 64; ++j) acc[c + j] = fmaf(as_f(v[j / 32][j % 32]), k, acc[c + j]);
+                }
+            }
+            // 16 columns at a time through shared memory: half a warp's store is
+            // 16 consecutive values of a row, whatever the pitch
+            const int rows = min(32, p.M - m0), hl = lane & 15, hw = lane >> 4;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                if (!good || rows <= 0 || n0 + c * 16 >= p.N) continue;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) turn[lane * 17 + j] = acc[c * 16 + j];
+                __syncwarp();
+                const int n = n0 + c * 16 + hl;
+                if (n < p.N) {
+                    float *o = p.out + (int64_t)(m0 + hw) * p.ldo + n;
+                    if (rows == 32) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i, o += 2 * p.ldo) *o = turn[(2 * i + hw) * 17 + hl];
+                    } else {
+                        for (int i = hw; i < rows; i += 2, o += 2 * p.ldo) *o = turn[i * 17 + hl];
+                    }
+                }
+                __syncwarp();
+            }
+        }
+    }
+    __syncwarp();
+    before_sync();
+    __syncthreads();
+    if (warp == 0) tmem_free(tmem, TBUF * BN);
+    if (threadIdx.x == 0 && *abort_) atomicOr(p.err, 4);
+}
+
+cudaError_t many_rows(const uint8_t *a, const uint8_t *w, const ProductArgs &p, int sms, cudaStream_t s) {
+    CUtensorMap mw, ma;
+    cudaError_t e = byte_map(&mw, w, p.N, p.K, BN);
+    if (e == cudaSuccess) e = byte_map(&ma, a, p.M, p.K, BM);
+    int device = 0;
+    static bmc::SharedMemory shm;
+    if (e == cudaSuccess) e = cudaGetDevice(&device);
+    if (e == cudaSuccess) e = shm.allow(reinterpret_cast<const void *>(many_rows_kernel), (int)MANY_SMEM, device);
+    if (e != cudaSuccess) return e;
+    const int64_t tiles = (int64_t)((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
     if (tiles > INT32_MAX / 2) return cudaErrorInvalidValue;
-    product_kernel<NB><<<(int)(tiles < sms ? tiles : sms), S::THREADS, S::SMEM, s>>>(mw, ma, p);
+    many_rows_kernel<<<(int)(tiles < sms ? tiles : sms), MANY_THREADS, MANY_SMEM, s>>>(ma, mw, p);
     return cudaGetLastError();
 }
 
-cudaError_t product(const uint8_t *a, const uint8_t *w, const ProductArgs &p, int sms,
-                    cudaStream_t s) {
-    if (p.M <= 16) return launch_product<16>(a, w, p, sms, s);
-    if (p.M <= 32) return launch_product<32>(a, w, p, sms, s);
-    if (p.M <= 64) return launch_product<64>(a, w, p, sms, s);
-    if (p.M <= 128) return launch_product<128>(a, w, p, sms, s);
-    return launch_product<256>(a, w, p, sms, s);
+cudaError_t product(const uint8_t *a, const uint8_t *w, const ProductArgs &p, int sms, cudaStream_t s) {
+    if (p.M <= 16) return few_rows<16>(a, w, p, sms, s);
+    if (p.M <= 32) return few_rows<32>(a, w, p, sms, s);
+    if (p.M <= 64) return few_rows<64>(a, w, p, sms, s);
+    if (p.M <= 128) return few_rows<128>(a, w, p, sms, s);
+    return many_rows(a, w, p, sms, s);
 }
 
 bool misaligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n != 0; }

@@ -42,12 +42,17 @@ __device__ __forceinline__ bool mbar_try(uint64_t *b, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
+// Bounded; the timer is read every 64th try only.
 __device__ __forceinline__ bool mbar_wait(uint64_t *b, uint32_t parity) {
     if (mbar_try(b, parity)) return true;
-    const unsigned long long t0 = gtimer();
-    for (unsigned it = 0; it < (1u << 30); ++it) {
+    unsigned long long t0 = 0;
+    for (unsigned it = 1; it < (1u << 30); ++it) {
         if (mbar_try(b, parity)) return true;
-        if (gtimer() - t0 > WAIT_NS) return false;
+        if ((it & 63u) == 0) {
+            const unsigned long long now = gtimer();
+            if (t0 == 0) t0 = now;
+            if (now - t0 > WAIT_NS) return false;
+        }
     }
     return false;
 }
