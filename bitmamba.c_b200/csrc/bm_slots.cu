@@ -53,9 +53,13 @@ __global__ void __launch_bounds__(NT)
     __syncthreads();
     const int n = n_moves;
     if (n == 0) return;
-    // columns per piece: a power of two of which n fit the room
+    // columns per piece: a power of two of which n fit the room, and small
+    // enough that every CTA has some
+    int64_t columns = 0;
+    for (int k = 0; k < g.n; ++k) columns += g.r[k].row_bytes * g.r[k].n_outer;
     int piece = PIECE_MAX;
-    while (piece > 16 && (int64_t)piece * n > room) piece >>= 1;
+    while (piece > 16 && ((int64_t)piece * n > room || (piece > 256 && columns < (int64_t)2 * piece * gridDim.x)))
+        piece >>= 1;
     const uint32_t buf0 = (uint32_t)__cvta_generic_to_shared(buf);
     int64_t item = blockIdx.x;
     for (int k = 0; k < g.n; ++k) {

@@ -798,30 +798,86 @@ int launch_prefill(Launch &l) {
     return BM_OK;
 }
 
+// ----------------------------------------------------------- single tokens --
+//
+// Bound by the bytes of the states: 4 of h and 3 inputs read and written per
+// channel against one x, z and y.  A thread has VEC channels (16 bytes of
+// fp32, 8 of bf16), loads everything of a row before it uses any of it, and
+// keeps its weights for the next row that it takes.
+template <typename T, int VEC>
+struct Pack;
+template <>
+struct Pack<float, 4> {
+    float4 v;
+    __device__ __forceinline__ float at(int i) const { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+    __device__ __forceinline__ void set(const float (&f)[4]) { v = make_float4(f[0], f[1], f[2], f[3]); }
+};
+template <>
+struct Pack<__nv_bfloat16, 4> {
+    uint2 v;
+    __device__ __forceinline__ float at(int i) const {
+        const uint32_t w = i < 2 ? v.x : v.y;
+        return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
+    }
+    __device__ __forceinline__ void set(const float (&f)[4]) {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(f[0], f[1]), b = __floats2bfloat162_rn(f[2], f[3]);
+        v = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+    }
+};
 template <typename T>
+struct Pack<T, 1> {
+    T v;
+    __device__ __forceinline__ float at(int) const { return to_f(v); }
+    __device__ __forceinline__ void set(const float (&f)[1]) { v = from_f<T>(f[0]); }
+};
+
+template <typename T, int VEC>
 __global__ void __launch_bounds__(128) step_kernel(const Args p) {
-    const int ch = blockIdx.x * 128 + threadIdx.x;
+    using W = Pack<T, VEC>;
+    using F = Pack<float, VEC>;
+    const int ch = (blockIdx.x * 128 + threadIdx.x) * VEC;
     if (ch >= p.l.C) return;
-    const float4 w = reinterpret_cast<const float4 *>(p.l.conv_w)[ch];
-    const float bias = p.l.conv_b[ch], d = p.l.d[ch];
-    const int hd = ch / p.l.P;
+    const int hd = ch / p.l.P;  // (VEC > 1: one head's channels)
+    float4 w[VEC];
+    float bias[VEC], d[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+        w[v] = reinterpret_cast<const float4 *>(p.l.conv_w)[ch + v];
+        bias[v] = p.l.conv_b[ch + v];
+        d[v] = p.l.d[ch + v];
+    }
+    const float dt_bias = p.l.dt_bias[hd], rate = expf(p.l.a_log[hd]);
     for (int r = blockIdx.y; r < p.rows; r += gridDim.y) {
         const int slot = p.slots ? p.slots[r] : r;
         if (slot < 0 || slot >= p.l.n_slots) continue;
-        T *cs = static_cast<T *>(p.l.conv) + ((int64_t)slot * 3) * p.l.C + ch;
-        float *hs = p.l.h + (int64_t)slot * p.l.C + ch;
-        const Head k = head_of<T>(p, r, hd);
-        const T x3 = cs[0], x2 = cs[p.l.C], x1 = cs[2 * p.l.C];
-        const T x0 = static_cast<const T *>(p.x)[r * p.ld + ch];
-        const float u = silu(fmaf(
-            w.w, to_f(x0), fmaf(w.z, to_f(x1), fmaf(w.y, to_f(x2), fmaf(w.x, to_f(x3), bias)))));
-        const float h = fmaf(k.a, *hs, k.g * u);
-        float y = fmaf(k.c, h, d * u);
-        if (p.z) y *= silu(to_f(static_cast<const T *>(p.z)[r * p.ld + ch]));
-        static_cast<T *>(p.y)[r * p.ldy + ch] = from_f<T>(y);
-        cs[0] = x2;
-        cs[p.l.C] = x1;
-        cs[2 * p.l.C] = x0;
+        W *c0 = reinterpret_cast<W *>(static_cast<T *>(p.l.conv) + (int64_t)slot * 3 * p.l.C + ch);
+        W *c1 = reinterpret_cast<W *>(reinterpret_cast<T *>(c0) + p.l.C), *c2 = reinterpret_cast<W *>(reinterpret_cast<T *>(c1) + p.l.C);
+        F *hs = reinterpret_cast<F *>(p.l.h + (int64_t)slot * p.l.C + ch);
+        const int64_t at = (int64_t)r * p.ld;
+        const W x3 = *c0, x2 = *c1, x1 = *c2;
+        F h = *hs;
+        const W x0 = *reinterpret_cast<const W *>(static_cast<const T *>(p.x) + at + ch);
+        W z = x0;
+        if (p.z) z = *reinterpret_cast<const W *>(static_cast<const T *>(p.z) + at + ch);
+        const T dt = static_cast<const T *>(p.dt)[at + hd], b = static_cast<const T *>(p.b)[at + hd],
+                c = static_cast<const T *>(p.c)[at + hd];
+        const Head k = head_of(to_f(dt) + dt_bias, rate, to_f(b), to_f(c));
+        float hn[VEC], y[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            const float u = silu(fmaf(
+                w[v].w, x0.at(v), fmaf(w[v].z, x1.at(v), fmaf(w[v].y, x2.at(v), fmaf(w[v].x, x3.at(v), bias[v])))));
+            hn[v] = fmaf(k.a, h.at(v), k.g * u);
+            y[v] = fmaf(k.c, hn[v], d[v] * u);
+            if (p.z) y[v] *= silu(z.at(v));
+        }
+        W o;
+        o.set(y);
+        *reinterpret_cast<W *>(static_cast<T *>(p.y) + (int64_t)r * p.ldy + ch) = o;
+        *c0 = x2;
+        *c1 = x1;
+        *c2 = x0;
+        h.set(hn);
         *hs = h;
     }
 }
@@ -940,11 +996,25 @@ int bm_ssm_step(bm_ctx_t *ctx, const bm_ssm_layer_t *layer, const void *d_x, con
     bmc::DeviceGuard guard(bm_detail_ctx(ctx, &sms, &err, &s));
     BMC_CK(guard.error);
     if (stream) s = static_cast<cudaStream_t>(stream);
-    const dim3 grid((unsigned)((a.l.C + 127) / 128), (unsigned)(rows < 65535 ? rows : 65535));
-    if (layer->type == BM_F32)
-        step_kernel<float><<<grid, 128, 0, s>>>(a);
-    else
-        step_kernel<__nv_bfloat16><<<grid, 128, 0, s>>>(a);
+    const size_t e = layer->type == BM_F32 ? 4 : 2;
+    const bool quads = a.l.P % 4 == 0 && ld % 4 == 0 && ldy % 4 == 0 && !misaligned(d_x, 4 * e) &&
+                       !misaligned(d_z, 4 * e) && !misaligned(d_y, 4 * e) &&
+                       !misaligned(layer->conv_state, 4 * e) && !misaligned(layer->h_state, 16);
+    const int vec = quads ? 4 : 1;
+    const unsigned across = (unsigned)((a.l.C + 128 * vec - 1) / (128 * vec));
+    // about 16 CTAs per SM in all; beyond that, several rows each
+    unsigned down = (unsigned)(16 * sms) / across + 1;
+    if (down > 65535) down = 65535;
+    if (down > (unsigned)rows) down = (unsigned)rows;
+    const dim3 grid(across, down);
+    using bf16 = __nv_bfloat16;
+    if (layer->type == BM_F32) {
+        if (quads) step_kernel<float, 4><<<grid, 128, 0, s>>>(a);
+        else step_kernel<float, 1><<<grid, 128, 0, s>>>(a);
+    } else {
+        if (quads) step_kernel<bf16, 4><<<grid, 128, 0, s>>>(a);
+        else step_kernel<bf16, 1><<<grid, 128, 0, s>>>(a);
+    }
     BMC_CK(cudaGetLastError());
     return BM_OK;
 }
