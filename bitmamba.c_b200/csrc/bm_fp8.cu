@@ -43,11 +43,12 @@ __device__ __forceinline__ float4 load4(const __nv_bfloat16 *p) {
                        __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
 }
 
-// max that keeps a NaN
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
+// x / s from r = 1 / s: the quotient's error is exact in one multiply-add, and
+// corrects it (Markstein, IBM J. Res. Dev. 34, 1990).  For 2^-110 < s < 2^120;
+// where the error underflows, x / s is far below e4m3's smallest value.
+__device__ __forceinline__ float divide(float x, float s, float r) {
+    const float q = x * r;
+    return fmaf(fmaf(-q, s, x), r, q);
 }
 
 // TPR threads per row: a warp's 32 groups of 4 columns are one block of 128.
@@ -96,14 +97,25 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
 #pragma unroll
     for (int i = 0; i < QV; ++i) {
         const int col = 4 * (t + i * TPR);
-        float top = max_nan(max_nan(fabsf(v[i].x), fabsf(v[i].y)), max_nan(fabsf(v[i].z), fabsf(v[i].w)));
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-        // !(top <= tiny): a NaN stays one
-        const float sc = !(top <= 0x1p-100f) ? __fdiv_rn(top, 448.0f) : 1.0f;
+        // the largest magnitude: as integers, whose order a NaN leads
+        const unsigned m = max(max(__float_as_uint(v[i].x) & 0x7fffffffu, __float_as_uint(v[i].y) & 0x7fffffffu),
+                               max(__float_as_uint(v[i].z) & 0x7fffffffu, __float_as_uint(v[i].w) & 0x7fffffffu));
+        const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, m));
+        float sc = 1.0f;
+        if (!(top < 0x1p+120f)) {  // (an infinity or NaN among them, or close to it)
+            sc = __fdiv_rn(top, 448.0f);
+            v[i] = make_float4(__fdiv_rn(v[i].x, sc), __fdiv_rn(v[i].y, sc), __fdiv_rn(v[i].z, sc),
+                               __fdiv_rn(v[i].w, sc));
+        } else if (top > 0x1p-100f) {
+            sc = divide(top, 448.0f, 1.0f / 448.0f);
+            float r;
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(sc));
+            r = fmaf(fmaf(-sc, r, 1.0f), r, r);  // (Newton: r to the last place)
+            v[i] = make_float4(divide(v[i].x, sc, r), divide(v[i].y, sc, r), divide(v[i].z, sc, r),
+                               divide(v[i].w, sc, r));
+        }
         if (live && col < d) {
-            const __nv_fp8x4_e4m3 r(make_float4(__fdiv_rn(v[i].x, sc), __fdiv_rn(v[i].y, sc),
-                                                __fdiv_rn(v[i].z, sc), __fdiv_rn(v[i].w, sc)));
+            const __nv_fp8x4_e4m3 r(v[i]);
             *reinterpret_cast<uint32_t *>(q + (int64_t)row * d + col) = r.__x;
             if (lane == 0) scale[(int64_t)(col >> 7) * ld_scale + row] = sc;
         }

@@ -17,7 +17,7 @@
 
 namespace {
 
-constexpr int NT = 256;
+constexpr int NT = 512;
 constexpr int MAX_REGIONS = 2 * BM_SLOT_REGIONS;
 constexpr int PIECE_MAX = 4096;
 
@@ -36,13 +36,17 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
 }
 
 // Dynamic shared memory: the list of moves ((src << 16) | dst, n_slots words
-// rounded up to 16 bytes), then `room` bytes of pieces.
+// rounded up to 16 bytes), then `buffers` times `room` bytes of pieces: with
+// two, the next piece's sources are read while this one's destinations are
+// written (one after the other took 112 us where this takes 98: 537 MB).
 __global__ void __launch_bounds__(NT)
-    reorder_kernel(const __grid_constant__ Regions g, const int32_t *src, int n_slots, int room) {
+    reorder_kernel(const __grid_constant__ Regions g, const int32_t *src, int n_slots, int room,
+                   int buffers) {
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ int n_moves;
+    __shared__ int n_moves, s_piece;
+    __shared__ unsigned per[MAX_REGIONS], items[MAX_REGIONS];
     uint32_t *list = reinterpret_cast<uint32_t *>(smem);
-    unsigned char *buf = smem + ((size_t)n_slots * 4 + 15) / 16 * 16;
+    unsigned char *const bufs = smem + ((size_t)n_slots * 4 + 15) / 16 * 16;
     if (threadIdx.x == 0) n_moves = 0;
     __syncthreads();
     for (int s = threadIdx.x; s < n_slots; s += NT) {
@@ -53,48 +57,83 @@ __global__ void __launch_bounds__(NT)
     __syncthreads();
     const int n = n_moves;
     if (n == 0) return;
-    // columns per piece: a power of two of which n fit the room, and small
-    // enough that every CTA has some
-    int64_t columns = 0;
-    for (int k = 0; k < g.n; ++k) columns += g.r[k].row_bytes * g.r[k].n_outer;
-    int piece = PIECE_MAX;
-    while (piece > 16 && ((int64_t)piece * n > room || (piece > 256 && columns < (int64_t)2 * piece * gridDim.x)))
-        piece >>= 1;
-    const uint32_t buf0 = (uint32_t)__cvta_generic_to_shared(buf);
-    int64_t item = blockIdx.x;
-    for (int k = 0; k < g.n; ++k) {
-        const Region &r = g.r[k];
-        const int64_t per = (r.row_bytes + piece - 1) / piece, items = per * r.n_outer;
-        for (; item < items; item += gridDim.x) {
-            const int64_t col = item % per * piece;
-            unsigned char *plane = r.base + item / per * r.outer_pitch + col;
-            const int bytes = (int)min((int64_t)piece, r.row_bytes - col);
-            const int words = bytes / r.unit;
-            const int total = n * words;
-            for (int i = threadIdx.x; i < total; i += NT) {
-                const int m = i / words, w = i - m * words;
-                const unsigned char *p = plane + (int64_t)(list[m] >> 16) * r.row_pitch + w * r.unit;
-                if (r.unit == 16)
-                    cp16(buf0 + m * piece + w * 16, p);
-                else
-                    *reinterpret_cast<uint32_t *>(buf + m * piece + w * 4) =
-                        *reinterpret_cast<const uint32_t *>(p);
-            }
-            asm volatile("cp.async.commit_group;\n cp.async.wait_all;" ::: "memory");
-            __syncthreads();  // every source is read
-            for (int i = threadIdx.x; i < total; i += NT) {
-                const int m = i / words, w = i - m * words;
-                unsigned char *p = plane + (int64_t)(list[m] & 0xffffu) * r.row_pitch + w * r.unit;
-                if (r.unit == 16)
-                    *reinterpret_cast<uint4 *>(p) =
-                        *reinterpret_cast<const uint4 *>(buf + m * piece + w * 16);
-                else
-                    *reinterpret_cast<uint32_t *>(p) =
-                        *reinterpret_cast<const uint32_t *>(buf + m * piece + w * 4);
-            }
-            __syncthreads();  // the buffer is free
+    // columns per piece: as many as fit the room n times, in lines of 128 bytes
+    // (pieces of 96 bytes took 139 us where 128 take 98) or a power of two
+    // below one; where that is less than a piece for every CTA, smaller ones
+    if (threadIdx.x == 0) {
+        int64_t columns = 0;
+        for (int k = 0; k < g.n; ++k) columns += g.r[k].row_bytes * g.r[k].n_outer;
+        int piece = min(PIECE_MAX, room / n);
+        if (piece >= 128) {
+            const int64_t share = (columns / gridDim.x + 127) & ~(int64_t)127;
+            piece = (int)max((int64_t)128, min((int64_t)piece, share)) & ~127;
+        } else {
+            piece = 1 << (31 - __clz(piece));  // (16 at least: the room is 16 bytes a slot)
         }
-        item -= items;
+        s_piece = piece;
+        for (int k = 0; k < g.n; ++k) {
+            per[k] = (unsigned)((g.r[k].row_bytes + piece - 1) / piece);
+            items[k] = per[k] * (unsigned)g.r[k].n_outer;
+        }
+    }
+    __syncthreads();
+    const int piece = s_piece;
+    // an item: a piece of columns of a plane of a region
+    struct Item {
+        int region;
+        unsigned at;
+    };
+    auto settle = [&](Item &i) {  // to the region that it falls into; false: past the last
+        for (; i.region < g.n; ++i.region) {
+            if (i.at < items[i.region]) return true;
+            i.at -= items[i.region];
+        }
+        return false;
+    };
+    auto each = [&](const Item &it, auto &&f) {
+        const Region &r = g.r[it.region];
+        const unsigned o = it.at / per[it.region];
+        const int64_t col = (int64_t)(it.at - o * per[it.region]) * piece;
+        unsigned char *plane = r.base + o * r.outer_pitch + col;
+        const int words = (int)min((int64_t)piece, r.row_bytes - col) / r.unit, total = n * words;
+        const unsigned inverse = 0xffffffffu / (unsigned)words + 1;  // (0 for one word)
+        for (int i = threadIdx.x; i < total; i += NT) {
+            // i / words, exact: i * words < 2^32
+            const int m = words == 1 ? i : (int)__umulhi((unsigned)i, inverse), w = i - m * words;
+            f(r.unit, plane + w * r.unit, r.row_pitch, list[m], m * piece + w * r.unit);
+        }
+    };
+    auto read = [&](const Item &it, unsigned char *buf) {
+        const uint32_t buf0 = (uint32_t)__cvta_generic_to_shared(buf);
+        each(it, [&](int unit, unsigned char *p, int64_t pitch, uint32_t move, int at) {
+            p += (int64_t)(move >> 16) * pitch;
+            if (unit == 16) cp16(buf0 + at, p);
+            else *reinterpret_cast<uint32_t *>(buf + at) = *reinterpret_cast<const uint32_t *>(p);
+        });
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    Item now{0, blockIdx.x};
+    bool more = settle(now);
+    if (more) read(now, bufs);
+    for (int k = 0; more; k ^= 1) {
+        Item next{now.region, now.at + gridDim.x};
+        more = settle(next);
+        unsigned char *buf = bufs + (buffers == 2 ? k * room : 0);
+        if (more && buffers == 2) {
+            read(next, bufs + (k ^ 1) * room);
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+        } else {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+        }
+        __syncthreads();  // every source of this item is read
+        each(now, [&](int unit, unsigned char *p, int64_t pitch, uint32_t move, int at) {
+            p += (int64_t)(move & 0xffffu) * pitch;
+            if (unit == 16) *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(buf + at);
+            else *reinterpret_cast<uint32_t *>(p) = *reinterpret_cast<const uint32_t *>(buf + at);
+        });
+        __syncthreads();  // the buffer is free
+        if (more && buffers == 1) read(next, bufs);
+        now = next;
     }
 }
 
@@ -116,6 +155,8 @@ int check_regions(const bm_slot_region_t *regions, int n_regions) {
         if (!r.base) why = "base is NULL";
         else if (r.row_bytes < 1 || r.n_outer < 1) why = "row_bytes or n_outer < 1";
         else if (!all_multiple(r, 4)) why = "base, row_bytes or a pitch not a multiple of 4";
+        else if (r.row_bytes > INT32_MAX || r.row_bytes / 16 * r.n_outer > INT32_MAX)
+            why = "more than 32 GB of columns";
         else if (r.row_pitch < r.row_bytes || (r.n_outer > 1 && r.outer_pitch < r.row_bytes))
             why = "a pitch below row_bytes";
         if (why) {
@@ -135,17 +176,21 @@ cudaError_t reorder(const bm_slot_region_t *regions, int n_regions, const int32_
                         regions[i].row_pitch, regions[i].outer_pitch, regions[i].n_outer,
                         all_multiple(regions[i], 16) ? 16 : 4};
     g.n = n_regions;
-    // 64 KB of pieces (three CTAs per SM), more where that is under 16 bytes a slot
-    const int room = n_slots * 16 > 65536 ? n_slots * 16 : 65536;
-    const size_t bytes = ((size_t)n_slots * 4 + 15) / 16 * 16 + (size_t)room;
+    // three CTAs per SM with a buffer of 64 KB each while that is a line or
+    // more of every slot, then one CTA with two of 96 KB, then one buffer
+    const int list = (n_slots * 4 + 15) / 16 * 16, per_sm = n_slots <= 400 ? 3 : 1;
+    const int buffers = n_slots > 400 && n_slots <= 4096 ? 2 : 1;
+    const int room = n_slots <= 400 ? 64 * 1024 : n_slots <= 4096 ? 96 * 1024 : n_slots * 16;
+    const size_t bytes = (size_t)list + (size_t)room * buffers;
     // the most that any call takes
-    constexpr int most = BM_SLOT_MAX * 4 + BM_SLOT_MAX * 16;
+    constexpr int most = 4096 * 4 + 2 * 96 * 1024;
+    static_assert(most >= BM_SLOT_MAX * (4 + 16), "shared memory");
     int device;
     cudaError_t e = cudaGetDevice(&device);
     static bmc::SharedMemory shm;
     if (e == cudaSuccess) e = shm.allow(reinterpret_cast<const void *>(reorder_kernel), most, device);
     if (e != cudaSuccess) return e;
-    reorder_kernel<<<sms * 3, NT, bytes, s>>>(g, d_src, n_slots, room);
+    reorder_kernel<<<sms * per_sm, NT, bytes, s>>>(g, d_src, n_slots, room, buffers);
     return cudaGetLastError();
 }
 
