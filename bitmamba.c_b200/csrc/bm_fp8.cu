@@ -219,7 +219,10 @@ struct ProductArgs {
 // Persistent CTAs with one tile after the other, or (split > 1) a cluster of
 // `split` CTAs per tile, each with a part of K: the others hand their sums to
 // the first through its shared memory, which adds them in order.  The scales
-// of a stay in shared memory, those of w in the lanes of a warp.
+// of a stay in shared memory, those of w in the lanes of a warp.  Two threads
+// issue copies and two MMAs, each every other block: one alone spends some 800
+// cycles a block on its waits, descriptors and commits (the blocks are
+// accumulations of their own, so their order does not matter).
 template <int NB>
 struct Few {
     static constexpr int BV = 128;
@@ -228,7 +231,7 @@ struct Few {
     static constexpr int TB = 4;                 // tensor memory buffers
     static constexpr int COLS = TB * NB;         // a power of two >= 32
     static constexpr int STAGE = BV * BKB + NB * BKB;
-    static constexpr int THREADS = 32 * (2 + PW);
+    static constexpr int THREADS = 32 * (4 + PW);
     static constexpr int MAX_STAGES = 12;
     static constexpr size_t BARS = (2 * MAX_STAGES + 2 * TB) * 8 + 16;
     static constexpr int SMEM = 220 * 1024;
@@ -279,54 +282,62 @@ __global__ void __launch_bounds__(Few<NB>::THREADS, 1)
     auto fail = [&]() { atomicOr(abort_, 1); };
     auto aborted = [&]() { return *reinterpret_cast<volatile int *>(abort_) != 0; };
 
-    if (threadIdx.x == 0) {
-        int s = 0, ph = 1;
-        for (int t = first; t < tiles && !aborted(); t += step) {
-            for (int kb = 0; kb < nkb; ++kb) {
-                if (!mbar_wait(&empty[s], ph)) {  // (a fresh barrier is past phase 1)
-                    fail();
-                    break;
+    // blocks and stages in turn: this thread's next ones
+    auto advance = [&](int &s, int &ph) {
+        s += 2;
+        if (s >= stages) {
+            s -= stages;
+            ph ^= 1;
+        }
+    };
+    if (warp < 2) {
+        if (lane == 0) {
+            int s = warp, ph = 1, g = 0;
+            for (int t = first; t < tiles && !aborted(); t += step) {
+                for (int kb = (g ^ warp) & 1; kb < nkb; kb += 2) {
+                    if (!mbar_wait(&empty[s], ph)) {  // (a fresh barrier is past phase 1)
+                        fail();
+                        break;
+                    }
+                    unsigned char *st = smem + (size_t)s * S::STAGE;
+                    mbar_expect_tx(&full[s], S::STAGE);
+                    tma_load_2d(st, &tmW, (kb0 + kb) * BKB, t * S::BV, &full[s]);
+                    tma_load_2d(st + S::BV * BKB, &tmA, (kb0 + kb) * BKB, 0, &full[s]);
+                    advance(s, ph);
                 }
-                unsigned char *st = smem + (size_t)s * S::STAGE;
-                mbar_expect_tx(&full[s], S::STAGE);
-                tma_load_2d(st, &tmW, (kb0 + kb) * BKB, t * S::BV, &full[s]);
-                tma_load_2d(st + S::BV * BKB, &tmA, (kb0 + kb) * BKB, 0, &full[s]);
-                if (++s == stages) {
-                    s = 0;
-                    ph ^= 1;
-                }
+                g += nkb;
             }
         }
-    } else if (threadIdx.x == 32) {
-        int s = 0, ph = 0, g = 0;
-        for (int t = first; t < tiles && !aborted(); t += step) {
-            for (int kb = 0; kb < nkb; ++kb, ++g) {
-                const int b = g % S::TB;
-                if (!mbar_wait(&acce[b], (g / S::TB + 1) & 1) || !mbar_wait(&full[s], ph)) {
-                    fail();
-                    break;
-                }
-                after_sync();
-                const uint32_t w0 = sa(smem + (size_t)s * S::STAGE), a0 = w0 + S::BV * BKB;
+    } else if (warp < 4) {
+        if (lane == 0) {
+            int s = warp - 2, ph = 0, g = 0;
+            for (int t = first; t < tiles && !aborted(); t += step) {
+                for (int kb = (g ^ warp) & 1; kb < nkb; kb += 2) {
+                    const int b = (g + kb) % S::TB;
+                    if (!mbar_wait(&acce[b], ((g + kb) / S::TB + 1) & 1) || !mbar_wait(&full[s], ph)) {
+                        fail();
+                        break;
+                    }
+                    after_sync();
+                    const uint32_t w0 = sa(smem + (size_t)s * S::STAGE), a0 = w0 + S::BV * BKB;
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    umma_f8(tmem + (uint32_t)(b * NB), sdesc(w0 + k * 32), sdesc(a0 + k * 32), f8_desc(NB),
-                            k > 0 ? 1u : 0u);
-                umma_commit(&empty[s]);
-                umma_commit(&accf[b]);
-                if (++s == stages) {
-                    s = 0;
-                    ph ^= 1;
+                    for (int k = 0; k < 4; ++k)
+                        umma_f8(tmem + (uint32_t)(b * NB), sdesc(w0 + k * 32), sdesc(a0 + k * 32), f8_desc(NB),
+                                k > 0 ? 1u : 0u);
+                    umma_commit(&empty[s]);
+                    umma_commit(&accf[b]);
+                    advance(s, ph);
                 }
+                g += nkb;
             }
         }
-    } else if (warp >= 2) {
-        for (int i = threadIdx.x - 64; i < nkb * NB; i += 32 * S::PW) {
+    } else {
+        for (int i = threadIdx.x - 128; i < nkb * NB; i += 32 * S::PW) {
             const int m = i % NB;
             scales[i] = m < p.M ? p.sa[(kb0 + i / NB) * p.ld_scale + m] : 0.0f;
         }
         asm volatile("bar.sync 1, %0;" ::"r"(32 * S::PW) : "memory");
-        const int q = warp & 3, c0 = ((warp - 2) >> 2) * S::CW;
+        const int q = warp & 3, c0 = ((warp - 4) >> 2) * S::CW;
         constexpr int LD = S::CW < 32 ? 16 : 32;
         int g = 0;
         // 32 blocks' scales of w in the lanes, the next ones on their way
@@ -417,7 +428,7 @@ __global__ void __launch_bounds__(Few<NB>::THREADS, 1)
             }
         }
     }
-    if (split > 1 && warp < 2) {
+    if (split > 1 && warp < 4) {
         // the cluster's two barriers, for the warps without sums
         __syncwarp();
         asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -465,8 +476,8 @@ cudaError_t few_rows(const uint8_t *a, const uint8_t *w, const ProductArgs &p, i
 // ---- many rows
 //
 // Persistent: CTA c takes tiles c, c + grid, ... (rows of a fastest, so CTAs
-// running together share w tiles).  Warp 0 lane 0 is the TMA producer, warp 1
-// lane 0 issues the MMAs, warps 4 to 11 promote: each has 32 rows by 128
+// running together share w tiles).  Warps 0 and 1 issue the copies, warps 2
+// and 3 the MMAs (as for few rows), warps 4 to 11 promote: each has 32 rows by 128
 // columns, a scale of a per thread and of w per warp.  128 sums and 64 values
 // on their way from tensor memory take more registers than an equal share, so
 // the first four warps give theirs up: 128 * 72 + 256 * 216 = 384 * 168, what
@@ -520,42 +531,51 @@ __global__ void __launch_bounds__(MANY_THREADS, 1)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     else
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-    if (threadIdx.x == 0) {
-        int g = 0;
-        for (int t = blockIdx.x; t < tiles && !aborted(); t += gridDim.x) {
-            const int m0 = t % MT * BM, n0 = t / MT * BN;
-            for (int kb = 0; kb < KB; ++kb, ++g) {
-                const int s = g % STAGES;
-                if (!mbar_wait(&empty[s], (g / STAGES + 1) & 1)) {
-                    fail();
-                    break;
+    static_assert(STAGES % 2 == 0 && TBUF == 2, "a thread has every other stage and its own buffer");
+    if (warp < 2) {
+        if (lane == 0) {
+            int g = 0;
+            for (int t = blockIdx.x; t < tiles && !aborted(); t += gridDim.x) {
+                const int m0 = t % MT * BM, n0 = t / MT * BN;
+                for (int kb = (g ^ warp) & 1; kb < KB; kb += 2) {
+                    const int s = (g + kb) % STAGES;
+                    if (!mbar_wait(&empty[s], ((g + kb) / STAGES + 1) & 1)) {
+                        fail();
+                        break;
+                    }
+                    unsigned char *st = smem + (size_t)s * STAGE_BYTES;
+                    mbar_expect_tx(&full[s], STAGE_BYTES);
+                    tma_load_2d(st, &tmA, kb * BKB, m0, &full[s]);
+                    tma_load_2d(st + BM * BKB, &tmW, kb * BKB, n0, &full[s]);
                 }
-                unsigned char *st = smem + (size_t)s * STAGE_BYTES;
-                mbar_expect_tx(&full[s], STAGE_BYTES);
-                tma_load_2d(st, &tmA, kb * BKB, m0, &full[s]);
-                tma_load_2d(st + BM * BKB, &tmW, kb * BKB, n0, &full[s]);
+                g += KB;
             }
         }
-    } else if (threadIdx.x == 32) {
-        int g = 0;
-        for (int t = blockIdx.x; t < tiles && !aborted(); t += gridDim.x) {
-            for (int kb = 0; kb < KB; ++kb, ++g) {
-                const int s = g % STAGES, b = g % TBUF;
-                if (!mbar_wait(&acce[b], (g / TBUF + 1) & 1) || !mbar_wait(&full[s], (g / STAGES) & 1)) {
-                    fail();
-                    break;
-                }
-                after_sync();
-                const uint32_t a0 = sa(smem + (size_t)s * STAGE_BYTES), w0 = a0 + BM * BKB;
+    } else if (warp < 4) {
+        if (lane == 0) {
+            const int b = warp & 1;
+            int g = 0;
+            for (int t = blockIdx.x; t < tiles && !aborted(); t += gridDim.x) {
+                for (int kb = (g ^ warp) & 1; kb < KB; kb += 2) {
+                    const int s = (g + kb) % STAGES;
+                    if (!mbar_wait(&acce[b], ((g + kb) / TBUF + 1) & 1) ||
+                        !mbar_wait(&full[s], ((g + kb) / STAGES) & 1)) {
+                        fail();
+                        break;
+                    }
+                    after_sync();
+                    const uint32_t a0 = sa(smem + (size_t)s * STAGE_BYTES), w0 = a0 + BM * BKB;
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    umma_f8(tmem + (uint32_t)(b * BN), sdesc(a0 + k * 32), sdesc(w0 + k * 32), f8_desc(BN),
-                            k > 0 ? 1u : 0u);
-                umma_commit(&empty[s]);
-                umma_commit(&accf[b]);
+                    for (int k = 0; k < 4; ++k)
+                        umma_f8(tmem + (uint32_t)(b * BN), sdesc(a0 + k * 32), sdesc(w0 + k * 32), f8_desc(BN),
+                                k > 0 ? 1u : 0u);
+                    umma_commit(&empty[s]);
+                    umma_commit(&accf[b]);
+                }
+                g += KB;
             }
         }
-    } else if (warp >= 4) {
+    } else {
         const int q = warp & 3, half = (warp - 4) >> 2, c0 = half * 128;
         float *turn = reinterpret_cast<float *>(smem + STAGES * STAGE_BYTES + (warp - 4) * TURN);
         const int NSW = (p.N + 127) / 128;
