@@ -13,7 +13,7 @@
 //   few rows    128 rows of w (the accumulator's lanes) by NB = 16 .. 128 rows
 //               of a (its columns), so that a few rows cost a narrow tile
 //               instead of a padded one.  Bound by the bytes of w.
-//   many rows   128 rows of a (lanes) by 256 rows of w: a thread's scale is
+//   many rows   128 rows of a (lanes) by 128 rows of w: a thread's scale is
 //               one value for its 128 columns.  (With w on the lanes every
 //               column has its own scale, and fetching 128 of them a block
 //               took twice as long as the tensor core's work.)
@@ -475,20 +475,23 @@ cudaError_t few_rows(const uint8_t *a, const uint8_t *w, const ProductArgs &p, i
 
 // ---- many rows
 //
-// Persistent: CTA c takes tiles c, c + grid, ... (rows of a fastest, so CTAs
-// running together share w tiles).  Warps 0 and 1 issue the copies, warps 2
-// and 3 the MMAs (as for few rows), warps 4 to 11 promote: each has 32 rows by 128
-// columns, a scale of a per thread and of w per warp.  128 sums and 64 values
-// on their way from tensor memory take more registers than an equal share, so
-// the first four warps give theirs up: 128 * 72 + 256 * 216 = 384 * 168, what
-// the block was launched with.
-constexpr int BM = 128, BN = 256, STAGES = 4, PROMOTE = 8, TBUF = 2;
+// Persistent: CTA c takes tiles c, c + grid, ... of 128 x 128 (rows of a
+// fastest, so CTAs running together share w tiles).  Warps 0 and 1 issue the
+// copies, warps 2 and 3 the MMAs (as for few rows).  Two groups of four warps
+// promote, every other tile each: while one group's sums go out, which takes
+// as long as several blocks, the tensor core works for the other.  (One tile of
+// 256 columns for all eight warps stood still then: 356 us for 2048 x 50257 x
+// 2048, of which 40 % were stores.)  A promotion thread has a row of a and 128
+// columns, so one scale a block; 128 sums and 64 values on their way from
+// tensor memory take more registers than an equal share, so the first four
+// warps give theirs up: 128 * 72 + 256 * 216 = 384 * 168, what the block was
+// launched with.
+constexpr int BM = 128, BN = 128, STAGES = 6, TBUF = 4;
 constexpr int STAGE_BYTES = (BM + BN) * BKB;
-constexpr int MANY_THREADS = 32 * (4 + PROMOTE);
+constexpr int MANY_THREADS = 32 * (4 + 8);
 constexpr int TURN = 17 * 32 * 4;  // a warp's 32 x 16 values on their way out
 constexpr int KRING = 8;           // blocks whose scales a thread has at hand
-constexpr size_t MANY_SMEM =
-    1024 + (size_t)STAGES * STAGE_BYTES + PROMOTE * TURN + KRING * PROMOTE * 32 * 4 + 256;
+constexpr size_t MANY_SMEM = 1024 + (size_t)STAGES * STAGE_BYTES + 8 * TURN + KRING * 256 * 4 + 256;
 
 __global__ void __launch_bounds__(MANY_THREADS, 1)
     many_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
@@ -496,16 +499,16 @@ __global__ void __launch_bounds__(MANY_THREADS, 1)
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     // (an offset, so that the compiler still knows it for shared memory)
     unsigned char *const smem = smem_raw + ((1024u - (sa(smem_raw) & 1023u)) & 1023u);
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + STAGES * STAGE_BYTES + PROMOTE * TURN +
-                                                  KRING * PROMOTE * 32 * 4);
+    unsigned char *const behind = smem + STAGES * STAGE_BYTES;
+    uint64_t *full = reinterpret_cast<uint64_t *>(behind + 8 * TURN + KRING * 256 * 4);
     uint64_t *empty = full + STAGES;
-    uint64_t *accf = empty + STAGES;
+    uint64_t *accf = empty + STAGES;  // [TBUF] buffers 2 w and 2 w + 1 are group w's
     uint64_t *acce = accf + TBUF;
     uint32_t *tslot = reinterpret_cast<uint32_t *>(acce + TBUF);
     int *abort_ = reinterpret_cast<int *>(tslot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int MT = (p.M + BM - 1) / BM, NTL = (p.N + BN - 1) / BN, KB = (p.K + BKB - 1) / BKB;
-    const int tiles = MT * NTL;
+    const int tiles = MT * NTL, step = gridDim.x;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) {
@@ -514,7 +517,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1)
         }
         for (int i = 0; i < TBUF; ++i) {
             mbar_init(&accf[i], 1);
-            mbar_init(&acce[i], PROMOTE);
+            mbar_init(&acce[i], 4);
         }
         *abort_ = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -531,15 +534,14 @@ __global__ void __launch_bounds__(MANY_THREADS, 1)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     else
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-    static_assert(STAGES % 2 == 0 && TBUF == 2, "a thread has every other stage and its own buffer");
+    static_assert(STAGES % 2 == 0, "a thread has every other stage");
     if (warp < 2) {
         if (lane == 0) {
-            int g = 0;
-            for (int t = blockIdx.x; t < tiles && !aborted(); t += gridDim.x) {
+            int g = 0, s = warp, ph = 1;
+            for (int t = blockIdx.x; t < tiles && !aborted(); t += step) {
                 const int m0 = t % MT * BM, n0 = t / MT * BN;
                 for (int kb = (g ^ warp) & 1; kb < KB; kb += 2) {
-                    const int s = (g + kb) % STAGES;
-                    if (!mbar_wait(&empty[s], ((g + kb) / STAGES + 1) & 1)) {
+                    if (!mbar_wait(&empty[s], ph)) {  // (a fresh barrier is past phase 1)
                         fail();
                         break;
                     }
@@ -547,19 +549,24 @@ __global__ void __launch_bounds__(MANY_THREADS, 1)
                     mbar_expect_tx(&full[s], STAGE_BYTES);
                     tma_load_2d(st, &tmA, kb * BKB, m0, &full[s]);
                     tma_load_2d(st + BM * BKB, &tmW, kb * BKB, n0, &full[s]);
+                    if ((s += 2) >= STAGES) {
+                        s -= STAGES;
+                        ph ^= 1;
+                    }
                 }
                 g += KB;
             }
         }
     } else if (warp < 4) {
         if (lane == 0) {
-            const int b = warp & 1;
-            int g = 0;
-            for (int t = blockIdx.x; t < tiles && !aborted(); t += gridDim.x) {
+            // a group's blocks go through its two buffers in turn; this thread
+            // has those of every other stage, as the copies do
+            int g = 0, s = warp & 1, ph = 0, w = 0, used[2] = {0, 0};
+            for (int t = blockIdx.x; t < tiles && !aborted(); t += step, w ^= 1) {
+                const int done = w ? used[1] : used[0];
                 for (int kb = (g ^ warp) & 1; kb < KB; kb += 2) {
-                    const int s = (g + kb) % STAGES;
-                    if (!mbar_wait(&acce[b], ((g + kb) / TBUF + 1) & 1) ||
-                        !mbar_wait(&full[s], ((g + kb) / STAGES) & 1)) {
+                    const int n = done + kb, b = 2 * w + (n & 1);
+                    if (!mbar_wait(&acce[b], (n / 2 + 1) & 1) || !mbar_wait(&full[s], ph)) {
                         fail();
                         break;
                     }
@@ -571,43 +578,49 @@ __global__ void __launch_bounds__(MANY_THREADS, 1)
                                 k > 0 ? 1u : 0u);
                     umma_commit(&empty[s]);
                     umma_commit(&accf[b]);
+                    if ((s += 2) >= STAGES) {
+                        s -= STAGES;
+                        ph ^= 1;
+                    }
                 }
                 g += KB;
+                if (w) used[1] += KB;
+                else used[0] += KB;
             }
         }
     } else {
-        const int q = warp & 3, half = (warp - 4) >> 2, c0 = half * 128;
-        float *turn = reinterpret_cast<float *>(smem + STAGES * STAGE_BYTES + (warp - 4) * TURN);
-        const int NSW = (p.N + 127) / 128;
-        int g = 0;
+        const int q = warp & 3, group = (warp - 4) >> 2;
+        float *turn = reinterpret_cast<float *>(behind + (warp - 4) * TURN);
         // This thread's scale for each block, in a ring of its own: four blocks
         // are loaded while the four before are used, and multiplied only then
-        // (a product right behind the loads would wait for them).
-        float *kr = reinterpret_cast<float *>(smem + STAGES * STAGE_BYTES + PROMOTE * TURN) + threadIdx.x - 128;
-        const float *pa = nullptr, *pw = nullptr;
-        int ahead_t = blockIdx.x, ahead_kb = 0;
+        // (a product right behind the loads would wait for them).  Rows and
+        // tiles past the last take the last one's.
+        float *kr = reinterpret_cast<float *>(behind + 8 * TURN) + threadIdx.x - 128;
+        const float *pa = p.sa, *pw = p.sw;
+        int ahead_t = blockIdx.x + group * step, ahead_kb = 0;
         float va[4], vw[4];
         auto load4 = [&]() {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if (ahead_kb == 0) {
-                    const int m = ahead_t % MT * BM + q * 32 + lane, nb = ahead_t / MT * 2 + half;
-                    pa = ahead_t < tiles && m < p.M && nb < NSW ? p.sa + m : nullptr;
-                    pw = p.sw + (int64_t)nb * KB;
+                    const int t = min(ahead_t, tiles - 1);
+                    pa = p.sa + min(t % MT * BM + q * 32 + lane, p.M - 1);
+                    pw = p.sw + (int64_t)(t / MT) * KB;
                 }
-                va[i] = pa ? *pa : 0.0f;
-                vw[i] = pa ? *pw : 0.0f;
-                if (pa) pa += p.ld_scale;
+                va[i] = *pa;
+                vw[i] = *pw;
+                pa += p.ld_scale;
                 ++pw;
                 if (++ahead_kb == KB) {
                     ahead_kb = 0;
-                    ahead_t += gridDim.x;
+                    ahead_t += 2 * step;
                 }
             }
         };
         load4();
-        for (int t = blockIdx.x; t < tiles && !aborted(); t += gridDim.x) {
-            const int m0 = t % MT * BM + q * 32, n0 = t / MT * BN + c0;
+        int g = 0;
+        for (int t = blockIdx.x + group * step; t < tiles && !aborted(); t += 2 * step) {
+            const int m0 = t % MT * BM + q * 32, n0 = t / MT * BN;
             float acc[128];
 #pragma unroll
             for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
@@ -615,19 +628,19 @@ __global__ void __launch_bounds__(MANY_THREADS, 1)
             for (int kb = 0; kb < KB; ++kb, ++g) {
                 if (g % 4 == 0) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) kr[(g + i) % KRING * (PROMOTE * 32)] = va[i] * vw[i];
+                    for (int i = 0; i < 4; ++i) kr[(g + i) % KRING * 256] = va[i] * vw[i];
                     load4();
                 }
-                const float k = kr[g % KRING * (PROMOTE * 32)];
-                const int b = g % TBUF;
-                const bool ok = mbar_wait(&accf[b], (g / TBUF) & 1);
+                const float k = kr[g % KRING * 256];
+                const int b = 2 * group + (g & 1);
+                const bool ok = mbar_wait(&accf[b], (g / 2) & 1);
                 if (__any_sync(0xffffffffu, !ok)) {
                     fail();
                     good = false;
                     break;
                 }
                 after_sync();
-                const uint32_t tb = tmem + (uint32_t)(b * BN + c0) + ((uint32_t)(q * 32) << 16);
+                const uint32_t tb = tmem + (uint32_t)(b * BN) + ((uint32_t)(q * 32) << 16);
 #pragma unroll
                 for (int c = 0; c < 128; c += 64) {
                     uint32_t v[2][32];
