@@ -257,7 +257,8 @@ __global__ void __launch_bounds__(Few<NB>::THREADS, 1)
     uint32_t *tslot = reinterpret_cast<uint32_t *>(acce + S::TB);
     int *abort_ = reinterpret_cast<int *>(tslot + 1);
     float *scales = reinterpret_cast<float *>(tslot + 4);  // [blocks][NB]
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // (from lane 0, so that the compiler knows it for one value a warp)
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int tiles = (p.N + S::BV - 1) / S::BV, KB = (p.K + BKB - 1) / BKB;
     const int rank = blockIdx.x % split, first = blockIdx.x / split, step = gridDim.x / split;
     const int kb0 = (int)((int64_t)KB * rank / split), nkb = (int)((int64_t)KB * (rank + 1) / split) - kb0;
@@ -476,22 +477,24 @@ cudaError_t few_rows(const uint8_t *a, const uint8_t *w, const ProductArgs &p, i
 // ---- many rows
 //
 // Persistent: CTA c takes tiles c, c + grid, ... of 128 x 128 (rows of a
-// fastest, so CTAs running together share w tiles).  Warps 0 and 1 issue the
-// copies, warps 2 and 3 the MMAs (as for few rows).  Two groups of four warps
-// promote, every other tile each: while one group's sums go out, which takes
-// as long as several blocks, the tensor core works for the other.  (One tile of
-// 256 columns for all eight warps stood still then: 356 us for 2048 x 50257 x
-// 2048, of which 40 % were stores.)  A promotion thread has a row of a and 128
-// columns, so one scale a block; 128 sums and 64 values on their way from
-// tensor memory take more registers than an equal share, so the first four
-// warps give theirs up: 128 * 72 + 256 * 216 = 384 * 168, what the block was
-// launched with.
-constexpr int BM = 128, BN = 128, STAGES = 6, TBUF = 4;
+// fastest, so CTAs running together share w tiles), in two pipelines of every
+// other tile each: a thread that issues copies (warps 0, 1), one that issues
+// MMAs (warps 2, 3), three stages, two tensor memory buffers and four warps
+// that promote.  A promotion thread has a row of a and 128 columns, so one
+// scale a block.  Promoting a block takes a warp longer than the tensor core
+// needs for it, and a tile's sums take as long as several blocks to go out:
+// with two pipelines, one works while the other waits.  (One tile of 256
+// columns for all eight warps: 356 us for 2048 x 50257 x 2048, 40 % of them
+// stores; two groups behind one pipeline: 327 us.)  128 sums and 64 values on
+// their way from tensor memory take more registers than an equal share, so the
+// first four warps give theirs up: 128 * 72 + 256 * 216 = 384 * 168, what the
+// block was launched with.
+constexpr int BM = 128, BN = 128, STAGES = 3, TBUF = 2;  // (of a pipeline)
 constexpr int STAGE_BYTES = (BM + BN) * BKB;
 constexpr int MANY_THREADS = 32 * (4 + 8);
 constexpr int TURN = 17 * 32 * 4;  // a warp's 32 x 16 values on their way out
 constexpr int KRING = 8;           // blocks whose scales a thread has at hand
-constexpr size_t MANY_SMEM = 1024 + (size_t)STAGES * STAGE_BYTES + 8 * TURN + KRING * 256 * 4 + 256;
+constexpr size_t MANY_SMEM = 1024 + (size_t)2 * STAGES * STAGE_BYTES + 8 * TURN + KRING * 256 * 4 + 256;
 
 __global__ void __launch_bounds__(MANY_THREADS, 1)
     many_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
@@ -499,97 +502,84 @@ __global__ void __launch_bounds__(MANY_THREADS, 1)
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     // (an offset, so that the compiler still knows it for shared memory)
     unsigned char *const smem = smem_raw + ((1024u - (sa(smem_raw) & 1023u)) & 1023u);
-    unsigned char *const behind = smem + STAGES * STAGE_BYTES;
-    uint64_t *full = reinterpret_cast<uint64_t *>(behind + 8 * TURN + KRING * 256 * 4);
-    uint64_t *empty = full + STAGES;
-    uint64_t *accf = empty + STAGES;  // [TBUF] buffers 2 w and 2 w + 1 are group w's
-    uint64_t *acce = accf + TBUF;
-    uint32_t *tslot = reinterpret_cast<uint32_t *>(acce + TBUF);
+    unsigned char *const behind = smem + 2 * STAGES * STAGE_BYTES;
+    // the pipeline of this thread, and its barriers
+    // (from lane 0, so that the compiler knows it for one value a warp)
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const int line = warp < 4 ? warp & 1 : (warp - 4) >> 2;
+    uint64_t *const bars = reinterpret_cast<uint64_t *>(behind + 8 * TURN + KRING * 256 * 4);
+    constexpr int BARS = 2 * STAGES + 2 * TBUF;
+    uint64_t *const full = bars + line * BARS, *const empty = full + STAGES;
+    uint64_t *const accf = empty + STAGES, *const acce = accf + TBUF;
+    uint32_t *tslot = reinterpret_cast<uint32_t *>(bars + 2 * BARS);
     int *abort_ = reinterpret_cast<int *>(tslot + 1);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    unsigned char *const stages = smem + line * STAGES * STAGE_BYTES;
     const int MT = (p.M + BM - 1) / BM, NTL = (p.N + BN - 1) / BN, KB = (p.K + BKB - 1) / BKB;
     const int tiles = MT * NTL, step = gridDim.x;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < STAGES; ++i) {
-            mbar_init(&full[i], 1);
-            mbar_init(&empty[i], 1);
-        }
-        for (int i = 0; i < TBUF; ++i) {
-            mbar_init(&accf[i], 1);
-            mbar_init(&acce[i], 4);
-        }
+        for (int i = 0; i < 2 * BARS; ++i) mbar_init(&bars[i], i % BARS < BARS - TBUF ? 1 : 4);
         *abort_ = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 0) tmem_alloc(tslot, TBUF * BN);
+    if (warp == 0) tmem_alloc(tslot, 2 * TBUF * BN);
     before_sync();
     __syncthreads();
     after_sync();
-    const uint32_t tmem = *tslot;
+    const uint32_t tmem = *tslot + (uint32_t)(line * TBUF * BN);
     auto fail = [&]() { atomicOr(abort_, 1); };
     auto aborted = [&]() { return *reinterpret_cast<volatile int *>(abort_) != 0; };
 
-    if (warp < 4)
+    const int first = blockIdx.x + line * step;
+    if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    else
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-    static_assert(STAGES % 2 == 0, "a thread has every other stage");
-    if (warp < 2) {
-        if (lane == 0) {
-            int g = 0, s = warp, ph = 1;
-            for (int t = blockIdx.x; t < tiles && !aborted(); t += step) {
+        if (warp < 2 && lane == 0) {
+            int s = 0, ph = 1;
+            for (int t = first; t < tiles && !aborted(); t += 2 * step) {
                 const int m0 = t % MT * BM, n0 = t / MT * BN;
-                for (int kb = (g ^ warp) & 1; kb < KB; kb += 2) {
+                for (int kb = 0; kb < KB; ++kb) {
                     if (!mbar_wait(&empty[s], ph)) {  // (a fresh barrier is past phase 1)
                         fail();
                         break;
                     }
-                    unsigned char *st = smem + (size_t)s * STAGE_BYTES;
+                    unsigned char *st = stages + s * STAGE_BYTES;
                     mbar_expect_tx(&full[s], STAGE_BYTES);
                     tma_load_2d(st, &tmA, kb * BKB, m0, &full[s]);
                     tma_load_2d(st + BM * BKB, &tmW, kb * BKB, n0, &full[s]);
-                    if ((s += 2) >= STAGES) {
-                        s -= STAGES;
+                    if (++s == STAGES) {
+                        s = 0;
                         ph ^= 1;
                     }
                 }
-                g += KB;
             }
         }
-    } else if (warp < 4) {
-        if (lane == 0) {
-            // a group's blocks go through its two buffers in turn; this thread
-            // has those of every other stage, as the copies do
-            int g = 0, s = warp & 1, ph = 0, w = 0, used[2] = {0, 0};
-            for (int t = blockIdx.x; t < tiles && !aborted(); t += step, w ^= 1) {
-                const int done = w ? used[1] : used[0];
-                for (int kb = (g ^ warp) & 1; kb < KB; kb += 2) {
-                    const int n = done + kb, b = 2 * w + (n & 1);
-                    if (!mbar_wait(&acce[b], (n / 2 + 1) & 1) || !mbar_wait(&full[s], ph)) {
+        if (warp >= 2 && lane == 0) {
+            int g = 0, s = 0, ph = 0;
+            for (int t = first; t < tiles && !aborted(); t += 2 * step) {
+                for (int kb = 0; kb < KB; ++kb, ++g) {
+                    const int b = g & 1;
+                    if (!mbar_wait(&acce[b], (g / 2 + 1) & 1) || !mbar_wait(&full[s], ph)) {
                         fail();
                         break;
                     }
                     after_sync();
-                    const uint32_t a0 = sa(smem + (size_t)s * STAGE_BYTES), w0 = a0 + BM * BKB;
+                    const uint32_t a0 = sa(stages + s * STAGE_BYTES), w0 = a0 + BM * BKB;
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
                         umma_f8(tmem + (uint32_t)(b * BN), sdesc(a0 + k * 32), sdesc(w0 + k * 32), f8_desc(BN),
                                 k > 0 ? 1u : 0u);
                     umma_commit(&empty[s]);
                     umma_commit(&accf[b]);
-                    if ((s += 2) >= STAGES) {
-                        s -= STAGES;
+                    if (++s == STAGES) {
+                        s = 0;
                         ph ^= 1;
                     }
                 }
-                g += KB;
-                if (w) used[1] += KB;
-                else used[0] += KB;
             }
         }
     } else {
-        const int q = warp & 3, group = (warp - 4) >> 2;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        const int q = warp & 3;
         float *turn = reinterpret_cast<float *>(behind + (warp - 4) * TURN);
         // This thread's scale for each block, in a ring of its own: four blocks
         // are loaded while the four before are used, and multiplied only then
@@ -597,7 +587,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1)
         // tiles past the last take the last one's.
         float *kr = reinterpret_cast<float *>(behind + 8 * TURN) + threadIdx.x - 128;
         const float *pa = p.sa, *pw = p.sw;
-        int ahead_t = blockIdx.x + group * step, ahead_kb = 0;
+        int ahead_t = first, ahead_kb = 0;
         float va[4], vw[4];
         auto load4 = [&]() {
 #pragma unroll
@@ -619,7 +609,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1)
         };
         load4();
         int g = 0;
-        for (int t = blockIdx.x + group * step; t < tiles && !aborted(); t += 2 * step) {
+        for (int t = first; t < tiles && !aborted(); t += 2 * step) {
             const int m0 = t % MT * BM + q * 32, n0 = t / MT * BN;
             float acc[128];
 #pragma unroll
@@ -632,7 +622,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1)
                     load4();
                 }
                 const float k = kr[g % KRING * 256];
-                const int b = 2 * group + (g & 1);
+                const int b = g & 1;
                 const bool ok = mbar_wait(&accf[b], (g / 2) & 1);
                 if (__any_sync(0xffffffffu, !ok)) {
                     fail();
@@ -683,7 +673,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1)
     __syncwarp();
     before_sync();
     __syncthreads();
-    if (warp == 0) tmem_free(tmem, TBUF * BN);
+    if (warp == 0) tmem_free(*tslot, 2 * TBUF * BN);
     if (threadIdx.x == 0 && *abort_) atomicOr(p.err, 4);
 }
 
