@@ -492,7 +492,7 @@ cudaError_t few_rows(const uint8_t *a, const uint8_t *w, const ProductArgs &p, i
 constexpr int BM = 128, BN = 128, STAGES = 3, TBUF = 2;  // (of a pipeline)
 constexpr int STAGE_BYTES = (BM + BN) * BKB;
 constexpr int MANY_THREADS = 32 * (4 + 8);
-constexpr int TURN = 17 * 32 * 4;  // a warp's 32 x 16 values on their way out
+constexpr int TURN = 33 * 16 * 4;  // a warp's 16 x 32 values on their way out
 constexpr int KRING = 8;           // blocks whose scales a thread has at hand
 constexpr size_t MANY_SMEM = 1024 + (size_t)2 * STAGES * STAGE_BYTES + 8 * TURN + KRING * 256 * 4 + 256;
 
@@ -647,26 +647,33 @@ __global__ void __launch_bounds__(MANY_THREADS, 1)
                     for (int j = 0; j < 64; ++j) acc[c + j] = fmaf(as_f(v[j / 32][j % 32]), k, acc[c + j]);
                 }
             }
-            // 16 columns at a time through shared memory: half a warp's store is
-            // 16 consecutive values of a row, whatever the pitch
-            const int rows = min(32, p.M - m0), hl = lane & 15, hw = lane >> 4;
+            // 32 columns of 16 rows at a time through shared memory: a store is
+            // 32 consecutive values of a row, whatever the pitch (two rows of 16
+            // took 6 % longer in all, whole 128-byte lines of rows staged in
+            // full 60 %, as the warp's own work)
+            const int rows = min(32, p.M - m0);
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                if (!good || rows <= 0 || n0 + c * 16 >= p.N) continue;
+            for (int c = 0; c < 4; ++c) {
+                if (!good || rows <= 0 || n0 + c * 32 >= p.N) continue;
+                const int n = n0 + c * 32 + lane;
 #pragma unroll
-                for (int j = 0; j < 16; ++j) turn[lane * 17 + j] = acc[c * 16 + j];
-                __syncwarp();
-                const int n = n0 + c * 16 + hl;
-                if (n < p.N) {
-                    float *o = p.out + (int64_t)(m0 + hw) * p.ldo + n;
-                    if (rows == 32) {
+                for (int r = 0; r < 32; r += 16) {
+                    if ((lane & 16) == r) {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i, o += 2 * p.ldo) *o = turn[(2 * i + hw) * 17 + hl];
-                    } else {
-                        for (int i = hw; i < rows; i += 2, o += 2 * p.ldo) *o = turn[i * 17 + hl];
+                        for (int j = 0; j < 32; ++j) turn[(lane & 15) * 33 + j] = acc[c * 32 + j];
                     }
+                    __syncwarp();
+                    if (n < p.N) {
+                        float *o = p.out + (int64_t)(m0 + r) * p.ldo + n;
+                        if (rows == 32) {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i, o += p.ldo) *o = turn[i * 33 + lane];
+                        } else {
+                            for (int i = 0; i < 16 && r + i < rows; ++i, o += p.ldo) *o = turn[i * 33 + lane];
+                        }
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
             }
         }
     }
