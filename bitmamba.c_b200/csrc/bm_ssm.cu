@@ -9,6 +9,7 @@
 // and 1 ulp) are not multiplied up.
 #include <climits>
 #include <cstdint>
+#include <type_traits>
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -239,8 +240,8 @@ struct Tile {
     // parts of a warp (of half a warp, for 8-byte words) meet in no bank
     static constexpr int PAD = CG * VEC * sizeof(T) >= 128 ? 0 : CG;
     static constexpr int WORDS = ROWS * CG + ST * PAD;
-    // x and z, twice
-    static constexpr size_t STAGED = 4 * (size_t)WORDS * VEC * sizeof(T);
+    // x and z
+    static constexpr size_t STAGED = 2 * (size_t)WORDS * VEC * sizeof(T);
     // a head's scalars (a, g, c, C times the part's decays up to the row) and
     // its parts' decays, twice
     static constexpr size_t PER_HEAD = 2 * (size_t)(ROWS * 16 + ST * 4);
@@ -296,7 +297,7 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
     __shared__ Word init_x[ST][3][CG];
     __shared__ V part_s[ST][CG + 1], came[ST][CG + 1], halo[3][CG];
     __shared__ float part_a[ST][CG + 1];
-    Word *const staged = reinterpret_cast<Word *>(smem);  // x0, z0, x1, z1
+    Word *const staged = reinterpret_cast<Word *>(smem);  // x, then z
     float4 *const tabs = reinterpret_cast<float4 *>(smem + L::STAGED);
     float *const decs = reinterpret_cast<float *>(tabs + 2 * heads * ROWS);
     const int C = p.l.C, P = p.l.P, tid = threadIdx.x, lane = tid & 31;
@@ -308,36 +309,37 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
     constexpr unsigned mask = LC == 32 ? 0xffffffffu : (1u << LC % 32) - 1u;
     const bool gate = p.z && !SUMS;
 
+    auto stage_rows = [&](int r0, const void *from, Word *dst) {
+        const int live = min(ROWS, seg1 - r0);
+        const T *src = static_cast<const T *>(from) + r0 * p.ld + c0;
+        if (wide) {  // 16 bytes at a time
+            constexpr int E = 16 / (int)sizeof(T), CH = CG * VEC / E;  // elements, chunks of a row
+            constexpr int STEP = NT / CH;                             // rows a pass
+            static_assert(STEP % LC == 0, "a pass is whole parts");
+            const int i = tid % CH, r = tid / CH;
+            const T *q = src + i * E + r * p.ld;
+            const uint32_t a0 = (uint32_t)__cvta_generic_to_shared(dst + r * CG + i * (E / VEC) + r / LC * L::PAD);
+            auto copy = [&](int n) {
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                                 a0 + n * (STEP * CG + STEP / LC * L::PAD) * (int)sizeof(Word)),
+                             "l"(q)
+                             : "memory");
+            };
+            if (live == ROWS) {
+#pragma unroll
+                for (int n = 0; n < ROWS / STEP; ++n, q += STEP * p.ld) copy(n);
+            } else {
+                for (int n = 0; r + n * STEP < live; ++n, q += STEP * p.ld) copy(n);
+            }
+        } else if (on) {
+            for (int r = part; r < live; r += ST)
+                stage(dst + r * CG + r / LC * L::PAD + cg, src + cg * VEC + r * p.ld, Word());
+        }
+    };
+    // x of a tile, and its head scalars
     auto stage_in = [&](int r0, int buf) {
         const int live = min(ROWS, seg1 - r0);
-        for (int k = 0; k < (gate ? 2 : 1); ++k) {
-            const T *src = static_cast<const T *>(k ? p.z : p.x) + r0 * p.ld + c0;
-            Word *dst = staged + (2 * buf + k) * L::WORDS;
-            if (wide) {  // 16 bytes at a time
-                constexpr int E = 16 / (int)sizeof(T), CH = CG * VEC / E;  // elements, chunks of a row
-                constexpr int STEP = NT / CH;                             // rows a pass
-                const int i = tid % CH, r = tid / CH;
-                const T *q = src + i * E + r * p.ld;
-                Word *d = dst + r * CG + i * (E / VEC);
-                static_assert(STEP % LC == 0, "a pass is whole parts");
-                const uint32_t a0 = (uint32_t)__cvta_generic_to_shared(d + r / LC * L::PAD);
-                auto copy = [&](int n) {
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                                     a0 + n * (STEP * CG + STEP / LC * L::PAD) * (int)sizeof(Word)),
-                                 "l"(q)
-                                 : "memory");
-                };
-                if (live == ROWS) {
-#pragma unroll
-                    for (int n = 0; n < ROWS / STEP; ++n, q += STEP * p.ld) copy(n);
-                } else {
-                    for (int n = 0; r + n * STEP < live; ++n, q += STEP * p.ld) copy(n);
-                }
-            } else if (on) {
-                for (int r = part; r < live; r += ST)
-                    stage(dst + r * CG + r / LC * L::PAD + cg, src + cg * VEC + r * p.ld, Word());
-            }
-        }
+        stage_rows(r0, p.x, staged);
         if (PRE) {
             const int parts = (live + LC - 1) / LC * LC;
             for (int i = tid; i < nh * ROWS; i += NT) {
@@ -351,8 +353,8 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
                     stage(decs + (buf * heads + h) * ST + t / LC, p.dec + (int64_t)(r0 + t) / LC * p.l.H + h0 + h, 0.0f);
             }
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    auto commit = []() { asm volatile("cp.async.commit_group;" ::: "memory"); };
     // consecutive lanes are consecutive rows
     auto head_table = [&](int r0, int buf) {
         for (int i = tid; i < nh * ROWS; i += NT) {
@@ -418,6 +420,7 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
 
     // ---- before the first tile
     if (seg0 < seg1) stage_in(seg0, 0);
+    commit();
     V w0, w1, w2, w3, bias, dd;
     {
         float4 a = make_float4(0, 0, 0, 0), b = a;
@@ -491,7 +494,7 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
         stage(&init_h[part][cg], p.l.h + (int64_t)(info >> 4) * C + ch, V());
 #pragma unroll
         for (int k = 0; k < 3; ++k) stage(&init_x[part][k][cg], conv_at(info >> 4, k), Word());
-        asm volatile("cp.async.commit_group;" ::: "memory");
+        commit();
     };
     __syncthreads();
     fetch_init();
@@ -503,7 +506,10 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         __syncthreads();
         const int r1 = r0 + ROWS;
-        if (r1 < seg1) stage_in(r1, buf ^ 1);
+        // z arrives during the scan of x; the next tile's x, when this one's is
+        // done with, during the outputs
+        if (gate) stage_rows(r0, p.z, staged + L::WORDS);
+        commit();
         unsigned valid = mask, start = 0, end = 0;
         if (!plain) {
             valid = row_valid[b0 / 32] >> b0 % 32 & mask;
@@ -512,7 +518,7 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
         }
         const int *info = row_info + b0;
         const float4 *tb = tabs + (buf * heads + hh) * ROWS + b0;
-        const Word *xw = staged + 2 * buf * L::WORDS + b0 * CG + part * L::PAD + cg, *zw = xw + L::WORDS;
+        const Word *xw = staged + b0 * CG + part * L::PAD + cg, *zw = xw + L::WORDS;
 
         // x1, x2, x3: the inputs 1, 2, 3 tokens back; from the slot before the
         // sequence's first
@@ -549,11 +555,13 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
             x1 = xt;
             return k.x;
         };
-        if (valid == mask && !start && !end && (plain || (info[0] & 3) == 3)) {
+        // (by warps: one with both kinds of part would run both loops)
+        const bool even = plain || (valid == mask && !start && !end && (info[0] & 3) == 3);
+        if (__all_sync(0xffffffffu, even)) {
 #pragma unroll
             for (int t = 0; t < LC; ++t) token(t);
         } else {
-            if ((valid & 1u) && !(start & 1u)) {
+            if (!even && (valid & 1u) && !(start & 1u)) {
                 const int place = info[0] & 3;
                 if (place < 3) x3 = back(3, place, info[0]);
                 if (place < 2) x2 = back(2, place, info[0]);
@@ -601,6 +609,8 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
         part_a[part][cg] = start ? SET : decs[(buf * heads + hh) * ST + part];
         if (!PRE && r1 < seg1) head_table(r1, buf ^ 1);
         __syncthreads();
+        if (r1 < seg1) stage_in(r1, buf ^ 1);
+        commit();
         if (part == ST - 1) {
             halo[0][cg] = x1;
             halo[1][cg] = x2;
@@ -635,6 +645,7 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
             }
             plain = same;
         }
+        asm volatile("cp.async.wait_group 1;" ::: "memory");  // z
         __syncthreads();
         if (r1 < seg1 && !plain) fetch_init();
         const V hin = came[part][cg];
@@ -658,26 +669,28 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
         if (!SUMS && on) {
             const int first = start ? __ffs(start) - 1 : LC;
             T *py = static_cast<T *>(p.y) + ch + (r0 + b0) * p.ldy;
-            auto finish = [&](int t, bool fix) {
+            auto finish = [&](int t, bool fix, auto gated) {
                 V o = y[t];
-                if (fix) {
-                    o = sfma(tb[t].w, hin, o);
-                }
-                if (gate) {
+                if (fix) o = sfma(tb[t].w, hin, o);
+                if (decltype(gated)::value) {
                     R zr;
                     zr.v = zw[t * CG];
                     o = vmul(o, silu(zr.get()));
                 }
                 put(py, o);
             };
-            if (valid == mask && !start) {
+            auto outputs = [&](auto gated) {
+                if (__all_sync(__activemask(), valid == mask && !start)) {
 #pragma unroll
-                for (int t = 0; t < LC; ++t, py += p.ldy) finish(t, true);
-            } else {
+                    for (int t = 0; t < LC; ++t, py += p.ldy) finish(t, true, gated);
+                } else {
 #pragma unroll
-                for (int t = 0; t < LC; ++t, py += p.ldy)
-                    if (valid >> t & 1u) finish(t, t < first);
-            }
+                    for (int t = 0; t < LC; ++t, py += p.ldy)
+                        if (valid >> t & 1u) finish(t, t < first, gated);
+                }
+            };
+            if (gate) outputs(std::true_type());
+            else outputs(std::false_type());
         }
     }
     if (SUMS) {
