@@ -144,11 +144,11 @@ __device__ __forceinline__ Head head_of(const Args &p, int64_t row, int h) {
 //
 // A CTA's channels are 64 to 128 bytes of a row, so a few dozen to hundreds of
 // CTAs share a prompt with nothing between them.  Where that leaves SMs idle
-// (few channels, many rows), the rows are cut into segments too: a first
-// launch takes each segment's (A, S) from a zero state, the second starts
-// every segment from those before it, and a third writes the states of
-// sequences that ended in another segment than they began in (before that,
-// their first segment may still have to read the slot).
+// (few channels, many rows), a cluster takes as many tiles at once as it has
+// CTAs: each leaves its tile's (A, S) in its shared memory, and after one
+// cluster barrier reads the others' to know the state that comes in.  (In a
+// launch for the sums of segments, one that starts from them and one that
+// writes the states of sequences across them, 2000 x 2048 fp32 took 41 us.)
 //
 // Measured against it: tiles joined by published words and a look-back (one
 // launch, any number of CTAs on an axis) took 0.91 ms for 65536 x 4096 bf16
@@ -221,16 +221,6 @@ __device__ __forceinline__ float2 shfl_at(float2 v, int l, int w) {
     return make_float2(shfl_at(v.x, l, w), shfl_at(v.y, l, w));
 }
 
-// Segments of the token axis, and what their launches hand on (in the
-// context's workspace): S [seg][C], A [seg][H], the states to write [seg][C]
-// with the inputs [seg][3][C], and their slots [seg][CTA] (-1: none).
-struct Segments {
-    int n, rows;  // rows of a segment, a multiple of the tile
-    float *S, *A, *h;
-    void *conv;
-    int *slot;
-};
-
 constexpr int SEQ_CACHE = 1024;  // sequences whose offsets a CTA keeps in shared memory
 
 template <typename T, int VEC, int CG, int ST, int LC>
@@ -276,10 +266,25 @@ __global__ void __launch_bounds__(128) heads_kernel(const Args p, float4 *tab, f
     dec[i] = prod;
 }
 
-// SUMS: only the segment's (A, S).  PRE: the head scalars come from p.tab.
-template <typename T, int VEC, int CG, int ST, int LC, int PER_SM, bool PRE, bool SUMS>
-__global__ void __launch_bounds__(CG *ST, PER_SM)
-    prefill_kernel(const Args p, const Segments g, int heads, int wide) {
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// a value in the shared memory of another CTA of the cluster
+__device__ __forceinline__ uint32_t remote(const void *p, int rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void load_remote(uint32_t at, float &v) {
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void load_remote(uint32_t at, float2 &v) {
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+}
+
+// PRE: the head scalars come from p.tab.  gridDim.y: CTAs of a cluster.
+template <typename T, int VEC, int CG, int ST, int LC, int PER_SM, bool PRE>
+__global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, int heads, int wide) {
     using L = Tile<T, VEC, CG, ST, LC>;
     using R = Raw<T, VEC>;
     using Word = typename R::Word;
@@ -295,22 +300,27 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
     // next tile takes from its slot
     __shared__ V init_h[ST][CG];
     __shared__ Word init_x[ST][3][CG];
-    __shared__ V part_s[ST][CG + 1], came[ST][CG + 1], halo[3][CG];
+    __shared__ V part_s[ST][CG + 1], came[ST][CG + 1];
     __shared__ float part_a[ST][CG + 1];
+    __shared__ Word halo[3][CG];  // the three rows above the tile
+    // the tile's (A, S), of this step and the one before
+    __shared__ V tile_s[2][CG];
+    __shared__ float tile_a[2][CG];
     Word *const staged = reinterpret_cast<Word *>(smem);  // x, then z
     float4 *const tabs = reinterpret_cast<float4 *>(smem + L::STAGED);
     float *const decs = reinterpret_cast<float *>(tabs + 2 * heads * ROWS);
     const int C = p.l.C, P = p.l.P, tid = threadIdx.x, lane = tid & 31;
     const int cg = tid % CG, part = tid / CG, b0 = part * LC;
-    const int seg = blockIdx.y, c0 = blockIdx.x * (CG * VEC), ch = c0 + cg * VEC;
-    const int seg0 = seg * g.rows, seg1 = min(p.rows, seg0 + g.rows);
+    const int rank = blockIdx.y, many = gridDim.y;  // (of a cluster)
+    const int c0 = blockIdx.x * (CG * VEC), ch = c0 + cg * VEC;
+    const int first = rank * ROWS, step = many * ROWS;  // this CTA's first row, and to its next tile
     const bool on = ch < C;
     const int h0 = c0 / P, nh = (min(c0 + CG * VEC, C) - 1) / P - h0 + 1, hh = (on ? ch : c0) / P - h0;
     constexpr unsigned mask = LC == 32 ? 0xffffffffu : (1u << LC % 32) - 1u;
-    const bool gate = p.z && !SUMS;
+    const bool gate = p.z != nullptr;
 
     auto stage_rows = [&](int r0, const void *from, Word *dst) {
-        const int live = min(ROWS, seg1 - r0);
+        const int live = min(ROWS, p.rows - r0);
         const T *src = static_cast<const T *>(from) + r0 * p.ld + c0;
         if (wide) {  // 16 bytes at a time
             constexpr int E = 16 / (int)sizeof(T), CH = CG * VEC / E;  // elements, chunks of a row
@@ -338,8 +348,9 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
     };
     // x of a tile, and its head scalars
     auto stage_in = [&](int r0, int buf) {
-        const int live = min(ROWS, seg1 - r0);
+        const int live = min(ROWS, p.rows - r0);
         stage_rows(r0, p.x, staged);
+        if (on && part < 3 && r0 > part) stage(&halo[part][cg], static_cast<const T *>(p.x) + ch + (r0 - 1 - part) * p.ld, Word());
         if (PRE) {
             const int parts = (live + LC - 1) / LC * LC;
             for (int i = tid; i < nh * ROWS; i += NT) {
@@ -360,7 +371,7 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
         for (int i = tid; i < nh * ROWS; i += NT) {
             const int h = i / ROWS, t = i % ROWS;
             Head k{0.0f, 0.0f, 0.0f};
-            if (r0 + t < seg1) k = head_of<T>(p, r0 + t, h0 + h);
+            if (r0 + t < p.rows) k = head_of<T>(p, r0 + t, h0 + h);
             float prod = k.a;
 #pragma unroll
             for (int o = 1; o < LC; o <<= 1) {
@@ -381,9 +392,9 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
         const int fresh = p.fresh ? p.fresh[s] != 0 : 1;
         return slot >= 0 && slot < p.l.n_slots ? slot << 4 | fresh << 2 : -1;
     };
-    // What the rows of a tile are, a thread a row.  row_info: slot << 4 | began
-    // before the segment << 3 | fresh << 2 | place in the sequence (3 and
-    // above: 3), or -1 for a row of no sequence; the masks have a bit per row.
+    // What the rows of a tile are, a thread a row.  row_info: slot << 4 | fresh
+    // << 2 | place in the sequence (3 and above: 3), or -1 for a row of no
+    // sequence; the masks have a bit per row.
     auto describe_rows = [&](int r0) {
         for (int i = tid; i < ROWS; i += NT) {  // (whole warps)
             const int r = r0 + i;
@@ -395,11 +406,11 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
             }
             const int sid = lo - 1;
             int info = -1, o0 = 0, o1 = 0;
-            if (r < seg1 && sid >= 0 && sid < p.n_seq) {
+            if (r < p.rows && sid >= 0 && sid < p.n_seq) {
                 info = cached ? s_info[sid] : load_info(sid);
                 o0 = off_at(sid);
                 o1 = off_at(sid + 1);
-                if (info >= 0) info |= (o0 < seg0 ? 8 : 0) | max(0, min(3, r - o0));
+                if (info >= 0) info |= max(0, min(3, r - o0));
             }
             const unsigned all = 0xffffffffu;
             const unsigned mv = __ballot_sync(all, info >= 0), ms = __ballot_sync(all, info >= 0 && r == o0),
@@ -419,7 +430,7 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
     };
 
     // ---- before the first tile
-    if (seg0 < seg1) stage_in(seg0, 0);
+    if (first < p.rows) stage_in(first, 0);
     commit();
     V w0, w1, w2, w3, bias, dd;
     {
@@ -441,32 +452,13 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
             if (i < p.n_seq) s_info[i] = load_info(i);
         }
     }
-    if (part == 0) {  // the three rows above
-#pragma unroll
-        for (int k = 0; k < 3; ++k) {
-            R r;
-            r.zero();
-            if (on && seg0 > k && seg0 < seg1)
-                r.v = *reinterpret_cast<const Word *>(static_cast<const T *>(p.x) + ch + (seg0 - 1 - k) * p.ld);
-            halo[k][cg] = r.get();
-        }
-    }
     // the scan's view of the threads: a lane a part
     const int sp = tid % ST, sc = tid / ST, sch = c0 + sc * VEC;
-    V carry;  // the state that comes into the tile, for channels sch
+    V carry;  // the state that comes into the cluster's tiles, for channels sch
     vset(carry, 0.0f, 0.0f);
-    float all = 1.0f;  // (SUMS) the decays of the segment so far
-    if (!SUMS && sch < C) {
-        for (int j = 0; j < seg; ++j) {
-            const float *S = g.S + (int64_t)j * C + sch;
-            V v;
-            vset(v, S[0], S[VEC - 1]);
-            carry = through(g.A[(int64_t)j * p.l.H + sch / P], carry, v);
-        }
-    }
-    if (!PRE) head_table(seg0, 0);
+    if (!PRE) head_table(first, 0);
     __syncthreads();
-    describe_rows(seg0);
+    describe_rows(first);
 
     auto conv_at = [&](int slot, int j) {
         return static_cast<T *>(p.l.conv) + ((int64_t)slot * 3 + j) * C + ch;
@@ -479,7 +471,7 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
         return r.get();
     };
     auto keep = [&](int slot, V a, V b, V c, V s) {
-        if (!on || SUMS) return;
+        if (!on) return;
         put(conv_at(slot, 0), a);
         put(conv_at(slot, 1), b);
         put(conv_at(slot, 2), c);
@@ -500,18 +492,20 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
     fetch_init();
 
     bool plain = false;
-    int left_slot = -1;  // the slot of a state left to the third launch
     int buf = 0;
-    for (int r0 = seg0; r0 < seg1; r0 += ROWS, buf ^= 1) {
+    // (every CTA of a cluster takes as many turns, with no rows in the last
+    // ones perhaps)
+    for (int r0 = first; r0 - first < p.rows; r0 += step, buf ^= 1) {
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         __syncthreads();
-        const int r1 = r0 + ROWS;
+        const int r1 = r0 + step;
         // z arrives during the scan of x; the next tile's x, when this one's is
         // done with, during the outputs
-        if (gate) stage_rows(r0, p.z, staged + L::WORDS);
+        if (gate && r0 < p.rows) stage_rows(r0, p.z, staged + L::WORDS);
         commit();
-        unsigned valid = mask, start = 0, end = 0;
-        if (!plain) {
+        const bool rows_left = r0 < p.rows;
+        unsigned valid = rows_left ? mask : 0, start = 0, end = 0;
+        if (rows_left && !plain) {
             valid = row_valid[b0 / 32] >> b0 % 32 & mask;
             start = row_start[b0 / 32] >> b0 % 32 & mask;
             end = row_end[b0 / 32] >> b0 % 32 & mask;
@@ -523,17 +517,13 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
         // x1, x2, x3: the inputs 1, 2, 3 tokens back; from the slot before the
         // sequence's first
         V x1, x2, x3;
-        if (part == 0) {
-            x1 = halo[0][cg];
-            x2 = halo[1][cg];
-            x3 = halo[2][cg];
-        } else {
+        {
             R r;
-            r.v = xw[-CG - L::PAD];
+            r.v = part ? xw[-CG - L::PAD] : halo[0][cg];
             x1 = r.get();
-            r.v = xw[-2 * CG - L::PAD];
+            r.v = part ? xw[-2 * CG - L::PAD] : halo[1][cg];
             x2 = r.get();
-            r.v = xw[-3 * CG - L::PAD];
+            r.v = part ? xw[-3 * CG - L::PAD] : halo[2][cg];
             x3 = r.get();
         }
         V h, y[LC];
@@ -549,14 +539,14 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
             const V xt = xr.get();
             const V u = silu(vfma(w3, xt, vfma(w2, x1, vfma(w1, x2, vfma(w0, x3, bias)))));
             h = sfma(k.x, h, smul(k.y, u));
-            if (!SUMS) y[t] = sfma(k.z, h, vmul(dd, u));
+            y[t] = sfma(k.z, h, vmul(dd, u));
             x3 = x2;
             x2 = x1;
             x1 = xt;
             return k.x;
         };
         // (by warps: one with both kinds of part would run both loops)
-        const bool even = plain || (valid == mask && !start && !end && (info[0] & 3) == 3);
+        const bool even = rows_left && (plain || (valid == mask && !start && !end && (info[0] & 3) == 3));
         if (__all_sync(0xffffffffu, even)) {
 #pragma unroll
             for (int t = 0; t < LC; ++t) token(t);
@@ -607,15 +597,10 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
         }
         part_s[part][cg] = h;
         part_a[part][cg] = start ? SET : decs[(buf * heads + hh) * ST + part];
-        if (!PRE && r1 < seg1) head_table(r1, buf ^ 1);
+        if (!PRE && r1 < p.rows) head_table(r1, buf ^ 1);
         __syncthreads();
-        if (r1 < seg1) stage_in(r1, buf ^ 1);
+        if (r1 < p.rows) stage_in(r1, buf ^ 1);
         commit();
-        if (part == ST - 1) {
-            halo[0][cg] = x1;
-            halo[1][cg] = x2;
-            halo[2][cg] = x3;
-        }
         {
             float a = part_a[sp][sc];
             V S = part_s[sp][sc];
@@ -628,17 +613,32 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
                     a = through(a1, a);
                 }
             }
-            const float a1 = shfl_up(a, 1, ST), an = shfl_at(a, ST - 1, ST);
-            const V S1 = shfl_up(S, 1, ST), Sn = shfl_at(S, ST - 1, ST);
-            came[sp][sc] = sp == 0 ? carry : through(a1, carry, S1);
-            carry = through(an, carry, Sn);
-            all = through(all, an);
+            const float a1 = shfl_up(a, 1, ST);
+            const V S1 = shfl_up(S, 1, ST);
+            float an = shfl_at(a, ST - 1, ST);
+            V Sn = shfl_at(S, ST - 1, ST), in = carry;
+            if (many > 1) {
+                if (sp == ST - 1) {
+                    tile_a[buf][sc] = a;
+                    tile_s[buf][sc] = S;
+                }
+                cluster_sync();
+                for (int j = 0; j < many; ++j) {
+                    load_remote(remote(&tile_a[buf][sc], j), an);
+                    load_remote(remote(&tile_s[buf][sc], j), Sn);
+                    carry = through(an, carry, Sn);
+                    if (j + 1 == rank) in = carry;
+                }
+            } else {
+                carry = through(an, carry, Sn);
+            }
+            came[sp][sc] = sp == 0 ? in : through(a1, in, S1);
         }
         // the next tile's rows: inside the sequence of this tile's last row,
         // nothing has to be looked up
-        if (r1 < seg1) {
+        if (r1 < p.rows) {
             const bool same = (plain || (row_info[ROWS - 1] >= 0 && last_info >= 0)) && r1 >= last_begin + 3 &&
-                              r1 + ROWS < last_end && r1 + ROWS <= seg1;
+                              r1 + ROWS < last_end && r1 + ROWS <= p.rows;
             if (!same) {
                 __syncthreads();  // every thread is done with this tile's rows
                 describe_rows(r1);
@@ -647,27 +647,16 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
         }
         asm volatile("cp.async.wait_group 1;" ::: "memory");  // z
         __syncthreads();
-        if (r1 < seg1 && !plain) fetch_init();
+        if (r1 < p.rows && !plain) fetch_init();
         const V hin = came[part][cg];
-        if (!SUMS && end_info >= 0) {
+        if (end_info >= 0) {
             V aa;
             vset(aa, Ae, Ae);
-            const V s = vfma(aa, hin, he);
-            if (end_info & 8) {
-                left_slot = end_info >> 4;
-                if (on) {
-                    T *cv = static_cast<T *>(g.conv) + (int64_t)seg * 3 * C + ch;
-                    put(cv, e3);
-                    put(cv + C, e2);
-                    put(cv + 2 * C, e1);
-                    put(g.h + (int64_t)seg * C + ch, s);
-                }
-            } else {
-                keep(end_info >> 4, e3, e2, e1, s);
-            }
+            keep(end_info >> 4, e3, e2, e1, vfma(aa, hin, he));
         }
-        if (!SUMS && on) {
-            const int first = start ? __ffs(start) - 1 : LC;
+        const bool whole = __all_sync(0xffffffffu, valid == mask && !start);
+        if (on) {
+            const int begin = start ? __ffs(start) - 1 : LC;
             T *py = static_cast<T *>(p.y) + ch + (r0 + b0) * p.ldy;
             auto finish = [&](int t, bool fix, auto gated) {
                 V o = y[t];
@@ -680,39 +669,22 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
                 put(py, o);
             };
             auto outputs = [&](auto gated) {
-                if (__all_sync(__activemask(), valid == mask && !start)) {
+                if (whole) {
 #pragma unroll
                     for (int t = 0; t < LC; ++t, py += p.ldy) finish(t, true, gated);
                 } else {
 #pragma unroll
                     for (int t = 0; t < LC; ++t, py += p.ldy)
-                        if (valid >> t & 1u) finish(t, t < first, gated);
+                        if (valid >> t & 1u) finish(t, t < begin, gated);
                 }
             };
             if (gate) outputs(std::true_type());
             else outputs(std::false_type());
         }
     }
-    if (SUMS) {
-        if (sp == 0 && sch < C) {
-            float *S = g.S + (int64_t)seg * C + sch;
-            S[0] = lane0(carry);
-            S[VEC - 1] = lane1(carry);
-            // (threads of the same head, and CTAs, write the same value)
-            g.A[(int64_t)seg * p.l.H + sch / P] = all;
-        }
-        return;
-    }
-    if (g.n > 1) {
-        const int left = __syncthreads_or(left_slot + 1) ? 1 : 0;
-        if (tid == 0) list[0] = -1;
-        __syncthreads();
-        if (left && left_slot >= 0) list[0] = left_slot;  // (one sequence: one slot)
-        __syncthreads();
-        if (tid == 0) g.slot[seg * gridDim.x + blockIdx.x] = list[0];
-    }
+    if (many > 1) cluster_sync();  // (nobody reads here any more)
     // sequences without tokens that start afresh: a zero state
-    if (seg == 0) {
+    if (rank == 0) {
         for (int s0 = 0; s0 < p.n_seq; s0 += NT) {
             const int s = s0 + tid;
             int slot = -1;
@@ -733,19 +705,6 @@ __global__ void __launch_bounds__(CG *ST, PER_SM)
     }
 }
 
-// The third launch: states that segments left, to their slots.
-template <typename T>
-__global__ void __launch_bounds__(128) left_kernel(const Layer l, const Segments g, int channels, int n_cb) {
-    const int ch = blockIdx.x * 128 + threadIdx.x, seg = blockIdx.y;
-    if (ch >= l.C) return;
-    const int slot = g.slot[seg * n_cb + ch / channels];
-    if (slot < 0) return;
-    const T *from = static_cast<const T *>(g.conv) + (int64_t)seg * 3 * l.C + ch;
-    T *to = static_cast<T *>(l.conv) + (int64_t)slot * 3 * l.C + ch;
-    for (int k = 0; k < 3; ++k) to[k * l.C] = from[k * l.C];
-    l.h[(int64_t)slot * l.C + ch] = g.h[(int64_t)seg * l.C + ch];
-}
-
 struct Launch {
     Args a;
     bm_ctx_t *ctx;
@@ -760,30 +719,17 @@ int launch_prefill(Launch &l) {
     const int C = a.l.C, P = a.l.P, H = a.l.H;
     const int n_cb = (C + CG * VEC - 1) / (CG * VEC);
     const int tiles = a.rows > 0 ? (int)(((int64_t)a.rows + L::ROWS - 1) / L::ROWS) : 1;
-    // segments for SMs that would be idle, of at least two tiles each
-    int segs = l.sms * PER_SM / n_cb;
-    if (segs > tiles / 2) segs = tiles / 2;
-    if (segs > 64) segs = 64;
-    if (segs < 1) segs = 1;
-    Segments g{};
-    g.rows = (tiles + segs - 1) / segs * L::ROWS;
-    g.n = segs = (int)(((int64_t)tiles * L::ROWS + g.rows - 1) / g.rows);
+    // clusters for SMs that would be idle
+    int many = 1;
+    while (many < 8 && many < tiles && n_cb * many * 2 <= l.sms * PER_SM) many *= 2;
     const int64_t parts = ((int64_t)a.rows + LC - 1) / LC;
     const size_t tab_bytes = PRE ? (size_t)parts * H * (LC * sizeof(float4) + sizeof(float)) : 0;
-    if (segs > 1 || PRE) {
+    if (PRE) {
         void *work;
-        const size_t words = segs > 1 ? (size_t)segs * ((size_t)2 * C + H + 3 * C + n_cb) : 0;
-        const int rc = bm_detail_work(l.ctx, BM_WORK_SCAN, tab_bytes + words * 4, &work);
+        const int rc = bm_detail_work(l.ctx, BM_WORK_SCAN, tab_bytes, &work);
         if (rc != BM_OK) return rc;
         a.tab = static_cast<const float4 *>(work);
-        a.dec = reinterpret_cast<const float *>(a.tab + (PRE ? parts * H * LC : 0));
-        g.S = reinterpret_cast<float *>(static_cast<unsigned char *>(work) + tab_bytes);
-        g.h = g.S + (size_t)segs * C;
-        g.conv = g.h + (size_t)segs * C;
-        g.A = g.h + (size_t)segs * 4 * C;
-        g.slot = reinterpret_cast<int *>(g.A + (size_t)segs * H);
-    }
-    if (PRE) {
+        a.dec = reinterpret_cast<const float *>(a.tab + parts * H * LC);
         const int64_t blocks = (parts * H + 127) / 128;
         if (blocks > INT32_MAX) return bm_detail_fail(BM_ERR_UNSUPPORTED, "rows * heads too large for one call");
         heads_kernel<T, LC><<<(unsigned)blocks, 128, 0, l.s>>>(a, const_cast<float4 *>(a.tab), const_cast<float *>(a.dec));
@@ -796,18 +742,21 @@ int launch_prefill(Launch &l) {
     if (bytes > most) return bm_detail_fail(BM_ERR_UNSUPPORTED, "too many heads in a tile");
     auto even = [&](const void *q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; };
     const int wide = C % (CG * VEC) == 0 && even(a.x) && even(a.z) && a.ld * (int64_t)sizeof(T) % 16 == 0;
-    auto *main = prefill_kernel<T, VEC, CG, ST, LC, PER_SM, PRE, false>;
-    static bmc::SharedMemory shm[2];
-    BMC_CK(shm[0].allow(reinterpret_cast<const void *>(main), most, l.device));
-    if (segs > 1) {
-        auto *sums = prefill_kernel<T, VEC, CG, ST, LC, PER_SM, PRE, true>;
-        BMC_CK(shm[1].allow(reinterpret_cast<const void *>(sums), most, l.device));
-        sums<<<dim3((unsigned)n_cb, (unsigned)segs - 1), L::NT, bytes, l.s>>>(a, g, heads, wide);
-    }
-    main<<<dim3((unsigned)n_cb, (unsigned)segs), L::NT, bytes, l.s>>>(a, g, heads, wide);
-    if (segs > 1)
-        left_kernel<T><<<dim3((unsigned)(C + 127) / 128, (unsigned)segs), 128, 0, l.s>>>(a.l, g, CG * VEC, n_cb);
-    BMC_CK(cudaGetLastError());
+    auto *k = prefill_kernel<T, VEC, CG, ST, LC, PER_SM, PRE>;
+    static bmc::SharedMemory shm;
+    BMC_CK(shm.allow(reinterpret_cast<const void *>(k), most, l.device));
+    cudaLaunchConfig_t c{};
+    cudaLaunchAttribute at[1];
+    c.gridDim = dim3((unsigned)n_cb, (unsigned)many);
+    c.blockDim = dim3(L::NT);
+    c.dynamicSmemBytes = bytes;
+    c.stream = l.s;
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = at[0].val.clusterDim.z = 1;
+    at[0].val.clusterDim.y = (unsigned)many;
+    c.attrs = at;
+    c.numAttrs = many > 1 ? 1 : 0;
+    BMC_CK(cudaLaunchKernelEx(&c, k, static_cast<const Args>(a), heads, wide));
     return BM_OK;
 }
 
