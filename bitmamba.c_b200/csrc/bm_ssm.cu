@@ -122,13 +122,6 @@ __device__ __forceinline__ Head head_of(float dt, float rate, float b, float c) 
     r.c = c;
     return r;
 }
-template <typename T>
-__device__ __forceinline__ Head head_of(const Args &p, int64_t row, int h) {
-    const int64_t at = row * p.ld + h;
-    return head_of(to_f(static_cast<const T *>(p.dt)[at]) + p.l.dt_bias[h], expf(p.l.a_log[h]),
-                   to_f(static_cast<const T *>(p.b)[at]), to_f(static_cast<const T *>(p.c)[at]));
-}
-
 // ---------------------------------------------------------------- prompts --
 //
 // The token axis of all sequences together is cut into tiles of ST * LC rows.
@@ -303,6 +296,7 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
     __shared__ V part_s[ST][CG + 1], came[ST][CG + 1];
     __shared__ float part_a[ST][CG + 1];
     __shared__ Word halo[3][CG];  // the three rows above the tile
+    __shared__ float head_bias[CG * VEC], head_rate[CG * VEC];
     // the tile's (A, S), of this step and the one before
     __shared__ V tile_s[2][CG];
     __shared__ float tile_a[2][CG];
@@ -366,12 +360,25 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
         }
     };
     auto commit = []() { asm volatile("cp.async.commit_group;" ::: "memory"); };
-    // consecutive lanes are consecutive rows
+    // The scalars of a tile's rows: entry i is row i % ROWS of head i / ROWS, so
+    // consecutive lanes are consecutive rows.  A thread's first entry is loaded
+    // early.
+    T raw[3];
+    auto load_head = [&](int r0, int i) {
+        const int64_t at = (int64_t)min(r0 + i % ROWS, p.rows - 1) * p.ld + h0 + i / ROWS;
+        raw[0] = static_cast<const T *>(p.dt)[at];
+        raw[1] = static_cast<const T *>(p.b)[at];
+        raw[2] = static_cast<const T *>(p.c)[at];
+    };
+    auto load_heads = [&](int r0) {
+        if (tid < nh * ROWS) load_head(r0, tid);
+    };
     auto head_table = [&](int r0, int buf) {
         for (int i = tid; i < nh * ROWS; i += NT) {
             const int h = i / ROWS, t = i % ROWS;
-            Head k{0.0f, 0.0f, 0.0f};
-            if (r0 + t < p.rows) k = head_of<T>(p, r0 + t, h0 + h);
+            if (i != tid) load_head(r0, i);
+            Head k = head_of(to_f(raw[0]) + head_bias[h], head_rate[h], to_f(raw[1]), to_f(raw[2]));
+            if (r0 + t >= p.rows) k = Head{0.0f, 0.0f, 0.0f};
             float prod = k.a;
 #pragma unroll
             for (int o = 1; o < LC; o <<= 1) {
@@ -432,6 +439,13 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
     // ---- before the first tile
     if (first < p.rows) stage_in(first, 0);
     commit();
+    if (!PRE) {
+        if (first < p.rows) load_heads(first);
+        if (tid < nh) {
+            head_bias[tid] = p.l.dt_bias[h0 + tid];
+            head_rate[tid] = expf(p.l.a_log[h0 + tid]);
+        }
+    }
     V w0, w1, w2, w3, bias, dd;
     {
         float4 a = make_float4(0, 0, 0, 0), b = a;
@@ -456,8 +470,8 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
     const int sp = tid % ST, sc = tid / ST, sch = c0 + sc * VEC;
     V carry;  // the state that comes into the cluster's tiles, for channels sch
     vset(carry, 0.0f, 0.0f);
-    if (!PRE) head_table(first, 0);
     __syncthreads();
+    if (!PRE && first < p.rows) head_table(first, 0);
     describe_rows(first);
 
     auto conv_at = [&](int slot, int j) {
@@ -503,6 +517,7 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
         // done with, during the outputs
         if (gate && r0 < p.rows) stage_rows(r0, p.z, staged + L::WORDS);
         commit();
+        if (!PRE && r1 < p.rows) load_heads(r1);
         const bool rows_left = r0 < p.rows;
         unsigned valid = rows_left ? mask : 0, start = 0, end = 0;
         if (rows_left && !plain) {
