@@ -223,8 +223,8 @@ struct Tile {
     // parts of a warp (of half a warp, for 8-byte words) meet in no bank
     static constexpr int PAD = CG * VEC * sizeof(T) >= 128 ? 0 : CG;
     static constexpr int WORDS = ROWS * CG + ST * PAD;
-    // x and z
-    static constexpr size_t STAGED = 2 * (size_t)WORDS * VEC * sizeof(T);
+    // x twice and z
+    static constexpr size_t STAGED = 3 * (size_t)WORDS * VEC * sizeof(T);
     // a head's scalars (a, g, c, C times the part's decays up to the row) and
     // its parts' decays, twice
     static constexpr size_t PER_HEAD = 2 * (size_t)(ROWS * 16 + ST * 4);
@@ -295,12 +295,12 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
     __shared__ Word init_x[ST][3][CG];
     __shared__ V part_s[ST][CG + 1], came[ST][CG + 1];
     __shared__ float part_a[ST][CG + 1];
-    __shared__ Word halo[3][CG];  // the three rows above the tile
+    __shared__ Word halo[2][3][CG];  // the three rows above the tile
     __shared__ float head_bias[CG * VEC], head_rate[CG * VEC];
     // the tile's (A, S), of this step and the one before
     __shared__ V tile_s[2][CG];
     __shared__ float tile_a[2][CG];
-    Word *const staged = reinterpret_cast<Word *>(smem);  // x, then z
+    Word *const sx = reinterpret_cast<Word *>(smem), *const sz = sx + 2 * L::WORDS;
     float4 *const tabs = reinterpret_cast<float4 *>(smem + L::STAGED);
     float *const decs = reinterpret_cast<float *>(tabs + 2 * heads * ROWS);
     const int C = p.l.C, P = p.l.P, tid = threadIdx.x, lane = tid & 31;
@@ -313,38 +313,45 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
     constexpr unsigned mask = LC == 32 ? 0xffffffffu : (1u << LC % 32) - 1u;
     const bool gate = p.z != nullptr;
 
-    auto stage_rows = [&](int r0, const void *from, Word *dst) {
+    // Copies of rows, 16 bytes a thread where that can be: COPIES for a tile,
+    // the n-th of them by copy(n).
+    constexpr int E = 16 / (int)sizeof(T), CH = CG * VEC / E;  // elements, chunks of a row
+    constexpr int STEP = NT / CH, COPIES = ROWS / STEP;        // rows a copy
+    static_assert(STEP % LC == 0 && COPIES * STEP == ROWS, "a copy is whole parts");
+    struct Copier {
+        const T *from;
+        uint32_t to;
+        int64_t pitch;
+        __device__ __forceinline__ void copy(int n) {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                             to + n * (STEP * CG + STEP / LC * L::PAD) * (int)sizeof(Word)),
+                         "l"(from)
+                         : "memory");
+            from += pitch;
+        }
+    };
+    const int copy_i = tid % CH, copy_r = tid / CH;
+    auto copier = [&](const void *from, int r0, Word *dst) {
+        return Copier{static_cast<const T *>(from) + (int64_t)(r0 + copy_r) * p.ld + c0 + copy_i * E,
+                      (uint32_t)__cvta_generic_to_shared(dst + copy_r * CG + copy_i * (E / VEC) + copy_r / LC * L::PAD),
+                      STEP * p.ld};
+    };
+    auto stage_rows = [&](int r0, const void *from, Word *dst) {  // (at once)
         const int live = min(ROWS, p.rows - r0);
-        const T *src = static_cast<const T *>(from) + r0 * p.ld + c0;
-        if (wide) {  // 16 bytes at a time
-            constexpr int E = 16 / (int)sizeof(T), CH = CG * VEC / E;  // elements, chunks of a row
-            constexpr int STEP = NT / CH;                             // rows a pass
-            static_assert(STEP % LC == 0, "a pass is whole parts");
-            const int i = tid % CH, r = tid / CH;
-            const T *q = src + i * E + r * p.ld;
-            const uint32_t a0 = (uint32_t)__cvta_generic_to_shared(dst + r * CG + i * (E / VEC) + r / LC * L::PAD);
-            auto copy = [&](int n) {
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                                 a0 + n * (STEP * CG + STEP / LC * L::PAD) * (int)sizeof(Word)),
-                             "l"(q)
-                             : "memory");
-            };
-            if (live == ROWS) {
-#pragma unroll
-                for (int n = 0; n < ROWS / STEP; ++n, q += STEP * p.ld) copy(n);
-            } else {
-                for (int n = 0; r + n * STEP < live; ++n, q += STEP * p.ld) copy(n);
-            }
+        if (wide) {
+            Copier k = copier(from, r0, dst);
+            for (int n = 0; copy_r + n * STEP < live; ++n) k.copy(n);
         } else if (on) {
+            const T *src = static_cast<const T *>(from) + r0 * p.ld + c0;
             for (int r = part; r < live; r += ST)
                 stage(dst + r * CG + r / LC * L::PAD + cg, src + cg * VEC + r * p.ld, Word());
         }
     };
-    // x of a tile, and its head scalars
-    auto stage_in = [&](int r0, int buf) {
+    // what a tile needs besides: the rows above, the head scalars
+    auto stage_rest = [&](int r0, int buf) {
         const int live = min(ROWS, p.rows - r0);
-        stage_rows(r0, p.x, staged);
-        if (on && part < 3 && r0 > part) stage(&halo[part][cg], static_cast<const T *>(p.x) + ch + (r0 - 1 - part) * p.ld, Word());
+        if (on && part < 3 && r0 > part)
+            stage(&halo[buf][part][cg], static_cast<const T *>(p.x) + ch + (r0 - 1 - part) * p.ld, Word());
         if (PRE) {
             const int parts = (live + LC - 1) / LC * LC;
             for (int i = tid; i < nh * ROWS; i += NT) {
@@ -437,7 +444,10 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
     };
 
     // ---- before the first tile
-    if (first < p.rows) stage_in(first, 0);
+    if (first < p.rows) {
+        stage_rows(first, p.x, sx);
+        stage_rest(first, 0);
+    }
     commit();
     if (!PRE) {
         if (first < p.rows) load_heads(first);
@@ -466,9 +476,13 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
             if (i < p.n_seq) s_info[i] = load_info(i);
         }
     }
-    // the scan's view of the threads: a lane a part
-    const int sp = tid % ST, sc = tid / ST, sch = c0 + sc * VEC;
-    V carry;  // the state that comes into the cluster's tiles, for channels sch
+    // the scan's view of the threads: each joins GP parts of a pair of channels
+    // (a lane a part took 700 cycles a tile more, in shuffles)
+    constexpr int GP = ST >= 16 ? 4 : 2, SG = ST / GP;
+    const int sp = tid % SG, sc = tid / SG;
+    const bool scans = tid < CG * SG;  // (whole warps)
+    static_assert(CG * SG % 32 == 0, "scan");
+    V carry;  // the state that comes into the cluster's tiles, of the scan's channels
     vset(carry, 0.0f, 0.0f);
     __syncthreads();
     if (!PRE && first < p.rows) head_table(first, 0);
@@ -513,10 +527,12 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         __syncthreads();
         const int r1 = r0 + step;
-        // z arrives during the scan of x; the next tile's x, when this one's is
-        // done with, during the outputs
-        if (gate && r0 < p.rows) stage_rows(r0, p.z, staged + L::WORDS);
-        commit();
+        // This tile's z and the next one's x, copied between the tokens of the
+        // scan: all at once, the copies' issue held every thread for 1000 cycles
+        // (of 9800 a tile).
+        const bool spread_z = gate && wide && r0 + ROWS <= p.rows, spread_x = wide && r1 + ROWS <= p.rows;
+        Copier kz = copier(p.z, r0, sz), kx = copier(p.x, r1, sx + (buf ^ 1) * L::WORDS);
+        if (r1 < p.rows) stage_rest(r1, buf ^ 1);
         if (!PRE && r1 < p.rows) load_heads(r1);
         const bool rows_left = r0 < p.rows;
         unsigned valid = rows_left ? mask : 0, start = 0, end = 0;
@@ -527,18 +543,18 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
         }
         const int *info = row_info + b0;
         const float4 *tb = tabs + (buf * heads + hh) * ROWS + b0;
-        const Word *xw = staged + b0 * CG + part * L::PAD + cg, *zw = xw + L::WORDS;
+        const Word *xw = sx + buf * L::WORDS + b0 * CG + part * L::PAD + cg, *zw = sz + b0 * CG + part * L::PAD + cg;
 
         // x1, x2, x3: the inputs 1, 2, 3 tokens back; from the slot before the
         // sequence's first
         V x1, x2, x3;
         {
             R r;
-            r.v = part ? xw[-CG - L::PAD] : halo[0][cg];
+            r.v = part ? xw[-CG - L::PAD] : halo[buf][0][cg];
             x1 = r.get();
-            r.v = part ? xw[-2 * CG - L::PAD] : halo[1][cg];
+            r.v = part ? xw[-2 * CG - L::PAD] : halo[buf][1][cg];
             x2 = r.get();
-            r.v = part ? xw[-3 * CG - L::PAD] : halo[2][cg];
+            r.v = part ? xw[-3 * CG - L::PAD] : halo[buf][2][cg];
             x3 = r.get();
         }
         V h, y[LC];
@@ -558,8 +574,23 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
             x3 = x2;
             x2 = x1;
             x1 = xt;
+            // z during the first half, x during the second
+            constexpr int HALF = LC / 2, EVERY = HALF / COPIES > 0 ? HALF / COPIES : 1;
+            constexpr int EACH = (COPIES + HALF / EVERY - 1) / (HALF / EVERY);
+            if (t < HALF ? spread_z : spread_x) {
+#pragma unroll
+                for (int n = 0; n < EACH; ++n) {
+                    const int c = (t % HALF) / EVERY * EACH + n;
+                    if ((t + 1) % EVERY == 0 && c < COPIES) {
+                        if (t < HALF) kz.copy(c);
+                        else kx.copy(c);
+                    }
+                }
+            }
+            if (t == HALF - 1) commit();
             return k.x;
         };
+        if (gate && rows_left && !spread_z) stage_rows(r0, p.z, sz);
         // (by warps: one with both kinds of part would run both loops)
         const bool even = rows_left && (plain || (valid == mask && !start && !end && (info[0] & 3) == 3));
         if (__all_sync(0xffffffffu, even)) {
@@ -613,31 +644,40 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
         part_s[part][cg] = h;
         part_a[part][cg] = start ? SET : decs[(buf * heads + hh) * ST + part];
         if (!PRE && r1 < p.rows) head_table(r1, buf ^ 1);
-        __syncthreads();
-        if (r1 < p.rows) stage_in(r1, buf ^ 1);
+        if (r1 < p.rows && !spread_x) stage_rows(r1, p.x, sx + (buf ^ 1) * L::WORDS);
         commit();
-        {
-            float a = part_a[sp][sc];
-            V S = part_s[sp][sc];
+        __syncthreads();
+        float a = 1.0f;
+        V S;
+        vset(S, 0.0f, 0.0f);
+        if (scans) {
 #pragma unroll
-            for (int o = 1; o < ST; o <<= 1) {
-                const float a1 = shfl_up(a, o, ST);
-                const V S1 = shfl_up(S, o, ST);
+            for (int i = 0; i < GP; ++i) {
+                const float ai = part_a[sp * GP + i][sc];
+                S = through(ai, S, part_s[sp * GP + i][sc]);
+                a = through(a, ai);
+            }
+#pragma unroll
+            for (int o = 1; o < SG; o <<= 1) {
+                const float a1 = shfl_up(a, o, SG);
+                const V S1 = shfl_up(S, o, SG);
                 if (sp >= o) {
                     S = through(a, S1, S);
                     a = through(a1, a);
                 }
             }
-            const float a1 = shfl_up(a, 1, ST);
-            const V S1 = shfl_up(S, 1, ST);
-            float an = shfl_at(a, ST - 1, ST);
-            V Sn = shfl_at(S, ST - 1, ST), in = carry;
+            if (many > 1 && sp == SG - 1) {
+                tile_a[buf][sc] = a;
+                tile_s[buf][sc] = S;
+            }
+        }
+        if (many > 1) cluster_sync();
+        if (scans) {
+            const float a1 = shfl_up(a, 1, SG);
+            const V S1 = shfl_up(S, 1, SG);
+            float an = shfl_at(a, SG - 1, SG);
+            V Sn = shfl_at(S, SG - 1, SG), in = carry;
             if (many > 1) {
-                if (sp == ST - 1) {
-                    tile_a[buf][sc] = a;
-                    tile_s[buf][sc] = S;
-                }
-                cluster_sync();
                 for (int j = 0; j < many; ++j) {
                     load_remote(remote(&tile_a[buf][sc], j), an);
                     load_remote(remote(&tile_s[buf][sc], j), Sn);
@@ -647,7 +687,12 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
             } else {
                 carry = through(an, carry, Sn);
             }
-            came[sp][sc] = sp == 0 ? in : through(a1, in, S1);
+            if (sp > 0) in = through(a1, in, S1);
+#pragma unroll
+            for (int i = 0; i < GP; ++i) {
+                came[sp * GP + i][sc] = in;
+                in = through(part_a[sp * GP + i][sc], in, part_s[sp * GP + i][sc]);
+            }
         }
         // the next tile's rows: inside the sequence of this tile's last row,
         // nothing has to be looked up
