@@ -318,29 +318,24 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
     constexpr int E = 16 / (int)sizeof(T), CH = CG * VEC / E;  // elements, chunks of a row
     constexpr int STEP = NT / CH, COPIES = ROWS / STEP;        // rows a copy
     static_assert(STEP % LC == 0 && COPIES * STEP == ROWS, "a copy is whole parts");
-    struct Copier {
-        const T *from;
-        uint32_t to;
-        int64_t pitch;
-        __device__ __forceinline__ void copy(int n) {
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                             to + n * (STEP * CG + STEP / LC * L::PAD) * (int)sizeof(Word)),
-                         "l"(from)
-                         : "memory");
-            from += pitch;
-        }
-    };
     const int copy_i = tid % CH, copy_r = tid / CH;
-    auto copier = [&](const void *from, int r0, Word *dst) {
-        return Copier{static_cast<const T *>(from) + (int64_t)(r0 + copy_r) * p.ld + c0 + copy_i * E,
-                      (uint32_t)__cvta_generic_to_shared(dst + copy_r * CG + copy_i * (E / VEC) + copy_r / LC * L::PAD),
-                      STEP * p.ld};
+    const int copy_to = (copy_r * CG + copy_i * (E / VEC) + copy_r / LC * L::PAD) * (int)sizeof(Word);
+    const int64_t copy_pitch = STEP * p.ld;
+    // the next tile's first chunk of this thread; a tile's copies move them on
+    const T *next_x = static_cast<const T *>(p.x) + (int64_t)(first + copy_r) * p.ld + c0 + copy_i * E;
+    const T *next_z = static_cast<const T *>(p.z) + (next_x - static_cast<const T *>(p.x));
+    auto copy = [&](const T *&from, uint32_t to, int n) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                         to + n * (STEP * CG + STEP / LC * L::PAD) * (int)sizeof(Word)),
+                     "l"(from)
+                     : "memory");
+        from += copy_pitch;
     };
-    auto stage_rows = [&](int r0, const void *from, Word *dst) {  // (at once)
+    auto stage_rows = [&](int r0, const void *from, const T *next, Word *dst) {  // (at once)
         const int live = min(ROWS, p.rows - r0);
         if (wide) {
-            Copier k = copier(from, r0, dst);
-            for (int n = 0; copy_r + n * STEP < live; ++n) k.copy(n);
+            const uint32_t to = (uint32_t)__cvta_generic_to_shared(dst) + copy_to;
+            for (int n = 0; copy_r + n * STEP < live; ++n) copy(next, to, n);
         } else if (on) {
             const T *src = static_cast<const T *>(from) + r0 * p.ld + c0;
             for (int r = part; r < live; r += ST)
@@ -348,24 +343,28 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
         }
     };
     // what a tile needs besides: the rows above, the head scalars
+    const bool halos = on && part < 3;
+    const T *next_halo = static_cast<const T *>(p.x) + ch + (first - 1 - part) * p.ld;
+    // (one head's entries are consecutive in a part, LC of them)
+    const float4 *next_tab = p.tab + ((int64_t)(first / LC + tid / LC) * p.l.H + h0) * LC + tid % LC;
+    const float *next_dec = p.dec + (int64_t)(first / LC + tid) * p.l.H + h0;
     auto stage_rest = [&](int r0, int buf) {
-        const int live = min(ROWS, p.rows - r0);
-        if (on && part < 3 && r0 > part)
-            stage(&halo[buf][part][cg], static_cast<const T *>(p.x) + ch + (r0 - 1 - part) * p.ld, Word());
+        if (halos && r0 > part) stage(&halo[buf][part][cg], next_halo, Word());
+        next_halo += step * p.ld;
         if (PRE) {
-            const int parts = (live + LC - 1) / LC * LC;
-            for (int i = tid; i < nh * ROWS; i += NT) {
-                const int h = i / ROWS, t = i % ROWS;
-                if (t >= parts) continue;
-                const uint32_t a = (uint32_t)__cvta_generic_to_shared(tabs + buf * heads * ROWS + i);
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(a),
-                             "l"(p.tab + ((int64_t)(r0 + t) / LC * p.l.H + h0 + h) * LC + t % LC)
-                             : "memory");
-                if (t % LC == 0)
-                    stage(decs + (buf * heads + h) * ST + t / LC, p.dec + (int64_t)(r0 + t) / LC * p.l.H + h0 + h, 0.0f);
+            const int live = min(ROWS, p.rows - r0);
+            for (int h = 0; h < nh; ++h) {
+                if (tid < ROWS && tid / LC * LC < live) {
+                    const uint32_t a = (uint32_t)__cvta_generic_to_shared(tabs + (buf * heads + h) * ROWS + tid);
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(a), "l"(next_tab + h * LC) : "memory");
+                }
+                if (tid < ST && tid * LC < live) stage(decs + (buf * heads + h) * ST + tid, next_dec + h, 0.0f);
             }
+            next_tab += (int64_t)step * p.l.H;
+            next_dec += (int64_t)(step / LC) * p.l.H;
         }
     };
+    static_assert(!PRE || ROWS <= NT, "an entry a thread");
     auto commit = []() { asm volatile("cp.async.commit_group;" ::: "memory"); };
     // The scalars of a tile's rows: entry i is row i % ROWS of head i / ROWS, so
     // consecutive lanes are consecutive rows.  A thread's first entry is loaded
@@ -445,9 +444,10 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
 
     // ---- before the first tile
     if (first < p.rows) {
-        stage_rows(first, p.x, sx);
+        stage_rows(first, p.x, next_x, sx);
         stage_rest(first, 0);
     }
+    next_x += step * p.ld;
     commit();
     if (!PRE) {
         if (first < p.rows) load_heads(first);
@@ -531,7 +531,9 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
         // scan: all at once, the copies' issue held every thread for 1000 cycles
         // (of 9800 a tile).
         const bool spread_z = gate && wide && r0 + ROWS <= p.rows, spread_x = wide && r1 + ROWS <= p.rows;
-        Copier kz = copier(p.z, r0, sz), kx = copier(p.x, r1, sx + (buf ^ 1) * L::WORDS);
+        const uint32_t to_z = (uint32_t)__cvta_generic_to_shared(sz) + copy_to,
+                       to_x = (uint32_t)__cvta_generic_to_shared(sx + (buf ^ 1) * L::WORDS) + copy_to;
+        const T *from_z = next_z, *from_x = next_x;
         if (r1 < p.rows) stage_rest(r1, buf ^ 1);
         if (!PRE && r1 < p.rows) load_heads(r1);
         const bool rows_left = r0 < p.rows;
@@ -582,15 +584,15 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
                 for (int n = 0; n < EACH; ++n) {
                     const int c = (t % HALF) / EVERY * EACH + n;
                     if ((t + 1) % EVERY == 0 && c < COPIES) {
-                        if (t < HALF) kz.copy(c);
-                        else kx.copy(c);
+                        if (t < HALF) copy(from_z, to_z, c);
+                        else copy(from_x, to_x, c);
                     }
                 }
             }
             if (t == HALF - 1) commit();
             return k.x;
         };
-        if (gate && rows_left && !spread_z) stage_rows(r0, p.z, sz);
+        if (gate && rows_left && !spread_z) stage_rows(r0, p.z, next_z, sz);
         // (by warps: one with both kinds of part would run both loops)
         const bool even = rows_left && (plain || (valid == mask && !start && !end && (info[0] & 3) == 3));
         if (__all_sync(0xffffffffu, even)) {
@@ -644,18 +646,26 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
         part_s[part][cg] = h;
         part_a[part][cg] = start ? SET : decs[(buf * heads + hh) * ST + part];
         if (!PRE && r1 < p.rows) head_table(r1, buf ^ 1);
-        if (r1 < p.rows && !spread_x) stage_rows(r1, p.x, sx + (buf ^ 1) * L::WORDS);
+        if (r1 < p.rows && !spread_x) stage_rows(r1, p.x, next_x, sx + (buf ^ 1) * L::WORDS);
+        next_x += step * p.ld;
+        next_z += step * p.ld;
         commit();
         __syncthreads();
         float a = 1.0f;
         V S;
         vset(S, 0.0f, 0.0f);
+        float av[GP];
+        V Sv[GP];
         if (scans) {
 #pragma unroll
             for (int i = 0; i < GP; ++i) {
-                const float ai = part_a[sp * GP + i][sc];
-                S = through(ai, S, part_s[sp * GP + i][sc]);
-                a = through(a, ai);
+                av[i] = part_a[sp * GP + i][sc];
+                Sv[i] = part_s[sp * GP + i][sc];
+            }
+#pragma unroll
+            for (int i = 0; i < GP; ++i) {
+                S = through(av[i], S, Sv[i]);
+                a = through(a, av[i]);
             }
 #pragma unroll
             for (int o = 1; o < SG; o <<= 1) {
@@ -691,7 +701,7 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
 #pragma unroll
             for (int i = 0; i < GP; ++i) {
                 came[sp * GP + i][sc] = in;
-                in = through(part_a[sp * GP + i][sc], in, part_s[sp * GP + i][sc]);
+                in = through(av[i], in, Sv[i]);
             }
         }
         // the next tile's rows: inside the sequence of this tile's last row,
