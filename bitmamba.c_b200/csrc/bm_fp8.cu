@@ -44,11 +44,22 @@ __device__ __forceinline__ float4 load4(const __nv_bfloat16 *p) {
 }
 
 // x / s from r = 1 / s: the quotient's error is exact in one multiply-add, and
-// corrects it (Markstein, IBM J. Res. Dev. 34, 1990).  For 2^-110 < s < 2^120;
-// where the error underflows, x / s is far below e4m3's smallest value.
+// corrects it (Markstein, IBM J. Res. Dev. 34, 1990).
 __device__ __forceinline__ float divide(float x, float s, float r) {
     const float q = x * r;
     return fmaf(fmaf(-q, s, x), r, q);
+}
+__device__ __forceinline__ uint32_t to_e4m3(float4 v) { return __nv_fp8x4_e4m3(v).__x; }
+__device__ __forceinline__ float4 times(float4 v, float k) {
+    return make_float4(v.x * k, v.y * k, v.z * k, v.w * k);
+}
+// e4m3(448 v / top) from the exact quotients
+__device__ __noinline__ uint32_t to_e4m3_exact(float4 v, float top) {
+    const double f[4] = {v.x, v.y, v.z, v.w};
+    uint32_t w = 0;
+    for (int i = 0; i < 4; ++i)
+        w |= (uint32_t)__nv_cvt_double_to_fp8(448.0 * f[i] / (double)top, __NV_SATFINITE, __NV_E4M3) << (8 * i);
+    return w;
 }
 
 // TPR threads per row: a warp's 32 groups of 4 columns are one block of 128.
@@ -68,6 +79,9 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
         v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (live && col < d) v[i] = load4(x + (int64_t)row * ldx + col);
     }
+    // The norm's factor of the row is in the scale alone: it drops out of
+    // x / scale, with its rounding.
+    float rms = 1.0f;
     if (NORM) {
         float s = 0.f;
 #pragma unroll
@@ -83,14 +97,13 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
 #pragma unroll
             for (int w = 0; w < TPR / 32; ++w) s += part[w0 + w];
         }
-        const float rms = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(s, (float)d) + 1e-6f));
+        rms = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(s, (float)d) + 1e-6f));
 #pragma unroll
         for (int i = 0; i < QV; ++i) {
             const int col = 4 * (t + i * TPR);
             if (col < d) {
                 const float4 w = load4(norm_w + col);
-                v[i] = make_float4(v[i].x * rms * w.x, v[i].y * rms * w.y, v[i].z * rms * w.z,
-                                   v[i].w * rms * w.w);
+                v[i] = make_float4(v[i].x * w.x, v[i].y * w.y, v[i].z * w.z, v[i].w * w.w);
             }
         }
     }
@@ -101,22 +114,27 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
         const unsigned m = max(max(__float_as_uint(v[i].x) & 0x7fffffffu, __float_as_uint(v[i].y) & 0x7fffffffu),
                                max(__float_as_uint(v[i].z) & 0x7fffffffu, __float_as_uint(v[i].w) & 0x7fffffffu));
         const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, m));
+        const float most = NORM ? top * rms : top;
         float sc = 1.0f;
-        if (!(top < 0x1p+120f)) {  // (an infinity or NaN among them, or close to it)
-            sc = __fdiv_rn(top, 448.0f);
-            v[i] = make_float4(__fdiv_rn(v[i].x, sc), __fdiv_rn(v[i].y, sc), __fdiv_rn(v[i].z, sc),
-                               __fdiv_rn(v[i].w, sc));
-        } else if (top > 0x1p-100f) {
-            sc = divide(top, 448.0f, 1.0f / 448.0f);
+        uint32_t w = 0;
+        if (!(top < 0x1p+120f && most < 0x1p+120f) || (top <= 0x1p-100f && most > 0x1p-100f)) {
+            // (an infinity or NaN among them, or close to the range's ends)
+            sc = __fdiv_rn(most, 448.0f);
+            w = to_e4m3(make_float4(__fdiv_rn(v[i].x * rms, sc), __fdiv_rn(v[i].y * rms, sc),
+                                    __fdiv_rn(v[i].z * rms, sc), __fdiv_rn(v[i].w * rms, sc)));
+        } else if (most > 0x1p-100f) {
+            sc = divide(most, 448.0f, 1.0f / 448.0f);
+            // Rounded from both sides of the approximate quotients, by more than
+            // these can be off (2 ulp of the reciprocal, 2 roundings: 2^-21.4);
+            // where that differs, a border is close and the exact ones decide.
             float r;
-            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(sc));
-            r = fmaf(fmaf(-sc, r, 1.0f), r, r);  // (Newton: r to the last place)
-            v[i] = make_float4(divide(v[i].x, sc, r), divide(v[i].y, sc, r), divide(v[i].z, sc, r),
-                               divide(v[i].w, sc, r));
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(top));
+            r *= 448.0f;
+            w = to_e4m3(times(v[i], r * (1.0f + 0x1p-21f)));
+            if (w != to_e4m3(times(v[i], r * (1.0f - 0x1p-21f)))) w = to_e4m3_exact(v[i], top);
         }
         if (live && col < d) {
-            const __nv_fp8x4_e4m3 r(v[i]);
-            *reinterpret_cast<uint32_t *>(q + (int64_t)row * d + col) = r.__x;
+            *reinterpret_cast<uint32_t *>(q + (int64_t)row * d + col) = w;
             if (lane == 0) scale[(int64_t)(col >> 7) * ld_scale + row] = sc;
         }
     }
