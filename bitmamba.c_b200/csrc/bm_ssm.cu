@@ -1008,8 +1008,9 @@ int bm_ssm_prefill(bm_ctx_t *ctx, const bm_ssm_layer_t *layer, const void *d_x, 
         return f32 ? launch_prefill<float, 1, 32, 16, 8, 1, false>(l) : launch_prefill<bf16, 1, 32, 16, 8, 1, false>(l);
     if (rows <= 64)
         return f32 ? launch_prefill<float, 2, 16, 8, 8, 4, false>(l) : launch_prefill<bf16, 2, 16, 8, 8, 4, false>(l);
-    // the head scalars of few tiles cost less in the CTAs than a launch
-    if (rows <= 2048)
+    // the head scalars of few tiles cost less in the CTAs than a launch, and a
+    // table of them is no use where it is larger than the inputs
+    if (rows <= 2048 || (int64_t)rows * a.l.H > ((int64_t)1 << 26))
         return f32 ? launch_prefill<float, 2, 16, 32, 8, 1, false>(l) : launch_prefill<bf16, 2, 16, 32, 8, 1, false>(l);
     return f32 ? launch_prefill<float, 2, 16, 32, 8, 1, true>(l) : launch_prefill<bf16, 2, 16, 32, 16, 1, true>(l);
 }

@@ -335,12 +335,12 @@ typedef struct {
  *            the inputs.  Rows of no sequence are left as they were.
  * Writes each sequence's state after its last token to its slot (an empty
  * sequence: unchanged, or zeros when fresh); other slots are not touched.
- * Stream-ordered (stream NULL: the context's stream).  The call uses a
- * workspace of the context that grows with rows * C and is kept until the
- * context is destroyed: the first call of a size must not be under stream
- * capture, later ones may be.  Calls on one context must not overlap in time
- * (two replayed graphs among them).  Errors of the kernel (a bounded wait)
- * show in bm_ctx_check.
+ * Stream-ordered (stream NULL: the context's stream).  Calls of more than
+ * 2048 rows use a workspace of the context (about 17 bytes per row and head,
+ * at most 1.1 GB) that is grown when needed and kept until the context is
+ * destroyed: the first call of a size must not be under stream capture, later
+ * ones may be, and such calls on one context must not overlap in time (two
+ * replayed graphs among them).
  */
 int bm_ssm_prefill(bm_ctx_t *ctx, const bm_ssm_layer_t *layer, const void *d_x, const void *d_z,
                    const void *d_b, const void *d_c, const void *d_dt, int64_t ld, int rows,

@@ -172,6 +172,34 @@ def test_prefill_long_many_tiles(gpu_ctx, sampler_lib, type_):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("H,P,rows,pad", [(16, 128, 600, 0), (9, 24, 2300, 0), (4, 64, 2300, 2), (3, 16, 2200, 4), (16, 64, 2100, 6),
+                                          (5, 7, 2100, 0), (64, 16, 300, 0), (2, 80, 4200, 8)])
+def test_prefill_tall(gpu_ctx, sampler_lib, type_, H, P, rows, pad):
+    """The ways of the taller prompts: clusters of two to eight, head scalars
+    from a launch of their own, copies of 16 bytes and of single words, heads
+    across the edges of a CTA's channels."""
+    off = offsets([rows // 3, 2, rows - rows // 3 - 2])
+    p = Problem(rows + P, type_, H, P, rows, 4, pad=pad)
+    p.prefill(sampler_lib, gpu_ctx, off, [2, 0, 3], [0, 0, 1])
+    p.check(off, [2, 0, 3], [0, 0, 1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+def test_prefill_thousands_of_sequences(gpu_ctx, sampler_lib, type_):
+    """More sequences than a CTA keeps offsets of; many without tokens."""
+    rng = np.random.default_rng(2)
+    lengths = list(rng.integers(0, 4, 1500))
+    off = offsets(lengths)
+    p = Problem(17, type_, 2, 16, off[-1], 1600)
+    slots = list(rng.permutation(1600)[:1500])
+    fresh = list((rng.random(1500) < 0.5).astype(int))
+    p.prefill(sampler_lib, gpu_ctx, off, slots, fresh)
+    p.check(off, slots, fresh)
+
+
+@pytest.mark.gpu
 def test_prefill_is_reproducible(gpu_ctx, sampler_lib):
     """The order in which tiles finish does not show in the results."""
     off = offsets([3000])
