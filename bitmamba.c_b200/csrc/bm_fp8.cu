@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(Few<NB>::THREADS, 1)
     };
     if (warp < 2) {
         if (lane == 0) {
-            int s = warp, ph = 1, g = 0;
+            int s = warp, ph = 1, g = 0, issued = 0;
             for (int t = first; t < tiles && !aborted(); t += step) {
                 for (int kb = (g ^ warp) & 1; kb < nkb; kb += 2) {
                     if (!mbar_wait(&empty[s], ph)) {  // (a fresh barrier is past phase 1)
@@ -323,13 +323,24 @@ __global__ void __launch_bounds__(Few<NB>::THREADS, 1)
                     tma_load_2d(st, &tmW, (kb0 + kb) * BKB, t * S::BV, &full[s]);
                     tma_load_2d(st + S::BV * BKB, &tmA, (kb0 + kb) * BKB, 0, &full[s]);
                     advance(s, ph);
+                    ++issued;
                 }
                 g += nkb;
+            }
+            if (aborted()) {  // no copy may outlive the CTA
+                for (int i = min(issued, (stages + 1) / 2); i > 0; --i) {
+                    s -= 2;
+                    if (s < 0) {
+                        s += stages;
+                        ph ^= 1;
+                    }
+                    mbar_wait(&full[s], ph ^ 1);
+                }
             }
         }
     } else if (warp < 4) {
         if (lane == 0) {
-            int s = warp - 2, ph = 0, g = 0;
+            int s = warp - 2, ph = 0, g = 0, last = -1;
             for (int t = first; t < tiles && !aborted(); t += step) {
                 for (int kb = (g ^ warp) & 1; kb < nkb; kb += 2) {
                     const int b = (g + kb) % S::TB;
@@ -346,9 +357,11 @@ __global__ void __launch_bounds__(Few<NB>::THREADS, 1)
                     umma_commit(&empty[s]);
                     umma_commit(&accf[b]);
                     advance(s, ph);
+                    last = g + kb;
                 }
                 g += nkb;
             }
+            if (aborted() && last >= 0) mbar_wait(&accf[last % S::TB], (last / S::TB) & 1);
         }
     } else {
         for (int i = threadIdx.x - 128; i < nkb * NB; i += 32 * S::PW) {
@@ -552,7 +565,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1)
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp < 2 && lane == 0) {
-            int s = 0, ph = 1;
+            int s = 0, ph = 1, issued = 0;
             for (int t = first; t < tiles && !aborted(); t += 2 * step) {
                 const int m0 = t % MT * BM, n0 = t / MT * BN;
                 for (int kb = 0; kb < KB; ++kb) {
@@ -564,10 +577,20 @@ __global__ void __launch_bounds__(MANY_THREADS, 1)
                     mbar_expect_tx(&full[s], STAGE_BYTES);
                     tma_load_2d(st, &tmA, kb * BKB, m0, &full[s]);
                     tma_load_2d(st + BM * BKB, &tmW, kb * BKB, n0, &full[s]);
+                    ++issued;
                     if (++s == STAGES) {
                         s = 0;
                         ph ^= 1;
                     }
+                }
+            }
+            if (aborted()) {  // no copy may outlive the CTA
+                for (int i = min(issued, STAGES); i > 0; --i) {
+                    if (--s < 0) {
+                        s += STAGES;
+                        ph ^= 1;
+                    }
+                    mbar_wait(&full[s], ph ^ 1);
                 }
             }
         }
@@ -594,6 +617,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1)
                     }
                 }
             }
+            if (aborted() && g > 0) mbar_wait(&accf[(g - 1) & 1], ((g - 1) / 2) & 1);
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
@@ -733,6 +757,12 @@ int check_d(int d) {
     return BM_OK;
 }
 
+int check_rows(int rows, int n) {  // (so that rounding up to a tile stays in range)
+    if (rows > INT32_MAX - 1024 || n > INT32_MAX - 1024)
+        return bm_detail_fail(BM_ERR_UNSUPPORTED, "rows or n > 2^31 - 1025");
+    return BM_OK;
+}
+
 int check_scale(const void *scale, int64_t ld_scale, int rows) {
     if (!scale || misaligned(scale, 16))
         return bm_detail_fail(BM_ERR_INVALID_ARG, "scales NULL or not 16-byte aligned");
@@ -754,6 +784,7 @@ int bm_fp8_quantize(bm_ctx_t *ctx, const void *d_x, int type, int rows, int d, i
         return bm_detail_fail(BM_ERR_UNSUPPORTED, "type must be BM_F32 or BM_BF16");
     if (rows < 0) return bm_detail_fail(BM_ERR_INVALID_ARG, "rows < 0");
     int rc = bml::check_d(d);
+    if (rc == BM_OK) rc = bml::check_rows(rows, 1);
     if (rc != BM_OK || rows == 0) return rc;
     if ((rc = bml::check_scale(d_scale, ld_scale, rows)) != BM_OK) return rc;
     if (!d_x || !d_q || ldx < d || ldx % 4)
@@ -786,6 +817,7 @@ int bm_fp8_product(bm_ctx_t *ctx, const uint8_t *d_a, const float *d_a_scale, in
     if (rows < 0 || n < 1 || ldo < n)
         return bm_detail_fail(BM_ERR_INVALID_ARG, "rows < 0, n < 1 or ldo < n");
     int rc = bml::check_d(d);
+    if (rc == BM_OK) rc = bml::check_rows(rows, n);
     if (rc != BM_OK || rows == 0) return rc;
     if ((rc = bml::check_scale(d_a_scale, ld_scale, rows)) != BM_OK) return rc;
     if (!d_a || !d_w || !d_w_scale || !d_out)
@@ -809,6 +841,7 @@ int bm_fp8_logits(bm_ctx_t *ctx, const float *d_hidden, int B, int d_model, cons
     if (!ctx) return bm_detail_fail(BM_ERR_INVALID_ARG, "ctx is NULL");
     if (B < 0 || V < 1 || ld < V) return bm_detail_fail(BM_ERR_INVALID_ARG, "B < 0, V < 1 or ld < V");
     int rc = bml::check_d(d_model);
+    if (rc == BM_OK) rc = bml::check_rows(B, V);
     if (rc != BM_OK || B == 0) return rc;
     if (!d_hidden || bml::misaligned(d_hidden, 16) || bml::misaligned(d_norm_w, 16))
         return bm_detail_fail(BM_ERR_INVALID_ARG, "hidden NULL, or hidden or norm weight not 16-byte aligned");

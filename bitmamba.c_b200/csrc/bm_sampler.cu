@@ -74,7 +74,7 @@ struct bm_ctx {
     // workspaces of the layer operators, by use.  A buffer that is outgrown is
     // kept until the context goes: a captured graph may still name it
     struct Work {
-        void *buf[24];
+        void *buf[40];
         int n;
         size_t cap;
     } work[BM_WORK_KINDS];

@@ -803,6 +803,7 @@ int launch_prefill(Launch &l) {
         const int64_t blocks = (parts * H + 127) / 128;
         if (blocks > INT32_MAX) return bm_detail_fail(BM_ERR_UNSUPPORTED, "rows * heads too large for one call");
         heads_kernel<T, LC><<<(unsigned)blocks, 128, 0, l.s>>>(a, const_cast<float4 *>(a.tab), const_cast<float *>(a.dec));
+        BMC_CK(cudaGetLastError());
     }
     int heads = (CG * VEC + P - 2) / P + 1;
     if (heads > H) heads = H;
@@ -938,6 +939,7 @@ int common(bm_ctx_t *ctx, const bm_ssm_layer_t *l, const void *x, const void *z,
         return bm_detail_fail(BM_ERR_INVALID_ARG,
                               "conv_w not 16-byte, or weights or states not element aligned");
     if (rows < 0) return bm_detail_fail(BM_ERR_INVALID_ARG, "rows < 0");
+    if (misaligned(slots, 4)) return bm_detail_fail(BM_ERR_INVALID_ARG, "slots not 4-byte aligned");
     const int C = l->n_heads * l->head_dim;
     if (rows > 0) {
         if (!x || !b || !c || !dt || !y)
@@ -980,6 +982,7 @@ int bm_ssm_prefill(bm_ctx_t *ctx, const bm_ssm_layer_t *layer, const void *d_x, 
     if (n_seq == 0) return BM_OK;
     if (!d_seq_off || misaligned(d_seq_off, 8))
         return bm_detail_fail(BM_ERR_INVALID_ARG, "seq_off NULL or not 8-byte aligned");
+    if (misaligned(d_fresh, 4)) return bm_detail_fail(BM_ERR_INVALID_ARG, "fresh not 4-byte aligned");
     a.off = d_seq_off;
     a.n_seq = n_seq;
     a.fresh = d_fresh;

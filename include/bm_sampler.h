@@ -326,8 +326,8 @@ typedef struct {
  * not decrease).  d_x, d_z ([rows x C]) and d_b, d_c, d_dt ([rows x n_heads])
  * are of the layer's type and share the row pitch ld (elements): columns of
  * one projection row, or arrays of their own.  d_z NULL: no gate.
- *   d_slots  [n_seq] slot of each sequence (NULL: slot i).  The slots of a
- *            call must differ; a sequence whose slot is outside
+ *   d_slots  [n_seq <= n_slots] slot of each sequence (NULL: slot i).  The
+ *            slots of a call must differ; a sequence whose slot is outside
  *            [0, n_slots) is skipped (its y rows are left as they were).
  *   d_fresh  [n_seq] non-zero: the sequence starts from a zero state, else it
  *            continues from its slot's (NULL: all start from zero).
@@ -347,8 +347,8 @@ int bm_ssm_prefill(bm_ctx_t *ctx, const bm_ssm_layer_t *layer, const void *d_x, 
                    const int64_t *d_seq_off, int n_seq, const int32_t *d_slots,
                    const int32_t *d_fresh, void *d_y, int64_t ldy, void *stream);
 
-/* One token for each of `rows` sequences: row r continues the state in slot
- * d_slots[r] (NULL: slot r; outside [0, n_slots): the row is skipped, its y
+/* One token for each of `rows` <= n_slots sequences: row r continues the state
+ * in slot d_slots[r] (NULL: slot r; the slots must differ; outside [0, n_slots): the row is skipped, its y
  * left as it was) and updates it.  Arguments as above; no workspace. */
 int bm_ssm_step(bm_ctx_t *ctx, const bm_ssm_layer_t *layer, const void *d_x, const void *d_z,
                 const void *d_b, const void *d_c, const void *d_dt, int64_t ld, int rows,
@@ -375,7 +375,8 @@ typedef struct {
  * to many, permutations (beam search) and compaction, in place.  A slot whose
  * d_src is itself, negative or >= n_slots is left as it is (a freed slot
  * needs no move: bm_ssm_prefill's fresh sequences start from zero).  The
- * region list is host memory.  Stream-ordered, no workspace.
+ * region list is host memory; regions must not overlap one another or d_src.
+ * Stream-ordered, no workspace.
  */
 int bm_slots_reorder(bm_ctx_t *ctx, const bm_slot_region_t *regions, int n_regions,
                      const int32_t *d_src, int n_slots, void *stream);

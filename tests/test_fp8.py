@@ -230,3 +230,31 @@ def test_refusals(sampler_lib):
         assert refuses(L.bm_fp8_logits, logits, **ch), ch
     for f, base, k in ((L.bm_fp8_quantize, quant, "rows"), (L.bm_fp8_product, prod, "rows"), (L.bm_fp8_logits, logits, "B")):
         assert f(*{**base, k: 0}.values()) == 0
+
+
+def test_refuses_rows_whose_tiles_overflow(sampler_lib):
+    L = sampler_lib.lib()
+    ctx = ctypes.create_string_buffer(1 << 16)
+    q, most = 1 << 20, 2 ** 31 - 1
+    assert L.bm_fp8_quantize(ctx, q, 0, most, 16, 16, q, q, q, most + 1, None) == -4
+    assert L.bm_fp8_product(ctx, q, q, most + 1, most, 16, q, q, 100, q, 100, None) == -4
+    assert L.bm_fp8_product(ctx, q, q, 8, 5, 16, q, q, most, q, most, None) == -4
+    assert L.bm_fp8_logits(ctx, q, most, 16, q, q, q, 100, q, 100, None) == -4
+
+
+@pytest.mark.gpu
+def test_products_at_once_on_two_streams(gpu_ctx):
+    """One context, no workspace: calls of both kinds of tile may overlap."""
+    import torch
+    few, many = make(21, 20, 2048, 4000), make(22, 700, 1024, 3000)
+    want = product(gpu_ctx, *few), product(gpu_ctx, *many)
+    outs = [torch.full_like(w, -3.0) for w in want]
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for (a, asc, w, wsc), out, s in zip((few, many), outs, streams):
+            gpu_ctx.fp8_product(a.data_ptr(), asc.data_ptr(), asc.shape[1], a.shape[0], a.shape[1], w.data_ptr(),
+                                wsc.data_ptr(), w.shape[0], out.data_ptr(), w.shape[0], s.cuda_stream)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+    gpu_ctx.check()

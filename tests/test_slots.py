@@ -215,3 +215,35 @@ def test_refusals(sampler_lib):
     for f, args in ((L.bm_decode_reorder, (None, q, None, 0, None)), (L.bm_decode_compact, (None, None, 0, None, None)),
                     (L.bm_decode_set_rows, (None, 1))):
         assert f(*args) == -1
+
+
+@pytest.mark.gpu
+def test_decode_compact_captured(gpu_ctx, sampler_lib):
+    """A compaction in a graph, replayed after more rows have stopped."""
+    import torch
+    B = 40
+    dec, step = _decode(gpu_ctx, sampler_lib, B, 6, [(3, 0), (20, 1)])
+    state = torch.randn(3, B, 16, device="cuda")
+    out = torch.empty(B, dtype=torch.int32, device="cuda")
+    r = sampler_lib.slot_regions([region(state)])
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        dec.compact(r, out.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    for k in range(3):
+        want = np.full(B, 50 + k)
+        want[[5 + k, 11 * k]] = 777
+        step(want)
+        before, held = dec.read(), state.clone()
+        live = np.flatnonzero(before["status"] == 0)
+        order = np.concatenate([live, np.flatnonzero(before["status"])])
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        after = dec.read()
+        for key in before:
+            assert np.array_equal(after[key], before[key][order]), key
+        assert np.array_equal(out.cpu().numpy(), order)
+        assert torch.equal(state[:, :len(live)], held[:, torch.from_numpy(live).cuda()])
+    dec.close()

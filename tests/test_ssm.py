@@ -359,3 +359,78 @@ def test_refusals(sampler_lib):
     assert refused(L.bm_ssm_prefill, base, n_seq=0) == 0
     with pytest.raises(ValueError):
         bm.SsmLayer(1, 1, 1, "f16", conv_w=q, conv_b=q, dt_bias=q, a_log=q, d=q, conv_state=q, h_state=q)
+
+
+@pytest.mark.gpu
+def test_captured_with_the_workspace(gpu_ctx, sampler_lib):
+    """A prompt long enough for the workspace, captured, then replayed after a
+    longer one has grown it: the graph still has its own."""
+    import torch
+    T = 2500
+    p = Problem(31, "bf16", 3, 32, T, 2)
+    o = torch.tensor([0, 700, T], device="cuda")
+    layer = p.layer(sampler_lib)
+
+    def call(stream):
+        gpu_ctx.ssm_prefill(layer, *p.ptrs(), p.ld, T, o.data_ptr(), 2, None, None, p.y.data_ptr(), p.C, stream)
+
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    call(s.cuda_stream)
+    s.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        call(torch.cuda.current_stream().cuda_stream)
+    big = Problem(32, "bf16", 40, 16, 6000, 1)
+    big.prefill(sampler_lib, gpu_ctx, [0, 6000])
+    big.check([0, 6000])
+    p.y.fill_(7.0)
+    p.dh.copy_(p.h)
+    p.dconv.copy_(p.conv)
+    torch.cuda.synchronize()
+    g.replay()
+    p.check([0, 700, T])
+
+
+@pytest.mark.gpu
+def test_two_contexts_at_once(gpu_ctx, sampler_lib):
+    """Prompts that use the workspace, on two contexts and two streams with
+    nothing between them."""
+    import torch
+    other = sampler_lib.Context(0)
+    a, b = Problem(33, "f32", 4, 32, 4000, 1), Problem(34, "f32", 4, 32, 4000, 1)
+    sa, sb = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    o = torch.tensor([0, 4000], device="cuda")
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for ctx, p, s in ((gpu_ctx, a, sa), (other, b, sb)):
+            ctx.ssm_prefill(p.layer(sampler_lib), *p.ptrs(), p.ld, 4000, o.data_ptr(), 1, None, None, p.y.data_ptr(),
+                            p.C, s.cuda_stream)
+    a.check([0, 4000])
+    b.check([0, 4000])
+    other.close()
+
+
+@pytest.mark.gpu
+def test_prefill_of_nothing(gpu_ctx, sampler_lib):
+    """No rows, no inputs: fresh slots are zeroed, the others stay."""
+    import torch
+    p = Problem(35, "f32", 2, 24, 0, 5)
+    slots, fresh = [3, 1, 9, 0], [1, 0, 1, 1]
+    i = [torch.tensor(v, dtype=torch.int32, device="cuda") for v in (slots, fresh)]
+    o = torch.zeros(5, dtype=torch.int64, device="cuda")
+    torch.cuda.synchronize()
+    gpu_ctx.ssm_prefill(p.layer(sampler_lib), None, None, None, None, None, 0, 0, o.data_ptr(), 4, i[0].data_ptr(),
+                        i[1].data_ptr(), None, 0, DEFAULT)
+    p.check([0] * 5, slots, fresh)
+
+
+def test_refuses_lists_off_their_alignment(sampler_lib):
+    L = sampler_lib.lib()
+    ctx = ctypes.create_string_buffer(1 << 16)
+    q = 1 << 20
+    layer = sampler_lib.SsmLayer(4, 8, 3, "f32", conv_w=q, conv_b=q, dt_bias=q, a_log=q, d=q, conv_state=q, h_state=q).ref
+    for slots, fresh in ((q + 2, q), (q, q + 2), (q + 1, None)):
+        assert L.bm_ssm_prefill(ctx, layer, q, q, q, q, q, 80, 5, q, 2, slots, fresh, q, 32, None) == -1
+    assert L.bm_ssm_step(ctx, layer, q, q, q, q, q, 80, 3, q + 2, q, 32, None) == -1
