@@ -56,10 +56,17 @@ __device__ __forceinline__ float4 times(float4 v, float k) {
 // e4m3(448 v / top) from the exact quotients
 __device__ __noinline__ uint32_t to_e4m3_exact(float4 v, float top) {
     const double f[4] = {v.x, v.y, v.z, v.w};
-    uint32_t w = 0;
+    uint32_t q = 0;
     for (int i = 0; i < 4; ++i)
-        w |= (uint32_t)__nv_cvt_double_to_fp8(448.0 * f[i] / (double)top, __NV_SATFINITE, __NV_E4M3) << (8 * i);
-    return w;
+        q |= (uint32_t)__nv_cvt_double_to_fp8(448.0 * f[i] / (double)top, __NV_SATFINITE, __NV_E4M3) << (8 * i);
+    return q;
+}
+__device__ __noinline__ uint32_t to_e4m3_exact(double x, double y, double z, double w, double top) {
+    const double f[4] = {x, y, z, w};
+    uint32_t q = 0;
+    for (int i = 0; i < 4; ++i)
+        q |= (uint32_t)__nv_cvt_double_to_fp8(448.0 * f[i] / top, __NV_SATFINITE, __NV_E4M3) << (8 * i);
+    return q;
 }
 
 // TPR threads per row: a warp's 32 groups of 4 columns are one block of 128.
@@ -125,13 +132,30 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
         } else if (most > 0x1p-100f) {
             sc = divide(most, 448.0f, 1.0f / 448.0f);
             // Rounded from both sides of the approximate quotients, by more than
-            // these can be off (2 ulp of the reciprocal, 2 roundings: 2^-21.4);
-            // where that differs, a border is close and the exact ones decide.
+            // these can be off (2 ulp of the reciprocal, 2 roundings: 2^-21.4;
+            // with the norm's weight 2 more); where that differs, a border is
+            // close and the exact ones decide.
+            constexpr float margin = NORM ? 0x1p-20f : 0x1p-21f;
             float r;
             asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(top));
             r *= 448.0f;
-            w = to_e4m3(times(v[i], r * (1.0f + 0x1p-21f)));
-            if (w != to_e4m3(times(v[i], r * (1.0f - 0x1p-21f)))) w = to_e4m3_exact(v[i], top);
+            w = to_e4m3(times(v[i], r * (1.0f + margin)));
+            const bool close = w != to_e4m3(times(v[i], r * (1.0f - margin)));
+            if (!NORM) {
+                if (close) w = to_e4m3_exact(v[i], top);
+            } else if (__any_sync(0xffffffffu, close)) {  // (top is the warp's)
+                // the products with the weight unrounded, and their largest
+                float4 f = make_float4(0.f, 0.f, 0.f, 0.f), k = f;
+                if (live && col < d) {
+                    f = load4(x + (int64_t)row * ldx + col);
+                    k = load4(norm_w + col);
+                }
+                const double e0 = (double)f.x * k.x, e1 = (double)f.y * k.y, e2 = (double)f.z * k.z,
+                             e3 = (double)f.w * k.w;
+                double most_e = fmax(fmax(fabs(e0), fabs(e1)), fmax(fabs(e2), fabs(e3)));
+                for (int o = 16; o > 0; o >>= 1) most_e = fmax(most_e, __shfl_xor_sync(0xffffffffu, most_e, o));
+                if (close) w = to_e4m3_exact(e0, e1, e2, e3, most_e);
+            }
         }
         if (live && col < d) {
             *reinterpret_cast<uint32_t *>(q + (int64_t)row * d + col) = w;

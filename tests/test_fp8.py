@@ -78,6 +78,27 @@ def test_quantize_rounds_to_even_exactly(gpu_ctx):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+def test_quantize_rounds_the_weighted_values_exactly(gpu_ctx, type_):
+    """With a norm too, q is what 64 bits give for x * weight / max, value by
+    value: the norm's factor drops out.  (A quotient of 64 bits closer than
+    2^-46 steps to a border is left out; there are none expected.)"""
+    import torch
+    rows, d = 1024, 2048
+    g = torch.Generator(device="cuda").manual_seed(8)
+    x = torch.randn(rows, d, generator=g, device="cuda").to(torch.float32 if type_ == "f32" else torch.bfloat16)
+    w = 1 + 0.02 * torch.randn(d, generator=g, device="cuda")
+    q, _ = quantize(gpu_ctx, x, w)
+    v = (x.double() * w.double()).view(rows, -1, 128)
+    v = (448.0 * v / v.abs().amax(2, keepdim=True)).view(rows, d)
+    grid = torch.exp2(torch.floor(torch.log2(v.abs().clamp(min=2.0 ** -6))) - 3)
+    t = v / grid
+    sure = ((t - torch.floor(t) - 0.5).abs() > 2.0 ** -46) | (t == torch.round(t))
+    assert torch.equal(q.double()[sure], (torch.round(t) * grid)[sure])
+    assert sure.float().mean() > 0.9999
+
+
+@pytest.mark.gpu
 def test_quantize_special_values(gpu_ctx):
     import torch
     x = torch.randn(6, 256, device="cuda")
