@@ -605,6 +605,51 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
                 if (place < 2) x2 = back(2, place, info[0]);
             }
             float A = 1.0f;
+            // One start at most and no end behind it: selects instead of
+            // branches, which would keep the tokens from overlapping (one warp
+            // took 250 cycles a token, and the others wait for it).
+            if (__all_sync(0xffffffffu, !(start & (start - 1u)) && !(start && end >= start))) {
+                const int first_t = __ffs(start) - 1, end_t = __ffs(end) - 1;
+                R i1, i2, i3;
+                i1.zero();
+                i2.zero();
+                i3.zero();
+                V ih;
+                vset(ih, 0.0f, 0.0f);
+                if (start && on && !(info[first_t] & 4)) {
+                    i1.v = init_x[part][2][cg];
+                    i2.v = init_x[part][1][cg];
+                    i3.v = init_x[part][0][cg];
+                    ih = init_h[part][cg];
+                }
+                if (end) {
+                    end_info = info[end_t];
+                    R r;
+                    r.v = xw[end_t * CG];
+                    e1 = r.get();
+                    e2 = x1;
+                    e3 = end_t ? x1 : x2;
+                    if (end_t >= 1) {
+                        r.v = xw[(end_t - 1) * CG];
+                        e2 = r.get();
+                    }
+                    if (end_t >= 2) {
+                        r.v = xw[(end_t - 2) * CG];
+                        e3 = r.get();
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < LC; ++t) {
+                    const bool here = t == first_t;
+                    x1 = here ? i1.get() : x1;
+                    x2 = here ? i2.get() : x2;
+                    x3 = here ? i3.get() : x3;
+                    h = here ? ih : h;
+                    A *= token(t);
+                    he = t == end_t ? h : he;
+                    Ae = t == end_t ? A : Ae;
+                }
+            } else {
 #pragma unroll
             for (int t = 0; t < LC; ++t) {
                 if (start >> t & 1u) {
@@ -641,6 +686,7 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
                         e3 = x3;
                     }
                 }
+            }
             }
         }
         part_s[part][cg] = h;
