@@ -94,16 +94,14 @@ __device__ __forceinline__ float rcp(float v) {
     return v;
 }
 // v / (1 + e^-v): where e^-v overflows the quotient's limit, -0
-template <typename V>
-__device__ __forceinline__ V silu(V v) {
-    V k, one, e;
-    vset(k, -1.44269504f, -1.44269504f);
-    vset(one, 1.0f, 1.0f);
-    const V t = vmul(v, k);
-    vset(e, ex2(lane0(t)), ex2(lane1(t)));
-    e = vadd(e, one);
-    vset(e, rcp(lane0(e)), rcp(lane1(e)));
-    return vmul(v, e);
+__device__ __forceinline__ float silu(float v) { return v * rcp(ex2(v * -1.44269504f) + 1.0f); }
+// Of a pair, with one reciprocal: 1 / a = b / (a b), e^-v held at 2^63 so that
+// the product is in range (below -43, where silu is under 2^-57, v 2^-63).
+__device__ __forceinline__ float2 silu(float2 v) {
+    const float2 t = __fmul2_rn(v, make_float2(-1.44269504f, -1.44269504f));
+    const float2 e = __fadd2_rn(make_float2(ex2(fminf(t.y, 63.0f)), ex2(fminf(t.x, 63.0f))), make_float2(1.0f, 1.0f));
+    const float r = rcp(e.x * e.y);
+    return __fmul2_rn(v, make_float2(e.x * r, e.y * r));
 }
 __device__ __forceinline__ float softplus(float v) {
     return fmaxf(v, 0.0f) + log1pf(expf(-fabsf(v)));
@@ -216,15 +214,20 @@ __device__ __forceinline__ float2 shfl_at(float2 v, int l, int w) {
 
 constexpr int SEQ_CACHE = 1024;  // sequences whose offsets a CTA keeps in shared memory
 
-template <typename T, int VEC, int CG, int ST, int LC>
+template <typename T, int VEC, int CG, int ST, int LC, bool PRE>
 struct Tile {
     static constexpr int NT = CG * ST, ROWS = ST * LC;
     // words: a part is shifted by CG words against the one before, so that the
     // parts of a warp (of half a warp, for 8-byte words) meet in no bank
     static constexpr int PAD = CG * VEC * sizeof(T) >= 128 ? 0 : CG;
     static constexpr int WORDS = ROWS * CG + ST * PAD;
-    // x twice and z
-    static constexpr size_t STAGED = 3 * (size_t)WORDS * VEC * sizeof(T);
+    // x twice; z once, copied while the tile's scan runs, or twice, copied a
+    // tile ahead.  Once, a long fp32 prompt's tiles waited for it (32768 x 4096
+    // 383 us, twice 345); 16 tokens of bf16 take long enough (65536 x 4096 522
+    // us, twice 528), and so do tiles that work out their head scalars (2048 x
+    // 4096 fp32 36.8, twice 38.0).
+    static constexpr int Z = PRE && sizeof(T) == 4 ? 2 : 1;
+    static constexpr size_t STAGED = (2 + Z) * (size_t)WORDS * VEC * sizeof(T);
     // a head's scalars (a, g, c, C times the part's decays up to the row) and
     // its parts' decays, twice
     static constexpr size_t PER_HEAD = 2 * (size_t)(ROWS * 16 + ST * 4);
@@ -278,7 +281,7 @@ __device__ __forceinline__ void load_remote(uint32_t at, float2 &v) {
 // PRE: the head scalars come from p.tab.  gridDim.y: CTAs of a cluster.
 template <typename T, int VEC, int CG, int ST, int LC, int PER_SM, bool PRE>
 __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, int heads, int wide) {
-    using L = Tile<T, VEC, CG, ST, LC>;
+    using L = Tile<T, VEC, CG, ST, LC, PRE>;
     using R = Raw<T, VEC>;
     using Word = typename R::Word;
     using V = typename Vec<VEC>::type;
@@ -519,19 +522,27 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
     __syncthreads();
     fetch_init();
 
+    constexpr bool Z2 = L::Z == 2;
+    if (Z2 && gate && first < p.rows) stage_rows(first, p.z, next_z, sz);
+    if (Z2) {
+        next_z += step * p.ld;
+        commit();
+    }
+
     bool plain = false;
     int buf = 0;
     // (every CTA of a cluster takes as many turns, with no rows in the last
     // ones perhaps)
     for (int r0 = first; r0 - first < p.rows; r0 += step, buf ^= 1) {
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        // (all but z, which is the last group)
+        asm volatile("cp.async.wait_group %0;" ::"n"(Z2 ? 1 : 0) : "memory");
         __syncthreads();
         const int r1 = r0 + step;
-        // This tile's z and the next one's x, copied between the tokens of the
-        // scan: all at once, the copies' issue held every thread for 1000 cycles
-        // (of 9800 a tile).
-        const bool spread_z = gate && wide && r0 + ROWS <= p.rows, spread_x = wide && r1 + ROWS <= p.rows;
-        const uint32_t to_z = (uint32_t)__cvta_generic_to_shared(sz) + copy_to,
+        // z (this tile's, or the next one's between the outputs) and the next
+        // tile's x are copied between the tokens: all at once, the copies' issue
+        // held every thread for 1000 cycles (of 9800 a tile).
+        const bool spread_x = wide && r1 + ROWS <= p.rows, spread_z = gate && wide && (Z2 ? r1 : r0) + ROWS <= p.rows;
+        const uint32_t to_z = (uint32_t)__cvta_generic_to_shared(sz + (Z2 ? (buf ^ 1) * L::WORDS : 0)) + copy_to,
                        to_x = (uint32_t)__cvta_generic_to_shared(sx + (buf ^ 1) * L::WORDS) + copy_to;
         const T *from_z = next_z, *from_x = next_x;
         if (r1 < p.rows) stage_rest(r1, buf ^ 1);
@@ -545,7 +556,7 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
         }
         const int *info = row_info + b0;
         const float4 *tb = tabs + (buf * heads + hh) * ROWS + b0;
-        const Word *xw = sx + buf * L::WORDS + b0 * CG + part * L::PAD + cg, *zw = sz + b0 * CG + part * L::PAD + cg;
+        const Word *xw = sx + buf * L::WORDS + b0 * CG + part * L::PAD + cg, *zw = sz + (Z2 ? buf * L::WORDS : 0) + b0 * CG + part * L::PAD + cg;
 
         // x1, x2, x3: the inputs 1, 2, 3 tokens back; from the slot before the
         // sequence's first
@@ -576,23 +587,23 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
             x3 = x2;
             x2 = x1;
             x1 = xt;
-            // z during the first half, x during the second
-            constexpr int HALF = LC / 2, EVERY = HALF / COPIES > 0 ? HALF / COPIES : 1;
-            constexpr int EACH = (COPIES + HALF / EVERY - 1) / (HALF / EVERY);
-            if (t < HALF ? spread_z : spread_x) {
+            // x during all of them, or z during the first half and x the second
+            constexpr int X0 = Z2 ? 0 : LC / 2, SPAN = LC - X0, EVERY = SPAN / COPIES > 0 ? SPAN / COPIES : 1;
+            constexpr int EACH = (COPIES + SPAN / EVERY - 1) / (SPAN / EVERY);
+            if (t < X0 ? spread_z : spread_x) {
 #pragma unroll
                 for (int n = 0; n < EACH; ++n) {
-                    const int c = (t % HALF) / EVERY * EACH + n;
+                    const int c = t % SPAN / EVERY * EACH + n;
                     if ((t + 1) % EVERY == 0 && c < COPIES) {
-                        if (t < HALF) copy(from_z, to_z, c);
+                        if (t < X0) copy(from_z, to_z, c);
                         else copy(from_x, to_x, c);
                     }
                 }
             }
-            if (t == HALF - 1) commit();
+            if (!Z2 && t == X0 - 1) commit();
             return k.x;
         };
-        if (gate && rows_left && !spread_z) stage_rows(r0, p.z, next_z, sz);
+        if (!Z2 && gate && rows_left && !spread_z) stage_rows(r0, p.z, next_z, sz);
         // (by warps: one with both kinds of part would run both loops)
         const bool even = rows_left && (plain || (valid == mask && !start && !end && (info[0] & 3) == 3));
         if (__all_sync(0xffffffffu, even)) {
@@ -694,7 +705,7 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
         if (!PRE && r1 < p.rows) head_table(r1, buf ^ 1);
         if (r1 < p.rows && !spread_x) stage_rows(r1, p.x, next_x, sx + (buf ^ 1) * L::WORDS);
         next_x += step * p.ld;
-        next_z += step * p.ld;
+        if (!Z2) next_z += step * p.ld;
         commit();
         __syncthreads();
         float a = 1.0f;
@@ -763,6 +774,7 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
         }
         asm volatile("cp.async.wait_group 1;" ::: "memory");  // z
         __syncthreads();
+        if (Z2 && gate && r1 < p.rows && !spread_z) stage_rows(r1, p.z, next_z, sz + (buf ^ 1) * L::WORDS);
         if (r1 < p.rows && !plain) fetch_init();
         const V hin = came[part][cg];
         if (end_info >= 0) {
@@ -774,6 +786,13 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
         if (on) {
             const int begin = start ? __ffs(start) - 1 : LC;
             T *py = static_cast<T *>(p.y) + ch + (r0 + b0) * p.ldy;
+            auto ahead = [&](int t) {  // the next tile's z
+                constexpr int EVERY = LC / COPIES > 0 ? LC / COPIES : 1, EACH = (COPIES + LC - 1) / LC;
+                if (!Z2 || !spread_z || (t + 1) % EVERY) return;
+#pragma unroll
+                for (int n = 0; n < EACH; ++n)
+                    if (t / EVERY * EACH + n < COPIES) copy(from_z, to_z, t / EVERY * EACH + n);
+            };
             auto finish = [&](int t, bool fix, auto gated) {
                 V o = y[t];
                 if (fix) o = sfma(tb[t].w, hin, o);
@@ -782,20 +801,29 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
                     zr.v = zw[t * CG];
                     o = vmul(o, silu(zr.get()));
                 }
-                put(py, o);
+                if (whole || (valid >> t & 1u)) put(py, o);
             };
             auto outputs = [&](auto gated) {
                 if (whole) {
 #pragma unroll
-                    for (int t = 0; t < LC; ++t, py += p.ldy) finish(t, true, gated);
+                    for (int t = 0; t < LC; ++t, py += p.ldy) {
+                        ahead(t);
+                        finish(t, true, gated);
+                    }
                 } else {
 #pragma unroll
-                    for (int t = 0; t < LC; ++t, py += p.ldy)
-                        if (valid >> t & 1u) finish(t, t < begin, gated);
+                    for (int t = 0; t < LC; ++t, py += p.ldy) {
+                        ahead(t);
+                        finish(t, t < begin, gated);  // (a branch for each would keep them from overlapping)
+                    }
                 }
             };
             if (gate) outputs(std::true_type());
             else outputs(std::false_type());
+        }
+        if (Z2) {
+            next_z += step * p.ld;
+            commit();
         }
     }
     if (many > 1) cluster_sync();  // (nobody reads here any more)
@@ -830,7 +858,7 @@ struct Launch {
 
 template <typename T, int VEC, int CG, int ST, int LC, int PER_SM, bool PRE>
 int launch_prefill(Launch &l) {
-    using L = Tile<T, VEC, CG, ST, LC>;
+    using L = Tile<T, VEC, CG, ST, LC, PRE>;
     Args &a = l.a;
     const int C = a.l.C, P = a.l.P, H = a.l.H;
     const int n_cb = (C + CG * VEC - 1) / (CG * VEC);
