@@ -243,6 +243,7 @@ __global__ void __launch_bounds__(128) heads_kernel(const Args p, float4 *tab, f
     const int h = (int)(i - part * p.l.H);
     if (part * LC >= p.rows) return;
     float4 *out = tab + i * LC;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const float bias = p.l.dt_bias[h], rate = expf(p.l.a_log[h]);
     T dt[LC], b[LC], c[LC];
 #pragma unroll
@@ -446,12 +447,8 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
     };
 
     // ---- before the first tile
-    if (first < p.rows) {
-        stage_rows(first, p.x, next_x, sx);
-        stage_rest(first, 0);
-    }
+    if (first < p.rows) stage_rows(first, p.x, next_x, sx);
     next_x += step * p.ld;
-    commit();
     if (!PRE) {
         if (first < p.rows) load_heads(first);
         if (tid < nh) {
@@ -490,6 +487,10 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
     __syncthreads();
     if (!PRE && first < p.rows) head_table(first, 0);
     describe_rows(first);
+    // until here the head scalars need not be there (launch_prefill)
+    if (PRE) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (first < p.rows) stage_rest(first, 0);
+    commit();
 
     auto conv_at = [&](int slot, int j) {
         return static_cast<T *>(p.l.conv) + ((int64_t)slot * 3 + j) * C + ch;
@@ -891,16 +892,23 @@ int launch_prefill(Launch &l) {
     static bmc::SharedMemory shm;
     BMC_CK(shm.allow(reinterpret_cast<const void *>(k), most, l.device));
     cudaLaunchConfig_t c{};
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     c.gridDim = dim3((unsigned)n_cb, (unsigned)many);
     c.blockDim = dim3(L::NT);
     c.dynamicSmemBytes = bytes;
     c.stream = l.s;
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = at[0].val.clusterDim.z = 1;
-    at[0].val.clusterDim.y = (unsigned)many;
     c.attrs = at;
-    c.numAttrs = many > 1 ? 1 : 0;
+    if (many > 1) {
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = at[0].val.clusterDim.z = 1;
+        at[0].val.clusterDim.y = (unsigned)many;
+        c.numAttrs = 1;
+    }
+    if (PRE) {  // starts while heads_kernel runs, and waits for it before it uses the table
+        at[c.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[c.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+        ++c.numAttrs;
+    }
     BMC_CK(cudaLaunchKernelEx(&c, k, static_cast<const Args>(a), heads, wide));
     return BM_OK;
 }
