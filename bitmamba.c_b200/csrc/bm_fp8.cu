@@ -547,7 +547,7 @@ cudaError_t few_rows(const uint8_t *a, const uint8_t *w, const ProductArgs &p, i
 constexpr int BM = 128, BN = 128, STAGES = 3, TBUF = 2;  // (of a pipeline)
 constexpr int STAGE_BYTES = (BM + BN) * BKB;
 constexpr int MANY_THREADS = 32 * (4 + 8);
-constexpr int TURN = 33 * 16 * 4;  // a warp's 16 x 32 values on their way out
+constexpr int TURN = 36 * 16 * 4;  // a warp's 16 x 32 values on their way out, 16-byte words of 8 lanes in all banks
 constexpr int KRING = 8;           // blocks whose scales a thread has at hand
 constexpr size_t MANY_SMEM = 1024 + (size_t)2 * STAGES * STAGE_BYTES + 8 * TURN + KRING * 256 * 4 + 256;
 
@@ -735,16 +735,18 @@ __global__ void __launch_bounds__(MANY_THREADS, 1)
                 for (int r = 0; r < 32; r += 16) {
                     if ((lane & 16) == r) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) turn[(lane & 15) * 33 + j] = acc[c * 32 + j];
+                        for (int j = 0; j < 32; j += 4)
+                            *reinterpret_cast<float4 *>(turn + (lane & 15) * 36 + j) =
+                                make_float4(acc[c * 32 + j], acc[c * 32 + j + 1], acc[c * 32 + j + 2], acc[c * 32 + j + 3]);
                     }
                     __syncwarp();
                     if (n < p.N) {
                         float *o = p.out + (int64_t)(m0 + r) * p.ldo + n;
                         if (rows == 32) {
 #pragma unroll
-                            for (int i = 0; i < 16; ++i, o += p.ldo) *o = turn[i * 33 + lane];
+                            for (int i = 0; i < 16; ++i, o += p.ldo) *o = turn[i * 36 + lane];
                         } else {
-                            for (int i = 0; i < 16 && r + i < rows; ++i, o += p.ldo) *o = turn[i * 33 + lane];
+                            for (int i = 0; i < 16 && r + i < rows; ++i, o += p.ldo) *o = turn[i * 36 + lane];
                         }
                     }
                     __syncwarp();
