@@ -10,14 +10,15 @@
 // works on the next buffer.
 //
 // Two shapes of tile:
-//   few rows    128 rows of w (the accumulator's lanes) by NB = 16 .. 128 rows
-//               of a (its columns), so that a few rows cost a narrow tile
-//               instead of a padded one.  Bound by the bytes of w.
+//   few rows    128 rows of w (the accumulator's lanes) by NB = 16, 32, 64, 96
+//               or 128 rows of a (its columns), so that a few rows cost a
+//               narrow tile instead of a padded one.  Bound by the bytes of w.
 //   many rows   128 rows of a (lanes) by 128 rows of w: a thread's scale is
 //               one value for its 128 columns.  (With w on the lanes every
 //               column has its own scale, and fetching 128 of them a block
 //               took twice as long as the tensor core's work.)
 #include <cstdint>
+#include <type_traits>
 
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
@@ -259,8 +260,8 @@ struct ProductArgs {
 // ---- few rows
 //
 // Persistent CTAs with one tile after the other, or (split > 1) a cluster of
-// `split` CTAs per tile, each with a part of K: the others hand their sums to
-// the first through its shared memory, which adds them in order.  The scales
+// `split` CTAs per tile, each with a part of K, whose sums they hand one
+// another through shared memory and add in order.  The scales
 // of a stay in shared memory, those of w in the lanes of a warp.  Two threads
 // issue copies and two MMAs, each every other block: one alone spends some 800
 // cycles a block on its waits, descriptors and commits (the blocks are
@@ -271,7 +272,7 @@ struct Few {
     static constexpr int PW = NB >= 64 ? 8 : 4;  // promotion warps
     static constexpr int CW = NB / (PW / 4);     // columns per promotion warp
     static constexpr int TB = 4;                 // tensor memory buffers
-    static constexpr int COLS = TB * NB;         // a power of two >= 32
+    static constexpr int COLS = NB == 96 ? 512 : TB * NB;  // a power of two >= 32
     static constexpr int STAGE = BV * BKB + NB * BKB;
     static constexpr int THREADS = 32 * (4 + PW);
     static constexpr int MAX_STAGES = 12;
@@ -394,7 +395,7 @@ __global__ void __launch_bounds__(Few<NB>::THREADS, 1)
         }
         asm volatile("bar.sync 1, %0;" ::"r"(32 * S::PW) : "memory");
         const int q = warp & 3, c0 = ((warp - 4) >> 2) * S::CW;
-        constexpr int LD = S::CW < 32 ? 16 : 32;
+        constexpr int LD = S::CW % 32 ? 16 : 32;
         int g = 0;
         // 32 blocks' scales of w in the lanes, the next ones on their way
         auto load_sw = [&](int t, int kb) {
@@ -448,40 +449,52 @@ __global__ void __launch_bounds__(Few<NB>::THREADS, 1)
                     }
                 }
             }
-            // sums of this CTA's part of K to the first of the cluster: [rank
-            // - 1][column][lane of w], over its stages, which are idle by then
-            // (its tensor core has read them, else it had not got this far)
-            const int at = (c0 * 128 + q * 32 + lane) * 4;
-            if (split > 1) {
-                asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
-                if (rank > 0) {
-                    const uint32_t mine = sa(smem) + (uint32_t)((rank - 1) * NB * 128 * 4 + at);
-                    uint32_t theirs;
-                    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(theirs) : "r"(mine));
+            const int n = t * S::BV + q * 32 + lane;
+            float *o = p.out + (int64_t)c0 * p.ldo + n;
+            if (split == 1) {
+                if (good && n < p.N) {
 #pragma unroll
-                    for (int j = 0; j < S::CW; ++j)
-                        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(theirs + j * 512),
-                                     "f"(j % 2 ? acc[j / 2].y : acc[j / 2].x)
-                                     : "memory");
+                    for (int j = 0; j < S::CW; ++j, o += p.ldo)
+                        if (c0 + j < p.M) *o = j % 2 ? acc[j / 2].y : acc[j / 2].x;
                 }
+                continue;
+            }
+            // Each CTA of the cluster adds up a share of the columns: the sums of
+            // this CTA's part of K go there, [part][column of the share][lane of
+            // w], over the stages, which are idle by then (every tensor core has
+            // read its own, else its CTA had not got to the barrier).  (100 x
+            // 2048 x 4096: 9.9 us; all sums to the first CTA 12.2.)
+            auto exchange = [&](auto parts) {
+                constexpr int SPLIT = decltype(parts)::value, SHARE = S::CW / SPLIT, OF = S::PW / 4;
+                const int of = (warp - 4) >> 2;
+                const uint32_t mine = sa(smem) + (uint32_t)(((rank * OF + of) * SHARE * 128 + q * 32 + lane) * 4);
                 asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
-                if (rank > 0) break;
-                for (int r = 0; r < split - 1; ++r) {
-                    const float *from = reinterpret_cast<const float *>(smem + (size_t)r * NB * 128 * 4 + at);
 #pragma unroll
-                    for (int j = 0; j < S::CW; ++j) {
-                        if (j % 2) acc[j / 2].y += from[j * 128];
-                        else acc[j / 2].x += from[j * 128];
+                for (int to = 0; to < SPLIT; ++to) {
+                    uint32_t theirs;
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(theirs) : "r"(mine), "r"(to));
+#pragma unroll
+                    for (int j = 0; j < SHARE; ++j) {
+                        const int c = to * SHARE + j;
+                        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(theirs + j * 512),
+                                     "f"(c % 2 ? acc[c / 2].y : acc[c / 2].x)
+                                     : "memory");
                     }
                 }
-            }
-            const int n = t * S::BV + q * 32 + lane;
-            if (good && n < p.N) {
-                float *o = p.out + (int64_t)c0 * p.ldo + n;
+                asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+                const float *from = reinterpret_cast<const float *>(smem) + of * SHARE * 128 + q * 32 + lane;
+                const int m0 = c0 + rank * SHARE;
+                o += (int64_t)rank * SHARE * p.ldo;
 #pragma unroll
-                for (int j = 0; j < S::CW; ++j, o += p.ldo)
-                    if (c0 + j < p.M) *o = j % 2 ? acc[j / 2].y : acc[j / 2].x;
-            }
+                for (int j = 0; j < SHARE; ++j, o += p.ldo) {
+                    float sum = from[j * 128];
+#pragma unroll
+                    for (int r = 1; r < SPLIT; ++r) sum += from[(r * OF * SHARE + j) * 128];
+                    if (good && n < p.N && m0 + j < p.M) *o = sum;
+                }
+            };
+            if (split == 2) exchange(std::integral_constant<int, 2>());
+            else exchange(std::integral_constant<int, 4>());
         }
     }
     if (split > 1 && warp < 4) {
@@ -510,11 +523,12 @@ cudaError_t few_rows(const uint8_t *a, const uint8_t *w, const ProductArgs &p, i
     if (e == cudaSuccess) e = shm.allow(reinterpret_cast<const void *>(k), S::SMEM, device);
     if (e != cudaSuccess) return e;
     const int tiles = (p.N + S::BV - 1) / S::BV, KB = (p.K + BKB - 1) / BKB;
-    // part of K each where tiles alone leave SMs idle: at least four blocks,
-    // and the others' sums fit over two thirds of the stages
+    // part of K each where tiles alone leave SMs idle: at least four blocks
+    // (the sums, NB * 512 bytes, fit over any three stages).  Clusters of 8 are
+    // slower: 16.2 us for 100 x 2048 x 4096 where those of 4 take 9.9.
     int split = 1;
-    while (split < 4 && tiles * split * 2 <= sms && KB >= split * 2 * 4 && (split * 2 - 1) * NB <= 256) split *= 2;
-    const int blocks = (KB + split - 1) / split, stages = S::stages(blocks);
+    while (split < 4 && tiles * split * 2 <= sms && KB >= split * 2 * 4) split *= 2;
+    const int stages = S::stages((KB + split - 1) / split);
     cudaLaunchConfig_t c{};
     cudaLaunchAttribute at[1];
     c.gridDim = dim3((unsigned)(split > 1 ? tiles * split : tiles < sms ? tiles : sms));
@@ -780,6 +794,7 @@ cudaError_t product(const uint8_t *a, const uint8_t *w, const ProductArgs &p, in
     if (p.M <= 16) return few_rows<16>(a, w, p, sms, s);
     if (p.M <= 32) return few_rows<32>(a, w, p, sms, s);
     if (p.M <= 64) return few_rows<64>(a, w, p, sms, s);
+    if (p.M <= 96) return few_rows<96>(a, w, p, sms, s);
     if (p.M <= 128) return few_rows<128>(a, w, p, sms, s);
     return many_rows(a, w, p, sms, s);
 }

@@ -184,6 +184,21 @@ def test_product_many_tiles(gpu_ctx, M, K, N):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("M", [2, 31, 48, 66, 95, 96, 97, 128])
+@pytest.mark.parametrize("K,N", [(1024, 300), (2000, 9000), (4096, 2047), (4112, 130)])
+def test_product_split_over_a_cluster(gpu_ctx, M, K, N):
+    """One, two and four CTAs a tile, each with a part of K and of the columns."""
+    a, asc, w, wsc = make(K + M, M, K, N)
+    out = product(gpu_ctx, a, asc, w, wsc, pad=3)
+    ad = a.double() * asc[:, :M].T.double().repeat_interleave(128, 1)[:, :K]
+    wd = w.double() * wsc.double().repeat_interleave(128, 0)[:N].repeat_interleave(128, 1)[:, :K]
+    want, mag = ad @ wd.T, ad.abs() @ wd.abs().T
+    assert ((out[:, :N] - want).abs() <= (256 + 2 + -(-K // 128)) * U * mag).all()
+    assert (out[:, N:] == -3.0).all()
+    gpu_ctx.check()
+
+
+@pytest.mark.gpu
 def test_product_nan_stays_in_its_row_and_column(gpu_ctx):
     a, asc, w, wsc = make(3, 20, 256, 300)
     clean = product(gpu_ctx, a, asc, w, wsc)
