@@ -328,10 +328,11 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
     // the next tile's first chunk of this thread; a tile's copies move them on
     const T *next_x = static_cast<const T *>(p.x) + (int64_t)(first + copy_r) * p.ld + c0 + copy_i * E;
     const T *next_z = static_cast<const T *>(p.z) + (next_x - static_cast<const T *>(p.x));
-    auto copy = [&](const T *&from, uint32_t to, int n) {
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+    // (a predicate, not a branch, which would keep the tokens from overlapping)
+    auto copy = [&](const T *&from, uint32_t to, int n, bool yes) {
+        asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %2, 0;\n @p cp.async.cg.shared.global [%0], [%1], 16;\n}" ::"r"(
                          to + n * (STEP * CG + STEP / LC * L::PAD) * (int)sizeof(Word)),
-                     "l"(from)
+                     "l"(from), "r"((int)yes)
                      : "memory");
         from += copy_pitch;
     };
@@ -339,7 +340,7 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
         const int live = min(ROWS, p.rows - r0);
         if (wide) {
             const uint32_t to = (uint32_t)__cvta_generic_to_shared(dst) + copy_to;
-            for (int n = 0; copy_r + n * STEP < live; ++n) copy(next, to, n);
+            for (int n = 0; copy_r + n * STEP < live; ++n) copy(next, to, n, true);
         } else if (on) {
             const T *src = static_cast<const T *>(from) + r0 * p.ld + c0;
             for (int r = part; r < live; r += ST)
@@ -557,6 +558,7 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
         }
         const int *info = row_info + b0;
         const float4 *tb = tabs + (buf * heads + hh) * ROWS + b0;
+        const uint32_t tb_at = (uint32_t)__cvta_generic_to_shared(tb);
         const Word *xw = sx + buf * L::WORDS + b0 * CG + part * L::PAD + cg, *zw = sz + (Z2 ? buf * L::WORDS : 0) + b0 * CG + part * L::PAD + cg;
 
         // x1, x2, x3: the inputs 1, 2, 3 tokens back; from the slot before the
@@ -578,7 +580,11 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
         V he = h, e1 = h, e2 = h, e3 = h;
         int end_info = -1;
         auto token = [&](int t) {
-            const float4 k = tb[t];
+            float4 k;
+            // (all four at once: the compiler would take two loads for the three that are used)
+            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(k.x), "=f"(k.y), "=f"(k.z), "=f"(k.w)
+                         : "r"(tb_at + t * 16));
             R xr;
             xr.v = xw[t * CG];
             const V xt = xr.get();
@@ -591,14 +597,12 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
             // x during all of them, or z during the first half and x the second
             constexpr int X0 = Z2 ? 0 : LC / 2, SPAN = LC - X0, EVERY = SPAN / COPIES > 0 ? SPAN / COPIES : 1;
             constexpr int EACH = (COPIES + SPAN / EVERY - 1) / (SPAN / EVERY);
-            if (t < X0 ? spread_z : spread_x) {
 #pragma unroll
-                for (int n = 0; n < EACH; ++n) {
-                    const int c = t % SPAN / EVERY * EACH + n;
-                    if ((t + 1) % EVERY == 0 && c < COPIES) {
-                        if (t < X0) copy(from_z, to_z, c);
-                        else copy(from_x, to_x, c);
-                    }
+            for (int n = 0; n < EACH; ++n) {
+                const int c = t % SPAN / EVERY * EACH + n;
+                if ((t + 1) % EVERY == 0 && c < COPIES) {
+                    if (t < X0) copy(from_z, to_z, c, spread_z);
+                    else copy(from_x, to_x, c, spread_x);
                 }
             }
             if (!Z2 && t == X0 - 1) commit();
@@ -789,10 +793,10 @@ __global__ void __launch_bounds__(CG *ST, PER_SM) prefill_kernel(const Args p, i
             T *py = static_cast<T *>(p.y) + ch + (r0 + b0) * p.ldy;
             auto ahead = [&](int t) {  // the next tile's z
                 constexpr int EVERY = LC / COPIES > 0 ? LC / COPIES : 1, EACH = (COPIES + LC - 1) / LC;
-                if (!Z2 || !spread_z || (t + 1) % EVERY) return;
+                if (!Z2 || (t + 1) % EVERY) return;
 #pragma unroll
                 for (int n = 0; n < EACH; ++n)
-                    if (t / EVERY * EACH + n < COPIES) copy(from_z, to_z, t / EVERY * EACH + n);
+                    if (t / EVERY * EACH + n < COPIES) copy(from_z, to_z, t / EVERY * EACH + n, spread_z);
             };
             auto finish = [&](int t, bool fix, auto gated) {
                 V o = y[t];
