@@ -187,6 +187,25 @@ def test_prefill_tall(gpu_ctx, sampler_lib, type_, H, P, rows, pad):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("gate", [True, False])
+@pytest.mark.parametrize("seed,H,P,most", [(1, 2, 32, 20), (2, 3, 32, 60), (3, 2, 48, 300), (4, 20, 128, 900)])
+def test_prefill_ragged_tall(gpu_ctx, sampler_lib, type_, gate, seed, H, P, most):
+    """Boundaries at every place of a part and of a tile, states taken up and
+    started, rows of no sequence before the first and behind the last."""
+    rng = np.random.default_rng(seed)
+    lengths = []
+    while sum(lengths) < 2600:
+        lengths.append(int(rng.integers(0, most)))
+    n = len(lengths)
+    off = offsets(lengths, first=7)
+    p = Problem(seed, type_, H, P, off[-1] + 30, n + 2, gate=gate)
+    slots, fresh = list(rng.permutation(n + 2)[:n]), list((rng.random(n) < 0.5).astype(int))
+    p.prefill(sampler_lib, gpu_ctx, off, slots, fresh)
+    p.check(off, slots, fresh)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
 def test_prefill_thousands_of_sequences(gpu_ctx, sampler_lib, type_):
     """More sequences than a CTA keeps offsets of; many without tokens."""
     rng = np.random.default_rng(2)
@@ -312,6 +331,30 @@ def test_captured_and_replayed(gpu_ctx, sampler_lib):
         # the replay continued nothing: every sequence started from zero, then took one token
         assert torch.equal(y, p.y) and torch.equal(h, p.dh)
     gpu_ctx.check()
+
+
+@pytest.mark.gpu
+def test_prefill_far_from_zero(gpu_ctx, sampler_lib):
+    """Sigmoids at their ends: inputs and gates of hundreds, next to small ones
+    in the same pair of channels; compared to the largest of each row."""
+    import torch
+    p = Problem(36, "f32", 2, 32, 200, 1)
+    g = torch.Generator().manual_seed(3)
+    scale = torch.exp2(torch.randint(-8, 9, (200, 4 * 32), generator=g).float())
+    p.proj[:, :2 * p.C] *= scale
+    p.dproj.copy_(p.proj)
+    torch.cuda.synchronize()
+    p.prefill(sampler_lib, gpu_ctx, [0, 200])
+    torch.cuda.synchronize()
+    f = p.proj.double().numpy()
+    C, H = p.C, p.H
+    w = {k: v.astype(np.float64) for k, v in p.w.items()}
+    y, ey, _, h, _ = ssm_ref.run(f[:, C:2 * C], f[:, :C], *(f[:, 2 * C + k * H:2 * C + (k + 1) * H] for k in range(3)), w, H,
+                                 p.P, np.zeros((3, C)), np.zeros(C), True)
+    got = p.y.double().cpu().numpy()
+    top = np.abs(y).max(1, keepdims=True)
+    assert np.isfinite(got).all()
+    assert (np.abs(got - y) <= 2 * ey + ssm_ref.U * np.abs(y) + 2.0 ** -40 * top).all()
 
 
 def refused(call, args, **changes):
