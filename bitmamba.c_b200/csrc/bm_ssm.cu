@@ -869,6 +869,15 @@ struct Launch {
     cudaStream_t s;
 };
 
+// CTAs of a cluster, for SMs that would be idle.  Clusters of 8 only where they
+// leave a third of the SMs: 16 of them do not fit the GPCs at once, and the
+// second turn costs more than they save (1500 x 512 bf16 17 us, of 4 14).
+int cluster_of(int n_cb, int64_t tiles, int at_once) {
+    int many = 1;
+    while (many < 8 && many < tiles && n_cb * many * 2 <= (many < 4 ? at_once : at_once * 2 / 3)) many *= 2;
+    return many;
+}
+
 template <typename T, int VEC, int CG, int ST, int LC, int PER_SM, bool PRE>
 int launch_prefill(Launch &l) {
     using L = Tile<T, VEC, CG, ST, LC, PRE>;
@@ -876,9 +885,7 @@ int launch_prefill(Launch &l) {
     const int C = a.l.C, P = a.l.P, H = a.l.H;
     const int n_cb = (C + CG * VEC - 1) / (CG * VEC);
     const int tiles = a.rows > 0 ? (int)(((int64_t)a.rows + L::ROWS - 1) / L::ROWS) : 1;
-    // clusters for SMs that would be idle
-    int many = 1;
-    while (many < 8 && many < tiles && n_cb * many * 2 <= l.sms * PER_SM) many *= 2;
+    const int many = cluster_of(n_cb, tiles, l.sms * PER_SM);
     const int64_t parts = ((int64_t)a.rows + LC - 1) / LC;
     const size_t tab_bytes = PRE ? (size_t)parts * H * (LC * sizeof(float4) + sizeof(float)) : 0;
     if (PRE) {
@@ -1106,9 +1113,19 @@ int bm_ssm_prefill(bm_ctx_t *ctx, const bm_ssm_layer_t *layer, const void *d_x, 
         return f32 ? launch_prefill<float, 1, 32, 16, 8, 1, false>(l) : launch_prefill<bf16, 1, 32, 16, 8, 1, false>(l);
     if (rows <= 64)
         return f32 ? launch_prefill<float, 2, 16, 8, 8, 4, false>(l) : launch_prefill<bf16, 2, 16, 8, 8, 4, false>(l);
-    // the head scalars of few tiles cost less in the CTAs than a launch, and a
-    // table of them is no use where it is larger than the inputs
-    if (rows <= 2048 || (int64_t)rows * a.l.H > ((int64_t)1 << 26))
+    // The head scalars of few tiles cost less in the CTAs than a launch for them
+    // (about 1 us), which in turn makes fp32's tiles of 256 rows 0.4 us shorter
+    // (4 turns: 22.2 us instead of 23.0 for 4096 channels, 3 the same) and lets
+    // bf16's have 512 rows (5.7 us a turn instead of 4.0 for 256).  A table
+    // larger than the inputs is no use.
+    const int n_cb = (a.l.C + 31) / 32;
+    auto turns = [&](int tile) {
+        const int64_t tiles = ((int64_t)rows + tile - 1) / tile;
+        const int many = cluster_of(n_cb, tiles, l.sms);
+        return (tiles + many - 1) / many;
+    };
+    const bool table = f32 ? turns(256) >= 4 : 57 * turns(512) + 10 < 40 * turns(256);
+    if (!table || (int64_t)rows * a.l.H > ((int64_t)1 << 26))
         return f32 ? launch_prefill<float, 2, 16, 32, 8, 1, false>(l) : launch_prefill<bf16, 2, 16, 32, 8, 1, false>(l);
     return f32 ? launch_prefill<float, 2, 16, 32, 8, 1, true>(l) : launch_prefill<bf16, 2, 16, 32, 16, 1, true>(l);
 }

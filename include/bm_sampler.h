@@ -336,7 +336,7 @@ typedef struct {
  * Writes each sequence's state after its last token to its slot (an empty
  * sequence: unchanged, or zeros when fresh); other slots are not touched.
  * Stream-ordered (stream NULL: the context's stream).  Calls of more than
- * 2048 rows use a workspace of the context (about 17 bytes per row and head,
+ * 256 rows may use a workspace of the context (about 17 bytes per row and head,
  * at most 1.1 GB) that is grown when needed and kept until the context is
  * destroyed: the first call of a size must not be under stream capture, later
  * ones may be, and such calls on one context must not overlap in time (two
