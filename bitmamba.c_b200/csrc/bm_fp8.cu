@@ -57,19 +57,29 @@ __device__ __forceinline__ uint32_t to_e4m3(float4 v) { return __nv_fp8x4_e4m3(v
 __device__ __forceinline__ float4 times(float4 v, float k) {
     return make_float4(v.x * k, v.y * k, v.z * k, v.w * k);
 }
-// e4m3(448 v / top) from the exact quotients
-__device__ __noinline__ uint32_t to_e4m3_exact(float4 v, float top) {
-    const double f[4] = {v.x, v.y, v.z, v.w};
-    uint32_t q = 0;
-    for (int i = 0; i < 4; ++i)
-        q |= (uint32_t)__nv_cvt_double_to_fp8(448.0 * f[i] / (double)top, __NV_SATFINITE, __NV_E4M3) << (8 * i);
-    return q;
+// Of two neighbouring codes the one that 448 v / top rounds to: which side of
+// the border (the mean of both, 5 bits) it is on, both multiplied by top, is
+// exact in 64 bits; on it, the even one.
+__device__ __forceinline__ uint32_t nearer(uint32_t lo, uint32_t hi, double v, double top) {
+    auto value = [](uint32_t c) { return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)c, __NV_E4M3))); };
+    const double border = 0.5f * fabsf(value(lo) + value(hi)), d = 448.0 * fabs(v) - border * top;
+    return d > 0.0 ? hi : d < 0.0 ? lo : lo & 1u ? hi : lo;
 }
-__device__ __noinline__ uint32_t to_e4m3_exact(double x, double y, double z, double w, double top) {
+__device__ __noinline__ uint32_t settle(uint32_t lo, uint32_t hi, double x, double y, double z, double w, double top) {
     const double f[4] = {x, y, z, w};
     uint32_t q = 0;
-    for (int i = 0; i < 4; ++i)
-        q |= (uint32_t)__nv_cvt_double_to_fp8(448.0 * f[i] / top, __NV_SATFINITE, __NV_E4M3) << (8 * i);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q |= nearer(lo >> (8 * i) & 255u, hi >> (8 * i) & 255u, f[i], top) << (8 * i);
+    return q;
+}
+__device__ __noinline__ uint32_t settle(uint32_t lo, uint32_t hi, float4 v, float top) {
+    const float f[4] = {v.x, v.y, v.z, v.w};
+    uint32_t q = lo;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t a = lo >> (8 * i) & 255u, b = hi >> (8 * i) & 255u;
+        if (a != b) q ^= (a ^ nearer(a, b, f[i], top)) << (8 * i);
+    }
     return q;
 }
 
@@ -144,11 +154,22 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
             constexpr float margin = NORM ? 0x1p-20f : 0x1p-21f;
             float r;
             asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(top));
-            r *= 448.0f;
-            w = to_e4m3(times(v[i], r * (1.0f + margin)));
-            const bool close = w != to_e4m3(times(v[i], r * (1.0f - margin)));
+            uint32_t lo = 0;
+            bool close = false;
+            if (!NORM && sizeof(T) == 2) {
+                // 448 v is exact, its quotient by the 8 bits of top is on a border
+                // or 2^-16 away: one corrected quotient is enough
+                const float4 x448 = times(v[i], 448.0f);
+                w = to_e4m3(make_float4(divide(x448.x, top, r), divide(x448.y, top, r), divide(x448.z, top, r),
+                                        divide(x448.w, top, r)));
+            } else {
+                r *= 448.0f;
+                w = to_e4m3(times(v[i], r * (1.0f + margin)));
+                lo = to_e4m3(times(v[i], r * (1.0f - margin)));
+                close = w != lo;
+            }
             if (!NORM) {
-                if (close) w = to_e4m3_exact(v[i], top);
+                if (close) w = settle(lo, w, v[i], top);
             } else if (__any_sync(0xffffffffu, close)) {  // (top is the warp's)
                 // the products with the weight unrounded, and their largest
                 float4 f = make_float4(0.f, 0.f, 0.f, 0.f), k = f;
@@ -160,7 +181,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
                              e3 = (double)f.w * k.w;
                 double most_e = fmax(fmax(fabs(e0), fabs(e1)), fmax(fabs(e2), fabs(e3)));
                 for (int o = 16; o > 0; o >>= 1) most_e = fmax(most_e, __shfl_xor_sync(0xffffffffu, most_e, o));
-                if (close) w = to_e4m3_exact(e0, e1, e2, e3, most_e);
+                if (close) w = settle(lo, w, e0, e1, e2, e3, most_e);
             }
         }
         if (live && col < d) {

@@ -78,6 +78,27 @@ def test_quantize_rounds_to_even_exactly(gpu_ctx):
 
 
 @pytest.mark.gpu
+def test_quantize_every_bf16_value(gpu_ctx):
+    """All pairs of a bf16 significand with a largest of its block, over the
+    exponents where e4m3 has values: ties among them."""
+    import torch
+    sig = (128 + torch.arange(128, device="cuda")).float()
+    blocks = []
+    for e in range(-2, 20):
+        for top in range(128):
+            b = sig * 2.0 ** -e
+            m = (128.0 + top) * 4
+            blocks.append(torch.cat([b[:64], -b[64:127], torch.tensor([m], device="cuda")]).clamp(-m, m))
+    x = torch.stack(blocks).to(torch.bfloat16)
+    q, _ = quantize(gpu_ctx, x)
+    v = x.double()
+    v = 448.0 * v / v.abs().amax(1, keepdim=True)
+    grid = torch.exp2(torch.floor(torch.log2(v.abs().clamp(min=2.0 ** -6))) - 3)
+    t = v / grid  # (a quotient of 64 bits is exact on a tie, and far from one elsewhere)
+    assert torch.equal(q.double(), torch.round(t) * grid)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("type_", ["f32", "bf16"])
 def test_quantize_rounds_the_weighted_values_exactly(gpu_ctx, type_):
     """With a norm too, q is what 64 bits give for x * weight / max, value by
