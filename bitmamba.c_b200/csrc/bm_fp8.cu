@@ -639,7 +639,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1)
             // (2048 x 50257 x 2048: 324 us without, 304 so, 313 over three
             // quarters of it; never slower where tried).
             const int extra = tiles % (2 * step);
-            if (first >= extra && tiles > 2 * step) {
+            if (extra > 0 && first >= extra && tiles > 2 * step) {
                 const long long t0 = clock64(), late = (long long)(KB * 600 + 4400) * (first - extra) / (2 * step - extra);
                 while (clock64() - t0 < late) {}
             }
