@@ -304,11 +304,19 @@ struct Few {
     static constexpr int MAX_STAGES = 12;
     static constexpr size_t BARS = (2 * MAX_STAGES + 2 * TB) * 8 + 16;
     static constexpr int SMEM = 220 * 1024;
-    // as many stages as fit beside the scales of kb blocks
-    static int stages(int kb) {
+    // As many stages as fit beside the scales of kb blocks, and an even number
+    // of them: block j is in stage j % stages, so every use of a stage is of one
+    // parity, by one of the copying threads and one of the MMA threads, and each
+    // waits for the other's last use of it.  With an odd number a stage's uses
+    // alternate between the threads, and the one parity bit of a wait tells a
+    // use from the second to last before it only while the four accumulators
+    // keep the threads closer than that: with five stages they do not, and a
+    // block was overwritten before its MMAs read it.
+    static constexpr int stages(int kb) {
         const int n = (int)((SMEM - 1024 - BARS - (size_t)kb * NB * 4) / STAGE);
-        return n < MAX_STAGES ? n : MAX_STAGES;
+        return (n < MAX_STAGES ? n : MAX_STAGES) & ~1;
     }
+    static_assert(MAX_STAGES % 2 == 0, "stages");
 };
 
 template <int NB>
@@ -943,6 +951,19 @@ int bm_fp8_logits(bm_ctx_t *ctx, const float *d_hidden, int B, int d_model, cons
     rc = bm_fp8_quantize(ctx, d_hidden, BM_F32, B, d_model, d_model, d_norm_w, q, sc, lds, stream);
     if (rc != BM_OK) return rc;
     return bm_fp8_product(ctx, q, sc, lds, B, d_model, d_w, d_w_scale, V, d_logits, ld, stream);
+}
+
+// The stages of a few-rows tile of nb rows with `blocks` blocks of K a CTA, 0
+// for other nb.  Not part of the public ABI: for tests on the host.
+int bm_detail_fp8_stages(int nb, int blocks) {
+    switch (nb) {
+        case 16: return bml::Few<16>::stages(blocks);
+        case 32: return bml::Few<32>::stages(blocks);
+        case 64: return bml::Few<64>::stages(blocks);
+        case 96: return bml::Few<96>::stages(blocks);
+        case 128: return bml::Few<128>::stages(blocks);
+        default: return 0;
+    }
 }
 
 }  // extern "C"

@@ -315,3 +315,20 @@ def test_products_at_once_on_two_streams(gpu_ctx):
     torch.cuda.synchronize()
     assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
     gpu_ctx.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N", [(97, 8192, 10000), (128, 8192, 10000), (128, 14976, 9600), (100, 16384, 9600),
+                                   (128, 16384, 9000), (97, 13584, 4800), (200, 16384, 3200)])
+def test_product_with_few_stages(gpu_ctx, M, K, N):
+    """Tiles of 128 rows whose scales leave room for four stages, whole rows of
+    K and parts of it: bounds as for test_product, twice with the same sums."""
+    import torch
+    a, asc, w, wsc = make(M + K, M, K, N)
+    out = product(gpu_ctx, a, asc, w, wsc)
+    ad = a.double() * asc[:, :M].T.double().repeat_interleave(128, 1)[:, :K]
+    wd = w.double() * wsc.double().repeat_interleave(128, 0)[:N].repeat_interleave(128, 1)[:, :K]
+    want, mag = ad @ wd.T, ad.abs() @ wd.abs().T
+    assert ((out - want).abs() <= (256 + 2 + -(-K // 128)) * U * mag).all()
+    assert torch.equal(out, product(gpu_ctx, a, asc, w, wsc))
+    gpu_ctx.check()
