@@ -83,6 +83,40 @@ __device__ __noinline__ uint32_t settle(uint32_t lo, uint32_t hi, float4 v, floa
     return q;
 }
 
+// A block near the ends of the range of fp32, past them as products with the
+// weight, or with values that are not finite: this thread's codes and the
+// block's scale.  x is taken by a power of two kx and the weight by kw, whose
+// product is back^-2; what is inexact then is far below the codes.
+template <bool NORM>
+__device__ __noinline__ uint2 at_the_ends(float4 x, float4 k, float rms, bool high) {
+    const float kx = !NORM ? 0x1p-64f : high ? 0x1p-66f : 0x1p+64f, back = !NORM ? 0x1p+32f : high ? 0x1p+65f : 0x1p-32f;
+    x = times(x, kx);
+    if (NORM && high) k = times(k, 0x1p-64f);
+    const float4 g = NORM ? make_float4(x.x * k.x, x.y * k.y, x.z * k.z, x.w * k.w) : x;
+    const unsigned m = max(max(__float_as_uint(g.x) & 0x7fffffffu, __float_as_uint(g.y) & 0x7fffffffu),
+                           max(__float_as_uint(g.z) & 0x7fffffffu, __float_as_uint(g.w) & 0x7fffffffu));
+    const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, m)), most = NORM ? top * rms : top;
+    const float sc = __fdiv_rn(most, 448.0f);
+    if (!(top < __int_as_float(0x7f800000)) || most != most) {  // an infinity or NaN
+        const float4 f = make_float4(__fdiv_rn(g.x * rms, sc), __fdiv_rn(g.y * rms, sc), __fdiv_rn(g.z * rms, sc),
+                                     __fdiv_rn(g.w * rms, sc));
+        return make_uint2(to_e4m3(f), __float_as_uint(sc));
+    }
+    if (!(most > 0.0f)) return make_uint2(0, __float_as_uint(1.0f));  // (rms is 0: the squares passed the range)
+    const float r = __fdiv_rn(448.0f, top);
+    const uint32_t lo = to_e4m3(times(g, r * (1.0f - 0x1p-20f))), hi = to_e4m3(times(g, r * (1.0f + 0x1p-20f)));
+    uint32_t q;
+    if (NORM) {
+        const double e0 = (double)x.x * k.x, e1 = (double)x.y * k.y, e2 = (double)x.z * k.z, e3 = (double)x.w * k.w;
+        double most_e = fmax(fmax(fabs(e0), fabs(e1)), fmax(fabs(e2), fabs(e3)));
+        for (int o = 16; o > 0; o >>= 1) most_e = fmax(most_e, __shfl_xor_sync(0xffffffffu, most_e, o));
+        q = settle(lo, hi, e0, e1, e2, e3, most_e);
+    } else {
+        q = settle(lo, hi, g, top);
+    }
+    return make_uint2(q, __float_as_uint(sc * back * back));
+}
+
 // TPR threads per row: a warp's 32 groups of 4 columns are one block of 128.
 // Bound by memory: a row is read once and stays in registers.  8192 x 4096 fp32
 // takes 28.7 us, 5.9 TB/s of reads and writes (the device copies at 6.5).
@@ -136,16 +170,31 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
         // the largest magnitude: as integers, whose order a NaN leads
         const unsigned m = max(max(__float_as_uint(v[i].x) & 0x7fffffffu, __float_as_uint(v[i].y) & 0x7fffffffu),
                                max(__float_as_uint(v[i].z) & 0x7fffffffu, __float_as_uint(v[i].w) & 0x7fffffffu));
-        const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, m));
-        const float most = NORM ? top * rms : top;
+        const unsigned bits = __reduce_max_sync(0xffffffffu, m);
+        const float top = __uint_as_float(bits), most = NORM ? top * rms : top;
         float sc = 1.0f;
         uint32_t w = 0;
-        if (!(top < 0x1p+120f && most < 0x1p+120f) || (top <= 0x1p-100f && most > 0x1p-100f)) {
-            // (an infinity or NaN among them, or close to the range's ends)
-            sc = __fdiv_rn(most, 448.0f);
-            w = to_e4m3(make_float4(__fdiv_rn(v[i].x * rms, sc), __fdiv_rn(v[i].y * rms, sc),
-                                    __fdiv_rn(v[i].z * rms, sc), __fdiv_rn(v[i].w * rms, sc)));
-        } else if (most > 0x1p-100f) {
+        // For bf16 alone one check of the bits, 2^-100 < top < 2^119 (448 times the
+        // largest is in range); beyond, both sides of the quotient by 512.
+        constexpr bool B16 = !NORM && sizeof(T) == 2;
+        constexpr unsigned LEAST = (127 - 100) << 23, MOST = (127 + 119) << 23;
+        if (B16 && bits - (LEAST + 1) >= MOST - (LEAST + 1)) {
+            if (bits >= MOST) {
+                const float4 f = times(v[i], 448.0f / 512.0f);
+                const float s = top * 0x1p-9f;
+                sc = __fdiv_rn(top, 448.0f);
+                w = to_e4m3(make_float4(__fdiv_rn(f.x, s), __fdiv_rn(f.y, s), __fdiv_rn(f.z, s), __fdiv_rn(f.w, s)));
+            }
+        } else if (!B16 && (!(top < 0x1p+119f && most < 0x1p+119f) || (top <= 0x1p-100f && most > 0x1p-100f))) {
+            float4 k = make_float4(1.f, 1.f, 1.f, 1.f);
+            if (NORM && live && col < d) {
+                v[i] = load4(x + (int64_t)row * ldx + col);
+                k = load4(norm_w + col);
+            }
+            const uint2 c = at_the_ends<NORM>(v[i], k, rms, !(top <= 0x1p-100f));
+            w = c.x;
+            sc = __uint_as_float(c.y);
+        } else if (B16 || most > 0x1p-100f) {
             sc = divide(most, 448.0f, 1.0f / 448.0f);
             // Rounded from both sides of the approximate quotients, by more than
             // these can be off (2 ulp of the reciprocal, 2 roundings: 2^-21.4;
@@ -156,7 +205,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
             asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(top));
             uint32_t lo = 0;
             bool close = false;
-            if (!NORM && sizeof(T) == 2) {
+            if (B16) {
                 // 448 v is exact, its quotient by the 8 bits of top is on a border
                 // or 2^-16 away: one corrected quotient is enough
                 const float4 x448 = times(v[i], 448.0f);

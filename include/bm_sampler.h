@@ -388,7 +388,9 @@ int bm_slots_reorder(bm_ctx_t *ctx, const bm_slot_region_t *regions, int n_regio
  * x * (1 / sqrtf(mean(x^2) + 1e-6f)) * norm_w first (d_norm_w NULL: none),
  * then scale = max|x| / 448 over the block (1 where max|x| <= 2^-100) and
  * q = e4m3(448 x / max|x|), rounded to nearest even from the exact quotient
- * (of x * norm_w unrounded; 0 where the scale is 1 for that reason).  A NaN in a block makes its scale
+ * (of x * norm_w unrounded; 0 where the scale is 1 for that reason), for all
+ * finite x and norm_w; a row whose squares pass the range of fp32 becomes
+ * zeros.  A NaN in a block (with a norm: in its row) makes its scale
  * NaN and the block NaN.  d_x: [rows x d] of `type` (BM_F32, BM_BF16),
  * row pitch ldx elements; d_q: [rows x d] e4m3 bytes; d_scale: scale of
  * (row r, block b) at d_scale[b * ld_scale + r], ld_scale >= rows and a

@@ -332,3 +332,94 @@ def test_product_with_few_stages(gpu_ctx, M, K, N):
     assert ((out - want).abs() <= (256 + 2 + -(-K // 128)) * U * mag).all()
     assert torch.equal(out, product(gpu_ctx, a, asc, w, wsc))
     gpu_ctx.check()
+
+
+def codes_of(v):
+    """e4m3 values of 448 v / max|v| by blocks of 128 columns, from 64 bits, and
+    where a quotient is too close to a border to tell (closer than 2^-46 steps)."""
+    import torch
+    b = v.view(v.shape[0], -1, 128)
+    b = (448.0 * b / b.abs().amax(2, keepdim=True)).view(v.shape)
+    grid = torch.exp2(torch.floor(torch.log2(b.abs().clamp(min=2.0 ** -6))) - 3)
+    t = b / grid
+    sure = ((t - torch.floor(t) - 0.5).abs() > 2.0 ** -46) | (t == torch.round(t))
+    return torch.round(t) * grid, sure
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+def test_quantize_at_the_ends_of_the_range(gpu_ctx, type_):
+    """Finite blocks whose largest lies in [2^115, 2^128) or [2^-100, 2^-97):
+    finite scales (a division's rounding off) and the codes of the exact
+    quotients.  In bf16 every significand of a value and of the largest, ties
+    among them: there a quotient is on a border or 2^-16 away."""
+    import torch
+    t = torch.float32 if type_ == "f32" else torch.bfloat16
+    g = torch.Generator(device="cuda").manual_seed(6)
+    bits = 24 if type_ == "f32" else 8
+    blocks = []
+    for e in list(range(115, 128)) + [-99, -98, -97]:
+        n = 128
+        top = 1.0 + torch.arange(n, device="cuda").double() / n
+        sig = 2 ** (bits - 1) + torch.randint(0, 2 ** (bits - 1), (n, 128), generator=g, device="cuda")
+        if type_ == "bf16":
+            sig = (128 + torch.arange(128, device="cuda")).expand(n, 128)
+        v = sig.double() / 2 ** (bits - 1) * torch.exp2(-torch.randint(0, 18, (n, 128), generator=g, device="cuda").double())
+        v = v * torch.where(torch.rand(n, 128, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+        v = torch.maximum(torch.minimum(v, top[:, None]), -top[:, None])
+        v[:, 5] = top
+        blocks.append(v * 2.0 ** e)
+    x = torch.cat(blocks).to(t)
+    assert torch.equal(x.double(), torch.cat(blocks))
+    q, scale = quantize(gpu_ctx, x)
+    want, sure = codes_of(x.double())
+    if type_ == "bf16":  # a quotient of 64 bits is exact on a tie, and far from one elsewhere
+        sure |= True
+    assert torch.equal(q.double()[sure], want[sure]) and sure.float().mean() > 0.9999
+    exact = x.double().abs().amax(1) / 448.0
+    assert ((scale[0, :x.shape[0]].double() - exact).abs() <= 2 * U * exact).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("ex,ew", [(0, 118), (0, 126), (3, 127), (-30, 127), (-52, -52), (-55, -50), (0, -99), (50, 80)])
+def test_quantize_with_a_norm_at_the_ends(gpu_ctx, type_, ex, ew):
+    """x about 2^ex, weights about 2^ew: products near the ends of the range and
+    past it; the scale is max|x w| / rms / 448 to the roundings of
+    test_quantize."""
+    import torch
+    rows, d = 64, 512
+    g = torch.Generator(device="cuda").manual_seed(7)
+    x = (torch.randn(rows, d, generator=g, device="cuda") * 2.0 ** ex).to(torch.float32 if type_ == "f32" else torch.bfloat16)
+    w = (1.0 + 0.9 * torch.rand(d, generator=g, device="cuda")) * 2.0 ** ew
+    q, scale = quantize(gpu_ctx, x, w)
+    v = x.double() * w.double()
+    want, sure = codes_of(v)
+    assert torch.equal(q.double()[sure], want[sure]) and sure.float().mean() > 0.9999
+    rms = torch.sqrt((x.double() ** 2).mean(1, keepdim=True) + 1e-6)
+    exact = (v.abs() / rms).view(rows, -1, 128).amax(2).T / 448.0
+    assert ((scale[:, :rows].double() - exact).abs() <= (d + 8) * U * exact * 1.01).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+def test_quantize_special_values_with_a_norm(gpu_ctx, type_):
+    """A NaN makes its row's factor NaN, an infinity 0; so do squares past the
+    range of fp32, whose row becomes zeros."""
+    import torch
+    x = torch.randn(5, 384, device="cuda")
+    x[0, 3] = float("nan")
+    x[1, 200] = -float("inf")
+    x[2] *= 2.0 ** 80
+    w = 1 + 0.1 * torch.rand(384, device="cuda")
+    q, s = quantize(gpu_ctx, x.to(torch.float32 if type_ == "f32" else torch.bfloat16), w)
+    f, s = q.float(), s.T
+    assert s[0].isnan().all() and f[0].isnan().all()
+    assert s[1, 1].isnan() and f[1, 128:256].isnan().all()
+    assert (s[1, [0, 2]] == 1.0).all() and (f[1, :128] == 0).all() and (f[1, 256:] == 0).all()
+    assert (s[2] == 1.0).all() and (f[2] == 0).all()
+    w[5] = float("inf")
+    q, s = quantize(gpu_ctx, x.to(torch.float32 if type_ == "f32" else torch.bfloat16), w)
+    f, s = q.float(), s.T
+    assert s[3:5, 0].isinf().all() and f[3:5, 5].isnan().all() and (f[3:5, 6:128] == 0).all()
+    assert s[3:5, 1:].isfinite().all() and f[3:5, 128:].isfinite().all()
