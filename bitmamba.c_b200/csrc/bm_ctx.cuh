@@ -24,7 +24,10 @@ int bm_detail_work(bm_ctx_t *c, int kind, size_t bytes, void **out);
 
 namespace bmc {
 
+// Reports a failed call, and clears the error that it leaves in the thread: a
+// later call that succeeds would report it.
 inline int cuda_fail(cudaError_t e, const char *what) {
+    cudaGetLastError();
     char buf[256];
     snprintf(buf, sizeof(buf), "%s: %s", what, cudaGetErrorString(e));
     return bm_detail_fail(e == cudaErrorMemoryAllocation ? BM_ERR_OOM : BM_ERR_CUDA, buf);
@@ -57,6 +60,18 @@ struct SharedMemory {
         return e;
     }
 };
+
+// A launch whose result is its own (what cudaGetLastError gives behind a launch
+// may be an earlier call's, and states would be taken for unchanged).
+template <typename... P, typename... A>
+cudaError_t launch(void (*kernel)(P...), dim3 grid, unsigned threads, size_t shared, cudaStream_t s, A &&...args) {
+    cudaLaunchConfig_t c{};
+    c.gridDim = grid;
+    c.blockDim = dim3(threads);
+    c.dynamicSmemBytes = shared;
+    c.stream = s;
+    return cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...);
+}
 
 }  // namespace bmc
 

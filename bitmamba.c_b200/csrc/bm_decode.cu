@@ -134,6 +134,7 @@ namespace {
 
 int dfail(int code, const char *what, cudaError_t e = cudaSuccess) {
     char buf[256];
+    if (e != cudaSuccess) cudaGetLastError();  // (a later call would report it)
     if (e != cudaSuccess)
         snprintf(buf, sizeof(buf), "%s: %s", what, cudaGetErrorString(e));
     else
@@ -164,10 +165,8 @@ void release(bm_decode_t *d) {
 
 int launch_update(bm_decode_t *d, int32_t *d_out_id, cudaStream_t s) {
     const int threads = 256, blocks = (d->rows + threads - 1) / threads;
-    decode_update_kernel<<<blocks, threads, 0, s>>>(d->d_id, d->rows, d->d_ring, d->d_pos, d->d_cur,
-                                                    d->d_status, d->d_ngen, d->d_stop, d->n_stop,
-                                                    d->max_tokens, d->d_active, d_out_id);
-    DCK(cudaGetLastError());
+    DCK(bmc::launch(decode_update_kernel, dim3((unsigned)blocks), threads, 0, s, d->d_id, d->rows, d->d_ring, d->d_pos,
+                    d->d_cur, d->d_status, d->d_ngen, d->d_stop, d->n_stop, d->max_tokens, d->d_active, d_out_id));
     return BM_OK;
 }
 
@@ -331,8 +330,7 @@ int bm_decode_reorder(bm_decode_t *d, const int32_t *d_src, const bm_slot_region
     bm_slot_region_t r[2 * BM_SLOT_REGIONS];
     const int n = all_regions(d, regions, n_regions, r);
     DCK(bms::reorder(r, n, d_src, d->B, sms, s));
-    count_active_kernel<<<1, 1024, 0, s>>>(d->d_status, d->B, d->d_active);
-    DCK(cudaGetLastError());
+    DCK(bmc::launch(count_active_kernel, dim3(1), 1024, 0, s, d->d_status, d->B, d->d_active));
     return BM_OK;
 }
 
@@ -350,8 +348,7 @@ int bm_decode_compact(bm_decode_t *d, const bm_slot_region_t *regions, int n_reg
     DCK(guard.error);
     if (stream) s = static_cast<cudaStream_t>(stream);
     int32_t *row_of = d->d_move, *live = d->d_move + d->B;
-    compact_map_kernel<<<1, 1024, 0, s>>>(d->d_status, d->B, row_of, live, d_map);
-    DCK(cudaGetLastError());
+    DCK(bmc::launch(compact_map_kernel, dim3(1), 1024, 0, s, d->d_status, d->B, row_of, live, d_map));
     bm_slot_region_t r[2 * BM_SLOT_REGIONS];
     const int n = all_regions(d, nullptr, 0, r);
     DCK(bms::reorder(r, n, row_of, d->B, sms, s));

@@ -246,9 +246,8 @@ cudaError_t quantize(const T *x, int rows, int d, int64_t ldx, const float *norm
 #define BM_Q(TPR)                                                                               \
     if (d <= 4 * QV * TPR) {                                                                    \
         constexpr int per = TPR < 256 ? 256 / TPR : 1;                                          \
-        quantize_kernel<T, TPR, NORM><<<(rows + per - 1) / per, TPR < 256 ? 256 : TPR, 0, s>>>( \
-            x, rows, d, ldx, norm_w, q, scale, ld_scale);                                       \
-        return cudaGetLastError();                                                              \
+        return bmc::launch(quantize_kernel<T, TPR, NORM>, dim3((unsigned)((rows + per - 1) / per)), \
+                           TPR < 256 ? 256 : TPR, 0, s, x, rows, d, ldx, norm_w, q, scale, ld_scale); \
     }
     BM_Q(32)
     BM_Q(128)
@@ -873,8 +872,7 @@ cudaError_t many_rows(const uint8_t *a, const uint8_t *w, const ProductArgs &p, 
     if (e != cudaSuccess) return e;
     const int64_t tiles = (int64_t)((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
     if (tiles > INT32_MAX / 2) return cudaErrorInvalidValue;
-    many_rows_kernel<<<(int)(tiles < sms ? tiles : sms), MANY_THREADS, MANY_SMEM, s>>>(ma, mw, p);
-    return cudaGetLastError();
+    return bmc::launch(many_rows_kernel, dim3((unsigned)(tiles < sms ? tiles : sms)), MANY_THREADS, MANY_SMEM, s, ma, mw, p);
 }
 
 cudaError_t product(const uint8_t *a, const uint8_t *w, const ProductArgs &p, int sms, cudaStream_t s) {

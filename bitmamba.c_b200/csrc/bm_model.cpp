@@ -328,6 +328,7 @@ int bm_model_head_load(bm_ctx_t *ctx, const char *path, bm_model_head_t **out) {
     I.d_packed = pd;
     I.d_w8 = w8;
     if (e != cudaSuccess) {
+        cudaGetLastError();  // (a later call would report it)
         bm_model_head_free(m);
         char buf[200];
         snprintf(buf, sizeof(buf), "model head upload: %s", cudaGetErrorString(e));
@@ -336,7 +337,10 @@ int bm_model_head_load(bm_ctx_t *ctx, const char *path, bm_model_head_t **out) {
     rc = bm_ternary_unpack(ctx, pd, V, dm, w8, nullptr);
     if (rc == BM_OK) {
         e = cudaStreamSynchronize(static_cast<cudaStream_t>(bm_ctx_stream(ctx)));
-        if (e != cudaSuccess) rc = bm_detail_fail(BM_ERR_CUDA, cudaGetErrorString(e));
+        if (e != cudaSuccess) {
+            cudaGetLastError();
+            rc = bm_detail_fail(BM_ERR_CUDA, cudaGetErrorString(e));
+        }
     }
     if (rc != BM_OK) {
         bm_model_head_free(m);

@@ -93,6 +93,7 @@ int fail(int code, const char *fmt, ...) {
 }
 
 int cuda_fail(cudaError_t e, const char *what) {
+    cudaGetLastError();  // (a later call would report it)
     int code = (e == cudaErrorMemoryAllocation) ? BM_ERR_OOM : BM_ERR_CUDA;
     return fail(code, "%s: %s", what, cudaGetErrorString(e));
 }
@@ -315,9 +316,11 @@ int bm_ctx_create(int device, bm_ctx_t **out) {
     *out = nullptr;
     int n = 0;
     cudaError_t e = cudaGetDeviceCount(&n);
-    if (e != cudaSuccess || n == 0)
+    if (e != cudaSuccess || n == 0) {
+        cudaGetLastError();
         return fail(BM_ERR_NO_DEVICE, "no CUDA device (%s)",
                     e == cudaSuccess ? "count 0" : cudaGetErrorString(e));
+    }
     if (device < 0 || device >= n)
         return fail(BM_ERR_NO_DEVICE, "device %d out of range (%d devices)", device, n);
     cudaDeviceProp prop;

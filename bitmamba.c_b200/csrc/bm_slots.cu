@@ -192,8 +192,7 @@ cudaError_t reorder(const bm_slot_region_t *regions, int n_regions, const int32_
     static bmc::SharedMemory shm;
     if (e == cudaSuccess) e = shm.allow(reinterpret_cast<const void *>(reorder_kernel), most, device);
     if (e != cudaSuccess) return e;
-    reorder_kernel<<<sms * per_sm, NT, bytes, s>>>(g, d_src, n_slots, room, buffers);
-    return cudaGetLastError();
+    return bmc::launch(reorder_kernel, dim3((unsigned)(sms * per_sm)), NT, bytes, s, g, d_src, n_slots, room, buffers);
 }
 
 }  // namespace bms

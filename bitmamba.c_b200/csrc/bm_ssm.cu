@@ -896,8 +896,8 @@ int launch_prefill(Launch &l) {
         a.dec = reinterpret_cast<const float *>(a.tab + parts * H * LC);
         const int64_t blocks = (parts * H + 127) / 128;
         if (blocks > INT32_MAX) return bm_detail_fail(BM_ERR_UNSUPPORTED, "rows * heads too large for one call");
-        heads_kernel<T, LC><<<(unsigned)blocks, 128, 0, l.s>>>(a, const_cast<float4 *>(a.tab), const_cast<float *>(a.dec));
-        BMC_CK(cudaGetLastError());
+        BMC_CK(bmc::launch(heads_kernel<T, LC>, dim3((unsigned)blocks), 128, 0, l.s, a, const_cast<float4 *>(a.tab),
+                           const_cast<float *>(a.dec)));
     }
     int heads = (CG * VEC + P - 2) / P + 1;
     if (heads > H) heads = H;
@@ -1156,14 +1156,9 @@ int bm_ssm_step(bm_ctx_t *ctx, const bm_ssm_layer_t *layer, const void *d_x, con
     if (down > (unsigned)rows) down = (unsigned)rows;
     const dim3 grid(across, down);
     using bf16 = __nv_bfloat16;
-    if (layer->type == BM_F32) {
-        if (quads) step_kernel<float, 4><<<grid, 128, 0, s>>>(a);
-        else step_kernel<float, 1><<<grid, 128, 0, s>>>(a);
-    } else {
-        if (quads) step_kernel<bf16, 4><<<grid, 128, 0, s>>>(a);
-        else step_kernel<bf16, 1><<<grid, 128, 0, s>>>(a);
-    }
-    BMC_CK(cudaGetLastError());
+    auto *k = layer->type == BM_F32 ? (quads ? step_kernel<float, 4> : step_kernel<float, 1>)
+                                    : (quads ? step_kernel<bf16, 4> : step_kernel<bf16, 1>);
+    BMC_CK(bmc::launch(k, grid, 128, 0, s, a));
     return BM_OK;
 }
 
