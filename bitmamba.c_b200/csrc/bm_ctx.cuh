@@ -11,6 +11,10 @@
 
 enum { BM_WORK_SCAN = 0, BM_WORK_FP8 = 1, BM_WORK_KINDS = 2 };
 
+// The largest workspace of bm_ssm_prefill: 2^26 rows times heads, the last part
+// of 16 rows of each of up to 2^16 heads filled up, 16.5 bytes each.
+constexpr size_t BM_WORK_SCAN_MOST = (((size_t)1 << 26) + ((size_t)1 << 20)) * 33 / 2;
+
 // The library's error channel: sets bm_last_error's text, returns code.
 int bm_detail_fail(int code, const char *msg);
 
@@ -19,7 +23,10 @@ int bm_detail_ctx(bm_ctx_t *c, int *sms, int **d_err, cudaStream_t *stream);
 
 // The context's workspace of a kind, at least `bytes` long, zeroed when it was
 // allocated and never freed before the context.  Growing it allocates and
-// synchronises the device, so it fails under stream capture.
+// synchronises the device, so it fails under stream capture.  It grows to twice
+// its size, so that all that were outgrown are together less than twice the
+// last of them, but not past the largest that its kind asks for, and to no more
+// than is asked for where twice cannot be had.
 int bm_detail_work(bm_ctx_t *c, int kind, size_t bytes, void **out);
 
 namespace bmc {
@@ -31,6 +38,14 @@ inline int cuda_fail(cudaError_t e, const char *what) {
     char buf[256];
     snprintf(buf, sizeof(buf), "%s: %s", what, cudaGetErrorString(e));
     return bm_detail_fail(e == cudaErrorMemoryAllocation ? BM_ERR_OOM : BM_ERR_CUDA, buf);
+}
+
+// The size that a workspace of `cap` bytes grows to when `bytes` are asked for,
+// and no call asks for more than `most`.
+inline size_t grown(size_t cap, size_t bytes, size_t most) {
+    size_t n = cap <= most / 2 ? 2 * cap : most;
+    if (n < bytes) n = bytes;
+    return (n + 255) & ~(size_t)255;
 }
 
 // Makes a context's device current, and the caller's again at the end.

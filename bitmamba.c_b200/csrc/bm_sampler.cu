@@ -917,16 +917,25 @@ int bm_detail_ctx(bm_ctx_t *c, int *sms, int **d_err, cudaStream_t *stream) {
     return c->device;
 }
 
+// (for tests on the host)
+extern "C" size_t bm_detail_grown(size_t cap, size_t bytes, int kind) {
+    return bmc::grown(cap, bytes, kind == BM_WORK_SCAN ? BM_WORK_SCAN_MOST : SIZE_MAX);
+}
+
 int bm_detail_work(bm_ctx_t *c, int kind, size_t bytes, void **out) {
     auto &w = c->work[kind];
     if (bytes > w.cap || w.n == 0) {
         constexpr int most = (int)(sizeof(w.buf) / sizeof(w.buf[0]));
         if (w.n == most) return fail(BM_ERR_OOM, "workspace grown %d times", most);
-        size_t n = 2 * w.cap;  // doubling: all buffers together stay under twice the largest
-        if (n < bytes) n = bytes;
-        n = (n + 255) & ~(size_t)255;
+        size_t n = bmc::grown(w.cap, bytes, kind == BM_WORK_SCAN ? BM_WORK_SCAN_MOST : SIZE_MAX);
+        const size_t least = (bytes + 255) & ~(size_t)255;
         void *p = nullptr;
         cudaError_t e = cudaMalloc(&p, n);
+        if (e == cudaErrorMemoryAllocation && n > least) {
+            cudaGetLastError();
+            n = least;
+            e = cudaMalloc(&p, n);
+        }
         if (e != cudaSuccess) return cuda_fail(e, "cudaMalloc(workspace)");
         e = cudaMemset(p, 0, n);
         // the memset is not ordered against the context's stream

@@ -887,6 +887,8 @@ int launch_prefill(Launch &l) {
     const int tiles = a.rows > 0 ? (int)(((int64_t)a.rows + L::ROWS - 1) / L::ROWS) : 1;
     const int many = cluster_of(n_cb, tiles, l.sms * PER_SM);
     const int64_t parts = ((int64_t)a.rows + LC - 1) / LC;
+    // (at most BM_WORK_SCAN_MOST: bm_ssm_prefill takes no table of more than 2^26
+    // rows times heads, and a pair's heads have 16 channels or more)
     const size_t tab_bytes = PRE ? (size_t)parts * H * (LC * sizeof(float4) + sizeof(float)) : 0;
     if (PRE) {
         void *work;

@@ -337,7 +337,9 @@ typedef struct {
  * sequence: unchanged, or zeros when fresh); other slots are not touched.
  * Stream-ordered (stream NULL: the context's stream).  Calls of more than
  * 256 rows may use a workspace of the context (about 17 bytes per row and head,
- * at most 1.1 GB) that is grown when needed and kept until the context is
+ * at most 1.13 GB) that is grown when needed, to twice its size where memory
+ * allows.  What it outgrows is kept too, since a captured graph may use it: in
+ * all less than three times the largest.  They go when the context is
  * destroyed: the first call of a size must not be under stream capture, later
  * ones may be, and such calls on one context must not overlap in time (two
  * replayed graphs among them).
