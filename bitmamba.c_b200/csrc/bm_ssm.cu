@@ -93,16 +93,13 @@ __device__ __forceinline__ float rcp(float v) {
     asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(v));
     return v;
 }
-// v / (1 + e^-v): where e^-v overflows the quotient's limit, -0
+// v / (1 + e^-v); where e^-v passes the range (v < -88.7) -0, as the quotient
+// in fp32 gives, and NaN for -infinity.
 __device__ __forceinline__ float silu(float v) { return v * rcp(ex2(v * -1.44269504f) + 1.0f); }
-// Of a pair, with one reciprocal: 1 / a = b / (a b), e^-v held at 2^63 so that
-// the product is in range (below -43, where silu is under 2^-57, v 2^-63).
-__device__ __forceinline__ float2 silu(float2 v) {
-    const float2 t = __fmul2_rn(v, make_float2(-1.44269504f, -1.44269504f));
-    const float2 e = __fadd2_rn(make_float2(ex2(fminf(t.y, 63.0f)), ex2(fminf(t.x, 63.0f))), make_float2(1.0f, 1.0f));
-    const float r = rcp(e.x * e.y);
-    return __fmul2_rn(v, make_float2(e.x * r, e.y * r));
-}
+// Of a pair, with a reciprocal each.  (One of the product for both has to hold
+// e^-v at 2^63, and then is v 2^-63 below -43, which grows with v; the same
+// time in fp32, 3 % less for 65536 x 4096 bf16.)
+__device__ __forceinline__ float2 silu(float2 v) { return make_float2(silu(v.x), silu(v.y)); }
 __device__ __forceinline__ float softplus(float v) {
     return fmaxf(v, 0.0f) + log1pf(expf(-fabsf(v)));
 }

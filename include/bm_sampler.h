@@ -293,7 +293,8 @@ int bm_ternary_sample_batch(bm_ctx_t *ctx, const float *d_hidden, int B, int d_m
  *   s_t[c] = a * s_{t-1}[c] + d * B_t[h] * u_t[c]
  *   y_t[c] = (C_t[h] * s_t[c] + D[c] * u_t[c]) * silu(z_t[c])
  *
- * evaluated in fp32; y is rounded once to its type.  Serves the layer loop
+ * evaluated in fp32, silu(v) = v / (1 + e^-v) (0 far below 0, NaN at
+ * -infinity); y is rounded once to its type.  Serves the layer loop
  * that the reference runs as block_step and block_step_batch
  * (src/block.c:272-448), between bm_ternary_logits or bm_fp8_logits as
  * in_proj and out_proj.

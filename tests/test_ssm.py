@@ -477,3 +477,106 @@ def test_refuses_lists_off_their_alignment(sampler_lib):
     for slots, fresh in ((q + 2, q), (q, q + 2), (q + 1, None)):
         assert L.bm_ssm_prefill(ctx, layer, q, q, q, q, q, 80, 5, q, 2, slots, fresh, q, 32, None) == -1
     assert L.bm_ssm_step(ctx, layer, q, q, q, q, q, 80, 3, q + 2, q, 32, None) == -1
+
+
+def strongly_negative(p, seed, mid):
+    """Some of a problem's gates and inputs replaced by -1e4 to -3e38 (as many
+    gates by -44 to -85 with `mid`), the convolution reduced to the newest
+    input; returns a mask over the projection's columns of the former."""
+    import torch
+    g = torch.Generator().manual_seed(seed)
+    n = 2 * p.C
+    far = torch.tensor([-1e4, -1e12, -1e19, -1e20, -1e30, -3e38])
+    pick = torch.rand(p.proj.shape[0], n, generator=g)
+    values = far[torch.randint(0, len(far), pick.shape, generator=g)].to(p.t)
+    hit = torch.zeros(p.proj.shape, dtype=torch.bool)
+    hit[:, :n] = pick < 0.3
+    p.proj[:, :n] = torch.where(hit[:, :n], values, p.proj[:, :n])
+    if mid:
+        between = (-44 - 41 * torch.rand(pick[:, :p.C].shape, generator=g)).to(p.t)
+        p.proj[:, :p.C] = torch.where(pick[:, :p.C] > 0.7, between, p.proj[:, :p.C])
+    p.dproj.copy_(p.proj)
+    p.conv.zero_()
+    p.dconv.zero_()
+    p.w["conv_b"][:] = 0
+    p.w["conv_w"][:] = [0, 0, 0, 1]
+    p.dev["conv_b"].zero_()
+    p.dev["conv_w"].copy_(torch.from_numpy(p.w["conv_w"]))
+    torch.cuda.synchronize()
+    return hit
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("P", [32, 15, 4])
+@pytest.mark.parametrize("rows", [40, 300, 2500])
+def test_sigmoids_of_strongly_negative_values(gpu_ctx, sampler_lib, type_, P, rows):
+    """silu is 0 far below 0 whatever the magnitude, next to ordinary channels,
+    and as exact between: what a prompt gives with such inputs and gates is what
+    the formula gives with zeros in their place (silu(0) = 0 too)."""
+    import torch
+    p = Problem(40, type_, 4, P, rows, 1)
+    hit = strongly_negative(p, rows, True)
+    p.prefill(sampler_lib, gpu_ctx, [0, rows])
+    torch.cuda.synchronize()
+    last = p.proj[-3:, p.C:2 * p.C].clone()
+    assert torch.equal(p.dconv[0].cpu(), last)
+    p.proj[hit] = 0.0
+    p.dconv[0] = p.proj[-3:, p.C:2 * p.C].cuda()
+    p.check([0, rows])
+    gpu_ctx.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("P", [32, 15])
+def test_step_with_strongly_negative_values(gpu_ctx, sampler_lib, type_, P):
+    import torch
+    p = Problem(41, type_, 4, P, 20, 20)
+    hit = strongly_negative(p, 5, True)
+    p.step(sampler_lib, gpu_ctx)
+    torch.cuda.synchronize()
+    assert torch.equal(p.dconv[:, 2].cpu(), p.proj[:, p.C:2 * p.C])
+    p.proj[hit] = 0.0
+    # One step from a state s: a s is off by err(a) |s| where ssm_ref.run, which
+    # bounds sums of many terms, has err(a) (a |s| + |g u|).  So its bound is
+    # widened by err(a) |s|, and the output's by that times |C silu(z)|, with
+    # err(a) as derived there: (13 |arg| + 4) u + 8 u d rate + u |v| rate
+    # relative for a = exp(-arg), arg = rate d, d = softplus(v).
+    f = p.proj.double().numpy()
+    C, H, u = p.C, p.H, ssm_ref.U
+    w = {k: v.astype(np.float64) for k, v in p.w.items()}
+    half = 2.0 ** -8 if type_ == "bf16" else u
+    for r in range(20):
+        z, x = f[r:r + 1, :C], f[r:r + 1, C:2 * C]
+        b, c, dt = (f[r:r + 1, 2 * C + k * H:2 * C + (k + 1) * H] for k in range(3))
+        h0 = p.h[r].double().numpy()
+        y, ey, _, h, eh = ssm_ref.run(x, z, b, c, dt, w, H, P, np.zeros((3, C)), h0, False)
+        v, rate = dt[0] + w["dt_bias"], np.exp(w["a_log"])
+        arg = rate * np.logaddexp(v, 0.0)
+        ea = ((13 * arg + 4) + 8 * arg + rate * np.abs(v)) * u * np.exp(-arg)
+        more = ea.repeat(P) * np.abs(h0)
+        got_h, got_y = p.dh[r].double().cpu().numpy(), p.y[r].double().cpu().numpy()
+        assert (np.abs(got_h - h) <= (eh + more) * 1.01 + 1e-30).all()
+        gate = np.abs(c[0].repeat(P) * z[0] / (1.0 + np.exp(-z[0])))
+        assert (np.abs(got_y - y[0]) <= (ey[0] + more * gate) * 1.01 + half * np.abs(y[0]) + 1e-30).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("P", [32, 15])
+def test_infinite_gates(gpu_ctx, sampler_lib, type_, P):
+    """A gate of -infinity is NaN (-inf / inf in the formula), in prompts and
+    steps, and the channels beside it are what they are without it."""
+    import torch
+    for step in (False, True):
+        p, q = (Problem(42, type_, 2, P, 50, 50) for _ in range(2))
+        at = torch.zeros(50, p.C, dtype=torch.bool, device="cuda")
+        at[::3, ::3] = True
+        p.dproj[:, :p.C][at] = -float("inf")
+        torch.cuda.synchronize()
+        for r in (p, q):
+            r.step(sampler_lib, gpu_ctx) if step else r.prefill(sampler_lib, gpu_ctx, [0, 20, 50])
+        torch.cuda.synchronize()
+        assert p.y[at].isnan().all() and torch.equal(p.y[~at], q.y[~at])
+        assert torch.equal(p.dh, q.dh) and torch.equal(p.dconv, q.dconv)
