@@ -156,8 +156,9 @@ int check_regions(const bm_slot_region_t *regions, int n_regions) {
         if (!r.base) why = "base is NULL";
         else if (r.row_bytes < 1 || r.n_outer < 1) why = "row_bytes or n_outer < 1";
         else if (!all_multiple(r, 4)) why = "base, row_bytes or a pitch not a multiple of 4";
-        else if (r.row_bytes > INT32_MAX || r.row_bytes / 16 * r.n_outer > INT32_MAX)
-            why = "more than 32 GB of columns";
+        // (pieces of 16 bytes or more, counted in 32 bits with a grid to spare)
+        else if (r.row_bytes > INT32_MAX || (r.row_bytes + 15) / 16 * r.n_outer > INT32_MAX)
+            why = "more than 2^31 - 1 pieces of 16 bytes in the rows of a slot";
         else if (r.row_pitch < r.row_bytes || (r.n_outer > 1 && r.outer_pitch < r.row_bytes))
             why = "a pitch below row_bytes";
         if (why) {

@@ -247,3 +247,18 @@ def test_decode_compact_captured(gpu_ctx, sampler_lib):
         assert np.array_equal(out.cpu().numpy(), order)
         assert torch.equal(state[:, :len(live)], held[:, torch.from_numpy(live).cuda()])
     dec.close()
+
+
+def test_refuses_more_pieces_than_are_counted(sampler_lib):
+    """Rows of a slot are cut into pieces of 16 bytes at least, whose number,
+    with the rest of each row as one, stays in 31 bits (on the host; no slots,
+    so nothing is launched)."""
+    L = sampler_lib.lib()
+    ctx = ctypes.create_string_buffer(1 << 16)
+    q, most = 1 << 20, 2 ** 31 - 1
+
+    def call(row, outer):
+        return L.bm_slots_reorder(ctx, sampler_lib.slot_regions([(q, row, row, outer, row)]), 1, q, 0, None)
+
+    assert call(16, most) == 0 and call(4, most) == 0 and call(32, most // 2) == 0
+    assert call(20, most) == -1 and call(28, most // 2 + 1) == -1 and call(32, most // 2 + 1) == -1
