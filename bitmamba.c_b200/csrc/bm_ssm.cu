@@ -1138,6 +1138,8 @@ int bm_ssm_step(bm_ctx_t *ctx, const bm_ssm_layer_t *layer, const void *d_x, con
     if (rc != BM_OK || rows == 0) return rc;
     if (rows > layer->n_slots)
         return bm_detail_fail(BM_ERR_INVALID_ARG, "more rows than slots");
+    // (a CTA's next row, up to 65535 further, stays in 31 bits)
+    if (rows > INT32_MAX - 65536) return bm_detail_fail(BM_ERR_UNSUPPORTED, "rows > 2^31 - 65537");
     int sms, *err;
     cudaStream_t s;
     bmc::DeviceGuard guard(bm_detail_ctx(ctx, &sms, &err, &s));

@@ -580,3 +580,12 @@ def test_infinite_gates(gpu_ctx, sampler_lib, type_, P):
         torch.cuda.synchronize()
         assert p.y[at].isnan().all() and torch.equal(p.y[~at], q.y[~at])
         assert torch.equal(p.dh, q.dh) and torch.equal(p.dconv, q.dconv)
+
+
+def test_step_refuses_rows_whose_next_overflows(sampler_lib):
+    L = sampler_lib.lib()
+    ctx = ctypes.create_string_buffer(1 << 16)
+    q, most = 1 << 20, 2 ** 31 - 1
+    layer = sampler_lib.SsmLayer(1, 1, most, "f32", conv_w=q, conv_b=q, dt_bias=q, a_log=q, d=q, conv_state=q, h_state=q).ref
+    assert L.bm_ssm_step(ctx, layer, q, q, q, q, q, 8, most, q, q, 8, None) == -4
+    assert L.bm_ssm_step(ctx, layer, q, q, q, q, q, 8, most - 65535, q, q, 8, None) == -4
