@@ -910,6 +910,14 @@ int check_scale(const void *scale, int64_t ld_scale, int rows) {
     return BM_OK;
 }
 
+int check_operands(const void *a, const void *w, const void *w_scale, const void *out) {
+    if (!a || !w || !w_scale || !out)
+        return bm_detail_fail(BM_ERR_INVALID_ARG, "a, w, w_scale and out must be non-NULL");
+    if (misaligned(a, 16) || misaligned(w, 16) || misaligned(w_scale, 4) || misaligned(out, 4))
+        return bm_detail_fail(BM_ERR_INVALID_ARG, "a or w not 16-byte, or w_scale or out not 4-byte aligned");
+    return BM_OK;
+}
+
 }  // namespace
 }  // namespace bml
 
@@ -959,11 +967,7 @@ int bm_fp8_product(bm_ctx_t *ctx, const uint8_t *d_a, const float *d_a_scale, in
     if (rc == BM_OK) rc = bml::check_rows(rows, n);
     if (rc != BM_OK || rows == 0) return rc;
     if ((rc = bml::check_scale(d_a_scale, ld_scale, rows)) != BM_OK) return rc;
-    if (!d_a || !d_w || !d_w_scale || !d_out)
-        return bm_detail_fail(BM_ERR_INVALID_ARG, "a, w, w_scale and out must be non-NULL");
-    if (bml::misaligned(d_a, 16) || bml::misaligned(d_w, 16) || bml::misaligned(d_w_scale, 4) ||
-        bml::misaligned(d_out, 4))
-        return bm_detail_fail(BM_ERR_INVALID_ARG, "a or w not 16-byte, or w_scale or out not 4-byte aligned");
+    if ((rc = bml::check_operands(d_a, d_w, d_w_scale, d_out)) != BM_OK) return rc;
     int sms, *err;
     cudaStream_t s;
     bmc::DeviceGuard guard(bm_detail_ctx(ctx, &sms, &err, &s));
@@ -984,6 +988,8 @@ int bm_fp8_logits(bm_ctx_t *ctx, const float *d_hidden, int B, int d_model, cons
     if (rc != BM_OK || B == 0) return rc;
     if (!d_hidden || bml::misaligned(d_hidden, 16) || bml::misaligned(d_norm_w, 16))
         return bm_detail_fail(BM_ERR_INVALID_ARG, "hidden NULL, or hidden or norm weight not 16-byte aligned");
+    // (the product's too, before anything is launched)
+    if ((rc = bml::check_operands(d_hidden, d_w, d_w_scale, d_logits)) != BM_OK) return rc;
     int sms, *err;
     cudaStream_t s;
     bmc::DeviceGuard guard(bm_detail_ctx(ctx, &sms, &err, &s));

@@ -423,3 +423,12 @@ def test_quantize_special_values_with_a_norm(gpu_ctx, type_):
     f, s = q.float(), s.T
     assert s[3:5, 0].isinf().all() and f[3:5, 5].isnan().all() and (f[3:5, 6:128] == 0).all()
     assert s[3:5, 1:].isfinite().all() and f[3:5, 128:].isfinite().all()
+
+
+def test_logits_refuses_the_products_operands_first(sampler_lib):
+    """Before the rows are quantised (the context stands for a real one)."""
+    L = sampler_lib.lib()
+    ctx = ctypes.create_string_buffer(1 << 16)
+    q = 1 << 20
+    for w, wsc, out in ((None, q, q), (q + 8, q, q), (q, None, q), (q, q + 2, q), (q, q, None), (q, q, q + 1)):
+        assert L.bm_fp8_logits(ctx, q, 5, 256, q, w, wsc, 100, out, 100, None) == -1
