@@ -15,7 +15,7 @@
 //               narrow tile instead of a padded one.  Bound by the bytes of w: 1 x 50257 x
 //               2048 takes 21 us, 4.9 TB/s.  In the middle, where a layer's
 //               projection is a tile or two an SM, by latency: 72 x 8288 x 2048
-//               takes 9.6 us, 16 x 2048 x 2048 already 5.6.
+//               takes 9.1 us, 16 x 2048 x 2048 already 5.5.
 //   many rows   128 rows of a (lanes) by 128 rows of w: a thread's scale is
 //               one value for its 128 columns.  (With w on the lanes every
 //               column has its own scale, and fetching 128 of them a block
@@ -119,7 +119,8 @@ __device__ __noinline__ uint2 at_the_ends(float4 x, float4 k, float rms, bool hi
 
 // TPR threads per row: a warp's 32 groups of 4 columns are one block of 128.
 // Bound by memory: a row is read once and stays in registers.  8192 x 4096 fp32
-// takes 28.7 us, 5.9 TB/s of reads and writes (the device copies at 6.5).
+// takes 27.9 us, 6.0 TB/s of reads and writes (the device copies at 6.5), bf16
+// 24.7, with a norm 40.3 and 38.6.
 template <typename T, int TPR, bool NORM>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
     quantize_kernel(const T *x, int rows, int d, int64_t ldx, const float *norm_w, uint8_t *q,
@@ -637,7 +638,8 @@ cudaError_t few_rows(const uint8_t *a, const uint8_t *w, const ProductArgs &p, i
 // scale a block.  Promoting a block takes a warp longer than the tensor core
 // needs for it, and a tile's sums take as long as several blocks to go out:
 // with two pipelines, one works while the other waits.  2048 x 50257 x 2048
-// takes 300 us (1.40 PFLOP/s; 412 MB of them stores): 225 without the stores,
+// takes 303 us alone and 350 among other work, under the power limit's clocks
+// (1.39 and 1.21 PFLOP/s; 412 MB of stores), 300 when this was taken: 225 without the stores,
 // 190 without the promotion's multiply-adds as well, 125 with one MMA of four;
 // half the copies change nothing.  (One tile of 256 columns for all eight warps
 // took 356 us, two groups behind one pipeline 327 when this took 322.)  128 sums and 64 values on

@@ -143,11 +143,12 @@ __device__ __forceinline__ Head head_of(float dt, float rate, float b, float c) 
 // and 123 us for 4099 x 4096 fp32; the chain over the tiles was what it spent
 // its time on.
 //
-// 65536 x 4096 bf16 takes 510 us (3.2 TB/s; 250 us at the device's 6.5): 78
+// 65536 x 4096 bf16 takes 526 us (3.1 TB/s; 250 us at the device's 6.5): 73
 // instructions a pair of channels and token keep the issue slots of the 128
-// SMs that have channels 59 % busy, the 6 special functions among them 36 %,
-// and two barriers a tile the rest.  32768 x 4096 fp32 takes 350 us (4.6 TB/s),
-// 4099 x 4096 fp32 in 13 sequences 61 us, 53 as one sequence: a tile with a
+// SMs that have channels 56 % busy, the 8 special functions among them half
+// of their units' rate; the rest are waits for those and for shared memory, and
+// two barriers a tile.  32768 x 4096 fp32 takes 351 us (4.7 TB/s), 4099 x 4096
+// fp32 in 13 sequences 60 us, 53 as one sequence: a tile with a
 // boundary has its rows looked up, and its warps wait for the one that has it.
 
 // Copies to shared memory: 4 or 8 bytes asynchronously, a 2-byte element
